@@ -29,6 +29,7 @@ enum mbx_itype { MBX_I16 = 0, MBX_I32 = 1, MBX_I64 = 2 };
 enum mbx_dtype { MBX_BF16 = 0, MBX_F16 = 1, MBX_F32 = 2 };
 enum mbx_layout { MBX_NN = 0, MBX_NT = 1, MBX_TN = 2 };
 enum mbx_activation { MBX_ACT_SILU = 0, MBX_ACT_GELU_TANH = 1 };
+enum mbx_score { MBX_SCORE_SOFTMAX = 0, MBX_SCORE_SIGMOID = 1 };
 
 #define MBX_EINVAL (-1)   /* bad enum / negative size / null pointer */
 #define MBX_ESCRATCH (-2) /* scratch buffer too small */
@@ -492,6 +493,33 @@ int mbx_loss_sum(const void* values, int dtype, const int32_t* counts, int64_t n
                  mbx_stream_t stream);
 int mbx_loss_gradient(const float* grad, const void* values, int dtype, const int32_t* counts, int64_t n, int period, float scale, void* out,
                       mbx_stream_t stream);
+
+/* ---- choice of experts by scores, bias and groups ----
+ * The router of layers whose experts are kept in balance by a bias and chosen in two steps; no counterpart in the reference, whose router is
+ * mbx_router_forward (softmax, top-k).  For `tokens` rows x of num_experts logits, scores s = softmax(x) or 1 / (1 + exp(-x)):
+ *   key     = s + bias (bias [num_experts], fp32), or without a bias (NULL) x, whose order is that of s
+ *   groups  of num_experts / groups neighbouring experts; a group's key is the sum of its group_best (1 or 2) largest keys (without a bias: scores);
+ *           the top_groups groups of largest key are open, ties to the lower one
+ *   indices = the top_k experts of open groups with the largest keys, in descending order, ties to the lower index, NaN first   [tokens, top_k]
+ *   weights = scale * s[indices] / ||s[indices]||_p with p = norm_p > 0 (0: not divided), rounded once; zero where the norm is zero   [tokens, top_k]
+ *   scores  = s, rounded (NULL: not wanted)   [tokens, num_experts];  lse = logsumexp(x), fp32 (NULL: not wanted)   [tokens]
+ * The choice is that of the exact keys: where fp32 does not tell two of them apart it is done in 64 bits.  indices32 (NULL: not wanted): the indices as
+ * int32.  top_k <= top_groups * num_experts / groups, groups divides num_experts (else MBX_EINVAL); up to 512 experts, top_k and groups up to 64 (else
+ * MBX_EUNSUPPORTED). */
+int mbx_choose_experts(const void* logits, int dtype, int64_t tokens, int num_experts, int top_k, int score, const float* bias, int groups, int top_groups,
+                       int group_best, float norm_p, float scale, void* scores, void* weights, int64_t* indices, int32_t* indices32, float* lse,
+                       mbx_stream_t stream);
+
+/* The gradient of the logits behind mbx_choose_experts, from those of weights, scores (both of type dtype) and lse (fp32), each NULL where there is none; the
+ * choice itself, and with it the bias, has none.  indices: the forward's (distinct experts of a token). */
+int mbx_choose_experts_backward(const void* grad_weights, const void* grad_scores, const float* grad_lse, const void* logits, const int64_t* indices, int dtype,
+                                int64_t tokens, int num_experts, int top_k, int score, float norm_p, float scale, void* grad_logits, mbx_stream_t stream);
+
+/* The update that keeps experts in balance, of all layers by one launch: out[l][e] = bias[l][e] + rate * sign(mean over the experts of n - n[e]), n[e] the
+ * sum of the rows[l] rows of counts[l] ([rows[l], num_experts], tokens per expert), compared in whole numbers.  out[l] may be bias[l].  The arrays of
+ * pointers and `rows` are in host memory, read before the call returns. */
+int mbx_balance_bias(const float* const* bias, const int32_t* const* counts, const int* rows, float* const* out, int layers, int num_experts, float rate,
+                     mbx_stream_t stream);
 
 #ifdef __cplusplus
 }

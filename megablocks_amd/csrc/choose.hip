@@ -1,0 +1,622 @@
+// The choice of experts by softmax or sigmoid scores, with a bias that keeps the experts in balance, by groups, its gradient, and the
+// update of the bias.
+//
+//   s = softmax(x) or 1 / (1 + exp(-x));  key = s + bias, without a bias x itself, whose order is the same
+//   group key = the sum of the group's `group_best` (1, 2) largest keys (without a bias: scores); the `top_groups` largest are open
+//   indices = the top_k open experts of largest key, in descending order; ties go to the lower index, NaN comes first
+//   weights = scale s[indices] / ||s[indices]||_p
+//
+// The order is that of the exact keys.  Scores in fp32 are off by some 2^-23, and of 256 scores of a token two neighbours in the order are closer
+// than that once in a few thousand tokens: where two keys next to each other in the order are within kCloseKeys without being made of the same logit and
+// bias, the wave does the choice over with keys in 64 bits.
+//
+// LANES (16 or 64) lanes have a token, R experts in a row each, so that a lane reads and writes its experts as one piece and most groups are a
+// power of two of neighbouring lanes.
+#include "common.h"
+
+namespace mbx {
+namespace {
+
+constexpr int kChooseThreads = 256;
+constexpr int kChooseMaxExperts = 512, kChooseMaxTopK = 64, kChooseMaxGroups = 64;
+constexpr float kCloseKeys = 0x1p-19f;   // of 1 + |key|: 16 times what the keys are off by
+
+struct Choose {
+  const void* logits;
+  const float* bias;
+  int64_t tokens;
+  int experts, top_k, sigmoid, groups, top_groups, group_best;
+  float norm_p, scale;
+  void* scores;
+  void* weights;
+  int64_t* indices;
+  int32_t* indices32;
+  float* lse;
+};
+
+// ---- between the LANES lanes of a token ----
+
+template <int CTRL, typename T>
+__device__ __forceinline__ T dpp(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+  }
+}
+
+// v of the rows of 16 (half waves) and of the other row of the pair (half wave), as first(..) and second(..)
+template <bool HALVES, typename T>
+__device__ __forceinline__ void swapped(T v, T& first, T& second) {
+  const auto swap = [](uint32_t x) {
+    if constexpr (HALVES) return __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    else return __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  };
+  if constexpr (sizeof(T) == 4) {
+    const auto p = swap(__builtin_bit_cast(uint32_t, v));
+    first = __builtin_bit_cast(T, (uint32_t)p[0]);
+    second = __builtin_bit_cast(T, (uint32_t)p[1]);
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+    first = __builtin_bit_cast(T, (uint64_t)(uint32_t)hi[0] << 32 | (uint32_t)lo[0]);
+    second = __builtin_bit_cast(T, (uint64_t)(uint32_t)hi[1] << 32 | (uint32_t)lo[1]);
+  }
+}
+
+constexpr int kQuadXor1 = 0xb1, kQuadXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+
+// all lanes of a token get v combined over them, for a commutative op
+template <int LANES, typename T, typename F>
+__device__ __forceinline__ T over_token(T v, F&& op) {
+  v = op(v, dpp<kQuadXor1>(v));
+  v = op(v, dpp<kQuadXor2>(v));
+  v = op(v, dpp<kHalfMirror>(v));   // the lanes of a quad are alike
+  v = op(v, dpp<kMirror>(v));
+  if constexpr (LANES == 64) {
+    T a, b;
+    swapped<false>(v, a, b);
+    v = op(a, b);
+    swapped<true>(v, a, b);
+    v = op(a, b);
+  }
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ T larger(T a, T b) { return a > b ? a : b; }
+template <typename T> __device__ __forceinline__ T smaller(T a, T b) { return a < b ? a : b; }
+
+template <int LANES, typename T> __device__ __forceinline__ T token_max(T v) { return over_token<LANES>(v, [](T a, T b) { return larger(a, b); }); }
+template <int LANES, typename T> __device__ __forceinline__ T token_min(T v) { return over_token<LANES>(v, [](T a, T b) { return smaller(a, b); }); }
+template <int LANES, typename T> __device__ __forceinline__ T token_sum(T v) { return over_token<LANES>(v, [](T a, T b) { return a + b; }); }
+
+// ---- keys as whole numbers in their order: 0 stands for "not a candidate", the largest for NaN ----
+
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.f);   // -0 as 0
+  return v != v ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.);
+  return v != v ? ~0ull : (u >> 63) ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ float unordered(uint32_t u) { return u == 0xffffffffu ? NAN : __builtin_bit_cast(float, (u & 0x80000000u) ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ double unordered(uint64_t u) {
+  return u == ~0ull ? (double)NAN : __builtin_bit_cast(double, (u >> 63) ? u & ~(1ull << 63) : ~u);
+}
+
+template <typename F> struct Keys;
+template <> struct Keys<float> { typedef uint32_t type; };
+template <> struct Keys<double> { typedef uint64_t type; };
+
+// The open groups of a token as a bit each, given its experts' keys (0: none).  close: whether two groups on either side of the border are
+// within what the keys may be off by.
+template <int LANES, int R, typename F>
+__device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&key)[R], const Choose& c, int lane, bool& close) {
+  typedef typename Keys<F>::type U;
+  const int size = c.experts / c.groups, base = lane * R;
+  const auto merge = [](U& m1, U& m2, U a1, U a2) {
+    const U low = smaller(m1, a1);
+    m1 = larger(m1, a1);
+    m2 = larger(low, larger(m2, a2));   // at most one of m2 and a2 is above `low`
+  };
+  const auto value = [&](U m1, U m2) {
+    const F first = unordered(m1);
+    return c.group_best == 2 && m2 != 0 ? first + unordered(m2) : first;
+  };
+  F mine = 0;   // of group `lane`
+  const int per = size / R;
+  if (per * R == size && per > 0 && (per & (per - 1)) == 0) {   // a group is `per` lanes next to each other
+    U m1 = 0, m2 = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) merge(m1, m2, key[r], 0);
+    if (per > 1) merge(m1, m2, dpp<kQuadXor1>(m1), dpp<kQuadXor1>(m2));
+    if (per > 2) merge(m1, m2, dpp<kQuadXor2>(m1), dpp<kQuadXor2>(m2));
+    if (per > 4) merge(m1, m2, dpp<kHalfMirror>(m1), dpp<kHalfMirror>(m2));
+    if (per > 8) merge(m1, m2, dpp<kMirror>(m1), dpp<kMirror>(m2));
+    if constexpr (LANES == 64) {
+      U a1, a2;
+      if (per > 16) { swapped<false>(m1, m1, a1); swapped<false>(m2, m2, a2); merge(m1, m2, a1, a2); }
+      if (per > 32) { swapped<true>(m1, m1, a1); swapped<true>(m2, m2, a2); merge(m1, m2, a1, a2); }
+    }
+    mine = __shfl(value(m1, m2), lane * per < LANES ? lane * per : 0, LANES);
+  } else {
+    for (int g = 0; g < c.groups; ++g) {
+      U m1 = 0, m2 = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int e = base + r;
+        merge(m1, m2, e >= g * size && e < (g + 1) * size ? key[r] : 0, 0);
+      }
+      merge(m1, m2, dpp<kQuadXor1>(m1), dpp<kQuadXor1>(m2));
+      merge(m1, m2, dpp<kQuadXor2>(m1), dpp<kQuadXor2>(m2));
+      merge(m1, m2, dpp<kHalfMirror>(m1), dpp<kHalfMirror>(m2));
+      merge(m1, m2, dpp<kMirror>(m1), dpp<kMirror>(m2));
+      if constexpr (LANES == 64) {
+        U a1, a2;
+        swapped<false>(m1, m1, a1); swapped<false>(m2, m2, a2); merge(m1, m2, a1, a2);
+        swapped<true>(m1, m1, a1); swapped<true>(m2, m2, a2); merge(m1, m2, a1, a2);
+      }
+      if (lane == g) mine = value(m1, m2);
+    }
+  }
+  const U order = ordered(mine);
+  int before = 0;
+  for (int g = 0; g < c.groups; ++g) {
+    const U other = __shfl(order, g, LANES);
+    before += other > order || (other == order && g < lane) ? 1 : 0;
+  }
+  const bool group = lane < c.groups, open = group && before < c.top_groups;
+  const F lowest = token_min<LANES>(open ? mine : (F)INFINITY), highest = token_max<LANES>(group && !open ? mine : (F)-INFINITY);
+  close = !(lowest - highest > (F)(2 * kCloseKeys) * (1 + (highest < 0 ? -highest : highest)));
+  const uint64_t all = __ballot(open);
+  return LANES == 64 ? all : (all >> (lane_id() & ~(LANES - 1))) & 0xffffu;
+}
+
+template <int R>
+__device__ __forceinline__ void keep_open(uint32_t (&key)[R], uint64_t open, int base, int size) {
+  int g = base / size, in = base - g * size;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (!((open >> g) & 1)) key[r] = 0;
+    if (++in == size) { in = 0; ++g; }
+  }
+}
+template <int R>
+__device__ __forceinline__ void keep_open(uint64_t (&key)[R], uint64_t open, int base, int size) {
+  int g = base / size, in = base - g * size;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (!((open >> g) & 1)) key[r] = 0;
+    if (++in == size) { in = 0; ++g; }
+  }
+}
+
+// The experts of the `count` largest keys, in order: lane j has the j-th in `mine`; the one after the first top_k in `next`.
+template <int LANES, int R, typename U>
+__device__ __forceinline__ void pick(U (&key)[R], int lane, int top_k, int count, int& mine, int& next) {
+  const int base = lane * R;
+  for (int j = 0; j < count; ++j) {
+    U best = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) best = larger(best, key[r]);
+    best = token_max<LANES>(best);
+    int e = 0x7fffffff;
+#pragma unroll
+    for (int r = R - 1; r >= 0; --r) e = key[r] == best ? base + r : e;
+    e = token_min<LANES>(e);
+    if (j == top_k) next = e;
+    else if (lane == j) mine = e;
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = base + r == e ? 0 : key[r];
+  }
+}
+
+// Where 16-bit numbers come out, the quick exponential and reciprocal do: they are off by a few 2^-24 of the largest score.
+template <int DT> __device__ __forceinline__ float exp_of(float v) { return DT == MBX_F32 ? expf(v) : __expf(v); }
+template <int DT> __device__ __forceinline__ float over(float a, float b) { return DT == MBX_F32 ? a / b : a * __builtin_amdgcn_rcpf(b); }
+
+// ||w||_p over a token's lanes
+template <int LANES>
+__device__ __forceinline__ float token_pnorm(float w, float p) {
+  const float a = fabsf(w);
+  const float sum = token_sum<LANES>(p == 1.f ? a : p == 2.f ? a * a : a == 0.f ? 0.f : powf(a, p));
+  return p == 1.f ? sum : p == 2.f ? sqrtf(sum) : powf(sum, 1.f / p);
+}
+
+// A lane's R experts of a row.  whole: rows and the base are whole pieces of R.
+template <int DT, int R>
+__device__ __forceinline__ void read_row(const typename Elem<DT>::type* __restrict__ row, int base, int experts, bool whole, float past, float (&x)[R]) {
+  typedef typename Elem<DT>::type E;
+  if (whole) {
+    struct alignas(R * sizeof(E) < 16 ? R * sizeof(E) : 16) Piece { E v[R]; };
+    Piece piece = {};
+    if (base < experts) piece = *(const Piece*)(row + base);
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = base < experts ? Elem<DT>::to_f32(piece.v[r]) : past;
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = base + r < experts ? Elem<DT>::to_f32(row[base + r]) : past;
+  }
+}
+template <int DT, int R>
+__device__ __forceinline__ void write_row(typename Elem<DT>::type* __restrict__ row, int base, int experts, bool whole, const float (&x)[R]) {
+  typedef typename Elem<DT>::type E;
+  if (whole) {
+    struct alignas(R * sizeof(E) < 16 ? R * sizeof(E) : 16) Piece { E v[R]; };
+    Piece piece;
+#pragma unroll
+    for (int r = 0; r < R; ++r) piece.v[r] = Elem<DT>::from_f32(x[r]);
+    if (base < experts) *(Piece*)(row + base) = piece;
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (base + r < experts) row[base + r] = Elem<DT>::from_f32(x[r]);
+  }
+}
+
+// A token's choice again, with keys in 64 bits
+template <int LANES, int R>
+__device__ __forceinline__ void pick_wide(const float (&x)[R], const float (&bias)[R], const Choose& c, int lane, int& mine) {
+  const int base = lane * R;
+  double s[R], sum = 0, top = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < R; ++r) top = larger(top, base + r < c.experts ? (double)x[r] : (double)-INFINITY);
+  top = token_max<LANES>(top);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const double v = x[r];
+    s[r] = base + r >= c.experts ? 0. : c.sigmoid ? 1. / (1. + exp(-v)) : exp(v - top);
+    sum += s[r];
+  }
+  if (!c.sigmoid) {
+    sum = token_sum<LANES>(sum);
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] /= sum;
+  }
+  uint64_t key[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = base + r < c.experts ? ordered(c.bias ? s[r] + (double)bias[r] : s[r]) : 0;
+  if (c.top_groups < c.groups) {
+    bool close;
+    const uint64_t open = open_groups<LANES, R, double>(key, c, lane, close);
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = c.bias ? key[r] : base + r < c.experts ? ordered((double)x[r]) : 0;
+    keep_open(key, open, base, c.experts / c.groups);
+  }
+  int next;
+  pick<LANES, R>(key, lane, c.top_k, c.top_k, mine, next);
+}
+
+template <int DT, int LANES, int R>
+__device__ __forceinline__ void choose_token(const float (&x)[R], const float (&bias)[R], const typename Elem<DT>::type* __restrict__ row, int64_t t, bool real,
+                                             const Choose& c, bool whole) {
+  typedef typename Elem<DT>::type E;
+  const int lane = lane_id() % LANES, base = lane * R;
+  float m = 0.f, sum = 1.f, s[R];
+  if (!c.sigmoid || c.lse) {
+    m = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r) m = fmaxf(m, x[r]);
+    m = token_max<LANES>(m);
+    sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r] = base + r < c.experts ? exp_of<DT>(x[r] - m) : 0.f;
+      sum += s[r];
+    }
+    sum = token_sum<LANES>(sum);
+    if (c.lse && lane == 0 && real) c.lse[t] = m == INFINITY || m == -INFINITY ? m : m + logf(sum);
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) s[r] = c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-x[r])) : over<DT>(s[r], sum);
+  if (c.scores && real) write_row<DT, R>((E*)c.scores + t * c.experts, base, c.experts, whole, s);
+
+  uint32_t key[R];
+  bool close = false;
+  const bool grouped = c.top_groups < c.groups;
+  uint64_t open = ~0ull;
+  if (grouped) {
+    // without a bias the best of a group by its logit, exactly
+    const bool by_logit = !c.bias && c.group_best == 1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = base + r < c.experts ? ordered(by_logit ? x[r] : c.bias ? s[r] + bias[r] : s[r]) : 0;
+    open = open_groups<LANES, R, float>(key, c, lane, close);
+    close = close && !by_logit;
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = base + r < c.experts ? ordered(c.bias ? s[r] + bias[r] : x[r]) : 0;
+  const int size = c.experts / c.groups;
+  if (grouped) keep_open(key, open, base, size);
+  int mine = 0, next = -1;
+  const int more = c.bias && c.top_k < c.top_groups * size ? 1 : 0;
+  pick<LANES, R>(key, lane, c.top_k, c.top_k + more, mine, next);
+
+  const bool live = lane < c.top_k;
+  const auto key_of = [&](int e, float& logit, float& by) {
+    logit = Elem<DT>::to_f32(row[e]);
+    by = c.bias[e];
+    return (c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-logit)) : over<DT>(exp_of<DT>(logit - m), sum)) + by;
+  };
+  if (c.bias) {
+    // each chosen key against the next in the order, of the next lane or behind the last
+    int after = __shfl_down(mine, 1, LANES);
+    if (lane == c.top_k - 1) after = next;
+    if (live && after >= 0 && (lane < c.top_k - 1 || more)) {
+      float x0, b0, x1, b1;
+      const float k0 = key_of(mine, x0, b0), k1 = key_of(after, x1, b1);
+      close = close || (!(k0 - k1 > kCloseKeys * (1.f + fabsf(k0))) && !(x0 == x1 && b0 == b1));
+    }
+  }
+  if (__any(close)) pick_wide<LANES, R>(x, bias, c, lane, mine);
+
+  float w = 0.f;
+  if (live) {
+    const float logit = Elem<DT>::to_f32(row[mine]);
+    w = c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-logit)) : over<DT>(exp_of<DT>(logit - m), sum);
+  }
+  if (c.norm_p > 0.f) {
+    const float norm = token_pnorm<LANES>(w, c.norm_p);
+    w = norm == 0.f ? 0.f : w / norm;   // scores that are all zero: weights of zero
+  }
+  if (live && real) {
+    ((E*)c.weights)[t * c.top_k + lane] = Elem<DT>::from_f32(w * c.scale);
+    c.indices[t * c.top_k + lane] = mine;
+    if (c.indices32) c.indices32[t * c.top_k + lane] = mine;
+  }
+}
+
+template <int R>
+__device__ __forceinline__ void read_bias(const Choose& c, int base, float (&bias)[R]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) bias[r] = c.bias && base + r < c.experts ? c.bias[base + r] : 0.f;
+}
+
+template <int DT, int LANES, int R>
+__global__ void __launch_bounds__(kChooseThreads) choose_kernel(const Choose c, bool whole) {
+  typedef typename Elem<DT>::type E;
+  constexpr int kTokens = kChooseThreads / LANES;
+  const int lane = lane_id() % LANES, base = lane * R;
+  float bias[R];
+  read_bias(c, base, bias);
+  const int64_t step = (int64_t)gridDim.x * kTokens;
+  for (int64_t first = (int64_t)blockIdx.x * kTokens; first < c.tokens; first += step) {
+    const int64_t token = first + threadIdx.x / LANES, t = token < c.tokens ? token : c.tokens - 1;   // all lanes stay: the last token again, not written
+    const E* const row = (const E*)c.logits + t * c.experts;
+    float x[R];
+    read_row<DT, R>(row, base, c.experts, whole, -INFINITY, x);
+    choose_token<DT, LANES, R>(x, bias, row, t, token < c.tokens, c, whole);
+  }
+}
+
+// grad_logits from the gradients of weights, scores and lse (each may be NULL), in fp32 from the logits:
+//   y = scale w / n, n = ||w||_p:   dw = scale (dy / n - (sum dy w) / n^2 (w / n)^(p - 1)), zero where n is;  ds = grad_scores + dw at the chosen experts
+//   dx = ds s (1 - s) (sigmoid), s (ds - sum ds s) (softmax);  + grad_lse softmax(x)
+template <int DT, int LANES, int R>
+__global__ void __launch_bounds__(kChooseThreads)
+choose_backward_kernel(const Choose c, const void* __restrict__ grad_weights, const void* __restrict__ grad_scores, const float* __restrict__ grad_lse,
+                       void* __restrict__ grad_logits, bool whole) {
+  typedef typename Elem<DT>::type E;
+  constexpr int kTokens = kChooseThreads / LANES;
+  const int lane = lane_id() % LANES, base = lane * R;
+  const int64_t step = (int64_t)gridDim.x * kTokens;
+  for (int64_t first = (int64_t)blockIdx.x * kTokens; first < c.tokens; first += step) {
+    const int64_t token = first + threadIdx.x / LANES, t = token < c.tokens ? token : c.tokens - 1;
+    const E* const row = (const E*)c.logits + t * c.experts;
+    float x[R], ds[R], soft[R];
+    read_row<DT, R>(row, base, c.experts, whole, -INFINITY, x);
+    if (grad_scores) read_row<DT, R>((const E*)grad_scores + t * c.experts, base, c.experts, whole, 0.f, ds);
+    else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) ds[r] = 0.f;
+    }
+    float m = 0.f, sum = 1.f;
+    const bool softmax = !c.sigmoid || grad_lse;
+    if (softmax) {
+      m = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < R; ++r) m = fmaxf(m, x[r]);
+      m = token_max<LANES>(m);
+      sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        soft[r] = base + r < c.experts ? exp_of<DT>(x[r] - m) : 0.f;
+        sum += soft[r];
+      }
+      sum = token_sum<LANES>(sum);
+#pragma unroll
+      for (int r = 0; r < R; ++r) soft[r] = over<DT>(soft[r], sum);
+    }
+    if (grad_weights) {
+      const bool live = lane < c.top_k;
+      int mine = live ? (int)c.indices[t * c.top_k + lane] : 0;
+      mine = mine < 0 || mine >= c.experts ? 0 : mine;
+      float w = 0.f, dy = 0.f;
+      if (live) {
+        const float logit = Elem<DT>::to_f32(row[mine]);
+        w = c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-logit)) : over<DT>(exp_of<DT>(logit - m), sum);
+        dy = Elem<DT>::to_f32(((const E*)grad_weights)[t * c.top_k + lane]) * c.scale;
+      }
+      float dw = dy;
+      if (c.norm_p > 0.f) {
+        const float p = c.norm_p, n = token_pnorm<LANES>(w, p), dot = token_sum<LANES>(dy * w);
+        const float u = w / n, dn = p == 1.f ? 1.f : p == 2.f ? u : powf(u, p - 1.f);
+        dw = n == 0.f || !live ? 0.f : (dy - dot / n * dn) / n;
+      }
+      for (int j = 0; j < c.top_k; ++j) {
+        const int e = __shfl(mine, j, LANES);
+        const float v = __shfl(dw, j, LANES);
+#pragma unroll
+        for (int r = 0; r < R; ++r) ds[r] += base + r == e ? v : 0.f;
+      }
+    }
+    float dx[R];
+    if (c.sigmoid) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        // s (1 - s) from exp(-|x|): exact towards either end
+        const float a = exp_of<DT>(-fabsf(x[r])), b = 1.f + a;
+        dx[r] = ds[r] * over<DT>(a, b * b);
+      }
+    } else {
+      float dot = 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) dot += ds[r] * soft[r];
+      dot = token_sum<LANES>(dot);
+#pragma unroll
+      for (int r = 0; r < R; ++r) dx[r] = soft[r] * (ds[r] - dot);
+    }
+    if (grad_lse) {
+      const float g = grad_lse[t];
+#pragma unroll
+      for (int r = 0; r < R; ++r) dx[r] += g * soft[r];
+    }
+    if (token < c.tokens) write_row<DT, R>((E*)grad_logits + t * c.experts, base, c.experts, whole, dx);
+  }
+}
+
+// bias + rate sign(mean count - count), the mean in whole numbers: of every layer a workgroup.
+constexpr int kBalanceLayers = 64;
+template <int MOST>
+struct Balance {
+  const float* bias[MOST];
+  const int32_t* counts[MOST];
+  float* out[MOST];
+  int rows[MOST];
+};
+
+template <int MOST>
+__global__ void __launch_bounds__(kChooseThreads) balance_kernel(const Balance<MOST> layers, int experts, float rate) {
+  __shared__ int64_t sums[kChooseThreads / kWave];
+  const float* const bias = layers.bias[blockIdx.x];
+  const int32_t* const counts = layers.counts[blockIdx.x];
+  float* const out = layers.out[blockIdx.x];
+  const int rows = layers.rows[blockIdx.x];
+  const auto count_of = [&](int e) {
+    int64_t n = 0;
+    for (int row = 0; row < rows; ++row) n += counts[(int64_t)row * experts + e];
+    return n;
+  };
+  int64_t total = 0;
+  for (int e = threadIdx.x; e < experts; e += kChooseThreads) total += count_of(e);
+  total = over_token<64>(total, [](int64_t a, int64_t b) { return a + b; });
+  if (lane_id() == 0) sums[threadIdx.x / kWave] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kChooseThreads / kWave; ++w) total += sums[w];
+  for (int e = threadIdx.x; e < experts; e += kChooseThreads) {
+    const int64_t off = total - count_of(e) * experts;
+    out[e] = bias[e] + (off > 0 ? rate : off < 0 ? -rate : 0.f);
+  }
+}
+
+template <int MOST>
+static void launch_balance(const float* const* bias, const int32_t* const* counts, const int* rows, float* const* out, int layers, int experts, float rate,
+                           hipStream_t s) {
+  Balance<MOST> of = {};
+  for (int l = 0; l < layers; ++l) {
+    of.bias[l] = bias[l];
+    of.counts[l] = counts[l];
+    of.out[l] = out[l];
+    of.rows[l] = rows[l];
+  }
+  balance_kernel<MOST><<<(unsigned)layers, kChooseThreads, 0, s>>>(of, experts, rate);
+}
+
+static unsigned choose_grid(int64_t tokens, int lanes) {
+  const int64_t blocks = ceil_div(tokens, kChooseThreads / lanes);
+  return (unsigned)(blocks < 4096 ? blocks : 4096);
+}
+
+static bool few_lanes(const Choose& c) { return c.experts <= 256 && c.top_k <= 16 && c.groups <= 16; }
+
+static bool pieces(const Choose& c, int r, int size, const void* a, const void* b, const void* d) {
+  const uintptr_t at = (uintptr_t)a | (uintptr_t)b | (uintptr_t)d, piece = (uintptr_t)(r * size < 16 ? r * size : 16);
+  return c.experts % r == 0 && at % piece == 0;
+}
+
+// KERNEL<DT, LANES, R> of the sizes
+#define MBX_CHOOSE(DT, KERNEL, SIZE, A, B, D, ...)                                                                                            \
+  do {                                                                                                                                        \
+    if (few_lanes(c)) {                                                                                                                       \
+      const unsigned grid = choose_grid(c.tokens, 16);                                                                                        \
+      if (c.experts <= 16) KERNEL<DT, 16, 1><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 1, SIZE, A, B, D));                       \
+      else if (c.experts <= 32) KERNEL<DT, 16, 2><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 2, SIZE, A, B, D));                  \
+      else if (c.experts <= 64) KERNEL<DT, 16, 4><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 4, SIZE, A, B, D));                  \
+      else if (c.experts <= 128) KERNEL<DT, 16, 8><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 8, SIZE, A, B, D));                 \
+      else KERNEL<DT, 16, 16><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 16, SIZE, A, B, D));                                     \
+    } else {                                                                                                                                  \
+      const unsigned grid = choose_grid(c.tokens, 64);                                                                                        \
+      if (c.experts <= 64) KERNEL<DT, 64, 1><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 1, SIZE, A, B, D));                       \
+      else if (c.experts <= 128) KERNEL<DT, 64, 2><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 2, SIZE, A, B, D));                 \
+      else if (c.experts <= 256) KERNEL<DT, 64, 4><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 4, SIZE, A, B, D));                 \
+      else KERNEL<DT, 64, 8><<<grid, kChooseThreads, 0, s>>>(__VA_ARGS__, pieces(c, 8, SIZE, A, B, D));                                       \
+    }                                                                                                                                         \
+  } while (0)
+
+static int choose_sizes(int dtype, int64_t tokens, int experts, int top_k, int score, int groups, int top_groups, int group_best, float norm_p, float scale) {
+  if (dtype != MBX_BF16 && dtype != MBX_F16 && dtype != MBX_F32) return MBX_EINVAL;
+  if (tokens < 0 || experts <= 0 || top_k <= 0 || (score != MBX_SCORE_SOFTMAX && score != MBX_SCORE_SIGMOID)) return MBX_EINVAL;
+  if (groups <= 0 || experts % groups || top_groups <= 0 || top_groups > groups || (group_best != 1 && group_best != 2)) return MBX_EINVAL;
+  if ((int64_t)top_k > (int64_t)top_groups * (experts / groups) || !(norm_p >= 0.f) || !(norm_p < INFINITY) || !(scale - scale == 0.f)) return MBX_EINVAL;
+  if (experts > kChooseMaxExperts || top_k > kChooseMaxTopK || groups > kChooseMaxGroups) return MBX_EUNSUPPORTED;
+  return 0;
+}
+
+}  // namespace
+}  // namespace mbx
+
+using namespace mbx;
+
+extern "C" {
+
+int mbx_choose_experts(const void* logits, int dtype, int64_t tokens, int num_experts, int top_k, int score, const float* bias, int groups, int top_groups,
+                       int group_best, float norm_p, float scale, void* scores, void* weights, int64_t* indices, int32_t* indices32, float* lse,
+                       mbx_stream_t stream) {
+  const int rc = choose_sizes(dtype, tokens, num_experts, top_k, score, groups, top_groups, group_best, norm_p, scale);
+  if (rc || tokens == 0) return rc;
+  if (!logits || !weights || !indices) return MBX_EINVAL;
+  const Choose c = {logits, bias, tokens, num_experts, top_k, score == MBX_SCORE_SIGMOID, groups, top_groups, group_best, norm_p, scale,
+                    scores, weights, indices, indices32, lse};
+  hipStream_t s = as_stream(stream);
+  if (dtype == MBX_BF16) MBX_CHOOSE(MBX_BF16, choose_kernel, 2, logits, scores, nullptr, c);
+  else if (dtype == MBX_F16) MBX_CHOOSE(MBX_F16, choose_kernel, 2, logits, scores, nullptr, c);
+  else MBX_CHOOSE(MBX_F32, choose_kernel, 4, logits, scores, nullptr, c);
+  return launch_status();
+}
+
+int mbx_choose_experts_backward(const void* grad_weights, const void* grad_scores, const float* grad_lse, const void* logits, const int64_t* indices, int dtype,
+                                int64_t tokens, int num_experts, int top_k, int score, float norm_p, float scale, void* grad_logits, mbx_stream_t stream) {
+  const int rc = choose_sizes(dtype, tokens, num_experts, top_k, score, 1, 1, 1, norm_p, scale);
+  if (rc || tokens == 0) return rc;
+  if (!logits || !grad_logits || (grad_weights && !indices)) return MBX_EINVAL;
+  const Choose c = {logits, nullptr, tokens, num_experts, top_k, score == MBX_SCORE_SIGMOID, 1, 1, 1, norm_p, scale,
+                    nullptr, nullptr, const_cast<int64_t*>(indices), nullptr, nullptr};
+  hipStream_t s = as_stream(stream);
+  if (dtype == MBX_BF16) MBX_CHOOSE(MBX_BF16, choose_backward_kernel, 2, logits, grad_scores, grad_logits, c, grad_weights, grad_scores, grad_lse, grad_logits);
+  else if (dtype == MBX_F16) MBX_CHOOSE(MBX_F16, choose_backward_kernel, 2, logits, grad_scores, grad_logits, c, grad_weights, grad_scores, grad_lse, grad_logits);
+  else MBX_CHOOSE(MBX_F32, choose_backward_kernel, 4, logits, grad_scores, grad_logits, c, grad_weights, grad_scores, grad_lse, grad_logits);
+  return launch_status();
+}
+
+int mbx_balance_bias(const float* const* bias, const int32_t* const* counts, const int* rows, float* const* out, int layers, int num_experts, float rate,
+                     mbx_stream_t stream) {
+  if (layers < 0 || num_experts <= 0) return MBX_EINVAL;
+  if (layers == 0) return 0;
+  if (!bias || !counts || !rows || !out) return MBX_EINVAL;
+  for (int l = 0; l < layers; ++l)
+    if (!bias[l] || !out[l] || rows[l] < 0 || (rows[l] > 0 && !counts[l])) return MBX_EINVAL;
+  hipStream_t s = as_stream(stream);
+  if (layers == 1) launch_balance<1>(bias, counts, rows, out, 1, num_experts, rate, s);
+  else
+    for (int first = 0; first < layers; first += kBalanceLayers)
+      launch_balance<kBalanceLayers>(bias + first, counts + first, rows + first, out + first, layers - first < kBalanceLayers ? layers - first : kBalanceLayers,
+                                     num_experts, rate, s);
+  return launch_status();
+}
+
+}  // extern "C"

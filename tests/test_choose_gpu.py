@@ -1,0 +1,265 @@
+"""The choice of experts by scores, bias and groups, its gradient and the update of the bias, against their restatement in float64.
+
+Tolerances.  fp32 arithmetic: exp and reciprocal as the hardware has them are off by 2^-23 each, the exponent x - m (16 bits out: times log2 e as well) by 2^-24
+of its size, sums of up to 512 positive terms by 2^-24 for each of some 16 steps: a score is off by at most (|x - m| + 24) 2^-23 of itself.  Rounding to the
+output's type is half a step of it, eps / 2."""
+import pytest
+import torch
+
+import megablocks_amd.ops as ops
+from oracle import choose as oracle
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _spread(x):
+    """How large the exponents of the scores are, per token."""
+    x = x.double().cpu()
+    return (x.abs().amax(1, keepdim=True) * 2).clamp(max=200.)
+
+
+def _close(got, want, bound, what):
+    got = got.double().cpu()
+    off = (got - want).abs()
+    assert bool((off <= bound).all()), (what, float((off / bound.clamp(min=1e-300)).max()))
+
+
+def _tiny(dtype):
+    return {BF16: 2.0 ** -126, F16: 2.0 ** -24, F32: 2.0 ** -126}[dtype]    # below the smallest normal number (fp16: its smallest step) nothing is promised
+
+
+def _check(logits, top_k, dtype, **how):
+    x = logits.to(dtype)
+    bias = how.get('bias')
+    got = ops.choose_experts(x.cuda(), top_k, want_lse=True, **{**how, 'bias': None if bias is None else bias.cuda()})
+    s, w, i, lse = oracle.choose(x, top_k, **how)
+    assert got[0].dtype == got[1].dtype == dtype and got[2].dtype == torch.int64 and got[3].dtype == torch.float32
+    assert torch.equal(got[2].cpu(), i), (got[2].cpu() != i).nonzero()[:5]
+    step, fp32 = torch.finfo(dtype).eps / 2, (_spread(x) + 24) * 2.0 ** -23
+    _close(got[0], s, s * (step + fp32) + _tiny(dtype), 'scores')
+    _close(got[1], w, w.abs() * (step + 4 * fp32) + _tiny(dtype), 'weights')
+    _close(got[3], lse, 24 * 2.0 ** -23 * (1 + lse.abs()), 'lse')
+    return x, got
+
+
+SHAPES = [   # tokens, experts, top_k, groups, top_groups, group_best
+    (1, 8, 2, 1, 1, 1), (7, 16, 1, 4, 2, 2), (33, 12, 2, 3, 2, 2), (17, 60, 4, 5, 3, 1), (64, 64, 6, 8, 3, 2), (50, 128, 8, 1, 1, 2), (129, 256, 8, 8, 4, 2),
+    (5, 250, 16, 10, 4, 2), (40, 160, 6, 8, 3, 1), (9, 512, 10, 16, 8, 2), (6, 500, 64, 20, 10, 2), (3, 96, 17, 2, 1, 2), (2, 1, 1, 1, 1, 1), (11, 4, 4, 2, 2, 1),
+    (19, 64, 64, 64, 64, 2), (13, 96, 8, 32, 9, 2), (21, 9, 2, 9, 4, 2), (8, 384, 8, 48, 5, 2), (25, 48, 4, 16, 3, 2)]
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('shape', SHAPES)
+def test_choice(shape, score, dtype):
+    tokens, experts, top_k, groups, top_groups, best = shape
+    g = torch.Generator().manual_seed(experts * 7 + tokens)
+    x = torch.randn(tokens, experts, generator=g) * 1.5
+    bias = torch.randint(-40, 41, (experts,), generator=g) * 0.001
+    print(f'choice {shape} {score} {dtype}', flush=True)
+    for b in (None, bias, torch.zeros(experts)):
+        for p, scale in ((0, 1.0), (1, 2.5)):
+            _check(x, top_k, dtype, score=score, bias=b, groups=groups, top_groups=top_groups, group_best=best, norm_p=p, scale=scale)
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('p', [2, 3, 0.5])
+def test_norms(score, p):
+    g = torch.Generator().manual_seed(5)
+    _check(torch.randn(31, 24, generator=g), 5, F32, score=score, norm_p=p, scale=0.5)
+
+
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('groups', [1, 8])
+def test_keys_that_32_bits_do_not_tell_apart(score, groups):
+    """Logits a step of fp32 apart around a value, and biases that nearly make up for the scores: the order is that of the exact keys."""
+    g = torch.Generator().manual_seed(11)
+    tokens, experts = 65, 64
+    x = 1.25 + torch.randint(-8, 9, (tokens, experts), generator=g) * 2.0 ** -22
+    bias = torch.randint(-2, 3, (experts,), generator=g) * 2.0 ** -25
+    _check(x, 6, F32, score=score, bias=bias, groups=groups, top_groups=max(1, groups // 2), norm_p=1)
+    _check(x, 6, F32, score=score, groups=groups, top_groups=max(1, groups // 2), norm_p=1)
+    big = torch.randn(tokens, experts, generator=g) * 2 + 24      # sigmoids within 2^-24 of one
+    _check(big, 6, F32, score=score, bias=bias * 0 + 0.125, groups=groups, top_groups=max(1, groups // 2))
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32])
+@pytest.mark.parametrize('with_bias', [False, True])
+def test_many_equal_logits(dtype, with_bias):
+    """Ties go to the lower index, also where the bias is the same for many."""
+    g = torch.Generator().manual_seed(12)
+    x = torch.randint(-2, 3, (70, 96), generator=g).float()
+    bias = torch.randint(0, 2, (96,), generator=g) * 0.25 if with_bias else None
+    for score in ('softmax', 'sigmoid'):
+        _check(x, 8, dtype, score=score, bias=bias, groups=6, top_groups=3, norm_p=1)
+
+
+def test_masked_infinite_and_undefined_logits():
+    inf, nan = float('inf'), float('nan')
+    x = torch.zeros(6, 16)
+    x[0, 3:] = -inf                 # fewer experts left than are chosen
+    x[1] = -inf                     # none left
+    x[2, 5] = nan
+    x[3, 7] = inf
+    x[4] = -200.                    # scores of zero in fp32
+    x[5] = torch.arange(16) * -1.
+    for bias in (None, torch.zeros(16)):
+        s, w, i, lse = ops.choose_experts(x.cuda(), 4, score='sigmoid', bias=None if bias is None else bias.cuda(), norm_p=1, want_lse=True)
+        i, w = i.cpu(), w.cpu()
+        assert i[0].tolist() == [0, 1, 2, 3] and w[0].tolist() == pytest.approx([1 / 3, 1 / 3, 1 / 3, 0])
+        assert i[1].tolist() == [0, 1, 2, 3] and w[1].tolist() == [0] * 4
+        assert i[2].tolist() == [5, 0, 1, 2] and w[2].isnan().all()
+        assert i[3].tolist() == [7, 0, 1, 2] and w[3].tolist() == pytest.approx([0.4, 0.2, 0.2, 0.2])
+        assert i[4].tolist() == [0, 1, 2, 3] and not w[4].isnan().any()
+        assert i[5].tolist() == [0, 1, 2, 3]
+        assert lse.cpu()[1] == -inf and lse.cpu()[3] == inf
+    # an expert that its bias shuts out, in a softmax and in groups; masked logits never bring in an expert of a closed group
+    bias = torch.zeros(16)
+    bias[0] = -inf
+    _, _, i, _ = ops.choose_experts(x.cuda(), 4, score='sigmoid', bias=bias.cuda())
+    assert i.cpu()[5].tolist() == [1, 2, 3, 4]
+    y = torch.full((2, 16), -inf)
+    y[:, 12] = 1.
+    for best in (1, 2):
+        _, _, i, _ = ops.choose_experts(y.cuda(), 4, score='sigmoid', groups=4, top_groups=1, group_best=best)
+        assert i.cpu().tolist() == [[12, 13, 14, 15]] * 2
+    i = ops.choose_experts(x[1:2].cuda(), 2, score='softmax', groups=4, top_groups=2)[2].cpu()   # softmax of nothing is undefined; the indices are experts
+    assert ((0 <= i) & (i < 16)).all()
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('shape', SHAPES)
+@pytest.mark.parametrize('p', [0, 1, 2])
+def test_gradient(shape, score, dtype, p):
+    tokens, experts, top_k, groups, top_groups, best = shape
+    g = torch.Generator().manual_seed(experts * 5 + tokens)
+    x = (torch.randn(tokens, experts, generator=g) * 1.5).to(dtype)
+    gs, gw, gl = torch.randn(tokens, experts, generator=g).to(dtype), torch.randn(tokens, top_k, generator=g).to(dtype), torch.randn(tokens, generator=g)
+    print(f'gradient {shape} {score} {dtype} {p}', flush=True)
+    leaf = x.cuda().requires_grad_()
+    bias = (torch.randint(-40, 41, (experts,), generator=g) * 0.001).cuda()
+    s, w, i, lse = ops.choose_experts(leaf, top_k, score=score, bias=bias, groups=groups, top_groups=top_groups, group_best=best, norm_p=p, scale=2.5,
+                                      want_lse=True)
+    # the gradient's terms go through exp, a division and up to 512 additions in fp32, each relative to the terms' sizes
+    for grads in ((gs, gw, gl), (None, gw, None), (gs, None, None), (None, None, gl)):
+        outs = [(o, d.cuda()) for o, d in zip((s, w, lse), grads) if d is not None]
+        got, = torch.autograd.grad([o for o, _ in outs], leaf, [d for _, d in outs], retain_graph=True)
+        want, size = oracle.gradient(x, i, score, p, 2.5, *grads)
+        assert got.dtype == dtype
+        _close(got, want, want.abs() * torch.finfo(dtype).eps / 2 + size * (_spread(x) + 40) * 2.0 ** -22 + _tiny(dtype), 'gradient')
+
+
+def test_gradient_of_scores_that_are_all_zero_and_of_masked_experts():
+    x = torch.full((2, 8), -300.)
+    x[1, 4:] = -float('inf')
+    leaf = x.cuda().requires_grad_()
+    w = ops.choose_experts(leaf, 6, score='sigmoid', norm_p=1)[1]
+    grad, = torch.autograd.grad(w.sum() + (w[:, 0] * 3).sum(), leaf)
+    assert (grad == 0).all()
+    y = torch.zeros(1, 8)
+    y[0, 4:] = -float('inf')
+    leaf = y.cuda().requires_grad_()
+    s, w, i, lse = ops.choose_experts(leaf, 2, score='softmax', norm_p=1, want_lse=True)
+    grad, = torch.autograd.grad((w * torch.tensor([[1., 2.]]).cuda()).sum() + lse.sum(), leaf)
+    want, _ = oracle.gradient(y, i, 'softmax', 1, 1.0, None, torch.tensor([[1., 2.]]), torch.ones(1))
+    assert torch.allclose(grad.cpu().double(), want, atol=1e-6)
+
+
+def test_gradients_are_given_once():
+    leaf = torch.randn(4, 8, device='cuda').requires_grad_()
+    s = ops.choose_experts(leaf, 2)[0]
+    grad, = torch.autograd.grad(s.square().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+
+
+def test_strides_types_and_no_tokens():
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(37, 80, generator=g)
+    view = wide.cuda()[:, 3:67]                      # rows that are no whole pieces
+    plain = wide[:, 3:67].contiguous()
+    for a, b in zip(ops.choose_experts(view, 4, score='sigmoid'), ops.choose_experts(plain.cuda(), 4, score='sigmoid')):
+        assert a is b is None or torch.equal(a, b)
+    flat = torch.zeros(37 * 64 + 1, device='cuda')
+    flat[1:] = plain.flatten().cuda()
+    off = flat[1:].view(37, 64)                      # a base that is no whole piece
+    assert torch.equal(ops.choose_experts(off, 4)[2], ops.choose_experts(plain.cuda(), 4)[2])
+    s, w, i, lse = ops.choose_experts(torch.zeros(0, 8, device='cuda'), 2, want_lse=True)
+    assert s.shape == (0, 8) and w.shape == i.shape == (0, 2) and lse.shape == (0,)
+    bias = torch.randn(64, 2, generator=g).cuda()[:, 0]
+    assert torch.equal(ops.choose_experts(plain.cuda(), 4, bias=bias)[2], ops.choose_experts(plain.cuda(), 4, bias=bias.contiguous())[2])
+    with pytest.raises(RuntimeError):
+        ops.choose_experts(torch.zeros(2, 8, device='cuda', dtype=torch.float64), 2)
+    with pytest.raises(RuntimeError):
+        ops.choose_experts(torch.zeros(2, 8, device='cuda'), 2, bias=torch.zeros(8, device='cuda').half())
+
+
+def test_rows_behind_the_last_token_are_left_as_they_were():
+    from megablocks_amd import _lib
+    tokens, experts, top_k = 21, 16, 2
+    x = torch.randn(tokens, experts, device='cuda')
+    full = [torch.full((tokens + 11, n), 7, dtype=d, device='cuda') for n, d in ((experts, F32), (top_k, F32), (top_k, torch.int64), (top_k, torch.int32), (1, F32))]
+    grad = torch.full((tokens + 11, experts), 7., device='cuda')
+    _lib.check(_lib.lib.mbx_choose_experts(x.data_ptr(), 2, tokens, experts, top_k, 1, None, 4, 2, 2, 1., 1., *(t.data_ptr() for t in full), _lib.stream()))
+    _lib.check(_lib.lib.mbx_choose_experts_backward(full[1].data_ptr(), None, None, x.data_ptr(), full[2].data_ptr(), 2, tokens, experts, top_k, 1, 1., 1.,
+                                                    grad.data_ptr(), _lib.stream()))
+    for t in (*full, grad):
+        assert (t[tokens:] == 7).all() and not (t[:tokens] == 7).all()
+
+
+def test_a_large_batch_and_a_captured_one():
+    g = torch.Generator().manual_seed(21)
+    x = torch.randn(70001, 16, generator=g).to(BF16)
+    bias = torch.randint(-40, 41, (16,), generator=g) * 0.001
+    got = ops.choose_experts(x.cuda(), 2, score='sigmoid', bias=bias.cuda(), groups=4, top_groups=2, norm_p=1)
+    some = torch.cat([torch.arange(0, 50), torch.arange(65500, 65600), torch.arange(69950, 70001)])
+    assert torch.equal(got[2].cpu()[some], oracle.choose(x[some], 2, 'sigmoid', bias, 4, 2, 2, 1)[2])
+    static, grad = x[:300].cuda().requires_grad_(), torch.randn(300, 2, generator=g).to(BF16).cuda()
+
+    def step(leaf):
+        s, w, i, _ = ops.choose_experts(leaf, 2, score='sigmoid', bias=device_bias, norm_p=1)
+        return s.detach(), w.detach(), i, torch.autograd.grad(w, leaf, grad)[0]
+    device_bias = bias.cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for first in (0, 1000, 40000):
+        new = x[first:first + 300].cuda()
+        with torch.no_grad():
+            static.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, step(new.requires_grad_())):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('layers,experts', [(1, 1), (1, 64), (2, 12), (32, 256), (65, 300), (130, 8)])
+def test_balance(layers, experts):
+    g = torch.Generator().manual_seed(layers)
+    biases = [torch.randn(experts, generator=g) * 0.01 for _ in range(layers)]
+    counts = [torch.randint(0, 4, (experts,) if l % 3 else (3, experts), generator=g).int() for l in range(layers)]
+    counts[0] = torch.full((experts,), 2 ** 31 - 1, dtype=torch.int32)     # sums pass 32 bits; all at the mean
+    got = ops.balance_bias([b.cuda() for b in biases], [n.cuda() for n in counts], 0.001)
+    again = [b.cuda() for b in biases]
+    assert ops.balance_bias(again, [n.cuda() for n in counts], 0.001, out=again) is again
+    for b, n, a, c in zip(biases, counts, got, again):
+        want = oracle.balance(b, n, 0.001)
+        assert (a.cpu().double() - want).abs().max() <= 2.0 ** -24 * (want.abs().max() + 0.001) and torch.equal(a, c)   # one rounding, and the rate's own
+    assert torch.equal(got[0].cpu(), biases[0])
+
+
+def test_balance_refuses_two_layers_with_one_output():
+    b, n = torch.zeros(8, device='cuda'), torch.zeros(8, dtype=torch.int32, device='cuda')
+    with pytest.raises(ValueError):
+        ops.balance_bias([b, b], [n, n], 0.001, out=[b, b])
+    with pytest.raises(ValueError):
+        ops.balance_bias([b], [n], 0.001, out=[torch.zeros(16, device='cuda')[::2]])
+    with pytest.raises(RuntimeError):
+        ops.balance_bias([b], [n.cpu()], 0.001)
