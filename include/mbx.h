@@ -494,6 +494,34 @@ int mbx_loss_sum(const void* values, int dtype, const int32_t* counts, int64_t n
 int mbx_loss_gradient(const float* grad, const void* values, int dtype, const int32_t* counts, int64_t n, int period, float scale, void* out,
                       mbx_stream_t stream);
 
+/* ---- experts with 4-bit weights ----
+ * Weights W of num_experts experts, n features of k columns each, in 4 bits with a scale (and, if wanted, a zero point) for every `group` (32, 64, 128)
+ * columns; no counterpart in the reference.  As they are kept, with T = ceil(n / 16) and B = ceil(k / 128):
+ *   words   uint32 [num_experts, T, B, 64, 4], 16-byte aligned: word j of lane 16 g + f holds feature 16 t + f, columns 128 b + 32 j + 8 g +
+ *           (0, 2, 4, 6, 1, 3, 5, 7), four bits each from the lowest
+ *   scales  [num_experts, T, B * 128 / group, 16] of scale_dtype: of feature 16 t + f and its p-th group
+ *   zeros   uint8 like scales, or NULL: 8 everywhere
+ * A code q stands for scale * (q - zero).  Features and columns past n and k are never used.
+ *
+ * mbx_quantize_4bit: from weights [num_experts, n, k] (layout MBX_NT, as w1 and v1 are kept) or [num_experts, k, n] (MBX_NN, as w2 is); scales in the weights'
+ * type.  Without zeros scale = round(max|w| / 7), q = clamp(rint(w / scale), -8, 7) + 8; with zeros, of low = min(w, 0) and high = max(w, 0),
+ * scale = round((high - low) / 15), zero = clamp(rint(-low / scale), 0, 15), q = clamp(rint(w / scale) + zero, 0, 15).  Quotients are taken exactly, halves
+ * go to even.  A group of zeros has scale 0, one with a number that is not finite scale NaN.
+ * mbx_dequantize_4bit: the values, rounded to `dtype`, in either layout. */
+int mbx_quantize_4bit(const void* weights, int dtype, int num_experts, int n, int k, int layout, int group, void* words, void* scales, uint8_t* zeros,
+                      mbx_stream_t stream);
+int mbx_dequantize_4bit(const void* words, const void* scales, const uint8_t* zeros, int scale_dtype, int num_experts, int n, int k, int layout, int group,
+                        void* out, int dtype, mbx_stream_t stream);
+
+/* c[r_e] = act(X[r_e] @ W[e]^T) (act -1: none; else an mbx_activation), with a second matrix (words2 not NULL) times X[r_e] @ W2[e]^T, rows [bins[e - 1],
+ * bins[e]) for expert e: the experts' products for few rows an expert, where reading the weights is what takes the time.  Rows of X: a's (indices NULL), or
+ * a[indices[r] / top_k] of a's a_rows rows.  16-bit activations, fp32 sums, rounded once.  The scales of both matrices are of type `dtype` or fp32; both
+ * have zeros or neither has.  Any number of rows is computed; with hundreds an expert mbx_dequantize_4bit and mbx_gmm are faster.  MBX_EUNSUPPORTED:
+ * fp32 activations, other scales, k = 0, more than 65535 pieces of 16 to 64 rows. */
+int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_k, const void* words, const void* scales, const uint8_t* zeros,
+                 const void* words2, const void* scales2, const uint8_t* zeros2, int scale_dtype, int group, void* c, int dtype, const int32_t* bins,
+                 int num_groups, int64_t rows, int k, int n, int act, mbx_stream_t stream);
+
 /* ---- choice of experts by scores, bias and groups ----
  * The router of layers whose experts are kept in balance by a bias and chosen in two steps; no counterpart in the reference, whose router is
  * mbx_router_forward (softmax, top-k).  For `tokens` rows x of num_experts logits, scores s = softmax(x) or 1 / (1 + exp(-x)):

@@ -82,6 +82,9 @@ _SIGNATURES = {
     'mbx_loss_gradients': (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp, _vp]),
     'mbx_router_input_gradient': (_i, [_vp, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp]),
     'mbx_sum_parts': (_i, [_vp, _i, _i64, _vp, _i, _i64, _vp]),
+    'mbx_quantize_4bit': (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    'mbx_dequantize_4bit': (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),
+    'mbx_gmm_4bit': (_i, [_vp, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i64, _i, _i, _i, _vp]),
     'mbx_choose_experts': (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp]),
     'mbx_choose_experts_backward': (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp]),
     'mbx_balance_bias': (_i, [_vp, _vp, _vp, _vp, _i, _i, ctypes.c_float, _vp]),

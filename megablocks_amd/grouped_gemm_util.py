@@ -13,6 +13,7 @@ import torch
 
 from megablocks_amd import _lib
 from megablocks_amd._lib import lib
+from megablocks_amd.weights_4bit import Weights4bit, quantize_4bit  # noqa: F401  (reached from here, as the products are)
 
 
 def grouped_gemm_is_available():
@@ -204,7 +205,7 @@ def gmm_dual(a, b, a2, b2, batch_sizes, trans_b=False, c=None):
     return c
 
 
-ACT_GELU_TANH = 1   # mbx_activation of include/mbx.h
+ACT_SILU, ACT_GELU_TANH = 0, 1   # mbx_activation of include/mbx.h
 # False: gmm_act / gmm_dact run the product and the element-wise pass as two launches (what they do anyway for shapes
 # the epilogue kernels do not take); a switch for measurements
 ACTIVATION_EPILOGUES = os.environ.get('MBX_ACTIVATION_EPILOGUES', '1') != '0'
@@ -829,6 +830,111 @@ def autocast_operands(*tensors):
 def _ops_gmm(a, b, batch_sizes, trans_b=False):
     a, b = autocast_operands(a, b)
     return GroupedGemm.apply(a, b, batch_sizes, trans_b)
+
+
+# Rows an expert, in the mean over those that can have some, above which 4-bit weights are turned into 16 bits for the products of those.
+FEW_ROWS_4BIT = 64
+
+
+def _operand_4bit(a, weights, batch_sizes, bins, what):
+    """(rows of a, their source or None, bins) of a product with 4-bit weights, checked."""
+    src = a if isinstance(a, GatheredRows) else None
+    x = a if src is None else src.x
+    first = weights[0]
+    if x.ndim != 2 or x.shape[1] != first.k:
+        raise ValueError(f'{what}: the rows must have the {first.k} columns of the weights')
+    if any((w.experts, w.n, w.k, w.group, w.scales.dtype, w.zeros is None) != (first.experts, first.n, first.k, first.group, first.scales.dtype, first.zeros is None)
+           for w in weights):
+        raise ValueError(f'{what}: both weights must have the same sizes, groups and types')
+    if (batch_sizes is None) == (bins is None and src is None):
+        raise ValueError(f'{what}: give the batch sizes or their inclusive sums' if src is None else f'{what}: gathered rows bring their bins')
+    _lib.require_cuda(x, bins, *(w.words for w in weights))
+    if any(w.device != x.device for w in weights):
+        raise RuntimeError(f'{what}: rows and weights must be on one device')
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f'{what}: expected bfloat16 or float16 rows but got {x.dtype}')
+    if first.scales.dtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f'{what}: the scales must be {x.dtype}, as the rows, or float32, not {first.scales.dtype}')
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError(f'{what}: products with 4-bit weights have no gradient; call them under torch.no_grad()')
+    if src is None:
+        rows = x.shape[0]
+        bins = _device_bins(batch_sizes, x.device, rows) if bins is None else bins
+    else:
+        if src.padded_bins is not None:
+            x, bins, src = src.materialize(), src.padded_bins, None
+            rows = x.shape[0]
+        else:
+            rows, bins = src.rows, src.bins
+            if src.indices.ndim != 1 or src.indices.dtype != torch.int32 or src.indices.shape[0] != x.shape[0] * src.top_k or rows != src.indices.shape[0]:
+                raise ValueError(f'{what}: one int32 assignment per token and top_k choice')
+    if bins.ndim != 1 or bins.shape[0] != first.experts or bins.dtype != torch.int32 or bins.device != x.device:
+        raise ValueError(f'{what}: the bins must be int32, one for each of the {first.experts} experts')
+    return x.contiguous(), src, bins.contiguous(), rows
+
+
+def _rows_4bit(x, src, bins, rows, b, b2, act, c, what):
+    """The product of few rows (`mbx_gmm_4bit`) into c; False where the library does not take it."""
+    indices = None if src is None else src.indices.contiguous()
+    with _lib.device_of(x), _lib.record(what, rows=rows, k=b.k, n=b.n * (1 if b2 is None else 2), elem=x.element_size(), groups=b.experts) as rec:
+        rc = lib.mbx_gmm_4bit(_lib.ptr(x), x.shape[0], _lib.ptr(indices), 1 if src is None else src.top_k, _lib.ptr(b.words), _lib.ptr(b.scales),
+                              _lib.ptr(b.zeros), None if b2 is None else _lib.ptr(b2.words), None if b2 is None else _lib.ptr(b2.scales),
+                              None if b2 is None else _lib.ptr(b2.zeros), _lib.DTYPE[b.scales.dtype], b.group, _lib.ptr(c), _lib.dtype_of(x),
+                              _lib.ptr(bins), b.experts, rows, b.k, b.n, -1 if act is None else act, _lib.stream())
+        if rc == _lib.EUNSUPPORTED:
+            rec.cancel()
+    if rc == _lib.EUNSUPPORTED:
+        return False
+    _lib.check(rc, what)
+    return True
+
+
+def _few_rows_4bit(rows, experts):
+    return rows <= FEW_ROWS_4BIT * min(rows, experts)
+
+
+def _gmm_nt_bins(a, b, bins):
+    """gmm(a, b, trans_b=True) by the bins themselves."""
+    c = torch.empty((a.shape[0], b.shape[1]), dtype=a.dtype, device=a.device)
+    with _lib.device_of(a), _lib.record('gmm_nt', rows=a.shape[0], k=a.shape[1], n=b.shape[1], elem=a.element_size(), groups=b.shape[0]):
+        _lib.check(lib.mbx_gmm(_lib.ptr(a), _lib.ptr(b), _lib.ptr(c), _lib.dtype_of(a), _lib.ptr(bins), b.shape[0], a.shape[0], a.shape[1], b.shape[1], _lib.NT,
+                               _lib.stream()), 'gmm')
+    return c
+
+
+def gmm_4bit(a, b: Weights4bit, batch_sizes=None, bins=None):
+    """out[r_e] = a[r_e] @ b[e]^T (as b's values are [experts, n, k]) with 4-bit weights b, without gradients: a [rows, k] in bf16 or fp16, or a GatheredRows;
+    batch_sizes as for `gmm`, or their inclusive int32 sums `bins` on the device (a GatheredRows brings its own).  fp32 sums, rounded once.  Few rows an
+    expert multiply the codes as they are (`mbx_gmm_4bit`); for many the values are made in a's type, 2 bytes a weight for the time of the call, and
+    go through `gmm`'s kernels."""
+    x, src, bins, rows = _operand_4bit(a, (b,), batch_sizes, bins, 'gmm_4bit')
+    if _few_rows_4bit(rows, b.experts):
+        c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
+        if _rows_4bit(x, src, bins, rows, b, None, None, c, 'gmm_4bit'):
+            return c
+    return _gmm_nt_bins(x if src is None else src.materialize(), b.dequantize(x.dtype, trans_b=True), bins)
+
+
+def gmm_4bit_act(a, b: Weights4bit, act, batch_sizes=None, bins=None, b2: Weights4bit = None):
+    """activation(a[r_e] @ b[e]^T), with b2 times a[r_e] @ b2[e]^T: the experts' first product(s) with 4-bit weights and their activation, operands as for
+    `gmm_4bit`.  act: ACT_SILU or ACT_GELU_TANH.  Few rows an expert: one launch, rounded once; many: as `gmm_act` / `gmm_glu` with the weights' values."""
+    if act not in (ACT_SILU, ACT_GELU_TANH):
+        raise ValueError('gmm_4bit_act: act must be ACT_SILU or ACT_GELU_TANH')
+    both = (b,) if b2 is None else (b, b2)
+    x, src, bins, rows = _operand_4bit(a, both, batch_sizes, bins, 'gmm_4bit_act')
+    if _few_rows_4bit(rows, b.experts):
+        c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
+        if _rows_4bit(x, src, bins, rows, b, b2, act, c, 'gmm_4bit_act' if b2 is None else 'gmm_4bit_glu'):
+            return c
+    values = [w.dequantize(x.dtype, trans_b=True) for w in both]
+    if ACTIVATION_EPILOGUES and (b2 is not None or act == ACT_GELU_TANH):
+        h = _hidden(x, src, values[0], None if b2 is None else values[1], bins, rows, act)
+        if h is not None:
+            return h
+    x = x if src is None else src.materialize()
+    products = [_gmm_nt_bins(x, v, bins).float() for v in values]
+    h = torch.nn.functional.silu(products[0]) if act == ACT_SILU else torch.nn.functional.gelu(products[0], approximate='tanh')
+    return (h if b2 is None else h * products[1]).to(x.dtype)
 
 
 backend = types.SimpleNamespace(gmm=gmm)
