@@ -522,6 +522,16 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
                  const void* words2, const void* scales2, const uint8_t* zeros2, int scale_dtype, int group, void* c, int dtype, const int32_t* bins,
                  int num_groups, int64_t rows, int k, int n, int act, mbx_stream_t stream);
 
+/* Everything behind the router of a dropless forward without gradients for few assignments, with 4-bit experts, by one call: mbx_route, mbx_gmm_4bit with the
+ * gather and the activation (v1_words NULL: no gate), mbx_gmm_4bit, mbx_scatter, with the same results.  w1, v1: ffn features of hidden columns, w2: hidden
+ * features of ffn columns, all with zeros or none.  scratch: mbx_experts_forward_scratch_bytes(tokens, top_k, num_experts, end_bit, hidden, ffn, dtype) bytes,
+ * 16-byte aligned.  MBX_EUNSUPPORTED: fp32, no assignment, what mbx_route or mbx_gmm_4bit does not take. */
+int mbx_experts_forward_4bit(const void* x, int64_t tokens, int hidden, int dtype, const int32_t* expert_ids, int top_k, const void* weights, int w_dtype,
+                             int num_experts, int end_bit, const void* w1_words, const void* w1_scales, const uint8_t* w1_zeros, const void* v1_words,
+                             const void* v1_scales, const uint8_t* v1_zeros, const void* w2_words, const void* w2_scales, const uint8_t* w2_zeros,
+                             int scale_dtype, int group, int ffn, int act, void* out, int32_t* tokens_per_expert, void* scratch, size_t scratch_bytes,
+                             mbx_stream_t stream);
+
 /* ---- choice of experts by scores, bias and groups ----
  * The router of layers whose experts are kept in balance by a bias and chosen in two steps; no counterpart in the reference, whose router is
  * mbx_router_forward (softmax, top-k).  For `tokens` rows x of num_experts logits, scores s = softmax(x) or 1 / (1 + exp(-x)):

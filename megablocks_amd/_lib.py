@@ -85,6 +85,7 @@ _SIGNATURES = {
     'mbx_quantize_4bit': (_i, [_vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp]),
     'mbx_dequantize_4bit': (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),
     'mbx_gmm_4bit': (_i, [_vp, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _i64, _i, _i, _i, _vp]),
+    'mbx_experts_forward_4bit': (_i, [_vp, _i64, _i, _i, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _sz, _vp]),
     'mbx_choose_experts': (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp]),
     'mbx_choose_experts_backward': (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp]),
     'mbx_balance_bias': (_i, [_vp, _vp, _vp, _vp, _i, _i, ctypes.c_float, _vp]),

@@ -133,6 +133,31 @@ int mbx_experts_forward(const void* x, int64_t tokens, int hidden_size, int dtyp
   return mbx_scatter(y, dtype, tokens, hidden_size, top_k, indices, bin_ids, bins, nullptr, num_experts, weights, w_dtype, out, slot_rows, nullptr, 0, stream);
 }
 
+int mbx_experts_forward_4bit(const void* x, int64_t tokens, int hidden_size, int dtype, const int32_t* expert_ids, int top_k, const void* weights, int w_dtype,
+                             int num_experts, int end_bit, const void* w1_words, const void* w1_scales, const uint8_t* w1_zeros, const void* v1_words,
+                             const void* v1_scales, const uint8_t* v1_zeros, const void* w2_words, const void* w2_scales, const uint8_t* w2_zeros,
+                             int scale_dtype, int group, int ffn, int act, void* out, int32_t* tokens_per_expert, void* scratch, size_t scratch_bytes,
+                             mbx_stream_t stream) {
+  if (!sizes_ok(tokens, top_k, num_experts, end_bit, hidden_size, ffn) || act < 0) return MBX_EINVAL;
+  if (dtype != MBX_BF16 && dtype != MBX_F16) return MBX_EUNSUPPORTED;
+  const int64_t slots = tokens * top_k;
+  if (slots == 0 || hidden_size == 0 || ffn == 0) return MBX_EUNSUPPORTED;
+  if (!x || !expert_ids || !w1_words || !w2_words || !out || !tokens_per_expert) return MBX_EINVAL;
+  const Parts parts(slots, num_experts, end_bit, hidden_size, ffn, dtype);
+  if (!scratch || scratch_bytes < parts.all.total || ((uintptr_t)scratch & 15)) return MBX_ESCRATCH;
+  char* const base = (char*)scratch;
+  int32_t *const indices = (int32_t*)(base + parts.indices), *const bin_ids = (int32_t*)(base + parts.bin_ids);
+  int32_t *const slot_rows = (int32_t*)(base + parts.slot_rows), *const bins = (int32_t*)(base + parts.bins);
+  void *const h = base + parts.hidden, *const y = base + parts.product;
+  int rc = mbx_route(expert_ids, slots, num_experts, end_bit, 0, indices, bin_ids, tokens_per_expert, bins, nullptr, slot_rows, base + parts.sort, parts.sort_bytes, stream);
+  if (!rc) rc = mbx_gmm_4bit(x, tokens, indices, top_k, w1_words, w1_scales, w1_zeros, v1_words, v1_scales, v1_zeros, scale_dtype, group, h, dtype, bins, num_experts,
+                             slots, hidden_size, ffn, act, stream);
+  if (!rc) rc = mbx_gmm_4bit(h, slots, nullptr, 1, w2_words, w2_scales, w2_zeros, nullptr, nullptr, nullptr, scale_dtype, group, y, dtype, bins, num_experts, slots, ffn,
+                             hidden_size, -1, stream);
+  if (rc) return rc;
+  return mbx_scatter(y, dtype, tokens, hidden_size, top_k, indices, bin_ids, bins, nullptr, num_experts, weights, w_dtype, out, slot_rows, nullptr, 0, stream);
+}
+
 // which: 0 what the forward keeps for the backward, 1 / 2 the scratch of the forward / the backward
 size_t mbx_experts_step_bytes(int64_t tokens, int top_k, int num_experts, int end_bit, int hidden_size, int ffn, int gate, int flags, int which) {
   if (!sizes_ok(tokens, top_k, num_experts, end_bit, hidden_size, ffn) || which < 0 || which > 2) return 0;

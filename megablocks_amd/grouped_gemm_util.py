@@ -937,5 +937,39 @@ def gmm_4bit_act(a, b: Weights4bit, act, batch_sizes=None, bins=None, b2: Weight
     return (h if b2 is None else h * products[1]).to(x.dtype)
 
 
+def experts_forward_4bit(x, expert_ids, expert_weights, num_experts, end_bit, top_k, w1: Weights4bit, v1, w2: Weights4bit, act):
+    """(out, tokens_per_expert) of the grouped dropless layer behind its router with 4-bit experts, from one call of the library
+    (`mbx_experts_forward_4bit`): `ops.route`, `gmm_4bit_act` on the gathered rows (v1 None: no gate), `gmm_4bit` and `ops.scatter`, with their results.  None: many
+    rows, or one of those does not take the operands."""
+    slots, dtype, device = expert_ids.numel(), x.dtype, x.device
+    if not 0 < slots <= EXPERTS_FORWARD_MAX_SLOTS or end_bit > 8 or dtype not in (torch.bfloat16, torch.float16) or not _few_rows_4bit(slots, num_experts) or \
+            _lib.profile_hook is not None or torch.is_grad_enabled():
+        return None
+    if any((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or t.device != device for t in (x, expert_ids, expert_weights)):
+        return None
+    for w in (w1, w2) if v1 is None else (w1, v1, w2):
+        if w.device != device or w.group != w1.group or w.scales.dtype != w1.scales.dtype or (w.zeros is None) != (w1.zeros is None) or w.experts != num_experts:
+            return None
+    if w1.scales.dtype not in (dtype, torch.float32) or x.shape[1] != w1.k or x.shape[0] * top_k != slots or expert_ids.dtype != torch.int32 or \
+            expert_weights.numel() != slots or expert_weights.dtype not in _lib.DTYPE or (w2.n, w2.k) != (w1.k, w1.n) or (v1 is not None and (v1.n, v1.k) != (w1.n, w1.k)):
+        return None
+    x, expert_ids, expert_weights = x.contiguous(), expert_ids.contiguous(), expert_weights.contiguous()
+    tokens, hidden = x.shape
+    code = _lib.DTYPE[dtype]
+    out = torch.empty_like(x)
+    tokens_per_expert = torch.empty(num_experts, dtype=torch.int32, device=device)
+    nbytes = lib.mbx_experts_forward_scratch_bytes(tokens, top_k, num_experts, end_bit, hidden, w1.n, code)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    operands = [_lib.ptr(t) for w in (w1, v1, w2) for t in ((None,) * 3 if w is None else (w.words, w.scales, w.zeros))]
+    with _lib.device_of(x):
+        rc = lib.mbx_experts_forward_4bit(x.data_ptr(), tokens, hidden, code, expert_ids.data_ptr(), top_k, expert_weights.data_ptr(),
+                                          _lib.DTYPE[expert_weights.dtype], num_experts, end_bit, *operands, _lib.DTYPE[w1.scales.dtype], w1.group, w1.n, act,
+                                          out.data_ptr(), tokens_per_expert.data_ptr(), scratch.data_ptr(), nbytes, _lib.stream())
+    if rc == _lib.EUNSUPPORTED:
+        return None
+    _lib.check(rc, 'experts_forward_4bit')
+    return out, tokens_per_expert
+
+
 backend = types.SimpleNamespace(gmm=gmm)
 ops = types.SimpleNamespace(gmm=_ops_gmm)

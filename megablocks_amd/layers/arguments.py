@@ -68,6 +68,17 @@ class Arguments:
     moe_zloss_weight: float = 0
     moe_zloss_in_fp32: bool = False
 
+    # Choice of experts (ops.choose_experts); the defaults are the reference's router.  Scores 'softmax' or 'sigmoid'; a bias for the choice alone, which
+    # layers.moe.update_balance_biases moves by moe_router_bias_rate towards equally many tokens an expert; experts in groups of which the best
+    # moe_router_top_groups are open, a group going by its moe_router_group_best best experts; the weights times moe_router_scale.
+    moe_router_score: str = 'softmax'
+    moe_router_bias: bool = False
+    moe_router_bias_rate: float = 0.001
+    moe_router_groups: int = 1
+    moe_router_top_groups: int = 1
+    moe_router_group_best: int = 2
+    moe_router_scale: float = 1.0
+
     def __post_init__(self):
         if self.moe_expert_model_parallelism:
             raise NotImplementedError('expert model parallelism is not part of this single-GPU build')

@@ -14,6 +14,7 @@ from megablocks_amd.layers import common, dmlp_registry, moe, mpu, router
 from megablocks_amd.layers.arguments import Arguments
 from megablocks_amd.layers.glu import GroupedGLU, _activation_code
 from megablocks_amd.layers.mlp import DEFAULT_ACTIVATION_FN, GroupedMLP, Topology
+from megablocks_amd.layers.mlp_4bit import Grouped4bitExperts
 
 
 _only_computed = common.only_computed
@@ -173,9 +174,27 @@ class ParallelDroplessMLP(moe.ParallelMLP):
             return None
         return act, experts.w1, v1, experts.w2
 
+    def quantize_experts_(self, group_size: int = 128, zero_points: bool = False):
+        """Puts the experts' weights into 4 bits, with a scale (and a zero point) for every group_size (32, 64, 128) columns of the reduction: `self.mlp` becomes a
+        Grouped4bitExperts, which has no gradients.  For grouped MLP and GLU experts.  Returns the layer."""
+        self.mlp = Grouped4bitExperts(self.mlp, group_size, zero_points)
+        self._takes_combine = None
+        return self
+
+    def _one_call_4bit(self, x, expert_weights, top_experts):
+        """grouped_forward_once from one call of the library (gg.experts_forward_4bit), as _one_call_forward."""
+        experts = self.mlp
+        if type(self) is not ParallelDroplessMLP or router._has_hooks(experts) or not _only_computed() or \
+                not self.__dict__.keys().isdisjoint(('indices_and_bins', 'grouped_permute_and_compute', 'permute_and_compute')):
+            return None
+        return gg.experts_forward_4bit(x.view(-1, x.shape[-1]), top_experts.int(), expert_weights, self.num_experts, self.sort_end_bit,
+                                       self.args.moe_top_k, experts.w1, experts.v1, experts.w2, experts.act)
+
     def _one_call_forward(self, x, expert_weights, top_experts):
         """grouped_forward_once from one call of the library (gg.experts_forward), where the layer and its experts are the
         built-in ones, nothing is traced or transformed and no gradient is recorded; else None."""
+        if type(self.mlp) is Grouped4bitExperts:
+            return self._one_call_4bit(x, expert_weights, top_experts)
         known = self._one_call_experts()
         if known is None or not _only_computed():
             return None
@@ -247,3 +266,8 @@ class dMoE(moe.MoE):
 
     def _init_experts_mlp(self, args: Arguments):
         return ParallelDroplessMLP(args)
+
+    def quantize_experts_(self, group_size: int = 128, zero_points: bool = False):
+        """The experts' weights in 4 bits, for serving (ParallelDroplessMLP.quantize_experts_).  Returns the layer."""
+        self.experts.quantize_experts_(group_size, zero_points)
+        return self

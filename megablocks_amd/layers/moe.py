@@ -26,6 +26,34 @@ def clear_load_balancing_loss():
     _LOAD_BALANCING_LOSS.clear()
 
 
+_EXPERT_LOADS = []
+
+
+def save_expert_load(bias, tokens_per_expert):
+    _EXPERT_LOADS.append((bias, tokens_per_expert))
+
+
+def get_expert_loads():
+    """(balance bias, tokens per expert) of every forward in training since the last update."""
+    return _EXPERT_LOADS
+
+
+def clear_expert_loads():
+    _EXPERT_LOADS.clear()
+
+
+def update_balance_biases(args: Arguments):
+    """Moves the balance biases of all layers that ran in training since the last call by moe_router_bias_rate: up for experts that got fewer tokens than the
+    mean, down for those that got more (ops.balance_bias; one launch for 64 layers).  Called once a step, after the backward; the forwards of a step
+    that accumulates gradients are added up."""
+    by_bias = {}
+    for bias, tokens_per_expert in get_expert_loads():
+        by_bias.setdefault(id(bias), (bias, []))[1].append(tokens_per_expert)
+    biases = [bias for bias, _ in by_bias.values()]
+    ops.balance_bias(biases, [loads[0] if len(loads) == 1 else torch.stack(loads) for _, loads in by_bias.values()], args.moe_router_bias_rate, out=biases)
+    clear_expert_loads()
+
+
 def batched_load_balancing_loss(args: Arguments):
     """moe.py:32-89: loss_weight * E / (layers * tokens * top_k) * <tokens_per_expert, mean scores>."""
     if args.moe_loss_weight == 0:
@@ -135,6 +163,7 @@ class ParallelMLP(torch.nn.Module):
         """moe.py:425-437."""
         in_shape = x.size()
         x, tokens_per_expert = self.forward_fn(x, expert_weights, top_experts)
+        self.tokens_per_expert = tokens_per_expert if self.args.moe_router_bias and self.training and torch.is_grad_enabled() else None
         if self.training and self.args.moe_loss_weight > 0:
             save_load_balancing_loss((tokens_per_expert, scores))
         x = x.view(in_shape)
@@ -168,4 +197,9 @@ class MoE(torch.nn.Module):
             scores, expert_weights, top_experts, x = module.forward_and_tokens(x)
         else:
             scores, expert_weights, top_experts = module(x)
-        return self.experts(x, scores, expert_weights, router.int32_indices(top_experts))
+        out = self.experts(x, scores, expert_weights, router.int32_indices(top_experts))
+        bias, load = getattr(module, 'balance_bias', None), getattr(self.experts, 'tokens_per_expert', None)
+        if bias is not None and load is not None:
+            save_expert_load(bias, load)
+            self.experts.tokens_per_expert = None
+        return out

@@ -10,6 +10,7 @@ import torch
 from megablocks_amd import _lib
 from megablocks_amd.layers import common
 from megablocks_amd.layers.arguments import Arguments
+from megablocks_amd.ops import choose
 
 _ROUTER_LOGITS = []
 
@@ -416,6 +417,29 @@ class LearnedRouter(torch.nn.Module):
         self.layer = torch.nn.Linear(args.hidden_size, args.moe_num_experts, bias=False, dtype=common.dtype(args),
                                      device=args.device)
         args.init_method(self.layer.weight)
+        # Scores, a bias or groups other than the reference's softmax and top-k (router.py:87-106): ops.choose_experts
+        self._chooses = (args.moe_router_score, args.moe_router_bias, args.moe_router_scale) != ('softmax', False, 1.0) or \
+            args.moe_router_top_groups != args.moe_router_groups
+        if self._chooses:
+            choose.check_choice(args.moe_num_experts, args.moe_top_k, args.moe_router_score, args.moe_router_groups, args.moe_router_top_groups,
+                                args.moe_router_group_best, args.moe_normalize_expert_weights or 0, args.moe_router_scale)
+        self.register_buffer('balance_bias', torch.zeros(args.moe_num_experts, dtype=torch.float32, device=args.device) if args.moe_router_bias else None)
+
+    def _apply(self, fn, *args, **kwargs):
+        """The balance bias goes along to other devices, not to other types: its steps are finer than 16 bits."""
+        bias = self.balance_bias
+        super()._apply(fn, *args, **kwargs)
+        if bias is not None and self.balance_bias.dtype != torch.float32:
+            self.balance_bias = bias.to(self.balance_bias.device)
+        return self
+
+    def _choose(self, logits: torch.Tensor):
+        args = self.args
+        if not logits.is_cuda:
+            raise RuntimeError('expected logits on the GPU: scores, biases and groups other than the softmax and top-k have no other implementation')
+        return choose.ChooseExpertsOp.apply(logits, self.balance_bias, args.moe_top_k, args.moe_router_score, args.moe_router_groups,
+                                            args.moe_router_top_groups, args.moe_router_group_best, float(args.moe_normalize_expert_weights or 0),
+                                            float(args.moe_router_scale), args.moe_zloss_weight != 0)
 
     def jitter(self, x: torch.Tensor):
         low = 1.0 - self.args.moe_jitter_eps
@@ -468,7 +492,7 @@ class LearnedRouter(torch.nn.Module):
             x = x * self.jitter(x)
         x2d = x.view(-1, x.shape[-1])
         args = self.args
-        if FUSED_SOFTMAX_TOPK and args.moe_zloss_weight == 0 and not args.uniform_expert_assignment:
+        if FUSED_SOFTMAX_TOPK and args.moe_zloss_weight == 0 and not args.uniform_expert_assignment and not self._chooses:
             for node in (_LinearSoftmaxTopK, _RecordedLinearSoftmaxTopK):   # without gradients, with
                 if node.supported(x2d, self.layer, args.moe_top_k):
                     return node.apply(x2d, self.layer.weight, args.moe_top_k, args.moe_normalize_expert_weights or 0)
@@ -481,7 +505,9 @@ class LearnedRouter(torch.nn.Module):
             # autocast runs softmax in fp32 (router.py:98 under torch.autocast): scores and weights come out in fp32
             logits = logits.float()
         expert_indices32 = None
-        if FUSED_SOFTMAX_TOPK and _SoftmaxTopK.supported(logits, self.args.moe_top_k):
+        if self._chooses:
+            scores, expert_weights, expert_indices, expert_indices32, lse = self._choose(logits)
+        elif FUSED_SOFTMAX_TOPK and _SoftmaxTopK.supported(logits, self.args.moe_top_k):
             scores, expert_weights, expert_indices, expert_indices32, lse = _SoftmaxTopK.apply(
                 logits, self.args.moe_top_k, self.args.moe_normalize_expert_weights or 0,
                 self.args.moe_zloss_weight != 0)

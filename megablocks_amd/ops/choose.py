@@ -137,6 +137,8 @@ def balance_bias(biases, tokens_per_expert, rate: float, out=None):
         raise ValueError('balance_bias: outputs must be contiguous')
     elif len({t.data_ptr() for t in out}) < layers:
         raise ValueError('balance_bias: two layers have the same output; pass the rows of their tokens per expert as one')
+    else:
+        torch.autograd.graph.increment_version(out)
     biases = [t.detach().contiguous() for t in biases]
     counts = [n.contiguous() for n in tokens_per_expert]
     pointers = lambda tensors: (ctypes.c_void_p * layers)(*map(_lib.ptr, tensors))

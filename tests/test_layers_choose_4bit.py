@@ -1,0 +1,60 @@
+"""The layers with a choice of experts by scores, bias and groups and with 4-bit experts, as far as they go without a GPU."""
+import pytest
+import torch
+
+from megablocks_amd.layers import moe as moe_layers
+from megablocks_amd.layers.arguments import Arguments
+from megablocks_amd.layers.dmoe import ParallelDroplessMLP
+from megablocks_amd.layers.router import LearnedRouter
+
+
+def _args(**changed):
+    return Arguments(**(dict(hidden_size=16, ffn_hidden_size=32, moe_num_experts=8, moe_top_k=2, device=torch.device('cpu'), fp16=False, bf16=True) | changed))
+
+
+def test_the_defaults_are_the_router_that_was_there():
+    router = LearnedRouter(_args())
+    assert not router._chooses and router.balance_bias is None and list(router.state_dict()) == ['layer.weight']
+    assert not LearnedRouter(_args(moe_router_groups=4, moe_router_top_groups=4))._chooses      # all groups open
+    for changed in (dict(moe_router_score='sigmoid'), dict(moe_router_bias=True), dict(moe_router_groups=4, moe_router_top_groups=2), dict(moe_router_scale=2.)):
+        assert LearnedRouter(_args(**changed))._chooses
+
+
+@pytest.mark.parametrize('changed', [
+    dict(moe_router_score='tanh'), dict(moe_router_groups=3), dict(moe_router_groups=4, moe_router_top_groups=5), dict(moe_router_bias=True, moe_router_group_best=0),
+    dict(moe_router_score='sigmoid', moe_top_k=9), dict(moe_router_scale=float('nan')), dict(moe_router_groups=8, moe_router_top_groups=1)])
+def test_routers_that_cannot_choose_are_refused(changed):
+    with pytest.raises(ValueError):
+        LearnedRouter(_args(**changed))
+
+
+def test_the_balance_bias_keeps_its_type():
+    router = LearnedRouter(_args(moe_router_bias=True))
+    assert sorted(router.state_dict()) == ['balance_bias', 'layer.weight'] and not router.balance_bias.requires_grad
+    router.balance_bias += 0.0011
+    router.half()
+    assert router.layer.weight.dtype == torch.float16 and router.balance_bias.dtype == torch.float32 and float(router.balance_bias[0]) == pytest.approx(0.0011)
+    with pytest.raises(RuntimeError):
+        router(torch.zeros(3, 1, 16).half())       # the choice has one implementation, on the GPU
+
+
+def test_updates_go_by_the_bias(monkeypatch):
+    calls = []
+    monkeypatch.setattr(moe_layers.ops, 'balance_bias', lambda biases, loads, rate, out: calls.append((biases, loads, rate, out)))
+    a, b = torch.zeros(4), torch.zeros(4)
+    for bias, load in ((a, [1, 2, 3, 4]), (b, [4, 3, 2, 1]), (a, [0, 0, 0, 8])):
+        moe_layers.save_expert_load(bias, torch.tensor(load, dtype=torch.int32))
+    assert len(moe_layers.get_expert_loads()) == 3
+    moe_layers.update_balance_biases(_args(moe_router_bias_rate=0.5))
+    (biases, loads, rate, out), = calls
+    assert biases[0] is a and biases[1] is b and out is biases and rate == 0.5
+    assert loads[0].tolist() == [[1, 2, 3, 4], [0, 0, 0, 8]] and loads[1].tolist() == [4, 3, 2, 1]
+    assert moe_layers.get_expert_loads() == []
+
+
+@pytest.mark.parametrize('changed', [dict(mlp_impl='sparse'), dict(activation_fn=torch.nn.functional.relu), dict(mlp_type='glu', activation_fn=torch.nn.functional.relu)])
+def test_experts_that_have_no_4_bit_form_are_refused(changed):
+    with pytest.raises(ValueError):
+        ParallelDroplessMLP(_args(**changed)).quantize_experts_()
+    with pytest.raises(RuntimeError):
+        ParallelDroplessMLP(_args()).quantize_experts_()       # on the CPU
