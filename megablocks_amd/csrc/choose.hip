@@ -176,22 +176,31 @@ __device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&k
   return LANES == 64 ? all : (all >> (lane_id() & ~(LANES - 1))) & 0xffffu;
 }
 
-template <int R>
-__device__ __forceinline__ void keep_open(uint32_t (&key)[R], uint64_t open, int base, int size) {
+// Keys of experts of closed groups, and of lanes' places past the last expert, as 0.
+template <int R, typename U>
+__device__ __forceinline__ void keep_open(U (&key)[R], uint64_t open, int base, int size) {
+  if (size % R == 0) {   // a lane is in one group
+    const bool in = (open >> (base / size)) & 1;
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = in ? key[r] : 0;
+    return;
+  }
   int g = base / size, in = base - g * size;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if (!((open >> g) & 1)) key[r] = 0;
-    if (++in == size) { in = 0; ++g; }
+    key[r] = (open >> g) & 1 ? key[r] : 0;
+    const bool next = ++in == size;
+    in = next ? 0 : in;
+    g += next ? 1 : 0;
   }
 }
-template <int R>
-__device__ __forceinline__ void keep_open(uint64_t (&key)[R], uint64_t open, int base, int size) {
-  int g = base / size, in = base - g * size;
+template <int R, typename U, typename F>
+__device__ __forceinline__ void order_keys(U (&key)[R], const F (&v)[R], int base, int experts) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (!((open >> g) & 1)) key[r] = 0;
-    if (++in == size) { in = 0; ++g; }
+  for (int r = 0; r < R; ++r) key[r] = ordered(v[r]);
+  if (base + R > experts) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) key[r] = base + r < experts ? key[r] : 0;
   }
 }
 
@@ -239,7 +248,10 @@ __device__ __forceinline__ void read_row(const typename Elem<DT>::type* __restri
     for (int r = 0; r < R; ++r) x[r] = base < experts ? Elem<DT>::to_f32(piece.v[r]) : past;
   } else {
 #pragma unroll
-    for (int r = 0; r < R; ++r) x[r] = base + r < experts ? Elem<DT>::to_f32(row[base + r]) : past;
+    for (int r = 0; r < R; ++r) {
+      const float v = Elem<DT>::to_f32(row[base + r < experts ? base + r : experts - 1]);   // one load after the other, no branches
+      x[r] = base + r < experts ? v : past;
+    }
   }
 }
 template <int DT, int R>
@@ -258,106 +270,132 @@ __device__ __forceinline__ void write_row(typename Elem<DT>::type* __restrict__ 
   }
 }
 
-// A token's choice again, with keys in 64 bits
-template <int LANES, int R>
-__device__ __forceinline__ void pick_wide(const float (&x)[R], const float (&bias)[R], const Choose& c, int lane, int& mine) {
-  const int base = lane * R;
-  double s[R], sum = 0, top = -INFINITY;
+// The largest logit of a token and the sum of exp(x - m), which the caller's e gets
+template <int DT, int LANES, int R>
+__device__ __forceinline__ void softmax_parts(const float (&x)[R], float& m, float& sum, float (&e)[R]) {
+  m = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < R; ++r) top = larger(top, base + r < c.experts ? (double)x[r] : (double)-INFINITY);
-  top = token_max<LANES>(top);
+  for (int r = 0; r < R; ++r) m = fmaxf(m, x[r]);
+  m = token_max<LANES>(m);
+  sum = 0.f;
+  // past the last expert x is -inf and adds nothing; of a token whose logits are all -inf the sum is not a number, as it should be
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const double v = x[r];
-    s[r] = base + r >= c.experts ? 0. : c.sigmoid ? 1. / (1. + exp(-v)) : exp(v - top);
-    sum += s[r];
+    e[r] = exp_of<DT>(x[r] - m);
+    sum += e[r];
   }
-  if (!c.sigmoid) {
-    sum = token_sum<LANES>(sum);
+  sum = token_sum<LANES>(sum);
+}
+
+template <int DT> __device__ __forceinline__ float sigmoid_of(float x) { return over<DT>(1.f, 1.f + exp_of<DT>(-x)); }
+
+// A token's choice again by the whole wave, with keys in 64 bits: lane j gets the j-th
+template <int DT, int R>
+__device__ __forceinline__ int pick_wide(const typename Elem<DT>::type* __restrict__ row, const Choose& c) {
+  const int lane = lane_id(), base = lane * R;
+  double x[R], s[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) x[r] = base + r < c.experts ? (double)Elem<DT>::to_f32(row[base + r]) : (double)-INFINITY;
+  if (c.sigmoid) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = 1. / (1. + exp(-x[r]));
+  } else {
+    double sum = 0, top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; ++r) top = larger(top, x[r]);
+    top = token_max<64>(top);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      s[r] = exp(x[r] - top);
+      sum += s[r];
+    }
+    sum = token_sum<64>(sum);
 #pragma unroll
     for (int r = 0; r < R; ++r) s[r] /= sum;
   }
-  uint64_t key[R];
+  if (c.bias) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) key[r] = base + r < c.experts ? ordered(c.bias ? s[r] + (double)bias[r] : s[r]) : 0;
+    for (int r = 0; r < R; ++r) s[r] += base + r < c.experts ? (double)c.bias[base + r] : 0.;
+  }
+  uint64_t key[R];
+  order_keys(key, s, base, c.experts);
   if (c.top_groups < c.groups) {
     bool close;
-    const uint64_t open = open_groups<LANES, R, double>(key, c, lane, close);
-#pragma unroll
-    for (int r = 0; r < R; ++r) key[r] = c.bias ? key[r] : base + r < c.experts ? ordered((double)x[r]) : 0;
+    const uint64_t open = open_groups<64, R, double>(key, c, lane, close);
+    if (!c.bias) order_keys(key, x, base, c.experts);
     keep_open(key, open, base, c.experts / c.groups);
   }
-  int next;
-  pick<LANES, R>(key, lane, c.top_k, c.top_k, mine, next);
+  int mine = 0, next;
+  pick<64, R>(key, lane, c.top_k, c.top_k, mine, next);
+  return mine;
 }
 
 template <int DT, int LANES, int R>
 __device__ __forceinline__ void choose_token(const float (&x)[R], const float (&bias)[R], const typename Elem<DT>::type* __restrict__ row, int64_t t, bool real,
                                              const Choose& c, bool whole) {
   typedef typename Elem<DT>::type E;
-  const int lane = lane_id() % LANES, base = lane * R;
+  const int lane = lane_id() % LANES, base = lane * R, size = c.experts / c.groups;
+  const bool grouped = c.top_groups < c.groups;
+  // the uniform conditions stay outside of the loops over a lane's experts: inside they become a branch for each
   float m = 0.f, sum = 1.f, s[R];
   if (!c.sigmoid || c.lse) {
-    m = -INFINITY;
-#pragma unroll
-    for (int r = 0; r < R; ++r) m = fmaxf(m, x[r]);
-    m = token_max<LANES>(m);
-    sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      s[r] = base + r < c.experts ? exp_of<DT>(x[r] - m) : 0.f;
-      sum += s[r];
-    }
-    sum = token_sum<LANES>(sum);
+    softmax_parts<DT, LANES, R>(x, m, sum, s);
     if (c.lse && lane == 0 && real) c.lse[t] = m == INFINITY || m == -INFINITY ? m : m + logf(sum);
   }
+  if (c.sigmoid) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) s[r] = c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-x[r])) : over<DT>(s[r], sum);
+    for (int r = 0; r < R; ++r) s[r] = sigmoid_of<DT>(x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] = over<DT>(s[r], sum);
+  }
   if (c.scores && real) write_row<DT, R>((E*)c.scores + t * c.experts, base, c.experts, whole, s);
 
   uint32_t key[R];
   bool close = false;
-  const bool grouped = c.top_groups < c.groups;
-  uint64_t open = ~0ull;
-  if (grouped) {
-    // without a bias the best of a group by its logit, exactly
-    const bool by_logit = !c.bias && c.group_best == 1;
-#pragma unroll
-    for (int r = 0; r < R; ++r) key[r] = base + r < c.experts ? ordered(by_logit ? x[r] : c.bias ? s[r] + bias[r] : s[r]) : 0;
-    open = open_groups<LANES, R, float>(key, c, lane, close);
-    close = close && !by_logit;
-  }
-#pragma unroll
-  for (int r = 0; r < R; ++r) key[r] = base + r < c.experts ? ordered(c.bias ? s[r] + bias[r] : x[r]) : 0;
-  const int size = c.experts / c.groups;
-  if (grouped) keep_open(key, open, base, size);
   int mine = 0, next = -1;
   const int more = c.bias && c.top_k < c.top_groups * size ? 1 : 0;
+  if (c.bias) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r] += bias[r];
+  }
+  // without a bias a group goes by its scores where two are added up, else by its best logit, exactly as the choice does
+  const bool by_score = c.bias || (grouped && c.group_best == 2);
+  if (by_score) order_keys(key, s, base, c.experts);
+  else order_keys(key, x, base, c.experts);
+  if (grouped) {
+    const uint64_t open = open_groups<LANES, R, float>(key, c, lane, close);
+    close = close && by_score;
+    if (by_score && !c.bias) order_keys(key, x, base, c.experts);
+    keep_open(key, open, base, size);
+  }
   pick<LANES, R>(key, lane, c.top_k, c.top_k + more, mine, next);
 
   const bool live = lane < c.top_k;
-  const auto key_of = [&](int e, float& logit, float& by) {
-    logit = Elem<DT>::to_f32(row[e]);
-    by = c.bias[e];
-    return (c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-logit)) : over<DT>(exp_of<DT>(logit - m), sum)) + by;
-  };
+  const auto score_of = [&](float logit) { return c.sigmoid ? sigmoid_of<DT>(logit) : over<DT>(exp_of<DT>(logit - m), sum); };
   if (c.bias) {
     // each chosen key against the next in the order, of the next lane or behind the last
-    int after = __shfl_down(mine, 1, LANES);
-    if (lane == c.top_k - 1) after = next;
-    if (live && after >= 0 && (lane < c.top_k - 1 || more)) {
-      float x0, b0, x1, b1;
-      const float k0 = key_of(mine, x0, b0), k1 = key_of(after, x1, b1);
-      close = close || (!(k0 - k1 > kCloseKeys * (1.f + fabsf(k0))) && !(x0 == x1 && b0 == b1));
+    const int last = live ? mine : 0;
+    const float x0 = Elem<DT>::to_f32(row[last]), b0 = c.bias[last], k0 = score_of(x0) + b0;
+    float x1 = __shfl_down(x0, 1, LANES), b1 = __shfl_down(b0, 1, LANES), k1 = __shfl_down(k0, 1, LANES);
+    if (lane == c.top_k - 1 && more) {
+      x1 = Elem<DT>::to_f32(row[next]);
+      b1 = c.bias[next];
+      k1 = score_of(x1) + b1;
     }
+    if (lane < c.top_k - 1 + more) close = close || (!(k0 - k1 > kCloseKeys * (1.f + fabsf(k0))) && !(x0 == x1 && b0 == b1));
   }
-  if (__any(close)) pick_wide<LANES, R>(x, bias, c, lane, mine);
+  for (uint64_t left = __ballot(close); left != 0;) {
+    const int first = __builtin_ctzll(left) & ~(LANES - 1);      // a token's lanes
+    left &= LANES == 64 ? 0 : ~(0xffffull << first);
+    const uint64_t at = (uint64_t)row;
+    const uint64_t of = (uint64_t)(uint32_t)lane_value((int)(uint32_t)(at >> 32), first) << 32 | (uint32_t)lane_value((int)(uint32_t)at, first);
+    const int wide = pick_wide<DT, (R * LANES + 63) / 64>((const E*)of, c);
+    const int moved = __shfl(wide, lane);
+    mine = (lane_id() & ~(LANES - 1)) == first ? moved : mine;
+  }
 
-  float w = 0.f;
-  if (live) {
-    const float logit = Elem<DT>::to_f32(row[mine]);
-    w = c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-logit)) : over<DT>(exp_of<DT>(logit - m), sum);
-  }
+  float w = live ? score_of(Elem<DT>::to_f32(row[mine])) : 0.f;
   if (c.norm_p > 0.f) {
     const float norm = token_pnorm<LANES>(w, c.norm_p);
     w = norm == 0.f ? 0.f : w / norm;   // scores that are all zero: weights of zero
@@ -414,19 +452,8 @@ choose_backward_kernel(const Choose c, const void* __restrict__ grad_weights, co
       for (int r = 0; r < R; ++r) ds[r] = 0.f;
     }
     float m = 0.f, sum = 1.f;
-    const bool softmax = !c.sigmoid || grad_lse;
-    if (softmax) {
-      m = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < R; ++r) m = fmaxf(m, x[r]);
-      m = token_max<LANES>(m);
-      sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        soft[r] = base + r < c.experts ? exp_of<DT>(x[r] - m) : 0.f;
-        sum += soft[r];
-      }
-      sum = token_sum<LANES>(sum);
+    if (!c.sigmoid || grad_lse) {
+      softmax_parts<DT, LANES, R>(x, m, sum, soft);
 #pragma unroll
       for (int r = 0; r < R; ++r) soft[r] = over<DT>(soft[r], sum);
     }
@@ -437,7 +464,7 @@ choose_backward_kernel(const Choose c, const void* __restrict__ grad_weights, co
       float w = 0.f, dy = 0.f;
       if (live) {
         const float logit = Elem<DT>::to_f32(row[mine]);
-        w = c.sigmoid ? over<DT>(1.f, 1.f + exp_of<DT>(-logit)) : over<DT>(exp_of<DT>(logit - m), sum);
+        w = c.sigmoid ? sigmoid_of<DT>(logit) : over<DT>(exp_of<DT>(logit - m), sum);
         dy = Elem<DT>::to_f32(((const E*)grad_weights)[t * c.top_k + lane]) * c.scale;
       }
       float dw = dy;

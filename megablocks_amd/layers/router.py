@@ -435,11 +435,9 @@ class LearnedRouter(torch.nn.Module):
 
     def _choose(self, logits: torch.Tensor):
         args = self.args
-        if not logits.is_cuda:
-            raise RuntimeError('expected logits on the GPU: scores, biases and groups other than the softmax and top-k have no other implementation')
-        return choose.ChooseExpertsOp.apply(logits, self.balance_bias, args.moe_top_k, args.moe_router_score, args.moe_router_groups,
-                                            args.moe_router_top_groups, args.moe_router_group_best, float(args.moe_normalize_expert_weights or 0),
-                                            float(args.moe_router_scale), args.moe_zloss_weight != 0)
+        return choose.choose(logits, self.balance_bias, args.moe_top_k, args.moe_router_score, args.moe_router_groups, args.moe_router_top_groups,
+                             args.moe_router_group_best, float(args.moe_normalize_expert_weights or 0), float(args.moe_router_scale), True,
+                             args.moe_zloss_weight != 0)
 
     def jitter(self, x: torch.Tensor):
         low = 1.0 - self.args.moe_jitter_eps

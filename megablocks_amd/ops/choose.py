@@ -5,7 +5,6 @@ import math
 from typing import Any, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from megablocks_amd import _lib
 from megablocks_amd._lib import lib
@@ -30,50 +29,85 @@ def check_choice(num_experts: int, top_k: int, score: str, groups: int, top_grou
         raise ValueError(f'choose_experts: up to {MAX_EXPERTS} experts, {MAX_TOP_K} a token and {MAX_GROUPS} groups')
 
 
+def _launch(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse):
+    """(scores, weights, indices, indices as int32 or None, lse or None) by `mbx_choose_experts`; logits and bias contiguous."""
+    tokens, experts = logits.shape
+    device, dtype = logits.device, logits.dtype
+    scores = torch.empty_like(logits)
+    weights = torch.empty((tokens, top_k), dtype=dtype, device=device)
+    indices = torch.empty((tokens, top_k), dtype=torch.int64, device=device)
+    indices32 = torch.empty((tokens, top_k), dtype=torch.int32, device=device) if want_int32 else None
+    lse = torch.empty((tokens,), dtype=torch.float32, device=device) if want_lse else None
+    with _lib.device_of(logits):
+        rc = lib.mbx_choose_experts(logits.data_ptr(), _lib.DTYPE[dtype], tokens, experts, top_k, SCORES[score], _lib.ptr(bias), groups, top_groups, group_best,
+                                    norm_p, scale, scores.data_ptr(), weights.data_ptr(), indices.data_ptr(), _lib.ptr(indices32), _lib.ptr(lse), _lib.stream())
+    _lib.check(rc, 'choose_experts')
+    return scores, weights, indices, indices32, lse
+
+
 class ChooseExpertsOp(torch.autograd.Function):
-    """(scores, weights, indices, indices as int32, lse or None) of `mbx_choose_experts`."""
+    """`_launch` with the logits' gradient."""
 
     @staticmethod
-    def forward(ctx: Any, logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_lse):
-        logits = logits.contiguous()
-        bias = None if bias is None else bias.detach().contiguous()
-        tokens, experts = logits.shape
-        scores = torch.empty_like(logits)
-        weights = torch.empty((tokens, top_k), dtype=logits.dtype, device=logits.device)
-        indices = torch.empty((tokens, top_k), dtype=torch.int64, device=logits.device)
-        indices32 = torch.empty((tokens, top_k), dtype=torch.int32, device=logits.device)
-        lse = torch.empty((tokens,), dtype=torch.float32, device=logits.device) if want_lse else None
-        with _lib.device_of(logits):
-            _lib.check(lib.mbx_choose_experts(_lib.ptr(logits), _lib.dtype_of(logits), tokens, experts, top_k, SCORES[score], _lib.ptr(bias), groups,
-                                              top_groups, group_best, norm_p, scale, _lib.ptr(scores), _lib.ptr(weights), _lib.ptr(indices),
-                                              _lib.ptr(indices32), _lib.ptr(lse), _lib.stream()), 'choose_experts')
+    def forward(ctx: Any, logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse):
+        scores, weights, indices, indices32, lse = _launch(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse)
         ctx.save_for_backward(logits, indices)
         ctx.choice = top_k, score, norm_p, scale
-        ctx.mark_non_differentiable(indices, indices32)
+        if want_int32:
+            ctx.mark_non_differentiable(indices, indices32)
+        else:
+            ctx.mark_non_differentiable(indices)
         ctx.set_materialize_grads(False)
         return scores, weights, indices, indices32, lse
 
     @staticmethod
-    @once_differentiable
     def backward(ctx: Any, grad_scores, grad_weights, _grad_indices, _grad_indices32, grad_lse):
         if grad_scores is None and grad_weights is None and grad_lse is None:
-            return (None,) * 10
+            return (None,) * 11
         logits, indices = ctx.saved_tensors
-        return (logits_gradient(logits, indices, *ctx.choice, grad_scores, grad_weights, grad_lse), *(None,) * 9)
+        # a backward that is differentiated itself (create_graph), or runs over a batch of gradients at once (is_grads_batched)
+        plain = torch.is_grad_enabled() or not all(_has_memory(g) for g in (grad_scores, grad_weights, grad_lse) if g is not None)
+        grad = _differentiable_gradient if plain else logits_gradient
+        return (grad(logits, indices, *ctx.choice, grad_scores, grad_weights, grad_lse),) + (None,) * 10
+
+
+def _has_memory(t):
+    try:
+        t.data_ptr()
+    except RuntimeError:
+        return False
+    return True
 
 
 def logits_gradient(logits, indices, top_k, score, norm_p, scale, grad_scores, grad_weights, grad_lse=None):
     """The gradient of the logits behind ChooseExpertsOp's outputs (`mbx_choose_experts_backward`); the outputs' may be None."""
     tokens, experts = logits.shape
     grad_logits = torch.empty_like(logits)
-    gs = None if grad_scores is None else grad_scores.to(logits.dtype).contiguous()
-    gw = None if grad_weights is None else grad_weights.to(logits.dtype).contiguous()
-    gl = None if grad_lse is None else grad_lse.float().contiguous()
+    plain = lambda g, dtype: None if g is None else (g if g.dtype == dtype else g.to(dtype)).contiguous()
+    gs, gw, gl = plain(grad_scores, logits.dtype), plain(grad_weights, logits.dtype), plain(grad_lse, torch.float32)
     with _lib.device_of(logits):
-        _lib.check(lib.mbx_choose_experts_backward(_lib.ptr(gw), _lib.ptr(gs), _lib.ptr(gl), _lib.ptr(logits), _lib.ptr(indices), _lib.dtype_of(logits),
-                                                   tokens, experts, top_k, SCORES[score], norm_p, scale, _lib.ptr(grad_logits), _lib.stream()),
-                   'choose_experts_backward')
+        rc = lib.mbx_choose_experts_backward(_lib.ptr(gw), _lib.ptr(gs), _lib.ptr(gl), logits.data_ptr(), indices.data_ptr(), _lib.DTYPE[logits.dtype], tokens,
+                                             experts, top_k, SCORES[score], norm_p, scale, grad_logits.data_ptr(), _lib.stream())
+    _lib.check(rc, 'choose_experts_backward')
     return grad_logits
+
+
+def _differentiable_gradient(logits, indices, top_k, score, norm_p, scale, grad_scores, grad_weights, grad_lse=None):
+    """logits_gradient in torch's operations, which have gradients themselves."""
+    x = logits.float()
+    soft = torch.softmax(x, 1) if score == 'softmax' or grad_lse is not None else None
+    s = soft if score == 'softmax' else torch.sigmoid(x)
+    ds = torch.zeros_like(x) if grad_scores is None else grad_scores.float()
+    if grad_weights is not None:
+        dw = grad_weights.float() * scale
+        if norm_p > 0:
+            w = s.gather(1, indices)
+            n = w.pow(norm_p).sum(1, keepdim=True).pow(1 / norm_p)
+            u = w / n
+            dw = (dw - (dw * u).sum(1, keepdim=True) * u.pow(norm_p - 1)) / n
+        ds = ds.scatter_add(1, indices, dw)
+    dx = s * (ds - (ds * s).sum(1, keepdim=True)) if score == 'softmax' else ds * s * torch.sigmoid(-x)
+    return (dx if grad_lse is None else dx + grad_lse.float().unsqueeze(1) * soft).to(logits.dtype)
 
 
 def choose_experts(logits: torch.Tensor, top_k: int, score: str = 'softmax', bias: Optional[torch.Tensor] = None, groups: int = 1, top_groups: int = 1,
@@ -92,15 +126,26 @@ def choose_experts(logits: torch.Tensor, top_k: int, score: str = 'softmax', bia
     norm_p, scale = float(norm_p or 0), float(scale)
     if logits.ndim != 2:
         raise ValueError('choose_experts: logits must be [tokens, experts]')
-    if bias is not None and (bias.ndim != 1 or bias.shape[0] != logits.shape[1]):
+    if bias is not None and bias.shape != logits.shape[1:]:
         raise ValueError('choose_experts: the bias must be a vector of a number for every expert')
     check_choice(logits.shape[1], top_k, score, groups, top_groups, group_best, norm_p, scale)
-    _lib.require_cuda(logits, bias)
-    _lib.dtype_of(logits)
-    if bias is not None and (bias.dtype != torch.float32 or bias.device != logits.device):
-        raise RuntimeError(f'choose_experts: expected a float32 bias on {logits.device} but got {bias.dtype} on {bias.device}')
-    scores, weights, indices, _, lse = ChooseExpertsOp.apply(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_lse)
+    scores, weights, indices, _, lse = choose(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, False, want_lse)
     return scores, weights, indices, lse
+
+
+def choose(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse):
+    """choose_experts of a choice that has been checked, with the indices as int32 too where want_int32: (scores, weights, indices, indices32, lse)."""
+    if not logits.is_cuda or (bias is not None and not bias.is_cuda):
+        raise RuntimeError('choose_experts: expected logits (and bias) on the GPU')
+    if logits.dtype not in _lib.DTYPE:
+        raise RuntimeError(f'choose_experts: expected bfloat16, float16 or float32 logits but got {logits.dtype}')
+    if bias is not None:
+        if bias.dtype != torch.float32 or bias.device != logits.device:
+            raise RuntimeError(f'choose_experts: expected a float32 bias on {logits.device} but got {bias.dtype} on {bias.device}')
+        bias = bias.detach().contiguous()
+    logits = logits.contiguous()
+    run = ChooseExpertsOp.apply if logits.requires_grad and torch.is_grad_enabled() else _launch    # a node of its own is 7 us of the host's time
+    return run(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse)
 
 
 def balance_bias(biases, tokens_per_expert, rate: float, out=None):
@@ -115,34 +160,47 @@ def balance_bias(biases, tokens_per_expert, rate: float, out=None):
         raise ValueError('balance_bias: the rate must be finite')
     if layers == 0:
         return []
-    experts, device = biases[0].shape[0] if biases[0].ndim == 1 else 0, biases[0].device
-    if experts == 0:
+    first = biases[0]
+    shape, index = first.shape, first.get_device()
+    if len(shape) != 1 or shape[0] == 0:
         raise ValueError('balance_bias: a bias must be a vector of a number for every expert')
-    for t in (*biases, *(() if out is None else out)):
-        if t.shape != (experts,):
+    experts = shape[0]
+    rows, b_ptrs, n_ptrs, kept, wrong = [1] * layers, [0] * layers, [0] * layers, [], None     # kept: copies the launch reads
+    for l in range(layers):
+        b, n = biases[l], tokens_per_expert[l]
+        if b.shape != shape:
             raise ValueError('balance_bias: all biases must be vectors of the same number of experts')
-        if t.dtype != torch.float32:
-            raise RuntimeError(f'balance_bias: expected float32 biases but got {t.dtype}')
-    for n in tokens_per_expert:
-        if n.ndim not in (1, 2) or n.shape[-1] != experts:
-            raise ValueError('balance_bias: tokens per expert must be [experts] or [rows, experts]')
-        if n.dtype != torch.int32:
-            raise RuntimeError(f'balance_bias: expected int32 tokens per expert but got {n.dtype}')
-    _lib.require_cuda(*biases, *tokens_per_expert, *(() if out is None else out))
-    if any(t.device != device for t in (*biases, *tokens_per_expert, *(() if out is None else out))):
-        raise RuntimeError('balance_bias: all tensors must be on one device')
+        if n.shape != shape:
+            if n.ndim != 2 or n.shape[1] != experts:
+                raise ValueError('balance_bias: tokens per expert must be [experts] or [rows, experts]')
+            rows[l] = n.shape[0]
+        if b.dtype != torch.float32 or n.dtype != torch.int32 or b.get_device() != index or n.get_device() != index or index < 0:
+            wrong = f'expected float32 biases and int32 tokens per expert on one GPU but got {b.dtype}, {n.dtype} on {b.device}, {n.device}'
+        if not b.is_contiguous():
+            kept.append(b.detach().contiguous())
+            b = kept[-1]
+        if not n.is_contiguous():
+            kept.append(n.contiguous())
+            n = kept[-1]
+        b_ptrs[l], n_ptrs[l] = b.data_ptr(), n.data_ptr()
+    for t in () if out is None else out:
+        if t.shape != shape or not t.is_contiguous():
+            raise ValueError('balance_bias: outputs must be contiguous vectors of a number for every expert')
+        if t.dtype != torch.float32 or t.get_device() != index:
+            wrong = f'expected float32 outputs on the device of the biases but got {t.dtype} on {t.device}'
+    if wrong is not None:
+        raise RuntimeError(f'balance_bias: {wrong}')
     if out is None:
-        out = list(torch.empty((layers, experts), dtype=torch.float32, device=device).unbind(0))
-    elif any(not t.is_contiguous() for t in out):
-        raise ValueError('balance_bias: outputs must be contiguous')
-    elif len({t.data_ptr() for t in out}) < layers:
-        raise ValueError('balance_bias: two layers have the same output; pass the rows of their tokens per expert as one')
+        made = torch.empty((layers, experts), dtype=torch.float32, device=first.device)
+        start = made.data_ptr()
+        out, o_ptrs = list(made.unbind(0)), range(start, start + 4 * layers * experts, 4 * experts)
     else:
+        o_ptrs = [t.data_ptr() for t in out]
+        if len(set(o_ptrs)) < layers:
+            raise ValueError('balance_bias: two layers have the same output; pass the rows of their tokens per expert as one')
         torch.autograd.graph.increment_version(out)
-    biases = [t.detach().contiguous() for t in biases]
-    counts = [n.contiguous() for n in tokens_per_expert]
-    pointers = lambda tensors: (ctypes.c_void_p * layers)(*map(_lib.ptr, tensors))
-    rows = (ctypes.c_int * layers)(*(1 if n.ndim == 1 else n.shape[0] for n in counts))
-    with _lib.device_of(biases[0]):
-        _lib.check(lib.mbx_balance_bias(pointers(biases), pointers(counts), rows, pointers(out), layers, experts, float(rate), _lib.stream()), 'balance_bias')
+    pointers = ctypes.c_void_p * layers
+    with _lib.device_of(first):
+        rc = lib.mbx_balance_bias(pointers(*b_ptrs), pointers(*n_ptrs), (ctypes.c_int * layers)(*rows), pointers(*o_ptrs), layers, experts, float(rate), _lib.stream())
+    _lib.check(rc, 'balance_bias')
     return out

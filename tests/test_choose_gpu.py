@@ -167,12 +167,28 @@ def test_gradient_of_scores_that_are_all_zero_and_of_masked_experts():
     assert torch.allclose(grad.cpu().double(), want, atol=1e-6)
 
 
-def test_gradients_are_given_once():
-    leaf = torch.randn(4, 8, device='cuda').requires_grad_()
-    s = ops.choose_experts(leaf, 2)[0]
-    grad, = torch.autograd.grad(s.square().sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError):
-        grad.sum().backward()
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('p', [0, 1, 2])
+def test_gradient_of_the_gradient(score, p):
+    """A backward that is differentiated itself: against autograd's of the formula in float64.  fp32 sums of 12 terms, twice."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(5, 12, generator=g)
+    gs, gw, gl, v = torch.randn(5, 12, generator=g), torch.randn(5, 3, generator=g), torch.randn(5, generator=g), torch.randn(5, 12, generator=g)
+    leaf = x.cuda().requires_grad_()
+    s, w, i, lse = ops.choose_experts(leaf, 3, score=score, norm_p=p, scale=1.5, want_lse=True)
+    plain, = torch.autograd.grad([s, w, lse], leaf, [gs.cuda(), gw.cuda(), gl.cuda()], retain_graph=True)
+    first, = torch.autograd.grad([s, w, lse], leaf, [gs.cuda(), gw.cuda(), gl.cuda()], create_graph=True)
+    second, = torch.autograd.grad(first, leaf, v.cuda())
+    wide = x.double().requires_grad_()
+    t = torch.softmax(wide, 1) if score == 'softmax' else torch.sigmoid(wide)
+    u = t.gather(1, i.cpu())
+    u = 1.5 * (u / u.norm(p=p, dim=1, keepdim=True) if p else u)
+    want, = torch.autograd.grad([t, u, torch.logsumexp(wide, 1)], wide, [gs.double(), gw.double(), gl.double()], create_graph=True)
+    want_second, = torch.autograd.grad(want, wide, v.double())
+    assert torch.allclose(plain, first, rtol=1e-5, atol=1e-5) and torch.allclose(first.cpu().double(), want, rtol=1e-5, atol=1e-5)
+    assert torch.allclose(second.cpu().double(), want_second, rtol=1e-4, atol=1e-4)
+    both, = torch.autograd.grad([s, w, lse], leaf, [torch.stack([t, 2 * t]).cuda() for t in (gs, gw, gl)], is_grads_batched=True)
+    assert torch.allclose(both[0], plain, rtol=1e-5, atol=1e-5) and torch.allclose(both[1], 2 * plain, rtol=1e-5, atol=1e-5)
 
 
 def test_strides_types_and_no_tokens():
