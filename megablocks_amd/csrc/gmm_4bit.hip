@@ -1,28 +1,16 @@
 // Weights in 4 bits with a scale (and a zero point) for every group of 32, 64 or 128 along the reduction: from 16- or 32-bit weights and back,
-// and the experts' products with them.
+// and the choice of the products' kernels (gmm_4bit_rows.hip, gmm_4bit_tile.hip).
 //
 // W [E, n, k] is kept in tiles of 16 features x 128 columns, in the order a wave multiplies them: 1 KiB in a row, 16 bytes a lane.  Lane
 // 16 g + f has feature f; its word j has the columns 32 j + 8 g + (0, 2, 4, 6, 1, 3, 5, 7) of the tile, four bits each from the lowest, so that word
 // j of all lanes is the operand of one v_mfma_f32_16x16x32 and a shift and a mask of a word give two neighbours in the halves of a register.
 // scales [E, n / 16, k / group, 16] (zeros alike, a byte each): a code q stands for scale (q - zero), zero 8 without zeros.  n and k are rounded up to
 // whole tiles; what lies past them is never used.
-#include "common.h"
+#include "gmm_4bit.h"
+
 
 namespace mbx {
 namespace {
-
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-
-constexpr int kTileFeatures = 16, kTileColumns = 128, kTileWords = 256;
-
-__device__ __host__ __forceinline__ int64_t tiles_of(int64_t n, int of) { return (n + of - 1) / of; }
-
-struct Packed {
-  const uint32_t* words;
-  const void* scales;
-  const uint8_t* zeros;
-};
 
 // ---- into 4 bits and back ----
 
@@ -248,227 +236,6 @@ dequantize_kernel(const Packed from, int scale_dtype, int64_t places, int n, int
   }
 }
 
-// ---- products of few rows ----
-//
-// A wave has WT tiles of features (with a second matrix WT / 2 of each) and MT sixteens of rows, the waves of a workgroup a share of the columns each, a
-// tile of 128 in turn; the shares are added up in the LDS, in order.  A word's codes become 16 + q in the activations' type by a shift, a mask and an or
-// for two of them (bf16: the mantissa's upper four bits are its bits 3 - 6, fp16: 6 - 9); the products with a column of ones are the sums of the rows' group,
-//   sum x scale (q - zero) = scale (sum x (16 + q) - (16 + zero) sum x)
-// in fp32, where 16 + q costs four bits of 24 of which 16-bit activations have eleven.
-constexpr int kRowsWaves = 4;
-
-template <int DT>
-__device__ __forceinline__ f32x4_t mfma_16x16x32(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
-  typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-  typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-  if constexpr (DT == MBX_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-}
-
-// eight codes as 16 + q
-template <int DT>
-__device__ __forceinline__ u32x4_t sixteen_and(uint32_t word) {
-  if constexpr (DT == MBX_BF16)
-    return u32x4_t{(word << 3 & 0x00780078u) | 0x41804180u, (word >> 1 & 0x00780078u) | 0x41804180u, (word >> 5 & 0x00780078u) | 0x41804180u,
-                   (word >> 9 & 0x00780078u) | 0x41804180u};
-  else
-    return u32x4_t{(word << 6 & 0x03c003c0u) | 0x4c004c00u, (word << 2 & 0x03c003c0u) | 0x4c004c00u, (word >> 2 & 0x03c003c0u) | 0x4c004c00u,
-                   (word >> 6 & 0x03c003c0u) | 0x4c004c00u};
-}
-
-__device__ __forceinline__ float activated(float x, int act) {
-  // x sigmoid(y): y = x (SiLU), or 2 sqrt(2 / pi) (x + 0.044715 x^3) (tanh-GELU)
-  const float y = act == MBX_ACT_SILU ? x : 1.5957691216057308f * (x + 0.044715f * x * x * x);
-  return x / (1.f + __expf(-y));
-}
-
-struct Rows4bit {
-  const void* a;
-  const int32_t* indices;   // NULL: row r of a is row r
-  int64_t a_rows;
-  int top_k;
-  Packed b[2];
-  int wide_scales;          // fp32 instead of the activations' type
-  void* c;
-  const int32_t* bins;
-  int num_groups;
-  int64_t rows;
-  int k, n, act;            // act < 0: none
-};
-
-// Tile `slot` of up to `height` rows: its expert, first and end row, false past the last.  bins need not be trusted: bounds stay in [0, rows].
-__device__ __forceinline__ bool find_rows(const Rows4bit& g, int slot, int height, int& expert, int64_t& first, int64_t& end) {
-  const int lane = lane_id(), per = (g.num_groups + kWave - 1) / kWave;
-  const auto bound = [&](int e) {   // rows before expert e
-    const int64_t b = e <= 0 ? 0 : g.bins[e - 1];
-    return b < 0 ? (int64_t)0 : b > g.rows ? g.rows : b;
-  };
-  const auto tiles = [&](int e) {
-    const int64_t count = bound(e + 1) - bound(e);
-    return count > 0 ? (int)((count + height - 1) / height) : 0;
-  };
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int e = lane * per + i;
-    if (e < g.num_groups) mine += tiles(e);
-  }
-  const int upto = wave_inclusive_scan(mine);
-  const uint64_t past = __ballot(upto > slot);
-  if (past == 0) return false;
-  const int at = __builtin_ctzll(past);
-  int left = slot - lane_value(upto - mine, at);
-  expert = at * per;
-  for (;;) {
-    const int count = __builtin_amdgcn_readfirstlane(tiles(expert));
-    if (left < count || expert + 1 >= g.num_groups) break;
-    left -= count;
-    ++expert;
-  }
-  const int64_t begin = bound(expert), last = bound(expert + 1);
-  first = begin + (int64_t)left * height;
-  end = first + height < last ? first + height : last;
-  return first < end;
-}
-
-template <int DT, int MT, int WT, bool TWO, int GROUP>
-__global__ void __launch_bounds__(kRowsWaves * kWave)
-rows_4bit_kernel(const Rows4bit g) {
-  typedef typename Elem<DT>::type E;
-  constexpr int kGroups = 128 / GROUP, kEach = GROUP / 32;
-  constexpr int kAhead = MT == 1 ? 4 : MT == 2 ? 2 : 1;    // tiles of columns whose loads are issued together
-  constexpr int kFeatureTiles = TWO ? WT / 2 : WT;
-  __shared__ float sums[kRowsWaves][WT * MT * 4][kWave];
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), f = lane % 16, part = lane / 16;
-  int expert;
-  int64_t first, end;
-  if (!find_rows(g, (int)blockIdx.y, 16 * MT, expert, first, end)) return;
-  const int tiles = (g.n + 15) / 16, blocks = (g.k + 127) / 128, tile0 = (int)blockIdx.x * kFeatureTiles;
-  // rows past the last are the last again: their results are not stored
-  const uint16_t* row[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    int64_t r = first + 16 * m + f;
-    r = r < end ? r : end - 1;
-    if (g.indices) {
-      r = g.indices[r] / g.top_k;
-      r = r < 0 ? 0 : r < g.a_rows ? r : g.a_rows - 1;
-    }
-    row[m] = (const uint16_t*)g.a + r * g.k;
-  }
-  f32x4_t y[WT][MT];
-#pragma unroll
-  for (int t = 0; t < WT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) y[t][m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const uint32_t one = DT == MBX_BF16 ? 0x3f803f80u : 0x3c003c00u;
-  const u32x4_t ones = {one, one, one, one};
-  int64_t at[WT];      // the tile's first block
-  Packed of[WT];
-#pragma unroll
-  for (int t = 0; t < WT; ++t) {
-    int tile = tile0 + (TWO ? t / 2 : t);
-    tile = tile < tiles ? tile : tiles - 1;
-    at[t] = ((int64_t)expert * tiles + tile) * blocks;
-    of[t] = g.b[TWO ? t % 2 : 0];
-  }
-  for (int block = wave; block < blocks; block += kRowsWaves * kAhead) {
-    u32x4_t words[kAhead][WT], x[kAhead][MT][4];
-    uint32_t scale[kAhead][WT][kGroups], zero[kAhead][WT][kGroups];   // as they are in memory: nothing waits for a load in this loop
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int b = block + u * kRowsWaves;
-      if (b >= blocks) continue;
-#pragma unroll
-      for (int t = 0; t < WT; ++t) words[u][t] = *(const u32x4_t*)(of[t].words + (at[t] + b) * kTileWords + lane * 4);
-      const auto each_scale = [&](auto&& set) {
-#pragma unroll
-        for (int t = 0; t < WT; ++t)
-#pragma unroll
-          for (int q = 0; q < kGroups; ++q) set(t, q, ((at[t] + b) * kGroups + q) * 16 + f);
-      };
-      if (g.wide_scales) each_scale([&](int t, int q, int64_t i) { scale[u][t][q] = ((const uint32_t*)of[t].scales)[i]; });
-      else each_scale([&](int t, int q, int64_t i) { scale[u][t][q] = ((const uint16_t*)of[t].scales)[i]; });
-      if (of[0].zeros) each_scale([&](int t, int q, int64_t i) { zero[u][t][q] = of[t].zeros[i]; });
-      else each_scale([&](int t, int q, int64_t) { zero[u][t][q] = 8; });
-      const int c0 = b * kTileColumns + 8 * part;
-      if ((b + 1) * kTileColumns <= g.k) {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) __builtin_memcpy(&x[u][m][j], row[m] + c0 + 32 * j, 16);
-      } else {
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = c0 + 32 * j;
-            if (c + 8 <= g.k) __builtin_memcpy(&x[u][m][j], row[m] + c, 16);
-            else
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                x[u][m][j][i] = (c + 2 * i < g.k ? (uint32_t)row[m][c + 2 * i] : 0u) | (c + 2 * i + 1 < g.k ? (uint32_t)row[m][c + 2 * i + 1] << 16 : 0u);
-          }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (block + u * kRowsWaves >= blocks) continue;
-#pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        f32x4_t of_ones[MT];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          of_ones[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = q * kEach; j < (q + 1) * kEach; ++j) of_ones[m] = mfma_16x16x32<DT>(x[u][m][j], ones, of_ones[m]);
-        }
-#pragma unroll
-        for (int t = 0; t < WT; ++t) {
-          f32x4_t acc[MT];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) acc[m] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = q * kEach; j < (q + 1) * kEach; ++j) {
-            const u32x4_t w = sixteen_and<DT>(words[u][t][j]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m] = mfma_16x16x32<DT>(x[u][m][j], w, acc[m]);
-          }
-          const float s = g.wide_scales ? __uint_as_float(scale[u][t][q]) : Elem<DT>::to_f32(__builtin_bit_cast(E, (uint16_t)scale[u][t][q]));
-          const float off = -16.f - (float)zero[u][t][q];
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(s, fmaf(off, of_ones[m][i], acc[m][i]), y[t][m][i]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < WT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[wave][(t * MT + m) * 4 + i][lane] = y[t][m][i];
-  __syncthreads();
-  // lane l, place i of a tile: row 4 (l / 16) + i, feature l % 16
-  for (int v = wave; v < kFeatureTiles * MT * 4; v += kRowsWaves) {
-    const int t = v / (MT * 4), rest = v % (MT * 4), m = rest / 4, i = rest % 4;
-    const auto sum = [&](int tile) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kRowsWaves; ++w) s += sums[w][tile * MT * 4 + rest][lane];
-      return s;
-    };
-    const int64_t r = first + 16 * m + 4 * part + i;
-    const int feature = (tile0 + t) * 16 + f;
-    if (r >= end || feature >= g.n) continue;
-    float c = sum(TWO ? 2 * t : t);
-    if (g.act >= 0) c = activated(c, g.act);
-    if constexpr (TWO) c *= sum(2 * t + 1);
-    ((E*)g.c)[r * g.n + feature] = Elem<DT>::from_f32(c);
-  }
-}
-
 static bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 
 static bool is_dtype(int d) { return d == MBX_BF16 || d == MBX_F16 || d == MBX_F32; }
@@ -478,8 +245,8 @@ struct PackGrid {
   int64_t places;
   unsigned grid;
   PackGrid(int64_t experts, int64_t n, int64_t k) {
-    feature_groups = (int)tiles_of(n, kPackFeatures);
-    blocks = (int)tiles_of(k, kTileColumns);
+    feature_groups = (int)pieces_of(n, kPackFeatures);
+    blocks = (int)pieces_of(k, kTileColumns);
     places = experts * feature_groups * blocks;
     grid = (unsigned)(places < 256 * 64 ? places : 256 * 64);
   }
@@ -542,37 +309,20 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   if (indices && (top_k <= 0 || a_rows < 0)) return MBX_EINVAL;
   if (words2 && (act < 0 || !zeros != !zeros2)) return MBX_EINVAL;
   if (dtype == MBX_F32 || (scale_dtype != dtype && scale_dtype != MBX_F32) || k == 0) return MBX_EUNSUPPORTED;
-  if (rows > 0x7fffffff || n > 0x7fffffff - 64 || k > 0x7fffffff - 128) return MBX_ERANGE;
+  if (rows > 0x7fffffff || n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (rows == 0 || n == 0 || num_groups == 0) return 0;
   if (!a || !words || !scales || !c || !bins || (words2 && !scales2) || (indices && a_rows == 0)) return MBX_EINVAL;
   if (((uintptr_t)words | (uintptr_t)words2) & 15) return MBX_EINVAL;
   hipStream_t s = as_stream(stream);
   const Rows4bit g = {a, indices, a_rows, top_k, {{(const uint32_t*)words, scales, zeros}, {(const uint32_t*)words2, scales2, zeros2}}, scale_dtype == MBX_F32,
                       c, bins, num_groups, rows, k, n, act};
-  const int64_t experts = rows < num_groups ? rows : num_groups, mean = ceil_div(rows, experts);
-  const int mt = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
-  const int64_t slots = experts + rows / (16 * mt);
+  // up to 12 rows an expert in the mean of those that can have some the one kernel, then the other (us, one / other: 8 gated experts of [4096, 14336], 8 rows
+  // 93 / 115, 16 rows 143 / 119; 64 of [2048, 1408], 3 rows 40 / 46, 15 rows 62 / 48)
+  const int64_t experts = rows < num_groups ? rows : num_groups;
+  const bool few = rows <= 12 * experts;
+  const int64_t slots = experts + rows / (few ? 16 : 32);
   if (slots > 65535) return MBX_EUNSUPPORTED;
-#define MBX_ROWS_GROUP(DT, MT, WT, TWO)                                                                                          \
-  do {                                                                                                                           \
-    const dim3 grid((unsigned)tiles_of(n, 16 * (TWO ? WT / 2 : WT)), (unsigned)slots);                                           \
-    if (group == 32) rows_4bit_kernel<DT, MT, WT, TWO, 32><<<grid, kRowsWaves * kWave, 0, s>>>(g);                               \
-    else if (group == 64) rows_4bit_kernel<DT, MT, WT, TWO, 64><<<grid, kRowsWaves * kWave, 0, s>>>(g);                          \
-    else rows_4bit_kernel<DT, MT, WT, TWO, 128><<<grid, kRowsWaves * kWave, 0, s>>>(g);                                          \
-  } while (0)
-#define MBX_ROWS(DT)                                                                                                             \
-  do {                                                                                                                           \
-    if (words2) {                                                                                                                \
-      if (mt == 1) MBX_ROWS_GROUP(DT, 1, 2, true); else if (mt == 2) MBX_ROWS_GROUP(DT, 2, 2, true); else MBX_ROWS_GROUP(DT, 4, 2, true); \
-    } else {                                                                                                                     \
-      if (mt == 1) MBX_ROWS_GROUP(DT, 1, 2, false); else if (mt == 2) MBX_ROWS_GROUP(DT, 2, 2, false); else MBX_ROWS_GROUP(DT, 4, 2, false); \
-    }                                                                                                                            \
-  } while (0)
-  if (dtype == MBX_BF16) MBX_ROWS(MBX_BF16);
-  else MBX_ROWS(MBX_F16);
-#undef MBX_ROWS
-#undef MBX_ROWS_GROUP
-  return launch_status();
+  return few ? launch_rows_4bit(g, dtype, group, slots, experts, s) : launch_tiles_4bit(g, dtype, group, slots, s);
 }
 
 }  // extern "C"

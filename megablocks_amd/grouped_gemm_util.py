@@ -832,8 +832,11 @@ def _ops_gmm(a, b, batch_sizes, trans_b=False):
     return GroupedGemm.apply(a, b, batch_sizes, trans_b)
 
 
-# Rows an expert, in the mean over those that can have some, above which 4-bit weights are turned into 16 bits for the products of those.
-FEW_ROWS_4BIT = 64
+# Rows an expert, in the mean over those that can have some, above which 4-bit weights are turned into 16 bits for the products of those; with groups of 32, whose
+# sums are four times as many, 3 / 5 of it.  (us, codes / values: 8 gated experts of [4096, 14336], 512 rows 1546 / 1799, 1024 rows 3011 / 2479; of [14336, 4096], 512
+# 864 / 1009, in groups of 32 256 605 / 959, 512 1189 / 1032.)  Sizes that are no multiples of 8 stay with the codes, the grouped kernels for them are slower at any number
+# (12 of [1031, 2727], 666 rows 138 / 1322).
+FEW_ROWS_4BIT = 640
 
 
 def _operand_4bit(a, weights, batch_sizes, bins, what):
@@ -889,8 +892,10 @@ def _rows_4bit(x, src, bins, rows, b, b2, act, c, what):
     return True
 
 
-def _few_rows_4bit(rows, experts):
-    return rows <= FEW_ROWS_4BIT * min(rows, experts)
+def _few_rows_4bit(rows, b):
+    if (b.k % 8 or b.n % 8) and FEW_ROWS_4BIT >= 0:
+        return True
+    return rows * (5 if b.group == 32 else 3) <= 3 * FEW_ROWS_4BIT * min(rows, b.experts)
 
 
 def _gmm_nt_bins(a, b, bins):
@@ -908,7 +913,7 @@ def gmm_4bit(a, b: Weights4bit, batch_sizes=None, bins=None):
     expert multiply the codes as they are (`mbx_gmm_4bit`); for many the values are made in a's type, 2 bytes a weight for the time of the call, and
     go through `gmm`'s kernels."""
     x, src, bins, rows = _operand_4bit(a, (b,), batch_sizes, bins, 'gmm_4bit')
-    if _few_rows_4bit(rows, b.experts):
+    if _few_rows_4bit(rows, b):
         c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
         if _rows_4bit(x, src, bins, rows, b, None, None, c, 'gmm_4bit'):
             return c
@@ -922,7 +927,7 @@ def gmm_4bit_act(a, b: Weights4bit, act, batch_sizes=None, bins=None, b2: Weight
         raise ValueError('gmm_4bit_act: act must be ACT_SILU or ACT_GELU_TANH')
     both = (b,) if b2 is None else (b, b2)
     x, src, bins, rows = _operand_4bit(a, both, batch_sizes, bins, 'gmm_4bit_act')
-    if _few_rows_4bit(rows, b.experts):
+    if _few_rows_4bit(rows, b):
         c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
         if _rows_4bit(x, src, bins, rows, b, b2, act, c, 'gmm_4bit_act' if b2 is None else 'gmm_4bit_glu'):
             return c
@@ -942,7 +947,7 @@ def experts_forward_4bit(x, expert_ids, expert_weights, num_experts, end_bit, to
     (`mbx_experts_forward_4bit`): `ops.route`, `gmm_4bit_act` on the gathered rows (v1 None: no gate), `gmm_4bit` and `ops.scatter`, with their results.  None: many
     rows, or one of those does not take the operands."""
     slots, dtype, device = expert_ids.numel(), x.dtype, x.device
-    if not 0 < slots <= EXPERTS_FORWARD_MAX_SLOTS or end_bit > 8 or dtype not in (torch.bfloat16, torch.float16) or not _few_rows_4bit(slots, num_experts) or \
+    if not 0 < slots <= EXPERTS_FORWARD_MAX_SLOTS or end_bit > 8 or dtype not in (torch.bfloat16, torch.float16) or not (_few_rows_4bit(slots, w1) and _few_rows_4bit(slots, w2)) or \
             _lib.profile_hook is not None or torch.is_grad_enabled():
         return None
     if any((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or t.device != device for t in (x, expert_ids, expert_weights)):
