@@ -17,238 +17,271 @@ namespace {
 constexpr int kPackThreads = 256;
 constexpr int kPackFeatures = 64;          // of a workgroup: a tile for each wave
 
-// rint(w / s), the quotient's exact value: ties to even.  inverse: 1 / (s lift)
-template <int DT>
-__device__ __forceinline__ float rounded_quotient(float w, float s, float inverse, float lift) {
-  const float t = w * lift * inverse, q = rintf(t);
+// rint(w / s) of the exact quotient, halves to even, plus a whole number: even if EVEN, which then costs nothing.  inverse: 1 / s.
+template <int DT, bool EVEN>
+__device__ __forceinline__ float rounded_quotient(float w, float s, float inverse, float add) {
   if constexpr (DT == MBX_F32) {
+    const float t = w * inverse, q = rintf(t);
     // t is off by up to 2^-20; where that may decide, in 64 bits
-    if (fabsf(fabsf(t - q) - 0.5f) < 0x1p-16f) return (float)rint((double)w / (double)s);
-    return q;
+    return (fabsf(fabsf(t - q) - 0.5f) < 0x1p-16f ? (float)rint((double)w / (double)s) : q) + add;
   } else {
-    // of numbers of up to 11 bits a quotient is half way between two whole numbers or further than t is off by from there; w - s q is exact
-    return fabsf(fmaf(-s, q, w)) == 0.5f * s ? 2.f * rintf(0.5f * t) : q;
+    // of two numbers of up to 11 bits the quotient is half way between two whole numbers or 2^-13 and more from there: to whole multiples of 2^-14, the last
+    // place of numbers from 512 to 1024, a quotient that is off by 2^-20 becomes the half that it is, or stays on its side
+    constexpr float kSnap = 768.f;
+    const float snapped = fmaf(w, inverse, kSnap);
+    return EVEN ? rintf(snapped - (kSnap - add)) : rintf(snapped - kSnap) + add;
   }
 }
 
 template <int DT> __device__ __forceinline__ float as_type(float v) { return Elem<DT>::to_f32(Elem<DT>::from_f32(v)); }
 
 // The 32 weights of a lane (its tile's columns 32 j + 8 g + i) as codes and scales.  GROUP: columns.
-template <int DT, int GROUP>
-__device__ __forceinline__ void encode(const float (&w)[4][8], bool zero_points, u32x4_t& words, float (&scale)[128 / GROUP], int (&zero)[128 / GROUP]) {
+template <int DT, int GROUP, bool ZEROS>
+__device__ __forceinline__ void encode(const float (&w)[4][8], u32x4_t& words, float (&scale)[128 / GROUP], int (&zero)[128 / GROUP]) {
   constexpr int kGroups = 128 / GROUP, kEach = GROUP / 32;
 #pragma unroll
   for (int p = 0; p < kGroups; ++p) {
-    float low = 0.f, high = 0.f, bad = 0.f;
+    float low = 0.f, high = 0.f;     // without zero points high is the largest size
+    bool bad = false;                // one is not a number
 #pragma unroll
     for (int j = p * kEach; j < (p + 1) * kEach; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        low = fminf(low, w[j][i]);
-        high = fmaxf(high, w[j][i]);
-        bad = fmaf(w[j][i], 0.f, bad);   // NaN if one is not finite
+      for (int i = 0; i < 8; i += 2) {
+        const float a = w[j][i], b = w[j][i + 1];
+        if constexpr (ZEROS) {
+          low = fminf(fminf(a, b), low);
+          high = fmaxf(fmaxf(a, b), high);
+        } else {
+          high = fmaxf(fmaxf(fabsf(a), fabsf(b)), high);
+        }
+        bad |= __builtin_isunordered(a, b);
       }
     // over the four lanes of a feature
-#pragma unroll
-    for (int step = 16; step <= 32; step += 16) {
-      low = fminf(low, __shfl_xor(low, step));
-      high = fmaxf(high, __shfl_xor(high, step));
-      bad += __shfl_xor(bad, step);
-    }
-    float s = as_type<DT>(zero_points ? (high - low) / 15.f : fmaxf(high, -low) / 7.f);
-    if (bad != 0.f || !(s < INFINITY)) s = NAN;
+    const uint64_t lanes = __ballot(bad);
+    bad = ((lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) >> (lane_id() % 16)) & 1;
+    const auto over = [](float v, auto&& op) {
+      const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      v = op(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+      const auto rows = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      return op(__uint_as_float(rows[0]), __uint_as_float(rows[1]));
+    };
+    high = over(high, [](float a, float b) { return fmaxf(a, b); });
+    if constexpr (ZEROS) low = over(low, [](float a, float b) { return fminf(a, b); });
+    float s = as_type<DT>(ZEROS ? (high - low) / 15.f : high / 7.f);
+    if (s < 0x1p-126f) s = 0.f;                   // no normal number of 32 bits: its inverse may be none
+    if (bad || !(s < INFINITY)) s = NAN;
     const bool usable = s > 0.f;
-    const float step = usable ? s : 1.f, lift = step < 0x1p-100f ? 0x1p64f : 1.f, inverse = 1.f / (step * lift);   // 1 / step may be infinite
+    const float inverse = 1.f / (usable ? s : 1.f);
     float z = 8.f;
-    if (zero_points) {
-      const float q = rounded_quotient<DT>(-low, step, inverse, lift);
-      z = usable ? fminf(fmaxf(q, 0.f), 15.f) : 0.f;
-    }
+    if constexpr (ZEROS) z = usable ? fminf(fmaxf(rounded_quotient<DT, true>(-low, s, inverse, 0.f), 0.f), 15.f) : 0.f;
     scale[p] = s;
     zero[p] = (int)z;
+    const uint32_t none = (uint32_t)(int)z * 0x11111111u;
 #pragma unroll
     for (int j = p * kEach; j < (p + 1) * kEach; ++j) {
-      uint32_t word = 0;
+      float half[2];       // of the word, a number below 2^16
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float q = fminf(fmaxf(rounded_quotient<DT>(w[j][i], step, inverse, lift) + z, 0.f), 15.f);
-        word |= (usable ? (uint32_t)q : (uint32_t)z) << (4 * (i / 2 + 4 * (i & 1)));
-      }
-      words[j] = word;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 6; i >= 0; i -= 2) {
+          const float q = __builtin_amdgcn_fmed3f(rounded_quotient<DT, !ZEROS>(w[j][i + h], s, inverse, z), 0.f, 15.f);
+          half[h] = i == 6 ? q : fmaf(half[h], 16.f, q);
+        }
+      words[j] = usable ? (uint32_t)half[1] << 16 | (uint32_t)half[0] : none;
     }
   }
 }
 
-// Where a workgroup of the two kernels is: 64 features, 128 columns of an expert
-struct PackPlace {
-  int64_t expert;
-  int tile, block;   // of features (the wave's), of columns
-};
-__device__ __forceinline__ PackPlace pack_place(int64_t at, int feature_groups, int blocks) {
-  PackPlace p;
-  p.block = (int)(at % blocks);
-  const int64_t rest = at / blocks;
-  p.tile = (int)(rest % feature_groups) * (kPackFeatures / kTileFeatures) + (int)(threadIdx.x / kWave);
-  p.expert = rest / feature_groups;
-  return p;
-}
+constexpr int kPitch = kPackFeatures + 2;   // of a column's features in the LDS: the four column groups of a read are 8 (fp32: 16) banks apart
 
-constexpr int kPitch = kPackFeatures + 2;
+// What a workgroup of the two kernels has: 64 features of an expert, a tile a wave, and blocks of 128 columns blockIdx.x, + gridDim.x, ...
+struct PackPlace {
+  int n, k, tiles, blocks, feature_groups, experts;
+};
 
 // Weights [E, n, k] (TRANSPOSED: [E, k, n]) into words, scales and zeros.  What bounds it: one reading of the weights.  A lane's eight columns of a word
-// are 16 bytes in a row of [n, k]; from [k, n] a workgroup's 64 features go through the LDS, whose pitch puts the four column groups of a read 8 (16) banks apart.
-template <int DT, int GROUP, bool TRANSPOSED>
+// are 16 bytes in a row of [n, k]; from [k, n] a workgroup's features go through the LDS.  whole: rows are whole 16-byte pieces at 16-byte addresses; the next
+// block's are then on their way while a block is encoded.
+template <int DT, int GROUP, bool TRANSPOSED, bool ZEROS>
 __global__ void __launch_bounds__(kPackThreads)
-quantize_kernel(const void* __restrict__ weights, int64_t places, int n, int k, int feature_groups, int blocks, bool whole, uint32_t* __restrict__ words,
-                void* __restrict__ scales, uint8_t* __restrict__ zeros) {
+quantize_kernel(const void* __restrict__ weights, const PackPlace place, bool whole, uint32_t* __restrict__ words, void* __restrict__ scales, uint8_t* __restrict__ zeros) {
   typedef typename Elem<DT>::type E;
+  constexpr int kGroups = 128 / GROUP, kEach = 16 / sizeof(E), kPieces = kTileColumns * kPackFeatures / kEach / kPackThreads;   // of a thread and block
   __shared__ alignas(16) E staged[TRANSPOSED ? kTileColumns * kPitch : 1];
-  const int lane = lane_id(), f = lane % 16, g = lane / 16, tiles = (n + 15) / 16;
-  for (int64_t at = blockIdx.x; at < places; at += gridDim.x) {
-    const PackPlace p = pack_place(at, feature_groups, blocks);
-    const E* const matrix = (const E*)weights + p.expert * n * k;
-    const int feature = p.tile * 16 + f, column = p.block * kTileColumns;
-    float w[4][8];
-    if constexpr (TRANSPOSED) {
-      const int first = p.tile / 4 * kPackFeatures;
-      __syncthreads();
-      if (whole && first + kPackFeatures <= n) {
-        constexpr int kEach = 16 / sizeof(E);
-        for (int i = threadIdx.x; i < kTileColumns * kPackFeatures / kEach; i += kPackThreads) {
-          const int row = i / (kPackFeatures / kEach), c = i % (kPackFeatures / kEach) * kEach;
-          u32x4_t v = {0, 0, 0, 0};
-          if (column + row < k) v = *(const u32x4_t*)(matrix + (int64_t)(column + row) * n + first + c);
-          uint32_t* const to = (uint32_t*)(staged + row * kPitch + c);
+  const int lane = lane_id(), f = lane % 16, g = lane / 16, n = place.n, k = place.k;
+  for (int64_t expert = blockIdx.z; expert < place.experts; expert += gridDim.z)
+    for (int group = blockIdx.y; group < place.feature_groups; group += gridDim.y) {
+      const int first = group * kPackFeatures, tile = group * 4 + (int)(threadIdx.x / kWave), feature = tile * 16 + f;
+      const E* const matrix = (const E*)weights + expert * n * k;
+      const bool pieces = whole && (!TRANSPOSED || first + kPackFeatures <= n);
+      u32x4_t next[kPieces];
+      const auto fetch = [&](int block) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) to[q] = v[q];
+        for (int q = 0; q < kPieces; ++q) {
+          next[q] = u32x4_t{0, 0, 0, 0};
+          if constexpr (TRANSPOSED) {
+            const int i = q * kPackThreads + (int)threadIdx.x, c = block * kTileColumns + i / (kPackFeatures / kEach);
+            if (c < k) next[q] = *(const u32x4_t*)(matrix + (int64_t)c * n + first + i % (kPackFeatures / kEach) * kEach);
+          } else {
+            const int c = block * kTileColumns + 32 * (q * kEach / 8) + 8 * g + q * kEach % 8;
+            if (feature < n && c < k) next[q] = *(const u32x4_t*)(matrix + (int64_t)feature * k + c);
+          }
         }
-      } else {
-        for (int i = threadIdx.x; i < kTileColumns * kPackFeatures; i += kPackThreads) {
-          const int row = i / kPackFeatures, c = i % kPackFeatures;
-          staged[row * kPitch + c] = column + row < k && first + c < n ? matrix[(int64_t)(column + row) * n + first + c] : E{};
-        }
-      }
-      __syncthreads();
+      };
+      if (pieces && (int)blockIdx.x < place.blocks) fetch(blockIdx.x);
+      for (int block = blockIdx.x; block < place.blocks; block += gridDim.x) {
+        const int column = block * kTileColumns, then = block + gridDim.x;
+        float w[4][8];
+        if constexpr (TRANSPOSED) {
+          __syncthreads();
+          if (pieces) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+            for (int q = 0; q < kPieces; ++q) {
+              const int i = q * kPackThreads + (int)threadIdx.x;
+              uint32_t* const to = (uint32_t*)(staged + i / (kPackFeatures / kEach) * kPitch + i % (kPackFeatures / kEach) * kEach);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[j][i] = Elem<DT>::to_f32(staged[(32 * j + 8 * g + i) * kPitch + (p.tile % 4) * 16 + f]);
-    } else {
+              for (int v = 0; v < 4; ++v) to[v] = next[q][v];
+            }
+          } else {
+            for (int i = threadIdx.x; i < kTileColumns * kPackFeatures; i += kPackThreads) {
+              const int c = i / kPackFeatures, r = i % kPackFeatures;
+              staged[c * kPitch + r] = column + c < k && first + r < n ? matrix[(int64_t)(column + c) * n + first + r] : E{};
+            }
+          }
+          __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = column + 32 * j + 8 * g;
-        struct alignas(16) Piece { E v[8]; };
-        if (whole) {
-          Piece piece = {};
-          if (feature < n && c < k) piece = *(const Piece*)(matrix + (int64_t)feature * k + c);
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[j][i] = Elem<DT>::to_f32(piece.v[i]);
+            for (int i = 0; i < 8; ++i) w[j][i] = Elem<DT>::to_f32(staged[(32 * j + 8 * g + i) * kPitch + (tile % 4) * 16 + f]);
+        } else if (pieces) {
+          E v[4][8];
+          __builtin_memcpy(v, next, sizeof(v));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[j][i] = Elem<DT>::to_f32(v[j][i]);
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[j][i] = feature < n && c + i < k ? Elem<DT>::to_f32(matrix[(int64_t)feature * k + c + i]) : 0.f;
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = column + 32 * j + 8 * g + i;
+              w[j][i] = feature < n && c < k ? Elem<DT>::to_f32(matrix[(int64_t)feature * k + c]) : 0.f;
+            }
+        }
+        if (pieces && then < place.blocks) fetch(then);
+        u32x4_t code;
+        float scale[kGroups];
+        int zero[kGroups];
+        encode<DT, GROUP, ZEROS>(w, code, scale, zero);
+        if (tile >= place.tiles) continue;   // no barrier between this and the head of the loop, which all waves reach
+        const int64_t at = (expert * place.tiles + tile) * place.blocks + block;
+        *(u32x4_t*)(words + at * kTileWords + lane * 4) = code;
+        // lane 16 q + f has group q's
+        float s = scale[0];
+        int z = zero[0];
+#pragma unroll
+        for (int q = 1; q < kGroups; ++q) {
+          s = g == q ? scale[q] : s;
+          z = g == q ? zero[q] : z;
+        }
+        if (g < kGroups) {
+          ((E*)scales)[at * kGroups * 16 + lane] = Elem<DT>::from_f32(s);
+          if constexpr (ZEROS) zeros[at * kGroups * 16 + lane] = (uint8_t)z;
         }
       }
     }
-    u32x4_t code;
-    float scale[128 / GROUP];
-    int zero[128 / GROUP];
-    encode<DT, GROUP>(w, zeros != nullptr, code, scale, zero);
-    if (p.tile >= tiles) continue;   // no barrier behind this that the others wait at: the next place's are at its head, which all reach
-    const int64_t tile = (p.expert * tiles + p.tile) * blocks + p.block;
-    *(u32x4_t*)(words + tile * kTileWords + lane * 4) = code;
-    if (g == 0) {
-#pragma unroll
-      for (int q = 0; q < 128 / GROUP; ++q) {
-        ((E*)scales)[(tile * (128 / GROUP) + q) * 16 + f] = Elem<DT>::from_f32(scale[q]);
-        if (zeros) zeros[(tile * (128 / GROUP) + q) * 16 + f] = (uint8_t)zero[q];
-      }
-    }
-  }
 }
 
 // The values: the reverse
 template <int DT, int GROUP, bool TRANSPOSED>
 __global__ void __launch_bounds__(kPackThreads)
-dequantize_kernel(const Packed from, int scale_dtype, int64_t places, int n, int k, int feature_groups, int blocks, bool whole, void* __restrict__ out) {
+dequantize_kernel(const Packed from, int scale_dtype, const PackPlace place, bool whole, void* __restrict__ out) {
   typedef typename Elem<DT>::type E;
-  constexpr int kGroups = 128 / GROUP;
+  constexpr int kGroups = 128 / GROUP, kEach = 16 / sizeof(E), kPieces = kTileColumns * kPackFeatures / kEach / kPackThreads;
   __shared__ alignas(16) E staged[TRANSPOSED ? kTileColumns * kPitch : 1];
-  const int lane = lane_id(), f = lane % 16, g = lane / 16, tiles = (n + 15) / 16;
-  for (int64_t at = blockIdx.x; at < places; at += gridDim.x) {
-    const PackPlace p = pack_place(at, feature_groups, blocks);
-    E* const matrix = (E*)out + p.expert * n * k;
-    const int feature = p.tile * 16 + f, column = p.block * kTileColumns;
-    E v[4][8] = {};
-    if (p.tile < tiles) {
-      const int64_t tile = (p.expert * tiles + p.tile) * blocks + p.block;
-      const u32x4_t code = *(const u32x4_t*)(from.words + tile * kTileWords + lane * 4);
-      float scale[kGroups], zero[kGroups];
+  const int lane = lane_id(), f = lane % 16, g = lane / 16, n = place.n, k = place.k;
+  for (int64_t expert = blockIdx.z; expert < place.experts; expert += gridDim.z)
+    for (int group = blockIdx.y; group < place.feature_groups; group += gridDim.y) {
+      const int first = group * kPackFeatures, tile = group * 4 + (int)(threadIdx.x / kWave), feature = tile * 16 + f;
+      E* const matrix = (E*)out + expert * n * k;
+      const bool pieces = whole && (!TRANSPOSED || first + kPackFeatures <= n);
+      u32x4_t code = {0, 0, 0, 0};
+      float lane_scale = 0.f, lane_zero = 8.f;    // of group lane / 16 (% the groups)
+      const auto fetch = [&](int block) {
+        const int64_t at = (expert * place.tiles + tile) * place.blocks + block, i = at * kGroups * 16 + lane % (kGroups * 16);
+        code = *(const u32x4_t*)(from.words + at * kTileWords + lane * 4);
+        lane_scale = load_as_f32(from.scales, i, scale_dtype);
+        if (from.zeros) lane_zero = (float)from.zeros[i];
+      };
+      if (tile < place.tiles && (int)blockIdx.x < place.blocks) fetch(blockIdx.x);
+      for (int block = blockIdx.x; block < place.blocks; block += gridDim.x) {
+        const int column = block * kTileColumns, then = block + gridDim.x;
+        uint32_t scale[kGroups], zero[kGroups];
+        spread<kGroups>(__float_as_uint(lane_scale), scale);
+        spread<kGroups>(__float_as_uint(lane_zero), zero);
+        E v[4][8];
 #pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        const int64_t i = (tile * kGroups + q) * 16 + f;
-        scale[q] = load_as_f32(from.scales, i, scale_dtype);
-        zero[q] = from.zeros ? (float)from.zeros[i] : 8.f;
-      }
+        for (int j = 0; j < 4; ++j) {
+          const float s = __uint_as_float(scale[j * kGroups / 4]), z = __uint_as_float(zero[j * kGroups / 4]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[j][i] = Elem<DT>::from_f32(((float)((code[j] >> (4 * (i / 2 + 4 * (i & 1)))) & 15u) - zero[j * kGroups / 4]) * scale[j * kGroups / 4]);
-    }
-    if constexpr (TRANSPOSED) {
-      const int first = p.tile / 4 * kPackFeatures;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) staged[(32 * j + 8 * g + i) * kPitch + (p.tile % 4) * 16 + f] = v[j][i];
-      __syncthreads();
-      if (whole && first + kPackFeatures <= n) {
-        constexpr int kEach = 16 / sizeof(E);
-        for (int i = threadIdx.x; i < kTileColumns * kPackFeatures / kEach; i += kPackThreads) {
-          const int row = i / (kPackFeatures / kEach), c = i % (kPackFeatures / kEach) * kEach;
-          const uint32_t* const at = (const uint32_t*)(staged + row * kPitch + c);
-          if (column + row < k) *(u32x4_t*)(matrix + (int64_t)(column + row) * n + first + c) = u32x4_t{at[0], at[1], at[2], at[3]};
+          for (int i = 0; i < 8; ++i) v[j][i] = Elem<DT>::from_f32(((float)((code[j] >> (4 * (i / 2 + 4 * (i & 1)))) & 15u) - z) * s);
         }
-      } else {
-        for (int i = threadIdx.x; i < kTileColumns * kPackFeatures; i += kPackThreads) {
-          const int row = i / kPackFeatures, c = i % kPackFeatures;
-          if (column + row < k && first + c < n) matrix[(int64_t)(column + row) * n + first + c] = staged[row * kPitch + c];
-        }
-      }
-    } else {
+        if (tile < place.tiles && then < place.blocks) fetch(then);
+        if constexpr (TRANSPOSED) {
+          __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = column + 32 * j + 8 * g;
-        struct alignas(16) Piece { E v[8]; };
-        if (whole) {
-          Piece piece;
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) piece.v[i] = v[j][i];
-          if (feature < n && c < k) *(Piece*)(matrix + (int64_t)feature * k + c) = piece;
+            for (int i = 0; i < 8; ++i) staged[(32 * j + 8 * g + i) * kPitch + (tile % 4) * 16 + f] = v[j][i];
+          __syncthreads();
+          if (pieces) {
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q) {
+              const int i = q * kPackThreads + (int)threadIdx.x, c = i / (kPackFeatures / kEach), r = i % (kPackFeatures / kEach) * kEach;
+              const uint32_t* const at = (const uint32_t*)(staged + c * kPitch + r);
+              if (column + c < k) *(u32x4_t*)(matrix + (int64_t)(column + c) * n + first + r) = u32x4_t{at[0], at[1], at[2], at[3]};
+            }
+          } else {
+            for (int i = threadIdx.x; i < kTileColumns * kPackFeatures; i += kPackThreads) {
+              const int c = i / kPackFeatures, r = i % kPackFeatures;
+              if (column + c < k && first + r < n) matrix[(int64_t)(column + c) * n + first + r] = staged[c * kPitch + r];
+            }
+          }
+        } else if (pieces) {
+          u32x4_t piece[kPieces];
+          __builtin_memcpy(piece, v, sizeof(v));
+#pragma unroll
+          for (int q = 0; q < kPieces; ++q) {
+            const int c = column + 32 * (q * kEach / 8) + 8 * g + q * kEach % 8;
+            if (feature < n && c < k) *(u32x4_t*)(matrix + (int64_t)feature * k + c) = piece[q];
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (feature < n && c + i < k) matrix[(int64_t)feature * k + c + i] = v[j][i];
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = column + 32 * j + 8 * g + i;
+              if (feature < n && c < k) matrix[(int64_t)feature * k + c] = v[j][i];
+            }
         }
       }
     }
-  }
 }
 
 static bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 
 static bool is_dtype(int d) { return d == MBX_BF16 || d == MBX_F16 || d == MBX_F32; }
 
+// Workgroups for all blocks up to 16384 (64 a compute unit), then as many that each has some in turn, up to eight
 struct PackGrid {
-  int feature_groups, blocks;
-  int64_t places;
-  unsigned grid;
-  PackGrid(int64_t experts, int64_t n, int64_t k) {
-    feature_groups = (int)pieces_of(n, kPackFeatures);
-    blocks = (int)pieces_of(k, kTileColumns);
-    places = experts * feature_groups * blocks;
-    grid = (unsigned)(places < 256 * 64 ? places : 256 * 64);
+  PackPlace place;
+  dim3 grid;
+  PackGrid(int experts, int n, int k) {
+    place = {n, k, (int)pieces_of(n, kTileFeatures), (int)pieces_of(k, kTileColumns), (int)pieces_of(n, kPackFeatures), experts};
+    const int64_t all = (int64_t)place.blocks * place.feature_groups * experts, turns = pieces_of(all, 16384);
+    const int64_t each = turns < 8 ? turns : 8;
+    grid = dim3((unsigned)pieces_of(place.blocks, (int)each), (unsigned)(place.feature_groups < 65535 ? place.feature_groups : 65535), (unsigned)(experts < 65535 ? experts : 65535));
   }
 };
 
@@ -262,43 +295,57 @@ extern "C" {
 int mbx_quantize_4bit(const void* weights, int dtype, int num_experts, int n, int k, int layout, int group, void* words, void* scales, uint8_t* zeros,
                       mbx_stream_t stream) {
   if (!is_dtype(dtype) || num_experts < 0 || n < 0 || k < 0 || (layout != MBX_NT && layout != MBX_NN) || !group_ok(group)) return MBX_EINVAL;
-  if (n > 0x7fffffff - 64 || k > 0x7fffffff - 128) return MBX_ERANGE;
+  if (n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (num_experts == 0 || n == 0 || k == 0) return 0;
   if (!weights || !words || !scales || ((uintptr_t)words & 15)) return MBX_EINVAL;
   const PackGrid p(num_experts, n, k);
   hipStream_t s = as_stream(stream);
   const int size = dtype_bytes(dtype), row = layout == MBX_NT ? k : n;
-  const bool whole = ((uintptr_t)weights & 15) == 0 && row % (layout == MBX_NT ? 8 : 16 / size) == 0;
+  const bool whole = ((uintptr_t)weights & 15) == 0 && row % (16 / size) == 0;
 #define MBX_PACK_GROUP(KERNEL, DT, T, ...)                                                      \
   do {                                                                                          \
-    if (group == 32) KERNEL<DT, 32, T><<<p.grid, kPackThreads, 0, s>>>(__VA_ARGS__);            \
-    else if (group == 64) KERNEL<DT, 64, T><<<p.grid, kPackThreads, 0, s>>>(__VA_ARGS__);       \
-    else KERNEL<DT, 128, T><<<p.grid, kPackThreads, 0, s>>>(__VA_ARGS__);                       \
+    if (group == 32) KERNEL(DT, 32, T, __VA_ARGS__);                                            \
+    else if (group == 64) KERNEL(DT, 64, T, __VA_ARGS__);                                       \
+    else KERNEL(DT, 128, T, __VA_ARGS__);                                                       \
   } while (0)
-#define MBX_PACK(KERNEL, ...)                                                                                                                \
-  do {                                                                                                                                       \
-    if (dtype == MBX_BF16) { if (layout == MBX_NN) MBX_PACK_GROUP(KERNEL, MBX_BF16, true, __VA_ARGS__); else MBX_PACK_GROUP(KERNEL, MBX_BF16, false, __VA_ARGS__); } \
-    else if (dtype == MBX_F16) { if (layout == MBX_NN) MBX_PACK_GROUP(KERNEL, MBX_F16, true, __VA_ARGS__); else MBX_PACK_GROUP(KERNEL, MBX_F16, false, __VA_ARGS__); } \
-    else { if (layout == MBX_NN) MBX_PACK_GROUP(KERNEL, MBX_F32, true, __VA_ARGS__); else MBX_PACK_GROUP(KERNEL, MBX_F32, false, __VA_ARGS__); } \
+#define MBX_PACK_TYPE(KERNEL, DT, ...)                                                          \
+  do {                                                                                          \
+    if (layout == MBX_NN) MBX_PACK_GROUP(KERNEL, DT, true, __VA_ARGS__);                        \
+    else MBX_PACK_GROUP(KERNEL, DT, false, __VA_ARGS__);                                        \
   } while (0)
-  MBX_PACK(quantize_kernel, weights, p.places, n, k, p.feature_groups, p.blocks, whole, (uint32_t*)words, scales, zeros);
+#define MBX_PACK(KERNEL, ...)                                                                   \
+  do {                                                                                          \
+    if (dtype == MBX_BF16) MBX_PACK_TYPE(KERNEL, MBX_BF16, __VA_ARGS__);                        \
+    else if (dtype == MBX_F16) MBX_PACK_TYPE(KERNEL, MBX_F16, __VA_ARGS__);                     \
+    else MBX_PACK_TYPE(KERNEL, MBX_F32, __VA_ARGS__);                                           \
+  } while (0)
+#define MBX_QUANTIZE(DT, GROUP, T, ...)                                                         \
+  do {                                                                                          \
+    if (zeros) quantize_kernel<DT, GROUP, T, true><<<p.grid, kPackThreads, 0, s>>>(__VA_ARGS__);  \
+    else quantize_kernel<DT, GROUP, T, false><<<p.grid, kPackThreads, 0, s>>>(__VA_ARGS__);     \
+  } while (0)
+#define MBX_DEQUANTIZE(DT, GROUP, T, ...) dequantize_kernel<DT, GROUP, T><<<p.grid, kPackThreads, 0, s>>>(__VA_ARGS__)
+  MBX_PACK(MBX_QUANTIZE, weights, p.place, whole, (uint32_t*)words, scales, zeros);
   return launch_status();
 }
 
 int mbx_dequantize_4bit(const void* words, const void* scales, const uint8_t* zeros, int scale_dtype, int num_experts, int n, int k, int layout, int group,
                         void* out, int dtype, mbx_stream_t stream) {
   if (!is_dtype(dtype) || !is_dtype(scale_dtype) || num_experts < 0 || n < 0 || k < 0 || (layout != MBX_NT && layout != MBX_NN) || !group_ok(group)) return MBX_EINVAL;
-  if (n > 0x7fffffff - 64 || k > 0x7fffffff - 128) return MBX_ERANGE;
+  if (n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (num_experts == 0 || n == 0 || k == 0) return 0;
   if (!out || !words || !scales || ((uintptr_t)words & 15)) return MBX_EINVAL;
   const PackGrid p(num_experts, n, k);
   hipStream_t s = as_stream(stream);
   const int size = dtype_bytes(dtype), row = layout == MBX_NT ? k : n;
-  const bool whole = ((uintptr_t)out & 15) == 0 && row % (layout == MBX_NT ? 8 : 16 / size) == 0;
+  const bool whole = ((uintptr_t)out & 15) == 0 && row % (16 / size) == 0;
   const Packed from = {(const uint32_t*)words, scales, zeros};
-  MBX_PACK(dequantize_kernel, from, scale_dtype, p.places, n, k, p.feature_groups, p.blocks, whole, out);
+  MBX_PACK(MBX_DEQUANTIZE, from, scale_dtype, p.place, whole, out);
 #undef MBX_PACK
+#undef MBX_PACK_TYPE
 #undef MBX_PACK_GROUP
+#undef MBX_QUANTIZE
+#undef MBX_DEQUANTIZE
   return launch_status();
 }
 

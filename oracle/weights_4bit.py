@@ -36,6 +36,7 @@ def quantize(w, group, zero_points):
     x = torch.where(bad[..., None], 0., parts.float())
     low, high = x.amin(3).clamp(max=0), x.amax(3).clamp(min=0)
     scales = ((high - low) / 15 if zero_points else torch.maximum(high, -low) / 7).to(w.dtype)
+    scales = torch.where(scales.float() < 2.0 ** -126, torch.zeros_like(scales), scales)
     step = torch.where(scales == 0, 1., scales.double())[..., None]
     zeros = torch.full(scales.shape, 8.).double()
     if zero_points:
