@@ -94,7 +94,8 @@ __device__ __forceinline__ void encode(const float (&w)[4][8], u32x4_t& words, f
 
 constexpr int kPitch = kPackFeatures + 2;   // of a column's features in the LDS: the four column groups of a read are 8 (fp32: 16) banks apart
 
-// What a workgroup of the two kernels has: 64 features of an expert, a tile a wave, and blocks of 128 columns blockIdx.x, + gridDim.x, ...
+// What a workgroup of the two kernels has: 64 features of an expert, a tile a wave, and every so many-th block of 128 columns.  Workgroups that run at the same time are
+// neighbours in the direction that the matrix is contiguous in: columns of [n, k], features of [k, n].
 struct PackPlace {
   int n, k, tiles, blocks, feature_groups, experts;
 };
@@ -109,8 +110,10 @@ quantize_kernel(const void* __restrict__ weights, const PackPlace place, bool wh
   constexpr int kGroups = 128 / GROUP, kEach = 16 / sizeof(E), kPieces = kTileColumns * kPackFeatures / kEach / kPackThreads;   // of a thread and block
   __shared__ alignas(16) E staged[TRANSPOSED ? kTileColumns * kPitch : 1];
   const int lane = lane_id(), f = lane % 16, g = lane / 16, n = place.n, k = place.k;
+  const int block0 = TRANSPOSED ? blockIdx.y : blockIdx.x, block_step = TRANSPOSED ? gridDim.y : gridDim.x;
+  const int group0 = TRANSPOSED ? blockIdx.x : blockIdx.y, group_step = TRANSPOSED ? gridDim.x : gridDim.y;
   for (int64_t expert = blockIdx.z; expert < place.experts; expert += gridDim.z)
-    for (int group = blockIdx.y; group < place.feature_groups; group += gridDim.y) {
+    for (int group = group0; group < place.feature_groups; group += group_step) {
       const int first = group * kPackFeatures, tile = group * 4 + (int)(threadIdx.x / kWave), feature = tile * 16 + f;
       const E* const matrix = (const E*)weights + expert * n * k;
       const bool pieces = whole && (!TRANSPOSED || first + kPackFeatures <= n);
@@ -128,9 +131,9 @@ quantize_kernel(const void* __restrict__ weights, const PackPlace place, bool wh
           }
         }
       };
-      if (pieces && (int)blockIdx.x < place.blocks) fetch(blockIdx.x);
-      for (int block = blockIdx.x; block < place.blocks; block += gridDim.x) {
-        const int column = block * kTileColumns, then = block + gridDim.x;
+      if (pieces && block0 < place.blocks) fetch(block0);
+      for (int block = block0; block < place.blocks; block += block_step) {
+        const int column = block * kTileColumns, then = block + block_step;
         float w[4][8];
         if constexpr (TRANSPOSED) {
           __syncthreads();
@@ -201,8 +204,10 @@ dequantize_kernel(const Packed from, int scale_dtype, const PackPlace place, boo
   constexpr int kGroups = 128 / GROUP, kEach = 16 / sizeof(E), kPieces = kTileColumns * kPackFeatures / kEach / kPackThreads;
   __shared__ alignas(16) E staged[TRANSPOSED ? kTileColumns * kPitch : 1];
   const int lane = lane_id(), f = lane % 16, g = lane / 16, n = place.n, k = place.k;
+  const int block0 = TRANSPOSED ? blockIdx.y : blockIdx.x, block_step = TRANSPOSED ? gridDim.y : gridDim.x;
+  const int group0 = TRANSPOSED ? blockIdx.x : blockIdx.y, group_step = TRANSPOSED ? gridDim.x : gridDim.y;
   for (int64_t expert = blockIdx.z; expert < place.experts; expert += gridDim.z)
-    for (int group = blockIdx.y; group < place.feature_groups; group += gridDim.y) {
+    for (int group = group0; group < place.feature_groups; group += group_step) {
       const int first = group * kPackFeatures, tile = group * 4 + (int)(threadIdx.x / kWave), feature = tile * 16 + f;
       E* const matrix = (E*)out + expert * n * k;
       const bool pieces = whole && (!TRANSPOSED || first + kPackFeatures <= n);
@@ -214,9 +219,9 @@ dequantize_kernel(const Packed from, int scale_dtype, const PackPlace place, boo
         lane_scale = load_as_f32(from.scales, i, scale_dtype);
         if (from.zeros) lane_zero = (float)from.zeros[i];
       };
-      if (tile < place.tiles && (int)blockIdx.x < place.blocks) fetch(blockIdx.x);
-      for (int block = blockIdx.x; block < place.blocks; block += gridDim.x) {
-        const int column = block * kTileColumns, then = block + gridDim.x;
+      if (tile < place.tiles && block0 < place.blocks) fetch(block0);
+      for (int block = block0; block < place.blocks; block += block_step) {
+        const int column = block * kTileColumns, then = block + block_step;
         uint32_t scale[kGroups], zero[kGroups];
         spread<kGroups>(__float_as_uint(lane_scale), scale);
         spread<kGroups>(__float_as_uint(lane_zero), zero);
@@ -277,11 +282,13 @@ static bool is_dtype(int d) { return d == MBX_BF16 || d == MBX_F16 || d == MBX_F
 struct PackGrid {
   PackPlace place;
   dim3 grid;
-  PackGrid(int experts, int n, int k) {
+  PackGrid(int experts, int n, int k, bool transposed) {
     place = {n, k, (int)pieces_of(n, kTileFeatures), (int)pieces_of(k, kTileColumns), (int)pieces_of(n, kPackFeatures), experts};
     const int64_t all = (int64_t)place.blocks * place.feature_groups * experts, turns = pieces_of(all, 16384);
     const int64_t each = turns < 8 ? turns : 8;
-    grid = dim3((unsigned)pieces_of(place.blocks, (int)each), (unsigned)(place.feature_groups < 65535 ? place.feature_groups : 65535), (unsigned)(experts < 65535 ? experts : 65535));
+    const auto most = [](int64_t v) { return (unsigned)(v < 65535 ? v : 65535); };
+    const int64_t columns = pieces_of(place.blocks, (int)each);
+    grid = transposed ? dim3((unsigned)place.feature_groups, most(columns), most(experts)) : dim3((unsigned)columns, most(place.feature_groups), most(experts));
   }
 };
 
@@ -298,7 +305,7 @@ int mbx_quantize_4bit(const void* weights, int dtype, int num_experts, int n, in
   if (n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (num_experts == 0 || n == 0 || k == 0) return 0;
   if (!weights || !words || !scales || ((uintptr_t)words & 15)) return MBX_EINVAL;
-  const PackGrid p(num_experts, n, k);
+  const PackGrid p(num_experts, n, k, layout == MBX_NN);
   hipStream_t s = as_stream(stream);
   const int size = dtype_bytes(dtype), row = layout == MBX_NT ? k : n;
   const bool whole = ((uintptr_t)weights & 15) == 0 && row % (16 / size) == 0;
@@ -335,7 +342,7 @@ int mbx_dequantize_4bit(const void* words, const void* scales, const uint8_t* ze
   if (n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (num_experts == 0 || n == 0 || k == 0) return 0;
   if (!out || !words || !scales || ((uintptr_t)words & 15)) return MBX_EINVAL;
-  const PackGrid p(num_experts, n, k);
+  const PackGrid p(num_experts, n, k, layout == MBX_NN);
   hipStream_t s = as_stream(stream);
   const int size = dtype_bytes(dtype), row = layout == MBX_NT ? k : n;
   const bool whole = ((uintptr_t)out & 15) == 0 && row % (16 / size) == 0;
