@@ -97,16 +97,19 @@ def _differentiable_gradient(logits, indices, top_k, score, norm_p, scale, grad_
     x = logits.float()
     soft = torch.softmax(x, 1) if score == 'softmax' or grad_lse is not None else None
     s = soft if score == 'softmax' else torch.sigmoid(x)
-    ds = torch.zeros_like(x) if grad_scores is None else grad_scores.float()
+    g = torch.zeros_like(x) if grad_scores is None else grad_scores.float() * s         # the gradient of log s
     if grad_weights is not None:
-        dw = grad_weights.float() * scale
+        dy = grad_weights.float() * scale
         if norm_p > 0:
-            w = s.gather(1, indices)
-            n = w.pow(norm_p).sum(1, keepdim=True).pow(1 / norm_p)
-            u = w / n
-            dw = (dw - (dw * u).sum(1, keepdim=True) * u.pow(norm_p - 1)) / n
-        ds = ds.scatter_add(1, indices, dw)
-    dx = s * (ds - (ds * s).sum(1, keepdim=True)) if score == 'softmax' else ds * s * torch.sigmoid(-x)
+            logs = norm_p * (torch.log_softmax(x, 1) if score == 'softmax' else torch.nn.functional.logsigmoid(x)).gather(1, indices)
+            parts = torch.softmax(logs, 1)                                               # u^p
+            u = ((logs - logs.logsumexp(1, keepdim=True)) / norm_p).exp()
+            here = dy * u - (dy * u).sum(1, keepdim=True) * parts
+            here = here.masked_fill(s.gather(1, indices).amax(1, keepdim=True) == 0, 0.)     # scores that are all zero: weights without a gradient
+        else:
+            here = dy * s.gather(1, indices)
+        g = g.scatter_add(1, indices, here)
+    dx = g - s * g.sum(1, keepdim=True) if score == 'softmax' else g * torch.sigmoid(-x)
     return (dx if grad_lse is None else dx + grad_lse.float().unsqueeze(1) * soft).to(logits.dtype)
 
 
@@ -122,7 +125,7 @@ def choose_experts(logits: torch.Tensor, top_k: int, score: str = 'softmax', bia
         lse     = logsumexp of the logits in fp32 where want_lse, else None
 
     The choice is that of the exact keys.  A token whose chosen scores are all zero has weights of zero.  Gradients go to the logits from scores, weights and
-    lse (once: the gradient has none itself); the bias gets none (it is updated by `balance_bias`)."""
+    lse (in fp32 from the logits), and on to the gradients' gradients; the bias gets none (it is updated by `balance_bias`)."""
     norm_p, scale = float(norm_p or 0), float(scale)
     if logits.ndim != 2:
         raise ValueError('choose_experts: logits must be [tokens, experts]')

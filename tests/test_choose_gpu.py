@@ -191,6 +191,44 @@ def test_gradient_of_the_gradient(score, p):
     assert torch.allclose(both[0], plain, rtol=1e-5, atol=1e-5) and torch.allclose(both[1], 2 * plain, rtol=1e-5, atol=1e-5)
 
 
+@pytest.mark.parametrize('p', [1, 2, 8])
+def test_norms_of_the_smallest_scores(p):
+    """Sigmoid scores of 1e-26 have squares below fp32 and weights all the same: off by the exponentials (the last bits of 60 as fp32, 2^-24 60, and 2^-22 of
+    their own) and the norm's powers (as much); scores of zero have weights and gradients of zero, the gradients' gradients too."""
+    x = torch.tensor([[-60.5, -60., -61.25, -90.], [-200., -200., -300., -250.], [1., 2., -3., 0.]])
+    leaf = x.cuda().requires_grad_()
+    s, w, i, _ = ops.choose_experts(leaf, 3, score='sigmoid', norm_p=p)
+    wide = x.double().requires_grad_()
+    u = torch.sigmoid(wide).gather(1, i.cpu())
+    most = u.detach().amax(1, keepdim=True)
+    u = u / (most * ((u / most) ** p).sum(1, keepdim=True) ** (1 / p))
+    real = torch.tensor([0, 2])
+    assert i[0].tolist() == [1, 0, 2] and not w[1].any()
+    assert torch.allclose(w[real].cpu().double(), u[real], rtol=2e-5, atol=0)
+    dy, v = torch.tensor([[1., -2., .5]] * 3), torch.tensor([[.5, 1., -1., 2.]] * 3)
+    plain, = torch.autograd.grad(w, leaf, dy.cuda(), retain_graph=True)
+    first, = torch.autograd.grad(w, leaf, dy.cuda(), create_graph=True)
+    second, = torch.autograd.grad(first, leaf, v.cuda())
+    want, = torch.autograd.grad(u, wide, dy.double(), create_graph=True)
+    want_second, = torch.autograd.grad(want, wide, v.double())
+    for got, is_ in ((plain, want), (first, want), (second, want_second)):
+        assert not got[1].any() and torch.allclose(got[real].cpu().double(), is_[real], rtol=1e-4, atol=1e-4)
+
+
+def test_more_tokens_than_a_launch():
+    """2^23 workgroups of 4 tokens are one launch: the last tokens of the first and those of the second, each with its own choice."""
+    tokens = 2**25 + 3
+    x = torch.zeros(tokens, 17, device='cuda', dtype=torch.bfloat16)
+    t = torch.arange(tokens, device='cuda')
+    x[t, t % 17] = 2.
+    x.requires_grad_()
+    _, w, i, _ = ops.choose_experts(x, 1, score='sigmoid', groups=17, top_groups=1, group_best=1)
+    assert torch.equal(i[:, 0], t % 17)
+    w.backward(torch.ones_like(w))
+    own = x.grad[t, t % 17]
+    assert bool((own == own[0]).all()) and own[0] > 0 and int((x.grad != 0).sum()) == tokens
+
+
 def test_strides_types_and_no_tokens():
     g = torch.Generator().manual_seed(2)
     wide = torch.randn(37, 80, generator=g)
