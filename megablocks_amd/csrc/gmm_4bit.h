@@ -28,11 +28,14 @@ struct Rows4bit {
   int num_groups;
   int64_t rows;
   int k, n, act;            // act < 0: none
+  int first_slot;           // the launch's first tile of rows
 };
 
-// Launches over `slots` pieces of 16 (rows) or 32 (tiles) rows at most; dtype, group and whether there is a second matrix are the arguments'.
+// The kernels: of tiles of 16 rows (few rows an expert), 32 (dozens) and 64 (hundreds), `slots` of them at most.  dtype, group, zeros and whether there is a
+// second matrix are the arguments'.
 int launch_rows_4bit(const Rows4bit& g, int dtype, int group, int64_t slots, int64_t experts, hipStream_t s);
 int launch_tiles_4bit(const Rows4bit& g, int dtype, int group, int64_t slots, hipStream_t s);
+int launch_long_4bit(const Rows4bit& g, int dtype, int group, int64_t slots, hipStream_t s);
 
 namespace {
 
@@ -50,13 +53,15 @@ template <int DT> struct Codes;
 template <> struct Codes<MBX_BF16> { static constexpr uint32_t kNibbles = 0x00780078u, kSixteens = 0x41804180u; static constexpr int kUp = 3; };
 template <> struct Codes<MBX_F16> { static constexpr uint32_t kNibbles = 0x03c003c0u, kSixteens = 0x4c004c00u; static constexpr int kUp = 6; };
 template <int DT>
+__device__ __forceinline__ uint32_t sixteen_and_pair(uint32_t word, int i, uint32_t mask, uint32_t bits) {
+  const int up = Codes<DT>::kUp - 4 * i;
+  return ((up >= 0 ? word << (up >= 0 ? up : 0) : word >> (up < 0 ? -up : 0)) & mask) | bits;
+}
+template <int DT>
 __device__ __forceinline__ u32x4_t sixteen_and(uint32_t word, uint32_t mask, uint32_t bits) {
   u32x4_t out;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int up = Codes<DT>::kUp - 4 * i;
-    out[i] = ((up >= 0 ? word << (up >= 0 ? up : 0) : word >> (up < 0 ? -up : 0)) & mask) | bits;
-  }
+  for (int i = 0; i < 4; ++i) out[i] = sixteen_and_pair<DT>(word, i, mask, bits);
   return out;
 }
 
@@ -66,8 +71,9 @@ __device__ __forceinline__ float activated(float x, int act) {
   return x / (1.f + __expf(-y));
 }
 
-// Tile `slot` of up to `height` rows: its expert, first and end row, false past the last.  bins need not be trusted: bounds stay in [0, rows].
-__device__ __forceinline__ bool find_rows(const Rows4bit& g, int slot, int height, int& expert, int& first, int& end) {
+// The workgroup's tile of up to `height` rows: its expert, first and end row, false past the last.  bins need not be trusted: bounds stay in [0, rows].
+__device__ __forceinline__ bool find_rows(const Rows4bit& g, int height, int& expert, int& first, int& end) {
+  const int slot = g.first_slot + (int)blockIdx.y;
   const int lane = lane_id(), per = (g.num_groups + kWave - 1) / kWave, rows = (int)g.rows;
   const auto clipped = [&](int b) { return b < 0 ? 0 : b > rows ? rows : b; };
   const auto bound = [&](int e) { return e <= 0 ? 0 : clipped(g.bins[e - 1]); };   // rows before expert e
@@ -140,6 +146,15 @@ __device__ __forceinline__ void spread(uint32_t v, uint32_t (&of)[GROUPS]) {
 
 inline int64_t pieces_of(int64_t n, int of) { return (n + of - 1) / of; }
 
+// launch(g, rows of the grid) for all slots, 65535 at a time
+template <typename F>
+void for_slots(Rows4bit g, int64_t slots, F&& launch) {
+  for (int64_t first = 0; first < slots; first += 65535) {
+    g.first_slot = (int)first;
+    launch(g, (unsigned)(slots - first < 65535 ? slots - first : 65535));
+  }
+}
+
 // A wave's WT tiles of weights of one expert (TWO: every other one of the second matrix), a block of 128 columns at a time.
 template <int DT, int WT, bool TWO, int GROUP>
 struct Weights4bit {
@@ -169,15 +184,14 @@ struct Weights4bit {
     with_zeros = zeros_at[0] != nullptr;
   }
 
-  // ONCE: read by nobody else, kept out of the caches (16 x 60 MiB of weights read alone: 9.7 us, with plain loads 10.9; 480 MiB: 69, 78)
+  // ONCE: read by nobody else, kept out of the caches (60 MiB of weights read alone: 9.7 us, with plain loads 10.9; 480 MiB: 69, 78)
   template <bool ONCE>
-  __device__ __forceinline__ void fetch(Block& to, int b) const {
-#pragma unroll
-    for (int t = 0; t < WT; ++t) {
-      const auto at = (const __attribute__((address_space(1))) u32x4_t*)(words_at[t] + (int64_t)b * (kTileWords * 4) + word_lane);
-      if constexpr (ONCE) to.words[t] = __builtin_nontemporal_load(at);
-      else to.words[t] = *at;
-    }
+  __device__ __forceinline__ void fetch_words(Block& to, int t, int b) const {
+    const auto at = (const __attribute__((address_space(1))) u32x4_t*)(words_at[t] + (int64_t)b * (kTileWords * 4) + word_lane);
+    if constexpr (ONCE) to.words[t] = __builtin_nontemporal_load(at);
+    else to.words[t] = *at;
+  }
+  __device__ __forceinline__ void fetch_scales(Block& to, int b) const {
     if (wide) {
 #pragma unroll
       for (int t = 0; t < WT; ++t) to.scale[t] = load_at<uint32_t>(scales_at[t], (int64_t)b * (kGroups * 64), scale_lane * 4);
@@ -189,6 +203,12 @@ struct Weights4bit {
 #pragma unroll
       for (int t = 0; t < WT; ++t) to.zero[t] = load_at<uint8_t>(zeros_at[t], (int64_t)b * (kGroups * 16), scale_lane);
     }
+  }
+  template <bool ONCE>
+  __device__ __forceinline__ void fetch(Block& to, int b) const {
+#pragma unroll
+    for (int t = 0; t < WT; ++t) fetch_words<ONCE>(to, t, b);
+    fetch_scales(to, b);
   }
 
   // scale and -(16 + zero) of the lane's feature for each group
@@ -208,11 +228,14 @@ struct CodeBits {
     asm("" : "+v"(bits));
   }
 };
+// Eight times v, which the type holds
 template <int DT>
-__device__ __forceinline__ u32x4_t ones_of() {
-  const uint32_t one = DT == MBX_BF16 ? 0x3f803f80u : 0x3c003c00u;
-  return u32x4_t{one, one, one, one};
+__device__ __forceinline__ u32x4_t all_of(float v) {
+  const uint32_t one = __builtin_bit_cast(uint16_t, Elem<DT>::from_f32(v)), two = one << 16 | one;
+  return u32x4_t{two, two, two, two};
 }
+template <int DT>
+__device__ __forceinline__ u32x4_t ones_of() { return all_of<DT>(1.f); }
 
 // Columns c ... c + 7 of a row of k, zeros past its end
 __device__ __forceinline__ void read_columns(const uint16_t* row, int c, int k, u32x4_t& to) {

@@ -274,6 +274,8 @@ dequantize_kernel(const Packed from, int scale_dtype, const PackPlace place, boo
     }
 }
 
+constexpr int kMostFeatures = 1 << 26;   // a launch's threads have to be fewer than 2^32
+
 static bool group_ok(int group) { return group == 32 || group == 64 || group == 128; }
 
 static bool is_dtype(int d) { return d == MBX_BF16 || d == MBX_F16 || d == MBX_F32; }
@@ -302,7 +304,7 @@ extern "C" {
 int mbx_quantize_4bit(const void* weights, int dtype, int num_experts, int n, int k, int layout, int group, void* words, void* scales, uint8_t* zeros,
                       mbx_stream_t stream) {
   if (!is_dtype(dtype) || num_experts < 0 || n < 0 || k < 0 || (layout != MBX_NT && layout != MBX_NN) || !group_ok(group)) return MBX_EINVAL;
-  if (n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
+  if (n > kMostFeatures || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (num_experts == 0 || n == 0 || k == 0) return 0;
   if (!weights || !words || !scales || ((uintptr_t)words & 15)) return MBX_EINVAL;
   const PackGrid p(num_experts, n, k, layout == MBX_NN);
@@ -339,7 +341,7 @@ int mbx_quantize_4bit(const void* weights, int dtype, int num_experts, int n, in
 int mbx_dequantize_4bit(const void* words, const void* scales, const uint8_t* zeros, int scale_dtype, int num_experts, int n, int k, int layout, int group,
                         void* out, int dtype, mbx_stream_t stream) {
   if (!is_dtype(dtype) || !is_dtype(scale_dtype) || num_experts < 0 || n < 0 || k < 0 || (layout != MBX_NT && layout != MBX_NN) || !group_ok(group)) return MBX_EINVAL;
-  if (n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
+  if (n > kMostFeatures || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (num_experts == 0 || n == 0 || k == 0) return 0;
   if (!out || !words || !scales || ((uintptr_t)words & 15)) return MBX_EINVAL;
   const PackGrid p(num_experts, n, k, layout == MBX_NN);
@@ -363,20 +365,20 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   if (indices && (top_k <= 0 || a_rows < 0)) return MBX_EINVAL;
   if (words2 && (act < 0 || !zeros != !zeros2)) return MBX_EINVAL;
   if (dtype == MBX_F32 || (scale_dtype != dtype && scale_dtype != MBX_F32) || k == 0) return MBX_EUNSUPPORTED;
-  if (rows > 0x7fffffff || n > 0x7fffffff - 1024 || k > 0x7fffffff - 256) return MBX_ERANGE;
+  if (rows > 0x7fffffff || n > kMostFeatures || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (rows == 0 || n == 0 || num_groups == 0) return 0;
   if (!a || !words || !scales || !c || !bins || (words2 && !scales2) || (indices && a_rows == 0)) return MBX_EINVAL;
   if (((uintptr_t)words | (uintptr_t)words2) & 15) return MBX_EINVAL;
   hipStream_t s = as_stream(stream);
   const Rows4bit g = {a, indices, a_rows, top_k, {{(const uint32_t*)words, scales, zeros}, {(const uint32_t*)words2, scales2, zeros2}}, scale_dtype == MBX_F32,
-                      c, bins, num_groups, rows, k, n, act};
-  // up to 12 rows an expert in the mean of those that can have some the one kernel, then the other (us, one / other: 8 gated experts of [4096, 14336], 8 rows
-  // 93 / 115, 16 rows 143 / 119; 64 of [2048, 1408], 3 rows 40 / 46, 15 rows 62 / 48)
+                      c, bins, num_groups, rows, k, n, act, 0};
+  // By rows an expert in the mean of those that can have some: up to 12, dozens, from 96 on (us, 8 gated experts of [4096, 14336]: 8 rows 93 / 115 with the first
+  // two, 16 rows 143 / 119; with the last two 64 rows 234 / 239, 128 rows 381 / 351, 1024 rows 2516 / 2114; 64 of [2048, 1408]: 3 rows 40 / 46, 15 rows 62 / 48;
+  // 93 rows 140 / 138).  The last one's rows are whole pieces of 16 bytes.
   const int64_t experts = rows < num_groups ? rows : num_groups;
-  const bool few = rows <= 12 * experts;
-  const int64_t slots = experts + rows / (few ? 16 : 32);
-  if (slots > 65535) return MBX_EUNSUPPORTED;
-  return few ? launch_rows_4bit(g, dtype, group, slots, experts, s) : launch_tiles_4bit(g, dtype, group, slots, s);
+  const bool few = rows <= 12 * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 28;
+  const int64_t slots = experts + rows / (few ? 16 : many ? 64 : 32);
+  return few ? launch_rows_4bit(g, dtype, group, slots, experts, s) : many ? launch_long_4bit(g, dtype, group, slots, s) : launch_tiles_4bit(g, dtype, group, slots, s);
 }
 
 }  // extern "C"

@@ -26,7 +26,7 @@ rows_4bit_kernel(const Rows4bit g) {
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), f = lane % 16, part = lane / 16;
   const int wk = wave % WK, wf = wave / WK;
   int expert, first, end;
-  if (!find_rows(g, (int)blockIdx.y, 16, expert, first, end)) return;   // alike for all waves: none is left at the barrier
+  if (!find_rows(g, 16, expert, first, end)) return;   // alike for all waves: none is left at the barrier
   const int tiles = (g.n + 15) / 16, blocks = (g.k + 127) / 128, tile0 = ((int)blockIdx.x * WF + wf) * kFeatureTiles;
   const Weights4bit<DT, WT, TWO, GROUP> weights(g, expert, tile0, tiles, blocks);
   typename Weights4bit<DT, WT, TWO, GROUP>::Block now;
@@ -97,7 +97,9 @@ rows_4bit_kernel(const Rows4bit g) {
 template <int DT, int WT, bool TWO, int GROUP, int WK>
 void launch(const Rows4bit& g, int64_t slots, hipStream_t s) {
   const int64_t waves = pieces_of(g.n, 16 * (TWO ? WT / 2 : WT));
-  rows_4bit_kernel<DT, WT, TWO, GROUP, WK><<<dim3((unsigned)pieces_of(waves, rows_waves(WK) / WK), (unsigned)slots), rows_waves(WK) * kWave, 0, s>>>(g);
+  for_slots(g, slots, [=](const Rows4bit& of, unsigned tiles) {
+    rows_4bit_kernel<DT, WT, TWO, GROUP, WK><<<dim3((unsigned)pieces_of(waves, rows_waves(WK) / WK), tiles), rows_waves(WK) * kWave, 0, s>>>(of);
+  });
 }
 
 // More tiles a wave share a reading of the rows, fewer leave more waves; the more waves share the columns the shorter the way of each.  By the tiles that

@@ -15,20 +15,21 @@ namespace {
 
 constexpr int kRowTiles = 2;   // of 16
 
-template <int DT, int WT, bool TWO, int GROUP>
+template <int DT, int WT, bool TWO, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(4 * kWave, WT == 2 ? 4 : 2)
 tile_4bit_kernel(const Rows4bit g) {
   typedef typename Elem<DT>::type E;
   constexpr int kGroups = 128 / GROUP, kEach = GROUP / 32, MT = kRowTiles;
   constexpr int kFeatureTiles = TWO ? WT / 2 : WT;
-  __shared__ u32x4_t staged[2][16 * MT][16];
+  __shared__ u32x4_t staged[3][16 * MT][16];
+  __shared__ f32x4_t sums[2][kGroups][4 * MT];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), f = lane % 16, part = lane / 16;
   int expert, first, end;
-  if (!find_rows(g, (int)blockIdx.y, 16 * MT, expert, first, end)) return;   // alike for all waves: none is left at a barrier
+  if (!find_rows(g, 16 * MT, expert, first, end)) return;   // alike for all waves: none is left at a barrier
   const int tiles = (g.n + 15) / 16, blocks = (g.k + 127) / 128, tile0 = ((int)blockIdx.x * 4 + wave) * kFeatureTiles;
   const Weights4bit<DT, WT, TWO, GROUP> weights(g, expert, tile0, tiles, blocks);
   typename Weights4bit<DT, WT, TWO, GROUP>::Block next;
-  // thread i stages piece i % 16 of rows i / 16 and i / 16 + 16; rows past the last are the last again
+  // thread i stages piece i % 16 of rows i / 16, i / 16 + 16, ...; rows past the last are the last again
   const int piece = (int)threadIdx.x % 16, stage_row = (int)threadIdx.x / 16;
   const uint16_t* row[MT];
 #pragma unroll
@@ -45,35 +46,61 @@ tile_4bit_kernel(const Rows4bit g) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) staged[buffer][16 * m + stage_row][piece ^ stage_row] = x_next[m];
   };
+  // Sums of the rows' columns of each group, a wave a tile of rows; without zeros times -24, which is what a code of 0 is off by
+  const u32x4_t ones = ZEROS ? ones_of<DT>() : all_of<DT>(-24.f);
+  const auto sum_up = [&](int buffer, int to) {
+    if (wave >= MT) return;
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      f32x4_t sum = {};
+#pragma unroll
+      for (int j = q * kEach; j < (q + 1) * kEach; ++j) sum = mfma_16x16x32<DT>(staged[buffer][16 * wave + f][(4 * j + part) ^ f], ones, sum);
+      if (f == 0) sums[to][q][4 * wave + part] = sum;
+    }
+  };
   f32x4_t y[WT][MT] = {};
-  const u32x4_t ones = ones_of<DT>();
   const CodeBits<DT> codes;
   fetch_rows(0);
   weights.template fetch<false>(next, 0);
   stage(0);
-  if (blocks > 1) fetch_rows(1);
+  if (blocks > 1) {
+    fetch_rows(1);
+    stage(1);
+  }
+  if (blocks > 2) fetch_rows(2);
+  __syncthreads();
+  sum_up(0, 0);
+  int buffer = 0;
   for (int b = 0; b < blocks; ++b) {
     const auto now = next;
-    __syncthreads();       // block b's rows are there, and those of block b - 1 no longer read
+    const int after = buffer == 2 ? 0 : buffer + 1;
+    __syncthreads();       // the rows of blocks b and b + 1 and the sums of b are there, and what is of block b - 1 no longer read
     if (b + 1 < blocks) {
-      stage((b + 1) & 1);
-      if (b + 2 < blocks) fetch_rows(b + 2);
+      if (b + 2 < blocks) stage(after == 2 ? 0 : after + 1);
+      if (b + 3 < blocks) fetch_rows(b + 3);
       weights.template fetch<false>(next, b + 1);
+      sum_up(after, (b + 1) & 1);
     }
-    const u32x4_t(*const x_now)[16] = staged[b & 1];
+    const u32x4_t(*const x_now)[16] = staged[buffer];
     uint32_t scale[WT][kGroups], off[WT][kGroups];
 #pragma unroll
     for (int t = 0; t < WT; ++t) weights.scales(now, t, scale[t], off[t]);
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) {
-      f32x4_t acc[WT][MT] = {}, of_ones[MT] = {};
+      f32x4_t acc[WT][MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const f32x4_t sum = sums[b & 1][q][4 * m + part];
+#pragma unroll
+        for (int t = 0; t < WT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][m][i] = ZEROS ? __uint_as_float(off[t][q]) * sum[i] : sum[i];
+      }
 #pragma unroll
       for (int j = q * kEach; j < (q + 1) * kEach; ++j) {
         u32x4_t x[MT];
 #pragma unroll
         for (int m = 0; m < MT; ++m) x[m] = x_now[16 * m + f][(4 * j + part) ^ f];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) of_ones[m] = mfma_16x16x32<DT>(x[m], ones, of_ones[m]);
 #pragma unroll
         for (int t = 0; t < WT; ++t) {
           const u32x4_t w = sixteen_and<DT>(now.words[t][j], codes.mask, codes.bits);
@@ -86,11 +113,11 @@ tile_4bit_kernel(const Rows4bit g) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            y[t][m][i] = fmaf(__uint_as_float(scale[t][q]), fmaf(__uint_as_float(off[t][q]), of_ones[m][i], acc[t][m][i]), y[t][m][i]);
+          for (int i = 0; i < 4; ++i) y[t][m][i] = fmaf(__uint_as_float(scale[t][q]), acc[t][m][i], y[t][m][i]);
           asm volatile("" : "+v"(y[t][m]));   // a group's sums before the next group's products
         }
     }
+    buffer = after;
   }
 #pragma unroll
   for (int t = 0; t < kFeatureTiles; ++t)
@@ -108,7 +135,11 @@ tile_4bit_kernel(const Rows4bit g) {
 
 template <int DT, int WT, bool TWO, int GROUP>
 void launch(const Rows4bit& g, int64_t slots, hipStream_t s) {
-  tile_4bit_kernel<DT, WT, TWO, GROUP><<<dim3((unsigned)pieces_of(g.n, 64 * (TWO ? WT / 2 : WT)), (unsigned)slots), 4 * kWave, 0, s>>>(g);
+  for_slots(g, slots, [=](const Rows4bit& of, unsigned tiles) {
+    const dim3 grid((unsigned)pieces_of(g.n, 64 * (TWO ? WT / 2 : WT)), tiles);
+    if (g.b[0].zeros) tile_4bit_kernel<DT, WT, TWO, GROUP, true><<<grid, 4 * kWave, 0, s>>>(of);
+    else tile_4bit_kernel<DT, WT, TWO, GROUP, false><<<grid, 4 * kWave, 0, s>>>(of);
+  });
 }
 
 // Four tiles a wave where that leaves six workgroups a compute unit (us, two / four: 8 gated experts of [4096, 14336], 32 rows, 1792 workgroups 158 / 150, 256 rows

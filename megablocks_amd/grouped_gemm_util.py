@@ -832,13 +832,6 @@ def _ops_gmm(a, b, batch_sizes, trans_b=False):
     return GroupedGemm.apply(a, b, batch_sizes, trans_b)
 
 
-# Rows an expert, in the mean over those that can have some, above which 4-bit weights are turned into 16 bits for the products of those; with groups of 32, whose
-# sums are four times as many, 3 / 5 of it.  (us, codes / values: 8 gated experts of [4096, 14336], 512 rows 1546 / 1799, 1024 rows 3011 / 2479; of [14336, 4096], 512
-# 864 / 1009, in groups of 32 256 605 / 959, 512 1189 / 1032.)  Sizes that are no multiples of 8 stay with the codes, the grouped kernels for them are slower at any number
-# (12 of [1031, 2727], 666 rows 138 / 1322).
-FEW_ROWS_4BIT = 640
-
-
 def _operand_4bit(a, weights, batch_sizes, bins, what):
     """(rows of a, their source or None, bins) of a product with 4-bit weights, checked."""
     src = a if isinstance(a, GatheredRows) else None
@@ -876,78 +869,40 @@ def _operand_4bit(a, weights, batch_sizes, bins, what):
     return x.contiguous(), src, bins.contiguous(), rows
 
 
-def _rows_4bit(x, src, bins, rows, b, b2, act, c, what):
-    """The product of few rows (`mbx_gmm_4bit`) into c; False where the library does not take it."""
+def _product_4bit(x, src, bins, rows, b, b2, act, what):
+    c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
     indices = None if src is None else src.indices.contiguous()
-    with _lib.device_of(x), _lib.record(what, rows=rows, k=b.k, n=b.n * (1 if b2 is None else 2), elem=x.element_size(), groups=b.experts) as rec:
-        rc = lib.mbx_gmm_4bit(_lib.ptr(x), x.shape[0], _lib.ptr(indices), 1 if src is None else src.top_k, _lib.ptr(b.words), _lib.ptr(b.scales),
-                              _lib.ptr(b.zeros), None if b2 is None else _lib.ptr(b2.words), None if b2 is None else _lib.ptr(b2.scales),
-                              None if b2 is None else _lib.ptr(b2.zeros), _lib.DTYPE[b.scales.dtype], b.group, _lib.ptr(c), _lib.dtype_of(x),
-                              _lib.ptr(bins), b.experts, rows, b.k, b.n, -1 if act is None else act, _lib.stream())
-        if rc == _lib.EUNSUPPORTED:
-            rec.cancel()
-    if rc == _lib.EUNSUPPORTED:
-        return False
-    _lib.check(rc, what)
-    return True
-
-
-def _few_rows_4bit(rows, b):
-    if (b.k % 8 or b.n % 8) and FEW_ROWS_4BIT >= 0:
-        return True
-    return rows * (5 if b.group == 32 else 3) <= 3 * FEW_ROWS_4BIT * min(rows, b.experts)
-
-
-def _gmm_nt_bins(a, b, bins):
-    """gmm(a, b, trans_b=True) by the bins themselves."""
-    c = torch.empty((a.shape[0], b.shape[1]), dtype=a.dtype, device=a.device)
-    with _lib.device_of(a), _lib.record('gmm_nt', rows=a.shape[0], k=a.shape[1], n=b.shape[1], elem=a.element_size(), groups=b.shape[0]):
-        _lib.check(lib.mbx_gmm(_lib.ptr(a), _lib.ptr(b), _lib.ptr(c), _lib.dtype_of(a), _lib.ptr(bins), b.shape[0], a.shape[0], a.shape[1], b.shape[1], _lib.NT,
-                               _lib.stream()), 'gmm')
+    with _lib.device_of(x), _lib.record(what, rows=rows, k=b.k, n=b.n * (1 if b2 is None else 2), elem=x.element_size(), groups=b.experts):
+        _lib.check(lib.mbx_gmm_4bit(_lib.ptr(x), x.shape[0], _lib.ptr(indices), 1 if src is None else src.top_k, _lib.ptr(b.words), _lib.ptr(b.scales),
+                                    _lib.ptr(b.zeros), None if b2 is None else _lib.ptr(b2.words), None if b2 is None else _lib.ptr(b2.scales),
+                                    None if b2 is None else _lib.ptr(b2.zeros), _lib.DTYPE[b.scales.dtype], b.group, _lib.ptr(c), _lib.dtype_of(x),
+                                    _lib.ptr(bins), b.experts, rows, b.k, b.n, -1 if act is None else act, _lib.stream()), what)
     return c
 
 
 def gmm_4bit(a, b: Weights4bit, batch_sizes=None, bins=None):
     """out[r_e] = a[r_e] @ b[e]^T (as b's values are [experts, n, k]) with 4-bit weights b, without gradients: a [rows, k] in bf16 or fp16, or a GatheredRows;
-    batch_sizes as for `gmm`, or their inclusive int32 sums `bins` on the device (a GatheredRows brings its own).  fp32 sums, rounded once.  Few rows an
-    expert multiply the codes as they are (`mbx_gmm_4bit`); for many the values are made in a's type, 2 bytes a weight for the time of the call, and
-    go through `gmm`'s kernels."""
+    batch_sizes as for `gmm`, or their inclusive int32 sums `bins` on the device (a GatheredRows brings its own).  The values are not rounded to a's type:
+    fp32 sums of a's rows with the codes, scaled in fp32 a group at a time, rounded once.  A row with an infinity gives infinities or NaN."""
     x, src, bins, rows = _operand_4bit(a, (b,), batch_sizes, bins, 'gmm_4bit')
-    if _few_rows_4bit(rows, b):
-        c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
-        if _rows_4bit(x, src, bins, rows, b, None, None, c, 'gmm_4bit'):
-            return c
-    return _gmm_nt_bins(x if src is None else src.materialize(), b.dequantize(x.dtype, trans_b=True), bins)
+    return _product_4bit(x, src, bins, rows, b, None, None, 'gmm_4bit')
 
 
 def gmm_4bit_act(a, b: Weights4bit, act, batch_sizes=None, bins=None, b2: Weights4bit = None):
-    """activation(a[r_e] @ b[e]^T), with b2 times a[r_e] @ b2[e]^T: the experts' first product(s) with 4-bit weights and their activation, operands as for
-    `gmm_4bit`.  act: ACT_SILU or ACT_GELU_TANH.  Few rows an expert: one launch, rounded once; many: as `gmm_act` / `gmm_glu` with the weights' values."""
+    """activation(a[r_e] @ b[e]^T), with b2 times a[r_e] @ b2[e]^T: the experts' first product(s) with 4-bit weights and their activation by one launch, rounded
+    once; operands as for `gmm_4bit`.  act: ACT_SILU or ACT_GELU_TANH."""
     if act not in (ACT_SILU, ACT_GELU_TANH):
         raise ValueError('gmm_4bit_act: act must be ACT_SILU or ACT_GELU_TANH')
-    both = (b,) if b2 is None else (b, b2)
-    x, src, bins, rows = _operand_4bit(a, both, batch_sizes, bins, 'gmm_4bit_act')
-    if _few_rows_4bit(rows, b):
-        c = torch.empty((rows, b.n), dtype=x.dtype, device=x.device)
-        if _rows_4bit(x, src, bins, rows, b, b2, act, c, 'gmm_4bit_act' if b2 is None else 'gmm_4bit_glu'):
-            return c
-    values = [w.dequantize(x.dtype, trans_b=True) for w in both]
-    if ACTIVATION_EPILOGUES and (b2 is not None or act == ACT_GELU_TANH):
-        h = _hidden(x, src, values[0], None if b2 is None else values[1], bins, rows, act)
-        if h is not None:
-            return h
-    x = x if src is None else src.materialize()
-    products = [_gmm_nt_bins(x, v, bins).float() for v in values]
-    h = torch.nn.functional.silu(products[0]) if act == ACT_SILU else torch.nn.functional.gelu(products[0], approximate='tanh')
-    return (h if b2 is None else h * products[1]).to(x.dtype)
+    x, src, bins, rows = _operand_4bit(a, (b,) if b2 is None else (b, b2), batch_sizes, bins, 'gmm_4bit_act')
+    return _product_4bit(x, src, bins, rows, b, b2, act, 'gmm_4bit_act' if b2 is None else 'gmm_4bit_glu')
 
 
 def experts_forward_4bit(x, expert_ids, expert_weights, num_experts, end_bit, top_k, w1: Weights4bit, v1, w2: Weights4bit, act):
     """(out, tokens_per_expert) of the grouped dropless layer behind its router with 4-bit experts, from one call of the library
-    (`mbx_experts_forward_4bit`): `ops.route`, `gmm_4bit_act` on the gathered rows (v1 None: no gate), `gmm_4bit` and `ops.scatter`, with their results.  None: many
-    rows, or one of those does not take the operands."""
+    (`mbx_experts_forward_4bit`): `ops.route`, `gmm_4bit_act` on the gathered rows (v1 None: no gate), `gmm_4bit` and `ops.scatter`, with their results.  None where
+    there are many rows, or one of those does not take the operands."""
     slots, dtype, device = expert_ids.numel(), x.dtype, x.device
-    if not 0 < slots <= EXPERTS_FORWARD_MAX_SLOTS or end_bit > 8 or dtype not in (torch.bfloat16, torch.float16) or not (_few_rows_4bit(slots, w1) and _few_rows_4bit(slots, w2)) or \
+    if not 0 < slots <= EXPERTS_FORWARD_MAX_SLOTS or end_bit > 8 or dtype not in (torch.bfloat16, torch.float16) or \
             _lib.profile_hook is not None or torch.is_grad_enabled():
         return None
     if any((type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter) or t.device != device for t in (x, expert_ids, expert_weights)):
