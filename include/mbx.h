@@ -515,10 +515,10 @@ int mbx_dequantize_4bit(const void* words, const void* scales, const uint8_t* ze
                         void* out, int dtype, mbx_stream_t stream);
 
 /* c[r_e] = act(X[r_e] @ W[e]^T) (act -1: none; else an mbx_activation), with a second matrix (words2 not NULL) times X[r_e] @ W2[e]^T, rows [bins[e - 1],
- * bins[e]) for expert e: the experts' products for few rows an expert, where reading the weights is what takes the time.  Rows of X: a's (indices NULL), or
- * a[indices[r] / top_k] of a's a_rows rows.  16-bit activations, fp32 sums, rounded once.  The scales of both matrices are of type `dtype` or fp32; both
- * have zeros or neither has.  Any number of rows is computed; with hundreds an expert mbx_dequantize_4bit and mbx_gmm are faster.  MBX_EUNSUPPORTED:
- * fp32 activations, other scales, k = 0, more than 65535 pieces of 16 to 64 rows. */
+ * bins[e]) for expert e: the experts' products, for a token's few rows (where reading the weights is what takes the time) to thousands.  Rows of X: a's (indices NULL), or
+ * a[indices[r] / top_k] of a's a_rows rows.  16-bit activations, fp32 sums of the rows with the codes, scaled in fp32 a group at a time, rounded once.  The
+ * scales of both matrices are of type `dtype` or fp32; both have zeros or neither has.  MBX_EUNSUPPORTED: fp32 activations, other scales, k = 0.
+ * MBX_ERANGE: more than 2^26 features (so too mbx_quantize_4bit and mbx_dequantize_4bit). */
 int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_k, const void* words, const void* scales, const uint8_t* zeros,
                  const void* words2, const void* scales2, const uint8_t* zeros2, int scale_dtype, int group, void* c, int dtype, const int32_t* bins,
                  int num_groups, int64_t rows, int k, int n, int act, mbx_stream_t stream);

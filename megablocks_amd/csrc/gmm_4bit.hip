@@ -1,5 +1,5 @@
 // Weights in 4 bits with a scale (and a zero point) for every group of 32, 64 or 128 along the reduction: from 16- or 32-bit weights and back,
-// and the choice of the products' kernels (gmm_4bit_rows.hip, gmm_4bit_tile.hip).
+// and the choice of the products' kernels (gmm_4bit_rows.hip, gmm_4bit_tile.hip, gmm_4bit_long.hip).
 //
 // W [E, n, k] is kept in tiles of 16 features x 128 columns, in the order a wave multiplies them: 1 KiB in a row, 16 bytes a lane.  Lane
 // 16 g + f has feature f; its word j has the columns 32 j + 8 g + (0, 2, 4, 6, 1, 3, 5, 7) of the tile, four bits each from the lowest, so that word
@@ -7,7 +7,6 @@
 // scales [E, n / 16, k / group, 16] (zeros alike, a byte each): a code q stands for scale (q - zero), zero 8 without zeros.  n and k are rounded up to
 // whole tiles; what lies past them is never used.
 #include "gmm_4bit.h"
-
 
 namespace mbx {
 namespace {
@@ -102,7 +101,8 @@ struct PackPlace {
 
 // Weights [E, n, k] (TRANSPOSED: [E, k, n]) into words, scales and zeros.  What bounds it: one reading of the weights.  A lane's eight columns of a word
 // are 16 bytes in a row of [n, k]; from [k, n] a workgroup's features go through the LDS.  whole: rows are whole 16-byte pieces at 16-byte addresses; the next
-// block's are then on their way while a block is encoded.
+// block's are then on their way while a block is encoded.  8 x [14336, 4096] in bf16 as [k, n]: 268 us for 1.18 GB read and written (4.4 TB/s, a copy
+// reaches 4.9), back in 215 (5.5 TB/s).
 template <int DT, int GROUP, bool TRANSPOSED, bool ZEROS>
 __global__ void __launch_bounds__(kPackThreads)
 quantize_kernel(const void* __restrict__ weights, const PackPlace place, bool whole, uint32_t* __restrict__ words, void* __restrict__ scales, uint8_t* __restrict__ zeros) {
@@ -372,11 +372,13 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   hipStream_t s = as_stream(stream);
   const Rows4bit g = {a, indices, a_rows, top_k, {{(const uint32_t*)words, scales, zeros}, {(const uint32_t*)words2, scales2, zeros2}}, scale_dtype == MBX_F32,
                       c, bins, num_groups, rows, k, n, act, 0};
-  // By rows an expert in the mean of those that can have some: up to 12, dozens, from 96 on (us, 8 gated experts of [4096, 14336]: 8 rows 93 / 115 with the first
-  // two, 16 rows 143 / 119; with the last two 64 rows 234 / 239, 128 rows 381 / 351, 1024 rows 2516 / 2114; 64 of [2048, 1408]: 3 rows 40 / 46, 15 rows 62 / 48;
-  // 93 rows 140 / 138).  The last one's rows are whole pieces of 16 bytes.
-  const int64_t experts = rows < num_groups ? rows : num_groups;
-  const bool few = rows <= 12 * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 28;
+  // By rows an expert in the mean of those that can have some.  The kernel for few goes over the weights again for every 16 rows and has the shorter way, which
+  // counts where the weights are few.  Us, of the kernels for few / dozens: 8 gated experts of [4096, 14336], 12 rows 95 / 118, 16 rows 135 / 110; 64 of [2048,
+  // 1408], 8 rows 42 / 47, 16 rows 65 / 47; 8 of [14336, 4096] without a gate, 16 rows 78 / 98, 24 rows 95 / 99; 12 of [1032, 2728], 16 rows 16 / 19, 33 rows
+  // 24 / 20.  Of those for dozens / hundreds, whose rows are whole pieces of 16 bytes: the first, 64 rows 234 / 239, 128 rows 381 / 351, 1024 rows 2516 / 2107; the
+  // second, 93 rows 140 / 138.
+  const int64_t experts = rows < num_groups ? rows : num_groups, tiles = pieces_of(n, kTileFeatures) * experts * (words2 ? 2 : 1);
+  const bool few = rows <= (tiles <= 4096 ? 20 : 12) * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 28;
   const int64_t slots = experts + rows / (few ? 16 : many ? 64 : 32);
   return few ? launch_rows_4bit(g, dtype, group, slots, experts, s) : many ? launch_long_4bit(g, dtype, group, slots, s) : launch_tiles_4bit(g, dtype, group, slots, s);
 }

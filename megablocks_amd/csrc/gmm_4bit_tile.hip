@@ -1,13 +1,13 @@
-// Products of some dozens to some hundreds of rows an expert with 4-bit weights.
+// Products of some dozens of rows an expert with 4-bit weights.
 //
-// A workgroup has 32 rows and each of its four waves WT tiles of features of its own (with a second matrix WT / 2 of each), all columns.  The rows' next
-// 128 columns are fetched while the last are multiplied, and shared through the LDS: 256 bytes a row, its 16-byte pieces in the order piece ^ row, so that the
-// 16 rows of a read are 16 different bank groups.  The weights go from memory to the operands as in gmm_4bit_rows.hip, each wave's own.
+// A workgroup has 32 rows and each of its four waves WT tiles of features of its own (with a second matrix WT / 2 of each), all columns.  The rows' columns
+// are fetched three blocks of 128 ahead and shared through the LDS: 256 bytes a row, its 16-byte pieces in the order piece ^ row, so that the 16 rows of a
+// read are 16 different bank groups.  The weights go from memory to the operands as in gmm_4bit_rows.hip, each wave's own.  What 16 + q is off by is taken off
+// at the start: sums of the next block's rows, made by two of the waves, are what its products are added to.
 //
-// What bounds it: the instructions that make operands of the codes and sums of the groups, 240 of 350 in a block of 128 columns with four tiles, next to 40
-// matrix instructions.  Us (and TFLOP/s) of the first products of 8 gated experts of [4096, 14336], by rows an expert: 16: 119, 32: 150, 64: 257 (470), 128: 421,
-// 256: 772 (620); the values in 16 bits and the grouped kernels 1380 - 1510.  With 64 rows a workgroup, and with waves of 8 in it, the waves that are
-// left on a unit cover each other's waits no better (256 rows: 809, 766 - 875).
+// What bounds it: the instructions that make operands of the codes, two for two weights, as many as the matrix instructions can hide or more, and a barrier a
+// block.  Us (and TFLOP/s) of the first products of 8 gated experts of [4096, 14336], by rows an expert: 16: 110, 32: 138 (437), 64: 234 (514), 96: 305;
+// 128: 381, 256: 698 (689).  With the sums made by every wave for itself, 40 matrix instructions a block in place of 32: 150 (32 rows), 469 (128).
 #include "gmm_4bit.h"
 
 namespace mbx {
@@ -142,8 +142,8 @@ void launch(const Rows4bit& g, int64_t slots, hipStream_t s) {
   });
 }
 
-// Four tiles a wave where that leaves six workgroups a compute unit (us, two / four: 8 gated experts of [4096, 14336], 32 rows, 1792 workgroups 158 / 150, 256 rows
-// 840 / 772; 64 of [2048, 1408], 65 rows, 1177: 116 / 123; 8 of [14336, 4096], 256 rows, 1152: 415 / 426, 16 rows, 192: 71 / 111)
+// Four tiles a wave where that leaves six workgroups a compute unit (us, two / four: 8 gated experts of [4096, 14336], 16 rows, 1344 workgroups 110 / 120, 32 rows,
+// 1792, 155 / 138; 64 of [2048, 1408], 31 rows, 1386: 64 / 63, 65 rows, 2134: 129 / 117; 8 of [14336, 4096] without a gate, 64 rows, 384: 143 / 170)
 template <int DT, bool TWO, int GROUP>
 void choose(const Rows4bit& g, int64_t slots, hipStream_t s) {
   if (pieces_of(g.n, 64 * (TWO ? 2 : 4)) * slots >= 1536) launch<DT, 4, TWO, GROUP>(g, slots, s);
