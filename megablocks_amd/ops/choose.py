@@ -1,5 +1,6 @@
 """The choice of experts by softmax or sigmoid scores, with a balance bias and by groups, and the update of that bias.  The reference has neither (its
 router is softmax and top-k, megablocks/layers/router.py:87-106)."""
+import bisect
 import ctypes
 import math
 from typing import Any, Optional
@@ -151,10 +152,25 @@ def choose(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, s
     return run(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse)
 
 
+_is_contiguous, _get_device, _data_ptr = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.data_ptr
+
+
+def _check_outputs(outputs, biases, size):
+    """ValueError where layers, which are computed side by side, have outputs that overlap, or one lies over another's bias."""
+    order = sorted(outputs)
+    clash = any(after - before < size for before, after in zip(order, order[1:]))
+    if outputs != biases and not clash:
+        for l, at in enumerate(biases):
+            near = bisect.bisect_left(order, at - size + 1)
+            clash = clash or any(o < at + size and (o, o) != (at, outputs[l]) for o in order[near:near + 2])
+    if clash:
+        raise ValueError('balance_bias: two layers have outputs, or an output and a bias, in the same place; rows of counts for one bias go into one entry')
+
+
 def balance_bias(biases, tokens_per_expert, rate: float, out=None):
     """bias + rate * sign(mean - n) for every layer's bias (fp32 [experts]) and n, its tokens per expert (int32, [experts] or rows of that, which are added
     up): experts with fewer tokens than the mean are made likelier, those with more less likely.  biases, tokens_per_expert, out: lists of one tensor a
-    layer, all of one number of experts; out (a list of fp32 vectors, which may be the biases themselves; no two of them the same) or None for new ones.
+    layer, all of one number of experts; out (a list of fp32 vectors, which may be the biases themselves, else in no layer's way) or None for new ones.
     Returns the list.  One launch for up to 64 layers."""
     layers = len(biases)
     if len(tokens_per_expert) != layers or (out is not None and len(out) != layers):
@@ -168,42 +184,40 @@ def balance_bias(biases, tokens_per_expert, rate: float, out=None):
     if len(shape) != 1 or shape[0] == 0:
         raise ValueError('balance_bias: a bias must be a vector of a number for every expert')
     experts = shape[0]
-    rows, b_ptrs, n_ptrs, kept, wrong = [1] * layers, [0] * layers, [0] * layers, [], None     # kept: copies the launch reads
-    for l in range(layers):
-        b, n = biases[l], tokens_per_expert[l]
-        if b.shape != shape:
+    # a property of all tensors at a time: 32 layers cost the host 0.2 us a step each, a layer's steps one after the other twice that
+    given = (*biases, *tokens_per_expert) if out is None else (*biases, *tokens_per_expert, *out)
+    shapes, rows = [t.shape for t in given], [1] * layers
+    if shapes.count(shape) < len(given):
+        if any(s != shape for s in shapes[:layers]):
             raise ValueError('balance_bias: all biases must be vectors of the same number of experts')
-        if n.shape != shape:
-            if n.ndim != 2 or n.shape[1] != experts:
-                raise ValueError('balance_bias: tokens per expert must be [experts] or [rows, experts]')
-            rows[l] = n.shape[0]
-        if b.dtype != torch.float32 or n.dtype != torch.int32 or b.get_device() != index or n.get_device() != index or index < 0:
-            wrong = f'expected float32 biases and int32 tokens per expert on one GPU but got {b.dtype}, {n.dtype} on {b.device}, {n.device}'
-        if not b.is_contiguous():
-            kept.append(b.detach().contiguous())
-            b = kept[-1]
-        if not n.is_contiguous():
-            kept.append(n.contiguous())
-            n = kept[-1]
-        b_ptrs[l], n_ptrs[l] = b.data_ptr(), n.data_ptr()
-    for t in () if out is None else out:
-        if t.shape != shape or not t.is_contiguous():
+        for l, s in enumerate(shapes[layers:2 * layers]):
+            if s != shape:
+                if len(s) != 2 or s[1] != experts:
+                    raise ValueError('balance_bias: tokens per expert must be [experts] or [rows, experts]')
+                rows[l] = s[0]
+        if any(s != shape for s in shapes[2 * layers:]):
             raise ValueError('balance_bias: outputs must be contiguous vectors of a number for every expert')
-        if t.dtype != torch.float32 or t.get_device() != index:
-            wrong = f'expected float32 outputs on the device of the biases but got {t.dtype} on {t.device}'
-    if wrong is not None:
-        raise RuntimeError(f'balance_bias: {wrong}')
+    contiguous = list(map(_is_contiguous, given))
+    if not all(contiguous[2 * layers:]):
+        raise ValueError('balance_bias: outputs must be contiguous vectors of a number for every expert')
+    dtypes = [t.dtype for t in given]
+    if set(map(_get_device, given)) != {index} or index < 0 or dtypes.count(torch.float32) != len(given) - layers or dtypes.count(torch.int32) != layers or \
+            dtypes[layers:2 * layers].count(torch.int32) != layers:
+        raise RuntimeError('balance_bias: expected float32 biases (and outputs) and int32 tokens per expert on one GPU but got '
+                           f'{sorted({f"{t.dtype} on {t.device}" for t in given})}')
+    if not all(contiguous):
+        given = [t if c else t.detach().contiguous() for t, c in zip(given, contiguous)]       # kept until the launch is under way
+    pointers = list(map(_data_ptr, given))
+    b_ptrs, n_ptrs, o_ptrs = pointers[:layers], pointers[layers:2 * layers], pointers[2 * layers:]
     if out is None:
         made = torch.empty((layers, experts), dtype=torch.float32, device=first.device)
         start = made.data_ptr()
         out, o_ptrs = list(made.unbind(0)), range(start, start + 4 * layers * experts, 4 * experts)
     else:
-        o_ptrs = [t.data_ptr() for t in out]
-        if len(set(o_ptrs)) < layers:
-            raise ValueError('balance_bias: two layers have the same output; pass the rows of their tokens per expert as one')
+        _check_outputs(o_ptrs, b_ptrs, 4 * experts)
         torch.autograd.graph.increment_version(out)
-    pointers = ctypes.c_void_p * layers
+    addresses = ctypes.c_void_p * layers
     with _lib.device_of(first):
-        rc = lib.mbx_balance_bias(pointers(*b_ptrs), pointers(*n_ptrs), (ctypes.c_int * layers)(*rows), pointers(*o_ptrs), layers, experts, float(rate), _lib.stream())
+        rc = lib.mbx_balance_bias(addresses(*b_ptrs), addresses(*n_ptrs), (ctypes.c_int * layers)(*rows), addresses(*o_ptrs), layers, experts, float(rate), _lib.stream())
     _lib.check(rc, 'balance_bias')
     return out

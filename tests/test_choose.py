@@ -82,3 +82,12 @@ def test_the_restatement_orders_and_differentiates():
                 d = torch.zeros_like(x)
                 d[t, e] = 1e-6
                 assert abs(float((loss(x + d) - loss(x - d)) / 2e-6) - float(got[t, e])) < 1e-7
+
+
+def test_outputs_of_layers_in_each_others_way():
+    from megablocks_amd.ops import choose
+    for outputs, biases in (([64, 128], [64, 128]), ([0, 64, 128], [256, 320, 384]), ([0], [0]), ([64, 192], [64, 128]), ([0, 64], [200, 264])):
+        choose._check_outputs(outputs, biases, 64)
+    for outputs, biases in (([64, 64], [64, 64]), ([64, 100], [64, 100]), ([128, 64], [64, 128]), ([0, 64], [64, 256]), ([0, 64], [256, 127]), ([32], [0]), ([0], [63])):
+        with pytest.raises(ValueError):
+            choose._check_outputs(outputs, biases, 64)
