@@ -378,7 +378,7 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   // 24 / 20.  Of those for dozens / hundreds, whose rows are whole pieces of 16 bytes: the first, 64 rows 234 / 239, 128 rows 381 / 351, 1024 rows 2516 / 2107; the
   // second, 93 rows 140 / 138.
   const int64_t experts = rows < num_groups ? rows : num_groups, tiles = pieces_of(n, kTileFeatures) * experts * (words2 ? 2 : 1);
-  const bool few = rows <= (tiles <= 4096 ? 20 : 12) * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 28;
+  const bool few = rows <= (tiles <= 4096 ? 20 : 12) * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 27;
   const int64_t slots = experts + rows / (few ? 16 : many ? 64 : 32);
   return few ? launch_rows_4bit(g, dtype, group, slots, experts, s) : many ? launch_long_4bit(g, dtype, group, slots, s) : launch_tiles_4bit(g, dtype, group, slots, s);
 }
