@@ -375,8 +375,8 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   // By rows an expert in the mean of those that can have some.  The kernel for few goes over the weights again for every 16 rows and has the shorter way, which
   // counts where the weights are few.  Us, of the kernels for few / dozens: 8 gated experts of [4096, 14336], 12 rows 95 / 118, 16 rows 135 / 110; 64 of [2048,
   // 1408], 8 rows 42 / 47, 16 rows 65 / 47; 8 of [14336, 4096] without a gate, 16 rows 78 / 98, 24 rows 95 / 99; 12 of [1032, 2728], 16 rows 16 / 19, 33 rows
-  // 24 / 20.  Of those for dozens / hundreds, whose rows are whole pieces of 16 bytes: the first, 64 rows 234 / 239, 128 rows 381 / 351, 1024 rows 2516 / 2107; the
-  // second, 93 rows 140 / 138.
+  // 24 / 20.  Of those for dozens / hundreds, whose rows are whole pieces of 16 bytes: the first, 64 rows 234 / 239, 128 rows 381 / 345, 1024 rows 2516 / 2030; the
+  // second, 93 rows 140 / 138, 384 rows 477 / 405.
   const int64_t experts = rows < num_groups ? rows : num_groups, tiles = pieces_of(n, kTileFeatures) * experts * (words2 ? 2 : 1);
   const bool few = rows <= (tiles <= 4096 ? 20 : 12) * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 27;
   const int64_t slots = experts + rows / (few ? 16 : many ? 64 : 32);

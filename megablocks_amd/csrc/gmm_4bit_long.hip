@@ -1,16 +1,17 @@
 // Products of hundreds to thousands of rows an expert with 4-bit weights.
 //
 // A workgroup has 64 rows, four waves with 64 features each (with a second matrix 32 of each), all columns; rows, weights and the start of the sums as in
-// gmm_4bit_tile.hip.  A wave goes over its block of 128 columns a unit at a time, a group of columns of one tile of features: 4 to 16 matrix instructions, and
-// next to each, in this order, two instructions of making the next operand of codes and one or two that scale and add up the unit before.  The rows of a
-// block are read from the LDS once, into the registers that the block before leaves with its last tile of features, and a tile's words are loaded
-// where its last operand has been made, three quarters of a block ahead.  That is the 256 registers there are for two waves on a SIMD.
+// gmm_4bit_tile.hip.  A wave multiplies by 32 x 32 x 16: a step of 16 columns is four matrix instructions, and next to each, in this order, a quarter of the
+// next step's operands is made of the codes; a group's sums are scaled and added up (64 instructions) while the next group's start is on its way.  A lane's
+// words of half a block are loaded half a block ahead, rows three blocks.  That is the 256 registers there are for two waves on a SIMD; where the rows are
+// is kept in the LDS for that.
 //
-// What bounds it: a SIMD issues one vector instruction in 4 cycles, a matrix instruction of 16 x 16 x 32 takes two such places (measured: 16 cycles alone, 9 ns
-// with three others, 12 ns with five): 70 of them and 297 others a block are 437 places, of which 80 % are used.  First products of 8 gated experts of
-// [4096, 14336], 256 / 512 / 1024 rows an expert: 623 / 1121 / 2107 us (772 / 858 / 913 TFLOP/s); values made in 16 bits and multiplied by the grouped kernels
-// 1380 / 1799 / 2016, each weight rounded on the way.  128 rows a workgroup and one wave a SIMD with all 512 registers: 2245, its instructions one after the other.
-// Groups of 32, 512 rows of 8 experts of [14336, 4096]: 827 us (582 TFLOP/s): four times the sums.
+// What bounds it: a SIMD issues a vector instruction every 4 cycles, and next to them a matrix instruction of 32 x 32 x 16 costs 2.4 such places, one of
+// 16 x 16 x 32, half the work, 2 (measured); 36 of them and some 260 others a block are 350 places, and at this rate the clock is down to 2.0 GHz.
+// First products of 8 gated experts of [4096, 14336], 128 / 256 / 512 / 1024 rows an expert: 345 / 608 / 1088 / 2030 us (698 / 792 / 885 / 948 TFLOP/s); by
+// 16 x 16 x 32 351 / 623 / 1121 / 2107; 128 rows a workgroup with one wave a SIMD and all 512 registers 2245; values made in 16 bits, which rounds each weight,
+// and multiplied by the grouped kernels 2016 for 1024 rows.  Workgroups of an XCD by 16 tiles of rows and a few features 2001, but 64 experts of [2048, 1408],
+// whose features do not divide by the XCDs, 405 -> 493.  Groups of 32, 512 rows of 8 experts of [14336, 4096]: 767 us (627 TFLOP/s): four times the sums.
 #include "gmm_4bit.h"
 
 namespace mbx {
