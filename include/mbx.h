@@ -518,7 +518,8 @@ int mbx_dequantize_4bit(const void* words, const void* scales, const uint8_t* ze
  * bins[e]) for expert e: the experts' products, for a token's few rows (where reading the weights is what takes the time) to thousands.  Rows of X: a's (indices NULL), or
  * a[indices[r] / top_k] of a's a_rows rows.  16-bit activations, fp32 sums of the rows with the codes, scaled in fp32 a group at a time, rounded once.  The
  * scales of both matrices are of type `dtype` or fp32; both have zeros or neither has.  MBX_EUNSUPPORTED: fp32 activations, other scales, k = 0.
- * MBX_ERANGE: more than 2^26 features (so too mbx_quantize_4bit and mbx_dequantize_4bit). */
+ * MBX_ERANGE: more than 2^31 - 65 rows or
+ * 2^26 features (the latter of mbx_quantize_4bit and mbx_dequantize_4bit too). */
 int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_k, const void* words, const void* scales, const uint8_t* zeros,
                  const void* words2, const void* scales2, const uint8_t* zeros2, int scale_dtype, int group, void* c, int dtype, const int32_t* bins,
                  int num_groups, int64_t rows, int k, int n, int act, mbx_stream_t stream);

@@ -365,7 +365,7 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   if (indices && (top_k <= 0 || a_rows < 0)) return MBX_EINVAL;
   if (words2 && (act < 0 || !zeros != !zeros2)) return MBX_EINVAL;
   if (dtype == MBX_F32 || (scale_dtype != dtype && scale_dtype != MBX_F32) || k == 0) return MBX_EUNSUPPORTED;
-  if (rows > 0x7fffffff || n > kMostFeatures || k > 0x7fffffff - 256) return MBX_ERANGE;
+  if (rows > 0x7fffffff - 64 || n > kMostFeatures || k > 0x7fffffff - 256) return MBX_ERANGE;
   if (rows == 0 || n == 0 || num_groups == 0) return 0;
   if (!a || !words || !scales || !c || !bins || (words2 && !scales2) || (indices && a_rows == 0)) return MBX_EINVAL;
   if (((uintptr_t)words | (uintptr_t)words2) & 15) return MBX_EINVAL;

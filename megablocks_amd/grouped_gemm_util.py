@@ -851,7 +851,8 @@ def _operand_4bit(a, weights, batch_sizes, bins, what):
         raise RuntimeError(f'{what}: expected bfloat16 or float16 rows but got {x.dtype}')
     if first.scales.dtype not in (x.dtype, torch.float32):
         raise RuntimeError(f'{what}: the scales must be {x.dtype}, as the rows, or float32, not {first.scales.dtype}')
-    if torch.is_grad_enabled() and x.requires_grad:
+    if (torch.is_grad_enabled() and x.requires_grad) or \
+            (getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0 and torch.autograd.forward_ad.unpack_dual(x).tangent is not None):
         raise RuntimeError(f'{what}: products with 4-bit weights have no gradient; call them under torch.no_grad()')
     if src is None:
         rows = x.shape[0]
@@ -864,6 +865,8 @@ def _operand_4bit(a, weights, batch_sizes, bins, what):
             rows, bins = src.rows, src.bins
             if src.indices.ndim != 1 or src.indices.dtype != torch.int32 or src.indices.shape[0] != x.shape[0] * src.top_k or rows != src.indices.shape[0]:
                 raise ValueError(f'{what}: one int32 assignment per token and top_k choice')
+            if src.indices.device != x.device:
+                raise RuntimeError(f'{what}: expected the assignments on {x.device} but got them on {src.indices.device}')
     if bins.ndim != 1 or bins.shape[0] != first.experts or bins.dtype != torch.int32 or bins.device != x.device:
         raise ValueError(f'{what}: the bins must be int32, one for each of the {first.experts} experts')
     return x.contiguous(), src, bins.contiguous(), rows

@@ -61,4 +61,4 @@ class Grouped4bitExperts(torch.nn.Module):
 
     def forward_tokens(self, src, tokens_per_expert):
         """forward on the rows of the tokens that `src` (a `gg.GatheredRows`) describes."""
-        return gg.gmm_4bit(gg.gmm_4bit_act(src, self.w1, self.act, b2=self.v1), self.w2, bins=src.bins)
+        return gg.gmm_4bit(gg.gmm_4bit_act(src, self.w1, self.act, b2=self.v1), self.w2, bins=src.bins if src.padded_bins is None else src.padded_bins)

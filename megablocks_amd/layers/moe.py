@@ -44,13 +44,18 @@ def clear_expert_loads():
 
 def update_balance_biases(args: Arguments):
     """Moves the balance biases of all layers that ran in training since the last call by moe_router_bias_rate: up for experts that got fewer tokens than the
-    mean, down for those that got more (ops.balance_bias; one launch for 64 layers).  Called once a step, after the backward; the forwards of a step
-    that accumulates gradients are added up."""
+    mean, down for those that got more (ops.balance_bias; one launch for 64 layers of a device).  Called once a step, after the backward; the forwards of a step
+    that accumulates gradients are added up.  Ranks that train on parts of a batch add up the counts of `get_expert_loads` between them first.  A step that
+    is captured into a graph has the update in the capture: a replay saves no loads."""
     by_bias = {}
     for bias, tokens_per_expert in get_expert_loads():
         by_bias.setdefault(id(bias), (bias, []))[1].append(tokens_per_expert)
-    biases = [bias for bias, _ in by_bias.values()]
-    ops.balance_bias(biases, [loads[0] if len(loads) == 1 else torch.stack(loads) for _, loads in by_bias.values()], args.moe_router_bias_rate, out=biases)
+    alike = {}     # layers of one device and number of experts
+    for bias, loads in by_bias.values():
+        alike.setdefault((bias.device, bias.shape), []).append((bias, loads[0] if len(loads) == 1 else torch.stack(loads)))
+    for layers in alike.values():
+        biases, loads = map(list, zip(*layers))
+        ops.balance_bias(biases, loads, args.moe_router_bias_rate, out=biases)
     clear_expert_loads()
 
 

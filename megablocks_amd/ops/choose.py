@@ -148,7 +148,9 @@ def choose(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, s
             raise RuntimeError(f'choose_experts: expected a float32 bias on {logits.device} but got {bias.dtype} on {bias.device}')
         bias = bias.detach().contiguous()
     logits = logits.contiguous()
-    run = ChooseExpertsOp.apply if logits.requires_grad and torch.is_grad_enabled() else _launch    # a node of its own is 7 us of the host's time
+    # a node of its own is 7 us of the host's time; one in forward differentiation says that it has none
+    recorded = (logits.requires_grad and torch.is_grad_enabled()) or getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0
+    run = ChooseExpertsOp.apply if recorded else _launch
     return run(logits, bias, top_k, score, groups, top_groups, group_best, norm_p, scale, want_int32, want_lse)
 
 

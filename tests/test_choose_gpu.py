@@ -229,6 +229,14 @@ def test_more_tokens_than_a_launch():
     assert bool((own == own[0]).all()) and own[0] > 0 and int((x.grad != 0).sum()) == tokens
 
 
+def test_no_derivative_forward():
+    x = torch.randn(3, 8, device='cuda')
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError):
+            ops.choose_experts(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), 2)
+        assert torch.equal(ops.choose_experts(x, 2)[1], ops.choose_experts(x.clone(), 2)[1])
+
+
 def test_strides_types_and_no_tokens():
     g = torch.Generator().manual_seed(2)
     wide = torch.randn(37, 80, generator=g)

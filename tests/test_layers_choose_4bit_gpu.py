@@ -111,6 +111,36 @@ def test_balance_over_steps():
     assert moe_layers.get_expert_loads() == []          # evaluation counts nothing
 
 
+def test_layers_of_different_numbers_of_experts_are_balanced_together():
+    torch.manual_seed(2)
+    layers = [dMoE(_args(moe_router_score='sigmoid', moe_router_bias=True, moe_router_bias_rate=0.01, moe_num_experts=e)) for e in (16, 8, 16)]
+    moe_layers.clear_expert_loads()
+    out = torch.randn(100, 1, 256, device='cuda').bfloat16().requires_grad_()
+    for layer in layers:
+        out = layer(out)
+    loads = [(b, n.clone()) for b, n in moe_layers.get_expert_loads()]
+    moe_layers.update_balance_biases(layers[0].router.args)
+    assert [b.numel() for b, _ in loads] == [16, 8, 16] and moe_layers.get_expert_loads() == []
+    for b, n in loads:
+        assert torch.allclose(b, 0.01 * torch.sign(n.sum() - n.numel() * n).float(), atol=1e-8)
+
+
+def test_4_bit_experts_of_padded_rows():
+    """Gathered rows that are padded for each expert, as the block-sparse layer has them: both products by the padded bins."""
+    _, kept = _quantized(_args(moe_num_experts=3, moe_top_k=1), 64, False)
+    mlp = kept.experts.mlp
+    x = torch.randn(9, 256, device='cuda').bfloat16()
+    ids = torch.tensor([2, 0, 0, 2, 2, 1, 0, 2, 2], device='cuda')
+    bin_ids, indices = ids.sort(stable=True)
+    bins = torch.bincount(ids, minlength=3).cumsum(0).int()
+    padded = torch.tensor([16, 32, 48], dtype=torch.int32, device='cuda')
+    with torch.no_grad():
+        out = mlp.forward_tokens(gg.GatheredRows(x, indices.int(), bin_ids.int(), bins, padded, 1, 48), None)
+        want = mlp(x[indices], torch.bincount(ids, minlength=3))
+    at = torch.cat([torch.arange(3), 16 + torch.arange(1), 32 + torch.arange(5)])
+    assert out.shape == (48, 256) and torch.equal(out[at.cuda()], want) and int((out != 0).any(1).sum()) == 9
+
+
 def test_other_scores_leave_auxiliary_losses_and_checkpoints_alone():
     """z-loss and load-balancing loss with sigmoid scores; a copy through a state_dict routes alike."""
     torch.manual_seed(2)

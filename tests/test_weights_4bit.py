@@ -84,6 +84,7 @@ def test_entry_points_refuse_without_touching_the_gpu():
     for unsupported in (dict(dtype=2), dict(scale_dtype=1), dict(k=0)):
         assert gmm(**unsupported) == _lib.EUNSUPPORTED
     assert gmm(rows=0) == gmm(n=0) == gmm(groups=0) == 0 and gmm(rows=1 << 31) == _lib.ERANGE
+    assert gmm(rows=(1 << 31) - 64) == gmm(n=(1 << 26) + 1) == _lib.ERANGE
     assert lib.mbx_quantize_4bit(None, 0, 1, 4, 4, _lib.TN, 32, None, None, None, None) == _lib.EINVAL
     assert lib.mbx_quantize_4bit(None, 0, 1, 4, 4, _lib.NT, 31, None, None, None, None) == _lib.EINVAL
     assert lib.mbx_quantize_4bit(None, 0, 1, 4, 4, _lib.NT, 32, None, None, None, None) == _lib.EINVAL

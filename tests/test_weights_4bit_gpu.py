@@ -191,6 +191,23 @@ def test_more_tiles_of_rows_than_a_grid():
     assert int((got != 0).any(1).sum()) == len(at)
 
 
+def test_what_is_refused():
+    kept, *_ = _weights(2, 16, 128, 128, False, BF16, 5)
+    x, bins, indices = torch.randn(4, 128, device='cuda').bfloat16(), torch.tensor([1, 4], dtype=torch.int32, device='cuda'), torch.arange(4, dtype=torch.int32, device='cuda')
+    src = lambda indices, rows=4: gg.GatheredRows(x, indices, indices, bins, None, 1, rows)
+    assert torch.equal(gg.gmm_4bit(src(indices), kept), gg.gmm_4bit(x, kept, bins=bins))
+    with pytest.raises(RuntimeError):
+        gg.gmm_4bit(src(indices.cpu()), kept)               # assignments on the host
+    for bad in (src(indices.long()), src(indices[:3]), src(indices, 5)):
+        with pytest.raises(ValueError):
+            gg.gmm_4bit(bad, kept)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError):
+            gg.gmm_4bit(dual, kept, bins=bins)              # no derivative forward either
+        assert torch.equal(gg.gmm_4bit(x, kept, bins=bins), gg.gmm_4bit(src(indices), kept))
+
+
 def test_strides_streams_and_captures():
     kept, *_ = _weights(4, 48, 200, 64, True, F16, 6)
     wide = torch.randn(30, 256, device='cuda').half()
