@@ -504,8 +504,8 @@ int mbx_loss_gradient(const float* grad, const void* values, int dtype, const in
  * A code q stands for scale * (q - zero).  Features and columns past n and k are never used.
  *
  * mbx_quantize_4bit: from weights [num_experts, n, k] (layout MBX_NT, as w1 and v1 are kept) or [num_experts, k, n] (MBX_NN, as w2 is); scales in the weights'
- * type.  Without zeros scale = round(max|w| / 7), q = clamp(rint(w / scale), -8, 7) + 8; with zeros, of low = min(w, 0) and high = max(w, 0),
- * scale = round((high - low) / 15), zero = clamp(rint(-low / scale), 0, 15), q = clamp(rint(w / scale) + zero, 0, 15).  Quotients are taken exactly, halves
+ * type.  Without zeros scale = round(max|w| * (1 / 7)), reciprocal and product in fp32, q = clamp(rint(w / scale), -8, 7) + 8; with zeros, of low = min(w, 0)
+ * and high = max(w, 0), scale = round((high - low) * (1 / 15)), zero = clamp(rint(-low / scale), 0, 15), q = clamp(rint(w / scale) + zero, 0, 15).  Quotients are taken exactly, halves
  * go to even.  A group of zeros has scale 0, as one whose
  * scale would be below 2^-126; one with a number that is not finite scale NaN.
  * mbx_dequantize_4bit: the values, rounded to `dtype`, in either layout. */

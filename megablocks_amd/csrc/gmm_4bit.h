@@ -164,7 +164,8 @@ struct Weights4bit {
     uint32_t scale[WT], zero[WT];   // as they are in memory: nothing waits for a load before the block is multiplied
   };
   wave_ptr words_at[WT], scales_at[WT], zeros_at[WT];
-  uint32_t word_lane, scale_lane;
+  uint32_t word_lane, scale_lane, scale_at, half_up, half_mask;
+  int scale_shift;
   bool wide, with_zeros;
 
   __device__ __forceinline__ Weights4bit(const Rows4bit& g, int expert, int tile0, int tiles, int blocks) {
@@ -182,6 +183,12 @@ struct Weights4bit {
     scale_lane = (uint32_t)lane_id() % (kGroups * 16);
     wide = g.wide_scales;
     with_zeros = zeros_at[0] != nullptr;
+    // The piece of 4 bytes with the lane's scale, one load whatever the type (of two in branches the second waits for the first); as 16 bits the lane's half
+    // is shifted up and the other cut off
+    scale_shift = wide ? 2 : 1;
+    scale_at = scale_lane << scale_shift & ~3u;
+    half_up = wide || scale_lane % 2 ? 0 : 16;
+    half_mask = wide ? ~0u : 0xffff0000u;
   }
 
   // ONCE: read by nobody else, kept out of the caches (60 MiB of weights read alone: 9.7 us, with plain loads 10.9; 480 MiB: 69, 78)
@@ -192,13 +199,8 @@ struct Weights4bit {
     else to.words[t] = *at;
   }
   __device__ __forceinline__ void fetch_scales(Block& to, int b) const {
-    if (wide) {
 #pragma unroll
-      for (int t = 0; t < WT; ++t) to.scale[t] = load_at<uint32_t>(scales_at[t], (int64_t)b * (kGroups * 64), scale_lane * 4);
-    } else {
-#pragma unroll
-      for (int t = 0; t < WT; ++t) to.scale[t] = load_at<uint16_t>(scales_at[t], (int64_t)b * (kGroups * 32), scale_lane * 2);
-    }
+    for (int t = 0; t < WT; ++t) to.scale[t] = load_at<uint32_t>(scales_at[t], (int64_t)b * (kGroups * 16) << scale_shift, scale_at);
     if (with_zeros) {
 #pragma unroll
       for (int t = 0; t < WT; ++t) to.zero[t] = load_at<uint8_t>(zeros_at[t], (int64_t)b * (kGroups * 16), scale_lane);
@@ -213,7 +215,9 @@ struct Weights4bit {
 
   // scale and -(16 + zero) of the lane's feature for each group
   __device__ __forceinline__ void scales(const Block& of, int t, uint32_t (&scale)[kGroups], uint32_t (&off)[kGroups]) const {
-    const float s = wide ? __uint_as_float(of.scale[t]) : Elem<DT>::to_f32(__builtin_bit_cast(typename Elem<DT>::type, (uint16_t)of.scale[t]));
+    const uint32_t raw = (of.scale[t] << half_up) & half_mask;
+    float s = __uint_as_float(raw);
+    if constexpr (DT == MBX_F16) s = wide ? s : Elem<DT>::to_f32(__builtin_bit_cast(typename Elem<DT>::type, (uint16_t)(raw >> 16)));
     spread<kGroups>(__float_as_uint(s), scale);
     spread<kGroups>(__float_as_uint(with_zeros ? -16.f - (float)of.zero[t] : -24.f), off);
   }

@@ -66,7 +66,9 @@ __device__ __forceinline__ void encode(const float (&w)[4][8], u32x4_t& words, f
     };
     high = over(high, [](float a, float b) { return fmaxf(a, b); });
     if constexpr (ZEROS) low = over(low, [](float a, float b) { return fminf(a, b); });
-    float s = as_type<DT>(ZEROS ? (high - low) / 15.f : high / 7.f);
+    float s = ZEROS ? (high - low) * (1.f / 15.f) : high * (1.f / 7.f);     // by the reciprocal in 32 bits, as torch divides by a number
+    asm("" : "+v"(s));                            // rounded there: a product and a rounding to fp16 in one instruction are rounded once
+    s = as_type<DT>(s);
     if (s < 0x1p-126f) s = 0.f;                   // no normal number of 32 bits: its inverse may be none
     if (bad || !(s < INFINITY)) s = NAN;
     const bool usable = s > 0.f;
@@ -373,9 +375,9 @@ int mbx_gmm_4bit(const void* a, int64_t a_rows, const int32_t* indices, int top_
   const Rows4bit g = {a, indices, a_rows, top_k, {{(const uint32_t*)words, scales, zeros}, {(const uint32_t*)words2, scales2, zeros2}}, scale_dtype == MBX_F32,
                       c, bins, num_groups, rows, k, n, act, 0};
   // By rows an expert in the mean of those that can have some.  The kernel for few goes over the weights again for every 16 rows and has the shorter way, which
-  // counts where the weights are few.  Us, of the kernels for few / dozens: 8 gated experts of [4096, 14336], 12 rows 95 / 118, 16 rows 135 / 110; 64 of [2048,
-  // 1408], 8 rows 42 / 47, 16 rows 65 / 47; 8 of [14336, 4096] without a gate, 16 rows 78 / 98, 24 rows 95 / 99; 12 of [1032, 2728], 16 rows 16 / 19, 33 rows
-  // 24 / 20.  Of those for dozens / hundreds, whose rows are whole pieces of 16 bytes: the first, 64 rows 234 / 239, 128 rows 381 / 345, 1024 rows 2516 / 2030; the
+  // counts where the weights are few.  Us, of the kernels for few / dozens: 8 gated experts of [4096, 14336], 12 rows 93 / 112, 16 rows 135 / 100; 64 of [2048,
+  // 1408], 8 rows 42 / 47, 16 rows 65 / 48; 8 of [14336, 4096] without a gate, 16 rows 75 / 98, 24 rows 95 / 81; 12 of [1032, 2728], 16 rows 16 / 19, 33 rows
+  // 24 / 20.  Of those for dozens / hundreds, whose rows are whole pieces of 16 bytes: the first, 64 rows 230 / 239, 128 rows 381 / 345, 1024 rows 2516 / 2030; the
   // second, 93 rows 140 / 138, 384 rows 477 / 405.
   const int64_t experts = rows < num_groups ? rows : num_groups, tiles = pieces_of(n, kTileFeatures) * experts * (words2 ? 2 : 1);
   const bool few = rows <= (tiles <= 4096 ? 20 : 12) * experts, many = rows >= 96 * experts && k % 8 == 0 && k <= 1 << 27;

@@ -6,7 +6,7 @@
 // at the start: sums of the next block's rows, made by two of the waves, are what its products are added to.
 //
 // What bounds it: the instructions that make operands of the codes, two for two weights, as many as the matrix instructions can hide or more, and a barrier a
-// block.  Us (and TFLOP/s) of the first products of 8 gated experts of [4096, 14336], by rows an expert: 16: 110, 32: 138 (437), 64: 234 (514), 96: 305;
+// block.  Us (and TFLOP/s) of the first products of 8 gated experts of [4096, 14336], by rows an expert: 16: 100, 32: 131 (460), 64: 230 (522), 96: 305;
 // 128: 381, 256: 698 (689).  With the sums made by every wave for itself, 40 matrix instructions a block in place of 32: 150 (32 rows), 469 (128).
 #include "gmm_4bit.h"
 
@@ -70,6 +70,7 @@ tile_4bit_kernel(const Rows4bit g) {
   if (blocks > 2) fetch_rows(2);
   __syncthreads();
   sum_up(0, 0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);     // all loads: the loop's waits are then for its own alone
   int buffer = 0;
   for (int b = 0; b < blocks; ++b) {
     const auto now = next;
@@ -143,7 +144,7 @@ void launch(const Rows4bit& g, int64_t slots, hipStream_t s) {
 }
 
 // Four tiles a wave where that leaves six workgroups a compute unit (us, two / four: 8 gated experts of [4096, 14336], 16 rows, 1344 workgroups 110 / 120, 32 rows,
-// 1792, 155 / 138; 64 of [2048, 1408], 31 rows, 1386: 64 / 63, 65 rows, 2134: 129 / 117; 8 of [14336, 4096] without a gate, 64 rows, 384: 143 / 170)
+// 1792, 155 / 138 (each some 5 % shorter since); 64 of [2048, 1408], 31 rows, 1386: 64 / 63, 65 rows, 2134: 129 / 117; 8 of [14336, 4096] without a gate, 64 rows, 384: 143 / 170)
 template <int DT, bool TWO, int GROUP>
 void choose(const Rows4bit& g, int64_t slots, hipStream_t s) {
   if (pieces_of(g.n, 64 * (TWO ? 2 : 4)) * slots >= 1536) launch<DT, 4, TWO, GROUP>(g, slots, s);

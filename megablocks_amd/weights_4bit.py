@@ -67,7 +67,7 @@ class Weights4bit:
 
 def quantize_4bit(w: torch.Tensor, group_size: int = 128, trans_b: bool = True, zero_points: bool = False) -> Weights4bit:
     """Weights w [experts, n, k] (trans_b False: [experts, k, n]) in 4 bits, for products x @ w[e]^T (x @ w[e]), with a scale in w's type for every
-    group_size (32, 64, 128) of the k columns: the largest weight of a group by 7, or with zero_points the distance of its largest and smallest (and 0) by 15."""
+    group_size (32, 64, 128) of the k columns: the largest weight of a group times 1 / 7 in fp32, or with zero_points the distance of its largest and smallest (and 0) times 1 / 15."""
     if w.ndim != 3:
         raise ValueError('quantize_4bit: w must be [experts, n, k] or [experts, k, n]')
     if group_size not in GROUP_SIZES:

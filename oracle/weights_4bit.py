@@ -35,7 +35,8 @@ def quantize(w, group, zero_points):
     bad = ~parts.isfinite().all(3)
     x = torch.where(bad[..., None], 0., parts.float())
     low, high = x.amin(3).clamp(max=0), x.amax(3).clamp(min=0)
-    scales = ((high - low) / 15 if zero_points else torch.maximum(high, -low) / 7).to(w.dtype)
+    one = torch.ones((), dtype=torch.float32)      # by the reciprocal in 32 bits
+    scales = ((high - low) * (one / 15) if zero_points else torch.maximum(high, -low) * (one / 7)).to(w.dtype)
     scales = torch.where(scales.float() < 2.0 ** -126, torch.zeros_like(scales), scales)
     step = torch.where(scales == 0, 1., scales.double())[..., None]
     zeros = torch.full(scales.shape, 8.).double()

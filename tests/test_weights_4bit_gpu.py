@@ -39,6 +39,31 @@ def test_quantized_weights(shape, group, zero_points, trans_b, dtype):
             assert got.dtype == out and torch.equal(got, want.to(out))
 
 
+def test_scales_next_to_a_rounding():
+    """A distance whose fifteenth lies half way between two numbers of the type: by the reciprocal in fp32, as torch on the GPU divides by a number."""
+    w = torch.zeros(1, 1, 32, dtype=BF16)
+    w[0, 0, 3], w[0, 0, 9] = -0.033203125, 0.00124359130859375
+    kept = gg.quantize_4bit(w.cuda(), 32, True, True)
+    assert kept.group_scales().item() == 0.0023040771484375 == oracle.quantize(w, 32, True)[1].item()
+    w = torch.zeros(1, 1, 32, dtype=F16)               # here the product in fp32 is half way itself: to even, as it is rounded twice
+    w[0, 0, 3], w[0, 0, 9] = -0.03240966796875, 0.0007925033569335938
+    kept = gg.quantize_4bit(w.cuda(), 32, True, True)
+    assert kept.group_scales().item() == 0.0022125244140625 == oracle.quantize(w, 32, True)[1].item()
+    for dtype in (BF16, F16):                          # distances of every last place
+        high = (torch.arange(2 ** 11, 2 ** 12, dtype=torch.float64) / 2 ** 12).to(dtype)[:, None]
+        low = -(torch.arange(1, 2 ** 8, 23, dtype=torch.float64) / 2 ** 12).to(dtype)[None]
+        w = torch.zeros(1, high.numel() * low.numel(), 32, dtype=dtype)
+        w[0, :, 0], w[0, :, 1] = high.expand(-1, low.numel()).flatten(), low.expand(high.numel(), -1).flatten()
+        for zero_points in (True, False):
+            codes, scales, _ = oracle.quantize(w, 32, zero_points)
+            kept = gg.quantize_4bit(w.cuda(), 32, True, zero_points)
+            assert torch.equal(kept.group_scales().cpu(), scales) and torch.equal(oracle.unpack(kept.words, w.shape[1], 32), codes)
+    x = torch.rand(1 << 20, generator=torch.Generator().manual_seed(13)).cuda()
+    for zero_points, by in ((True, 15), (False, 7)):
+        kept = gg.quantize_4bit(torch.nn.functional.pad(x[None, :, None], (0, 31)), 32, True, zero_points)
+        assert torch.equal(kept.group_scales().flatten(), x / by)
+
+
 @pytest.mark.parametrize('dtype', [BF16, F16, F32])
 def test_groups_that_are_not_finite_tiny_or_huge(dtype):
     w = torch.ones(1, 8, 96, dtype=dtype)
