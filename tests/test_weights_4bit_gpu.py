@@ -216,6 +216,21 @@ def test_more_tiles_of_rows_than_a_grid():
     assert int((got != 0).any(1).sum()) == len(at)
 
 
+@pytest.mark.parametrize('rows', [3, 40, 200])      # a kernel each
+@pytest.mark.parametrize('dtype', [BF16, F16])
+def test_scales_and_rows_at_odd_addresses(rows, dtype):
+    kept, values, sizes = _weights(2, 80, 264, 64, True, dtype, 21)
+    flat = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+    odd = gg.Weights4bit(kept.words, flat(kept.scales), flat(kept.zeros), kept.n, kept.k, kept.group)
+    assert odd.scales.data_ptr() % 4 == 2 and odd.zeros.data_ptr() % 2 == 1
+    x = torch.randn(2 * rows, 264, device='cuda').to(dtype)
+    bins = torch.tensor([rows, 2 * rows], dtype=torch.int32, device='cuda')
+    want = gg.gmm_4bit(x, kept, bins=bins)
+    assert torch.equal(gg.gmm_4bit(x, odd, bins=bins), want) and torch.equal(gg.gmm_4bit(flat(x), odd, bins=bins), want)
+    _close(want, *_products(x.cpu(), [rows, rows], values, sizes), dtype)
+    assert torch.equal(odd.dequantize(), kept.dequantize())
+
+
 def test_what_is_refused():
     kept, *_ = _weights(2, 16, 128, 128, False, BF16, 5)
     x, bins, indices = torch.randn(4, 128, device='cuda').bfloat16(), torch.tensor([1, 4], dtype=torch.int32, device='cuda'), torch.arange(4, dtype=torch.int32, device='cuda')
