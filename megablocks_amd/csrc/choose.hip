@@ -8,7 +8,7 @@
 //
 // The order is that of the exact keys.  Scores in fp32 are off by some 2^-23, and of 256 scores of a token two neighbours in the order are closer
 // than that once in a few thousand tokens: where two keys next to each other in the order are within kCloseKeys without being made of the same logit and
-// bias, the wave does the choice over with keys in 64 bits.
+// bias, or the last chosen one and the largest left out that is not made of the same, the wave does the choice over with keys in 64 bits.
 //
 // LANES (16 or 64) lanes have a token, R experts in a row each, so that a lane reads and writes its experts as one piece and most groups are a
 // power of two of neighbouring lanes.  What bounds it is instructions: a token's rounds of "largest of all, then its place" (top_k + 1 of them) take most.
@@ -390,7 +390,21 @@ __device__ __forceinline__ void choose_token(const float (&x)[R], const typename
       b1 = c.bias[next];
       k1 = score_of(x1) + b1;
     }
-    if (lane < c.top_k - 1 + more) close = close || (!(k0 - k1 > kCloseKeys * (1.f + fabsf(k0))) && !(x0 == x1 && b0 == b1));
+    const bool twins = x0 == x1 && b0 == b1, border = lane == c.top_k - 1 && more;
+    if (lane < c.top_k - 1 + more) close = close || (!(k0 - k1 > kCloseKeys * (1.f + fabsf(k0))) && !twins);
+    // Twins on either side of the border say nothing of the keys behind them: the last chosen one against the largest left that is no twin of it.  16-bit logits and
+    // equal biases make some tokens in a hundred such (32768 tokens, 8 of 256 experts, biases of zero: 20.9 us without this, 22.0 with it)
+    if (__any(border && twins)) {
+      const float x_last = __shfl(x0, c.top_k - 1, LANES), b_last = __shfl(b0, c.top_k - 1, LANES);
+      float left[R], bias[R];
+      read_row<DT, R, WHOLE>(row, base, c.experts, -INFINITY, left);
+      read_row<MBX_F32, R, WHOLE>(c.bias, base, c.experts, 0.f, bias);
+      uint32_t best = 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) best = larger(best, left[r] == x_last && bias[r] == b_last ? 0 : key[r]);
+      best = token_max<LANES>(best);
+      if (border && twins && best != 0) close = close || !(k0 - unordered(best) > kCloseKeys * (1.f + fabsf(k0)));
+    }
   }
   for (uint64_t left = __ballot(close); left != 0;) {
     const int first = __builtin_ctzll(left) & ~(LANES - 1);      // a token's lanes

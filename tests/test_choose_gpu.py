@@ -84,6 +84,46 @@ def test_keys_that_32_bits_do_not_tell_apart(score, groups):
     _check(big, 6, F32, score=score, bias=bias * 0 + 0.125, groups=groups, top_groups=max(1, groups // 2))
 
 
+def _border(experts, top_k, groups, score, dtype):
+    """(logits, bias): top_k - 1 experts far in front; at the border two of the same logit and bias, and at a higher index one whose exact key is the larger
+    and whose key in fp32 is theirs."""
+    x, bias = torch.full((1, experts), -9.), torch.zeros(experts)
+    x[0, :top_k - 1], bias[:top_k - 1] = 0., 2. + torch.arange(top_k - 1)
+    at = experts // groups if groups > 1 else top_k - 1        # in a group of their own, the second best
+    if score == 'sigmoid':
+        x[0, [at, at + 1, at + 3]] = torch.tensor([20., 20., 20.125])        # 1 - 2.1e-9 and 1 - 1.8e-9
+    else:
+        x[0, experts - 1] = 0.
+        x[0, [at, at + 1, at + 3]] = torch.tensor([-16., -16., -15.875])     # below 1.3e-7, next to a bias of one
+        bias[[at, at + 1, at + 3]] = 1.
+    return x.to(dtype), bias
+
+
+@pytest.mark.parametrize('dtype', [BF16, F16, F32])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('experts,top_k,groups', [(5, 1, 1), (12, 4, 1), (64, 6, 4), (256, 8, 1), (256, 8, 8), (384, 17, 4), (500, 2, 1)])
+@pytest.mark.parametrize('tokens', [3, 2100])
+def test_a_tie_at_the_border_hides_no_larger_key(tokens, experts, top_k, groups, score, dtype):
+    """The last chosen and the first left out are made of the same logit and bias: what follows them counts all the same."""
+    x, bias = _border(experts, top_k, groups, score, dtype)
+    how = dict(score=score, bias=bias, groups=groups, top_groups=min(groups, 2))
+    want = oracle.choose(x, top_k, **how)[2]
+    assert int(want[0, -1]) == (experts // groups if groups > 1 else top_k - 1) + 3
+    got = ops.choose_experts(x.repeat(tokens, 1).cuda(), top_k, **{**how, 'bias': bias.cuda()})[2].cpu()
+    assert torch.equal(got, want.expand(tokens, -1))
+
+
+def test_ties_at_the_border_without_a_larger_key():
+    """Many of the same logit and bias, nothing behind them or only smaller keys: the lower indices."""
+    for experts in (16, 40, 300):
+        x, bias = torch.zeros(4, experts), torch.full((experts,), 0.25)
+        x[1, experts // 2:] = -1.
+        x[2, experts // 2:] = -float('inf')
+        x[3, 0] = 1.
+        _check(x, 3, F32, score='sigmoid', bias=bias)
+        _check(x, 3, BF16, score='softmax', bias=bias, groups=2, top_groups=1)
+
+
 @pytest.mark.parametrize('dtype', [BF16, F16, F32])
 @pytest.mark.parametrize('with_bias', [False, True])
 def test_many_equal_logits(dtype, with_bias):
