@@ -115,7 +115,7 @@ template <> struct Keys<float> { typedef uint32_t type; };
 template <> struct Keys<double> { typedef uint64_t type; };
 
 // The open groups of a token as a bit each, given its experts' keys (0: none).  close: whether two groups on either side of the border are
-// within what the keys may be off by.
+// within what the keys may be off by, which goes by the sizes of the keys that are added up: large biases may leave little of them.
 template <int LANES, int R, typename F>
 __device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&key)[R], const Choose& c, int lane, bool& close) {
   typedef typename Keys<F>::type U;
@@ -129,7 +129,11 @@ __device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&k
     const F first = unordered(m1);
     return c.group_best == 2 && m2 != 0 ? first + unordered(m2) : first;
   };
-  F mine = 0;   // of group `lane`
+  const auto off_by = [&](U m1, U m2) {
+    const F first = unordered(m1), second = c.group_best == 2 && m2 != 0 ? unordered(m2) : (F)0;
+    return (F)kCloseKeys * (1 + (first < 0 ? -first : first) + (second < 0 ? -second : second));
+  };
+  F mine = 0, off = 0;   // of group `lane`
   const int per = size / R;
   if (per * R == size && per > 0 && (per & (per - 1)) == 0) {   // a group is `per` lanes next to each other
     U m1 = 0, m2 = 0;
@@ -144,7 +148,9 @@ __device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&k
       if (per > 16) { swapped<false>(m1, m1, a1); swapped<false>(m2, m2, a2); merge(m1, m2, a1, a2); }
       if (per > 32) { swapped<true>(m1, m1, a1); swapped<true>(m2, m2, a2); merge(m1, m2, a1, a2); }
     }
-    mine = __shfl(value(m1, m2), lane * per < LANES ? lane * per : 0, LANES);
+    const int from = lane * per < LANES ? lane * per : 0;
+    mine = __shfl(value(m1, m2), from, LANES);
+    off = __shfl(off_by(m1, m2), from, LANES);
   } else {
 #pragma unroll 1
     for (int g = 0; g < c.groups; ++g) {
@@ -163,7 +169,10 @@ __device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&k
         swapped<false>(m1, m1, a1); swapped<false>(m2, m2, a2); merge(m1, m2, a1, a2);
         swapped<true>(m1, m1, a1); swapped<true>(m2, m2, a2); merge(m1, m2, a1, a2);
       }
-      if (lane == g) mine = value(m1, m2);
+      if (lane == g) {
+        mine = value(m1, m2);
+        off = off_by(m1, m2);
+      }
     }
   }
   const U order = ordered(mine);
@@ -174,8 +183,8 @@ __device__ __forceinline__ uint64_t open_groups(const typename Keys<F>::type (&k
     before += other > order || (other == order && g < lane) ? 1 : 0;
   }
   const bool group = lane < c.groups, open = group && before < c.top_groups;
-  const F lowest = token_min<LANES>(open ? mine : (F)INFINITY), highest = token_max<LANES>(group && !open ? mine : (F)-INFINITY);
-  close = !(lowest - highest > (F)(2 * kCloseKeys) * (1 + (highest < 0 ? -highest : highest)));
+  const F lowest = token_min<LANES>(open ? mine - off : (F)INFINITY), highest = token_max<LANES>(group && !open ? mine + off : (F)-INFINITY);
+  close = !(lowest > highest) || (group && !(off < (F)INFINITY));
   const uint64_t all = __ballot(open);
   return LANES == 64 ? all : (all >> (lane_id() & ~(LANES - 1))) & 0xffffu;
 }

@@ -124,6 +124,33 @@ def test_ties_at_the_border_without_a_larger_key():
         _check(x, 3, BF16, score='softmax', bias=bias, groups=2, top_groups=1)
 
 
+@pytest.mark.parametrize('experts', [4, 12, 96, 128])
+@pytest.mark.parametrize('size', [64., 8192., 1e6])
+def test_groups_whose_keys_cancel(size, experts):
+    """One expert of a group is wanted by its bias and the rest shut out by theirs: the group's key is what two large numbers leave, with their rounding."""
+    g = torch.Generator().manual_seed(31)
+    bias = torch.zeros(experts)
+    bias[0], bias[1:experts // 2] = size, -size
+    x = torch.randn(200, experts, generator=g)
+    x[:, 2:experts // 2], x[:, experts // 2 + 2:] = -4., -4.
+    x[:, experts // 2:experts // 2 + 2] = x[:, :2] + torch.randn(200, 2, generator=g) * 2.0 ** -10
+    how = dict(score='sigmoid', bias=bias, groups=2, top_groups=1, group_best=2)
+    want = oracle.choose(x, 1, **how)[2]
+    assert 50 < int((want < experts // 2).sum()) < 150
+    assert torch.equal(ops.choose_experts(x.cuda(), 1, **{**how, 'bias': bias.cuda()})[2].cpu(), want)
+
+
+def test_groups_shut_out_by_the_lowest_number():
+    """Biases of the type's lowest number or of -infinity in whole groups: their sums are none, and the open groups' experts are chosen."""
+    low = torch.finfo(F32).min
+    x = torch.randn(50, 32, generator=torch.Generator().manual_seed(32))
+    for out in (low, -float('inf')):
+        for top_groups in (1, 2):
+            bias = torch.full((32,), out)
+            bias[8:24] = 0.
+            _check(x, 4, F32, score='sigmoid', bias=bias, groups=4, top_groups=top_groups, norm_p=1)
+
+
 @pytest.mark.parametrize('dtype', [BF16, F16, F32])
 @pytest.mark.parametrize('with_bias', [False, True])
 def test_many_equal_logits(dtype, with_bias):
