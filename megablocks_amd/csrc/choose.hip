@@ -352,7 +352,17 @@ __device__ __forceinline__ void choose_token(const float (&x)[R], const typename
   float m = 0.f, sum = 1.f, s[R];
   if (!c.sigmoid || c.lse) {
     softmax_parts<DT, LANES, R>(x, m, sum, s);
-    if (c.lse && lane == 0 && real) c.lse[t] = m == INFINITY || m == -INFINITY ? m : m + logf(sum);
+    if (c.lse) {
+      float lse = m + logf(sum);
+      if (__any(m == INFINITY || m == -INFINITY)) {     // the largest is none of the logits that are not numbers, which the sum then does not show
+        float bad = 0.f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) bad = x[r] != x[r] ? 1.f : bad;
+        bad = token_max<LANES>(bad);
+        lse = bad != 0.f ? NAN : m == INFINITY || m == -INFINITY ? m : lse;
+      }
+      if (lane == 0 && real) c.lse[t] = lse;
+    }
   }
   if (c.sigmoid) {
 #pragma unroll

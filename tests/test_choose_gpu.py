@@ -195,6 +195,26 @@ def test_masked_infinite_and_undefined_logits():
     assert ((0 <= i) & (i < 16)).all()
 
 
+@pytest.mark.parametrize('experts', [5, 64, 300])
+@pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
+def test_lse_of_logits_that_are_not_numbers(score, experts):
+    """A logit that is not a number makes lse none, also next to infinities; without one infinities are the sum."""
+    inf, nan = float('inf'), float('nan')
+    x = torch.zeros(8, experts)
+    x[0] = nan
+    x[1], x[1, -1] = -inf, nan
+    x[2, 0], x[2, -1] = inf, nan
+    x[3, 1] = nan
+    x[4] = -inf
+    x[5, 2] = inf
+    x[6], x[6, 3] = -inf, 1.5
+    for dtype in (BF16, F16, F32):
+        lse = ops.choose_experts(x.to(dtype).cuda(), 2, score=score, want_lse=True)[3].cpu()
+        want = torch.logsumexp(x.double(), 1)
+        assert torch.equal(lse.isnan(), want.isnan()) and lse[:4].isnan().all()
+        assert torch.equal(lse[4:6].double(), want[4:6]) and torch.allclose(lse[6:].double(), want[6:], rtol=24 * 2.0 ** -23, atol=0)
+
+
 @pytest.mark.parametrize('dtype', [BF16, F16, F32])
 @pytest.mark.parametrize('score', ['softmax', 'sigmoid'])
 @pytest.mark.parametrize('shape', SHAPES)
