@@ -165,7 +165,7 @@ struct Weights4bit {
   };
   wave_ptr words_at[WT], scales_at[WT], zeros_at[WT];
   uint32_t word_lane, scale_lane, scale_at, half_up, half_mask;
-  int scale_shift;
+  int scale_shift, groups;
   bool wide, with_zeros;
 
   __device__ __forceinline__ Weights4bit(const Rows4bit& g, int expert, int tile0, int tiles, int blocks) {
@@ -189,6 +189,7 @@ struct Weights4bit {
     scale_at = scale_lane << scale_shift & ~3u;
     half_up = wide || scale_lane % 2 ? 0 : 16;
     half_mask = wide ? ~0u : 0xffff0000u;
+    groups = (g.k + GROUP - 1) / GROUP;
   }
 
   // ONCE: read by nobody else, kept out of the caches (60 MiB of weights read alone: 9.7 us, with plain loads 10.9; 480 MiB: 69, 78)
@@ -213,9 +214,11 @@ struct Weights4bit {
     fetch_scales(to, b);
   }
 
-  // scale and -(16 + zero) of the lane's feature for each group
-  __device__ __forceinline__ void scales(const Block& of, int t, uint32_t (&scale)[kGroups], uint32_t (&off)[kGroups]) const {
-    const uint32_t raw = (of.scale[t] << half_up) & half_mask;
+  // The bits of a scale's piece that are used in block b: none of groups that lie wholly past k, whose sums are 0, but 0 times a scale that is not finite is not
+  __device__ __forceinline__ uint32_t mask_of(int b) const { return kGroups > 1 && scale_lane >= (uint32_t)(groups - b * kGroups) * 16 ? 0u : half_mask; }
+  // scale and -(16 + zero) of the lane's feature for each group; mask: mask_of the block
+  __device__ __forceinline__ void scales(const Block& of, int t, uint32_t mask, uint32_t (&scale)[kGroups], uint32_t (&off)[kGroups]) const {
+    const uint32_t raw = (of.scale[t] << half_up) & mask;
     float s = __uint_as_float(raw);
     if constexpr (DT == MBX_F16) s = wide ? s : Elem<DT>::to_f32(__builtin_bit_cast(typename Elem<DT>::type, (uint16_t)(raw >> 16)));
     spread<kGroups>(__float_as_uint(s), scale);

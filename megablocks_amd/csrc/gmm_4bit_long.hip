@@ -85,8 +85,9 @@ long_4bit_kernel(const Rows4bit g) {
       if constexpr (ZEROS) zero_raw[t] = load_at<uint8_t>(zeros_at[t], 0, zero_at[t] + (uint32_t)group * 16);
     }
   };
-  const auto scale_of = [&](int t) {
-    const uint32_t raw = (scale_raw[t] << half_up) & half_mask;
+  // of groups that lie wholly past k 0: their sums are 0, but 0 times a scale that is not finite is not
+  const auto scale_of = [&](int t, int group) {
+    const uint32_t raw = (scale_raw[t] << half_up) & (kGroups > 1 && group * GROUP >= g.k ? 0u : half_mask);
     if constexpr (DT == MBX_F16) return wide ? __uint_as_float(raw) : Elem<DT>::to_f32(__builtin_bit_cast(typename Elem<DT>::type, (uint16_t)(raw >> 16)));
     else return __uint_as_float(raw);
   };
@@ -186,7 +187,7 @@ long_4bit_kernel(const Rows4bit g) {
       float off[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        of_last[t] = scale_of(t);
+        of_last[t] = scale_of(t, b * kGroups + q);
         if constexpr (ZEROS) off[t] = -16.f - (float)zero_raw[t];
       }
       fetch_scales(q + 1 < kGroups ? b * kGroups + q + 1 : b_next * kGroups);

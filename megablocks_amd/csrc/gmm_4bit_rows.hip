@@ -49,8 +49,9 @@ rows_4bit_kernel(const Rows4bit g) {
       }
     }
     uint32_t scale[WT][kGroups], off[WT][kGroups];
+    const uint32_t scale_mask = weights.mask_of(b);
 #pragma unroll
-    for (int t = 0; t < WT; ++t) weights.scales(now, t, scale[t], off[t]);
+    for (int t = 0; t < WT; ++t) weights.scales(now, t, scale_mask, scale[t], off[t]);
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) {
       f32x4_t of_ones = {0.f, 0.f, 0.f, 0.f};

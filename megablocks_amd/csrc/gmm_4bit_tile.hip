@@ -84,8 +84,9 @@ tile_4bit_kernel(const Rows4bit g) {
     }
     const u32x4_t(*const x_now)[16] = staged[buffer];
     uint32_t scale[WT][kGroups], off[WT][kGroups];
+    const uint32_t scale_mask = weights.mask_of(b);
 #pragma unroll
-    for (int t = 0; t < WT; ++t) weights.scales(now, t, scale[t], off[t]);
+    for (int t = 0; t < WT; ++t) weights.scales(now, t, scale_mask, scale[t], off[t]);
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) {
       f32x4_t acc[WT][MT];

@@ -231,6 +231,41 @@ def test_scales_and_rows_at_odd_addresses(rows, dtype):
     assert torch.equal(odd.dequantize(), kept.dequantize())
 
 
+@pytest.mark.parametrize('dtype', [BF16, F16])
+@pytest.mark.parametrize('wide', [False, True])
+@pytest.mark.parametrize('zeros', [False, True])
+@pytest.mark.parametrize('rows', [3, 40, 200])      # a kernel each
+@pytest.mark.parametrize('k,group', [(8, 32), (40, 32), (96, 32), (136, 64), (264, 32), (1032, 32), (129, 64), (130, 128)])
+def test_padding_is_never_used(k, group, rows, zeros, wide, dtype):
+    """Codes, scales and zeros past n and k may be anything, scales that are no numbers among it: the products are those of padding of zeros."""
+    n, experts = 24, 2
+    g = torch.Generator().manual_seed(k)
+    whole, features = -(-k // 128) * 128, -(-n // 16) * 16
+    codes = torch.randint(0, 16, (experts, features, whole), generator=g)
+    scales = ((torch.rand(experts, features, whole // group, generator=g) + 0.2) * 0.01).to(F32 if wide else dtype)
+    offs = torch.randint(0, 16, scales.shape, generator=g)
+
+    def made(fill_codes, fill_scales):
+        c, s, z = codes.clone(), scales.clone(), offs.clone()
+        for t, end, fill in ((c, k, fill_codes), (s, -(-k // group), fill_scales), (z, -(-k // group), fill_codes)):
+            t[:, :, end:] = fill
+            t[:, n:] = fill
+        return gg.Weights4bit(oracle.pack(c).cuda(), oracle.kept(s).cuda(), oracle.kept(z).to(torch.uint8).cuda() if zeros else None, n, k, group)
+
+    x = torch.randn(2 * rows, k, generator=g).to(dtype).cuda()
+    bins = torch.tensor([rows, 2 * rows], dtype=torch.int32, device='cuda')
+    plain = made(0, 0.)
+    want, gated = gg.gmm_4bit(x, plain, bins=bins), gg.gmm_4bit_act(x, plain, gg.ACT_SILU, bins=bins, b2=plain)
+    assert want.isfinite().all()
+    for fill in (float('nan'), float('inf'), -float('inf')):
+        other = made(13, fill)
+        assert torch.equal(gg.gmm_4bit(x, other, bins=bins), want) and torch.equal(gg.gmm_4bit_act(x, other, gg.ACT_SILU, bins=bins, b2=other), gated)
+        assert torch.equal(other.dequantize(), plain.dequantize())
+    bad = made(0, 0.)
+    bad.scales[0, 0, 0, 3] = float('nan')            # within k it counts
+    assert gg.gmm_4bit(x, bad, bins=bins)[:rows, 3].isnan().all()
+
+
 def test_what_is_refused():
     kept, *_ = _weights(2, 16, 128, 128, False, BF16, 5)
     x, bins, indices = torch.randn(4, 128, device='cuda').bfloat16(), torch.tensor([1, 4], dtype=torch.int32, device='cuda'), torch.arange(4, dtype=torch.int32, device='cuda')
