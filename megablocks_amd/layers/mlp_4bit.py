@@ -31,8 +31,18 @@ class Grouped4bitExperts(torch.nn.Module):
                 self.register_buffer(f'{name}_{part}', getattr(made, part))
         self._wrap()
 
+    def _of_buffers(self, name):
+        return Weights4bit(*(getattr(self, f'{name}_{part}') for part in ('words', 'scales', 'zeros')), *self._sizes[name])
+
     def _wrap(self):
-        self._weights = {name: Weights4bit(*(getattr(self, f'{name}_{part}') for part in ('words', 'scales', 'zeros')), *self._sizes[name]) for name in self._names}
+        self._weights = {name: self._of_buffers(name) for name in self._names}
+
+    def _kept(self, name):
+        """The weights that the buffers are now: made once (5 us) while nobody puts others in their place, as an assignment and torch.func.functional_call do."""
+        kept, buffers = self._weights[name], self._buffers
+        if buffers.get(f'{name}_words') is kept.words and buffers.get(f'{name}_scales') is kept.scales and buffers.get(f'{name}_zeros', self) is kept.zeros:
+            return kept
+        return self._of_buffers(name)
 
     def _apply(self, fn, *args, **kwargs):
         super()._apply(fn, *args, **kwargs)
@@ -45,15 +55,15 @@ class Grouped4bitExperts(torch.nn.Module):
 
     @property
     def w1(self):
-        return self._weights['w1']
+        return self._kept('w1')
 
     @property
     def v1(self):
-        return self._weights.get('v1')
+        return self._kept('v1') if 'v1' in self._weights else None
 
     @property
     def w2(self):
-        return self._weights['w2']
+        return self._kept('w2')
 
     def forward(self, x, tokens_per_expert):
         x, = gg.autocast_operands(x)

@@ -58,3 +58,44 @@ def test_experts_that_have_no_4_bit_form_are_refused(changed):
         ParallelDroplessMLP(_args(**changed)).quantize_experts_()
     with pytest.raises(RuntimeError):
         ParallelDroplessMLP(_args()).quantize_experts_()       # on the CPU
+
+
+@pytest.mark.parametrize('changed', [dict(zero_points=False), dict(zero_points=True)])
+def test_4_bit_experts_go_by_the_buffers_there_are(monkeypatch, changed):
+    """Buffers that a call or an assignment puts in the place of others are the ones multiplied by."""
+    from megablocks_amd import grouped_gemm_util as gg
+    from megablocks_amd.layers import mlp_4bit
+
+    def made(w, group, trans_b, zero_points):
+        n, k = (w.shape[1], w.shape[2]) if trans_b else (w.shape[2], w.shape[1])
+        shape = (w.shape[0], -(-n // 16), -(-k // 128) * 128 // group, 16)
+        return gg.Weights4bit(torch.zeros(w.shape[0], -(-n // 16), -(-k // 128), 64, 4, dtype=torch.int32), torch.ones(shape, dtype=w.dtype),
+                              torch.zeros(shape, dtype=torch.uint8) if zero_points else None, n, k, group, trans_b)
+    monkeypatch.setattr(mlp_4bit, 'quantize_4bit', made)
+    experts = ParallelDroplessMLP(_args(mlp_type='glu', activation_fn=torch.nn.functional.silu)).quantize_experts_(32, **changed).mlp
+    seen = []
+    monkeypatch.setattr(gg, 'gmm_4bit_act', lambda x, b, act, *sizes, b2=None: (seen.append((b, b2)), x)[1])
+    monkeypatch.setattr(gg, 'gmm_4bit', lambda x, b, *sizes: (seen.append(b), x)[1])
+    x, sizes = torch.zeros(2, 16, dtype=torch.bfloat16), torch.tensor([2] + [0] * 7)
+
+    def used():
+        (w1, v1), w2 = seen[-2:]
+        return {f'{name}_{part}': getattr(w, part) for name, w in (('w1', w1), ('v1', v1), ('w2', w2)) for part in ('words', 'scales', 'zeros')}
+    experts(x, sizes)
+    first = dict(experts.named_buffers())
+    assert all(t is first.get(name) for name, t in used().items())
+    others = {name: t.clone() for name, t in first.items()}
+    for name in others:                                    # one at a time, and all
+        torch.func.functional_call(experts, {name: others[name]}, (x, sizes))
+        assert all(t is (others if name == at else first).get(at) for at, t in used().items())
+    torch.func.functional_call(experts, others, (x, sizes))
+    assert all(t is others.get(name) for name, t in used().items())
+    experts(x, sizes)
+    assert all(t is first.get(name) for name, t in used().items())
+    for name in others:
+        setattr(experts, name, others[name])
+        experts(x, sizes)
+        assert used()[name] is others[name] is dict(experts.named_buffers())[name]
+    experts.w1_scales = torch.ones(3, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        experts(x, sizes)                                  # that do not fit
