@@ -184,7 +184,7 @@ class ParallelDroplessMLP(moe.ParallelMLP):
     def _one_call_4bit(self, x, expert_weights, top_experts):
         """grouped_forward_once from one call of the library (gg.experts_forward_4bit), as _one_call_forward."""
         experts = self.mlp
-        if type(self) is not ParallelDroplessMLP or router._has_hooks(experts) or not _only_computed() or \
+        if type(self) is not ParallelDroplessMLP or router._has_hooks(experts) or not _only_computed() or 'forward_tokens' in experts.__dict__ or \
                 not self.__dict__.keys().isdisjoint(('indices_and_bins', 'grouped_permute_and_compute', 'permute_and_compute')):
             return None
         return gg.experts_forward_4bit(x.view(-1, x.shape[-1]), top_experts.int(), expert_weights, self.num_experts, self.sort_end_bit,

@@ -60,18 +60,36 @@ def test_experts_that_have_no_4_bit_form_are_refused(changed):
         ParallelDroplessMLP(_args()).quantize_experts_()       # on the CPU
 
 
+def _made(w, group, trans_b, zero_points):
+    """quantize_4bit's weights in shape, all zeros, without a GPU."""
+    from megablocks_amd import grouped_gemm_util as gg
+    n, k = (w.shape[1], w.shape[2]) if trans_b else (w.shape[2], w.shape[1])
+    shape = (w.shape[0], -(-n // 16), -(-k // 128) * 128 // group, 16)
+    return gg.Weights4bit(torch.zeros(w.shape[0], -(-n // 16), -(-k // 128), 64, 4, dtype=torch.int32), torch.ones(shape, dtype=w.dtype),
+                          torch.zeros(shape, dtype=torch.uint8) if zero_points else None, n, k, group, trans_b)
+
+
+@pytest.mark.parametrize('name', ['forward', 'forward_tokens'])
+def test_a_replaced_method_of_the_4_bit_experts_is_called(monkeypatch, name):
+    """The call that does everything behind the router at once stands aside for it."""
+    from megablocks_amd import grouped_gemm_util as gg
+    from megablocks_amd.layers import mlp_4bit
+    monkeypatch.setattr(mlp_4bit, 'quantize_4bit', _made)
+    layer = ParallelDroplessMLP(_args()).quantize_experts_(32)
+    monkeypatch.setattr(gg, 'experts_forward_4bit', lambda *a: 'by one call')
+    x, weights, experts = torch.zeros(3, 16, dtype=torch.bfloat16), torch.ones(6, dtype=torch.bfloat16), torch.zeros(6, dtype=torch.int32)
+    with torch.no_grad():
+        assert layer._one_call_forward(x, weights, experts) == 'by one call'
+        setattr(layer.mlp, name, lambda *a: None)
+        assert layer._one_call_forward(x, weights, experts) is None
+
+
 @pytest.mark.parametrize('changed', [dict(zero_points=False), dict(zero_points=True)])
 def test_4_bit_experts_go_by_the_buffers_there_are(monkeypatch, changed):
     """Buffers that a call or an assignment puts in the place of others are the ones multiplied by."""
     from megablocks_amd import grouped_gemm_util as gg
     from megablocks_amd.layers import mlp_4bit
-
-    def made(w, group, trans_b, zero_points):
-        n, k = (w.shape[1], w.shape[2]) if trans_b else (w.shape[2], w.shape[1])
-        shape = (w.shape[0], -(-n // 16), -(-k // 128) * 128 // group, 16)
-        return gg.Weights4bit(torch.zeros(w.shape[0], -(-n // 16), -(-k // 128), 64, 4, dtype=torch.int32), torch.ones(shape, dtype=w.dtype),
-                              torch.zeros(shape, dtype=torch.uint8) if zero_points else None, n, k, group, trans_b)
-    monkeypatch.setattr(mlp_4bit, 'quantize_4bit', made)
+    monkeypatch.setattr(mlp_4bit, 'quantize_4bit', _made)
     experts = ParallelDroplessMLP(_args(mlp_type='glu', activation_fn=torch.nn.functional.silu)).quantize_experts_(32, **changed).mlp
     seen = []
     monkeypatch.setattr(gg, 'gmm_4bit_act', lambda x, b, act, *sizes, b2=None: (seen.append((b, b2)), x)[1])
