@@ -410,6 +410,7 @@ def int32_indices(expert_indices: torch.Tensor) -> torch.Tensor:
 
 
 class LearnedRouter(torch.nn.Module):
+    _chooses = False     # of a router made without __init__ below
 
     def __init__(self, args: Arguments):
         super().__init__()
@@ -427,7 +428,7 @@ class LearnedRouter(torch.nn.Module):
 
     def _apply(self, fn, *args, **kwargs):
         """The balance bias goes along to other devices, not to other types: its steps are finer than 16 bits."""
-        bias = self.balance_bias
+        bias = self._buffers.get('balance_bias')
         super()._apply(fn, *args, **kwargs)
         if bias is not None and self.balance_bias.dtype != torch.float32:
             self.balance_bias = bias.to(self.balance_bias.device)

@@ -117,3 +117,19 @@ def test_4_bit_experts_go_by_the_buffers_there_are(monkeypatch, changed):
     experts.w1_scales = torch.ones(3, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         experts(x, sizes)                                  # that do not fit
+
+
+def test_routers_made_without_the_choice_route_as_before():
+    """A router of a class with an __init__ of its own, or pickled before there was a choice: softmax and top-k, casts and moves too."""
+    class Own(LearnedRouter):
+
+        def __init__(self, args):
+            torch.nn.Module.__init__(self)
+            self.args, self.layer = args, torch.nn.Linear(args.hidden_size, args.moe_num_experts, bias=False, dtype=torch.bfloat16)
+    args = _args()
+    own, plain = Own(args), LearnedRouter(args)
+    x = torch.randn(5, 1, 16).bfloat16()
+    with torch.no_grad():
+        own.layer.weight.copy_(plain.layer.weight)
+        assert all(torch.equal(a, b) for a, b in zip(own(x), plain(x)))
+        assert own.float().layer.weight.dtype == torch.float32 and own(x.float())[0].shape == (5, 8)
