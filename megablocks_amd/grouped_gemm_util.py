@@ -842,7 +842,7 @@ def _operand_4bit(a, weights, batch_sizes, bins, what):
     if any((w.experts, w.n, w.k, w.group, w.scales.dtype, w.zeros is None) != (first.experts, first.n, first.k, first.group, first.scales.dtype, first.zeros is None)
            for w in weights):
         raise ValueError(f'{what}: both weights must have the same sizes, groups and types')
-    if (batch_sizes is None) == (bins is None and src is None):
+    if (batch_sizes is not None) + (bins is not None) != (src is None):
         raise ValueError(f'{what}: give the batch sizes or their inclusive sums' if src is None else f'{what}: gathered rows bring their bins')
     _lib.require_cuda(x, bins, *(w.words for w in weights))
     if any(w.device != x.device for w in weights):

@@ -91,3 +91,17 @@ def test_entry_points_refuse_without_touching_the_gpu():
     assert lib.mbx_quantize_4bit(None, 0, 0, 4, 4, _lib.NT, 32, None, None, None, None) == 0
     assert lib.mbx_dequantize_4bit(None, None, None, 0, 1, 4, 4, _lib.NT, 32, None, 5, None) == _lib.EINVAL
     assert lib.mbx_dequantize_4bit(None, None, None, 0, 1, 0, 4, _lib.NT, 32, None, 0, None) == 0
+
+
+def test_gathered_rows_bring_their_bins():
+    """Sizes or bins next to gathered rows are refused, not passed over."""
+    w, bins = weights(), torch.tensor([3, 5], dtype=torch.int32)
+    indices = torch.arange(5, dtype=torch.int32)
+    src = gg.GatheredRows(torch.zeros(5, 40, dtype=torch.bfloat16), indices, indices, bins, None, 1, 5)
+    for given in (dict(bins=bins), dict(batch_sizes=torch.tensor([3, 2])), dict(bins=bins, batch_sizes=torch.tensor([3, 2]))):
+        with pytest.raises(ValueError):
+            gg.gmm_4bit(src, w, **given)
+        with pytest.raises(ValueError):
+            gg.gmm_4bit_act(src, w, gg.ACT_SILU, **given)
+    with pytest.raises(RuntimeError):
+        gg.gmm_4bit(src, w)              # on the CPU
