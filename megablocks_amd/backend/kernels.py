@@ -42,6 +42,9 @@ def _scratch(n_slots, device):
 
 
 def _slot_rows_key(indices, bins, padded_bins):
+    """What a kept map is told by; None for tensors made in inference mode, whose changes nothing shows: no map is kept on or used for them."""
+    if indices.is_inference() or bins.is_inference() or (padded_bins is not None and padded_bins.is_inference()):
+        return None
     return (_lib.stream_of(indices), indices._version, bins.data_ptr(), bins._version,
             None if padded_bins is None else (padded_bins.data_ptr(), padded_bins._version))
 
@@ -51,8 +54,11 @@ def remember_slot_rows(indices, bins, padded_bins, rows):
     Not under stream capture, where nothing is kept (see _slot_rows)."""
     if torch.cuda.is_current_stream_capturing():
         return
+    key = _slot_rows_key(indices, bins, padded_bins)
+    if key is None:
+        return
     try:
-        indices._mbx_slot_rows = (_slot_rows_key(indices, bins, padded_bins), rows, bins, padded_bins)
+        indices._mbx_slot_rows = (key, rows, bins, padded_bins)
     except AttributeError:
         pass
 
@@ -70,7 +76,7 @@ def forget_slot_rows(indices):
 
 def _kept_slot_rows(indices, key):
     cached = getattr(indices, '_mbx_slot_rows', None)
-    return cached[1] if cached is not None and cached[0] == key else None
+    return cached[1] if key is not None and cached is not None and cached[0] == key else None
 
 
 def _slot_rows(indices, bin_ids, bins, padded_bins):
@@ -86,14 +92,14 @@ def _slot_rows(indices, bin_ids, bins, padded_bins):
     capturing = torch.cuda.is_current_stream_capturing()
     key = _slot_rows_key(indices, bins, padded_bins)
     cached = getattr(indices, '_mbx_slot_rows', None)   # _kept_slot_rows, without the call: five times a layer step
-    if not capturing and cached is not None and cached[0] == key:
+    if not capturing and key is not None and cached is not None and cached[0] == key:
         return cached[1]
     n_slots = indices.shape[0]
     rows = _scratch(n_slots, indices.device)
     with _lib.device_of(indices):
         _lib.check(lib.mbx_slot_rows(_lib.ptr(indices), _lib.ptr(bin_ids), _lib.ptr(bins), _lib.ptr(padded_bins),
                                      bins.shape[0], n_slots, _lib.ptr(rows), _lib.stream()), 'slot_rows')
-    if not capturing:
+    if not capturing and key is not None:
         try:
             indices._mbx_slot_rows = (key, rows, bins, padded_bins)   # the references keep the data pointers of the key alive
         except AttributeError:   # a tensor type without instance attributes: the map is built on every call

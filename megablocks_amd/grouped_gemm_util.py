@@ -36,12 +36,13 @@ def _device_bins(batch_sizes: torch.Tensor, device, rows: int) -> torch.Tensor:
     operation has written to it.  A write torch does not see (a kernel launched on its raw pointer, the replay of
     a captured graph into it) does not invalidate them: hand such a tensor to `forget_bins` first, or pass a new
     one.  Nothing is kept or reused under stream capture, where a graph must contain the kernel that computes
-    the bins it uses."""
+    the bins it uses, nor for sizes made in inference mode, which have no version."""
     if batch_sizes.ndim != 1:
         raise ValueError('batch_sizes must be a vector')
     capturing = batch_sizes.is_cuda and torch.cuda.is_current_stream_capturing()
+    keeps = not capturing and not batch_sizes.is_inference()
     cached = getattr(batch_sizes, '_mbx_bins', None)
-    if not capturing and cached is not None and cached[1] == batch_sizes._version and cached[0].device == device:
+    if keeps and cached is not None and cached[1] == batch_sizes._version and cached[0].device == device:
         if cached[2] is not None and cached[2] != rows:
             raise ValueError(f'gmm: batch_sizes add up to {cached[2]} rows but the operand has {rows}')
         return cached[0]
@@ -56,7 +57,7 @@ def _device_bins(batch_sizes: torch.Tensor, device, rows: int) -> torch.Tensor:
         if total != rows:
             raise ValueError(f'gmm: batch_sizes add up to {total} rows but the operand has {rows}')
         bins = torch.cumsum(batch_sizes, 0).to(torch.int32).to(device)
-    if not capturing:
+    if keeps:
         _remember(batch_sizes, (bins, batch_sizes._version, total))
     return bins
 
@@ -78,7 +79,7 @@ def note_bins(batch_sizes: torch.Tensor, bins: torch.Tensor):
     """A caller that has already computed the inclusive cumsum of `batch_sizes` (int32, on the same device) hands
     it over, and the products of this step do not compute it again."""
     if batch_sizes.is_cuda and bins.dtype == torch.int32 and bins.device == batch_sizes.device \
-            and bins.numel() == batch_sizes.numel() and not torch.cuda.is_current_stream_capturing():
+            and bins.numel() == batch_sizes.numel() and not batch_sizes.is_inference() and not torch.cuda.is_current_stream_capturing():
         _remember(batch_sizes, (bins.view(-1), batch_sizes._version, None))
 
 

@@ -453,8 +453,8 @@ class LearnedRouter(torch.nn.Module):
 
     def forward(self, x: torch.Tensor):
         scores, expert_weights, expert_indices, expert_indices32 = self.route(x)
-        if expert_indices32 is not None:
-            # out of band: the same indices as int32, valid while the int64 tensor is the one returned here, unmodified
+        if expert_indices32 is not None and not expert_indices.is_inference():
+            # out of band: the same indices as int32, valid while the int64 tensor is the one returned here, unmodified (which one made in inference mode does not show)
             expert_indices._mbx_int32 = (expert_indices32, expert_indices._version)
         return scores, expert_weights, expert_indices
 

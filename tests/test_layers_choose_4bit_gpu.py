@@ -290,3 +290,43 @@ def test_decoding_replays_from_a_captured_graph():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize('tokens', [3, 700, 2500])
+@pytest.mark.parametrize('choice', [dict(), CHOICES[0]])
+def test_serving_in_inference_mode(choice, tokens):
+    """Tensors made in inference mode have no version by which a kept map, bins or indices are told: the layers run without, with 16 and 4 bits, by one call and by
+    several, and what ordinary calls keep stays right next to it."""
+    for changed in (dict(), dict(mlp_impl='sparse', mlp_type='mlp', activation_fn=Arguments().activation_fn)):
+        args = _args(**choice, **changed)
+        layer = dMoE(args).eval()
+        layers = [layer] if changed else [layer, copy.deepcopy(layer).quantize_experts_(64, True), MoE(args).eval()]
+        x = torch.randn(tokens, 1, 256, device='cuda').bfloat16()
+        for layer in layers:
+            with torch.no_grad():
+                want = layer(x)
+            with torch.inference_mode():
+                got, again = layer(x), layer(x.clone())
+            assert torch.equal(got, want) and torch.equal(again, want)
+            with torch.no_grad():
+                assert torch.equal(layer(x), want)
+
+
+def test_products_and_permutation_of_inference_tensors():
+    """Batch sizes and a routing made in inference mode, used there and outside."""
+    kept = _quantized(_args(moe_num_experts=3, moe_top_k=2), 64, False)[1].experts.mlp
+    x, ids = torch.randn(40, 256, device='cuda').bfloat16(), torch.randint(0, 3, (80,), device='cuda').int()
+
+    def step():
+        indices, bin_ids, counts, bins, _ = ops.routing.route(ids, 3, 2)
+        rows = ops.gather(x, indices, bin_ids, bins, 2)
+        y = kept(rows, counts)
+        return ops.scatter(y, indices, bin_ids, torch.ones(80, device='cuda').bfloat16(), bins, 2), (rows, counts, indices, bin_ids, bins, y)
+    with torch.no_grad():
+        want, _ = step()
+    with torch.inference_mode():
+        got, (rows, counts, indices, bin_ids, bins, y) = step()
+        counts.copy_(counts)
+    assert torch.equal(got, want)
+    with torch.no_grad():
+        assert torch.equal(kept(rows, counts), y) and torch.equal(ops.gather(x, indices, bin_ids, bins, 2), rows)
