@@ -71,7 +71,8 @@ __device__ __forceinline__ float activated(float x, int act) {
   return x / (1.f + __expf(-y));
 }
 
-// The workgroup's tile of up to `height` rows: its expert, first and end row, false past the last.  bins need not be trusted: bounds stay in [0, rows].
+// The workgroup's tile of up to `height` rows: its expert, first and end row, false past the last.  bins need not be trusted: bounds stay in [0, rows], and a lane
+// counts no further than it has the slot, so that falling bins of many experts, each with all rows, do not pass 32 bits: up to the lane that has it sums are exact.
 __device__ __forceinline__ bool find_rows(const Rows4bit& g, int height, int& expert, int& first, int& end) {
   const int slot = g.first_slot + (int)blockIdx.y;
   const int lane = lane_id(), per = (g.num_groups + kWave - 1) / kWave, rows = (int)g.rows;
@@ -87,7 +88,7 @@ __device__ __forceinline__ bool find_rows(const Rows4bit& g, int height, int& ex
   } else {
     for (int i = 0; i < per; ++i) {
       const int e = lane * per + i;
-      if (e < g.num_groups) mine += tiles(bound(e), bound(e + 1));
+      if (e < g.num_groups && mine <= slot) mine += tiles(bound(e), bound(e + 1));
     }
   }
   const int upto = wave_inclusive_scan(mine);

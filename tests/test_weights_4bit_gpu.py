@@ -203,6 +203,23 @@ def test_bins_that_do_not_fit_stay_in_range_and_rows_behind_the_last_are_left():
     assert gg.gmm_4bit(src, kept).isfinite().all()
 
 
+@pytest.mark.parametrize('rows,experts', [(200, 700), (3000, 100), (20000, 130)])      # a kernel each
+def test_falling_bins_of_many_experts(rows, experts):
+    """More experts than lanes, every other one with all rows: the tiles there are room for are those of the first that have some, the rest is left out, as is what
+    lies behind the rows."""
+    from megablocks_amd import _lib
+    kept, values, sizes = _weights(experts, 16, 40, 32, False, BF16, 5)
+    x = torch.randn(rows, 40, device='cuda').bfloat16()
+    bins = torch.tensor([rows, 0], dtype=torch.int32, device='cuda').repeat(experts // 2)
+    kept.words[1:], kept.scales[1:] = kept.words[:1], kept.scales[:1]       # all alike: whichever has a row, its product is the same
+    out = torch.full((rows + 64, 16), 7., device='cuda').bfloat16()
+    _lib.check(_lib.lib.mbx_gmm_4bit(x.data_ptr(), rows, None, 1, kept.words.data_ptr(), kept.scales.data_ptr(), None, None, None, None, 0, 32, out.data_ptr(), 0,
+                                     bins.data_ptr(), experts, rows, 40, 16, -1, _lib.stream()))
+    torch.cuda.synchronize()
+    assert (out[rows:] == 7).all()
+    _close(out[:rows], *_products(x.cpu(), [rows], values, sizes), BF16)
+
+
 def test_more_tiles_of_rows_than_a_grid():
     """65535 tiles of 64 rows are one launch: rows on either side of its end and the last ones, each a product of its own."""
     rows = 65535 * 64 + 70
