@@ -412,3 +412,14 @@ def test_balance_refuses_two_layers_with_one_output():
         ops.balance_bias([b], [n], 0.001, out=[torch.zeros(16, device='cuda')[::2]])
     with pytest.raises(RuntimeError):
         ops.balance_bias([b], [n.cpu()], 0.001)
+
+
+@pytest.mark.parametrize('experts,spread', [(256, 0.02), (256, 0.1), (512, 0.02), (64, 0.02)])
+def test_flat_scores_with_a_bias_of_zero(experts, spread):
+    """Where training starts: softmax scores of many experts that are nearly alike, most tokens within what 32 bits tell apart.  With a bias of zero everywhere the
+    order is that of the logits."""
+    x = torch.randn(4099, experts, generator=torch.Generator().manual_seed(experts)) * spread
+    for dtype in (F32, BF16):
+        logits = x.to(dtype)
+        want = logits.double().sort(dim=1, descending=True, stable=True).indices[:, :8]
+        assert torch.equal(ops.choose_experts(logits.cuda(), 8, bias=torch.zeros(experts, device='cuda'))[2].cpu(), want)
