@@ -501,13 +501,14 @@ int mbx_loss_gradient(const float* grad, const void* values, int dtype, const in
  *           (0, 2, 4, 6, 1, 3, 5, 7), four bits each from the lowest
  *   scales  [num_experts, T, B * 128 / group, 16] of scale_dtype: of feature 16 t + f and its p-th group
  *   zeros   uint8 like scales, or NULL: 8 everywhere
- * A code q stands for scale * (q - zero).  Features and columns past n and k are never used.
+ * A code q stands for scale * (q - zero).  Features and columns past n and k are never used, nor scales and zeros of groups that lie wholly past k: they may be
+ * anything.
  *
  * mbx_quantize_4bit: from weights [num_experts, n, k] (layout MBX_NT, as w1 and v1 are kept) or [num_experts, k, n] (MBX_NN, as w2 is); scales in the weights'
  * type.  Without zeros scale = round(max|w| * (1 / 7)), reciprocal and product in fp32, q = clamp(rint(w / scale), -8, 7) + 8; with zeros, of low = min(w, 0)
  * and high = max(w, 0), scale = round((high - low) * (1 / 15)), zero = clamp(rint(-low / scale), 0, 15), q = clamp(rint(w / scale) + zero, 0, 15).  The
  * quotients by the scale are taken exactly, halves go to even.  A group of zeros has scale 0, as one whose scale would be below 2^-126; one with a number
- * that is not finite scale NaN.
+ * that is not finite scale NaN, as one with zeros whose high - low fp32 does not hold.
  * mbx_dequantize_4bit: the values, rounded to `dtype`, in either layout. */
 int mbx_quantize_4bit(const void* weights, int dtype, int num_experts, int n, int k, int layout, int group, void* words, void* scales, uint8_t* zeros,
                       mbx_stream_t stream);

@@ -103,8 +103,8 @@ struct PackPlace {
 
 // Weights [E, n, k] (TRANSPOSED: [E, k, n]) into words, scales and zeros.  What bounds it: one reading of the weights.  A lane's eight columns of a word
 // are 16 bytes in a row of [n, k]; from [k, n] a workgroup's features go through the LDS.  whole: rows are whole 16-byte pieces at 16-byte addresses; the next
-// block's are then on their way while a block is encoded.  8 x [14336, 4096] in bf16 as [k, n]: 268 us for 1.18 GB read and written (4.4 TB/s, a copy
-// reaches 4.9), back in 215 (5.5 TB/s).
+// block's are then on their way while a block is encoded.  8 x [14336, 4096] in bf16 as [k, n]: 278 us for 1.18 GB read and written (4.2 TB/s, a copy
+// reaches 4.9), back in 225 (5.2 TB/s).
 template <int DT, int GROUP, bool TRANSPOSED, bool ZEROS>
 __global__ void __launch_bounds__(kPackThreads)
 quantize_kernel(const void* __restrict__ weights, const PackPlace place, bool whole, uint32_t* __restrict__ words, void* __restrict__ scales, uint8_t* __restrict__ zeros) {

@@ -6,12 +6,15 @@
 // words of half a block are loaded half a block ahead, rows three blocks.  That is the 256 registers there are for two waves on a SIMD; where the rows are
 // is kept in the LDS for that.
 //
-// What bounds it: a SIMD issues a vector instruction every 4 cycles, and next to them a matrix instruction of 32 x 32 x 16 costs 2.4 such places, one of
-// 16 x 16 x 32, half the work, 2 (measured); 36 of them and some 260 others a block are 350 places, and at this rate the clock is down to 2.0 GHz.
+// What bounds it: issuing, and waiting with two waves a SIMD.  A SIMD issues a vector instruction every 4 cycles, and next to them a matrix instruction of 32 x 32 x 16
+// costs 2.4 such places, one of 16 x 16 x 32, half the work, 2 (measured); 36 of them and some 290 others a block are 370 places of 4 cycles, 2960 for both waves, where a
+// block takes 4100 cycles of a clock that is down to 1.84 GHz.  Counted, 1024 rows an expert: the matrix pipe is busy in 52 % of the cycles, 63 % of the places are
+// taken; of its time a wave issues vector instructions for 33 %, waits for its turn to issue for 38 %, and for loads, the LDS or the barrier for 17 %.  128 rows: 46 %, 56 %;
+// 33, 36 and 20 %.
 // First products of 8 gated experts of [4096, 14336], 128 / 256 / 512 / 1024 rows an expert: 345 / 608 / 1088 / 2030 us (698 / 792 / 885 / 948 TFLOP/s); by
 // 16 x 16 x 32 351 / 623 / 1121 / 2107; 128 rows a workgroup with one wave a SIMD and all 512 registers 2245; values made in 16 bits, which rounds each weight,
 // and multiplied by the grouped kernels 2016 for 1024 rows.  Workgroups of an XCD by 16 tiles of rows and a few features 2001, but 64 experts of [2048, 1408],
-// whose features do not divide by the XCDs, 405 -> 493.  Groups of 32, 512 rows of 8 experts of [14336, 4096]: 767 us (627 TFLOP/s): four times the sums.
+// whose features do not divide by the XCDs, 405 -> 493.  Groups of 32, 512 rows of 8 experts of [14336, 4096]: 784 us (614 TFLOP/s): four times the sums.
 #include "gmm_4bit.h"
 
 namespace mbx {

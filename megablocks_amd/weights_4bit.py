@@ -21,6 +21,7 @@ class Weights4bit:
         scales  [experts, ceil(n / 16), ceil(k / 128) * 128 / group, 16], fp32 or of a 16-bit type
         zeros   uint8 like the scales, or None: 8 everywhere
 
+    What lies past n and k, whole groups of scales and zeros among it, is never used and may be anything.
     trans_b: whether the weights came (and come back, `dequantize`) as [experts, n, k], else as [experts, k, n]; products are x @ W[e]^T either way."""
 
     def __init__(self, words: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], n: int, k: int, group: int, trans_b: bool = True):
