@@ -562,6 +562,30 @@ int mbx_choose_experts_backward(const void* grad_weights, const void* grad_score
 int mbx_balance_bias(const float* const* bias, const int32_t* const* counts, const int* rows, float* const* out, int layers, int num_experts, float rate,
                      mbx_stream_t stream);
 
+/* ---- rows of a table by token ----
+ * No counterpart in the reference.  out[i] = scale * table[ids[i]], in fp32, rounded once: table [words, hidden] of `dtype`, ids [tokens] (MBX_I32 or
+ * MBX_I64), out [tokens, hidden]; an id outside [0, words) gives zeros.  All contiguous, at any address their types may have.
+ * mbx_embedding_gradient: out[v] = scale * (the sum of grad[i] over ids[i] = v, i ascending, fp32), rounded once, for all words; zeros for the word `padding`
+ * (negative: none) and those no id names.  The order of a sum depends on the ids alone.  scratch: mbx_embedding_gradient_scratch_bytes bytes, 16-byte aligned.
+ * MBX_ERANGE: 2^31 - 256 tokens, 2^31 - 1 words or 2^24 columns and more. */
+int mbx_embedding(const void* ids, int itype, int64_t tokens, const void* table, int dtype, int64_t words, int64_t hidden, float scale, void* out, mbx_stream_t stream);
+size_t mbx_embedding_gradient_scratch_bytes(int64_t tokens, int64_t words, int64_t hidden);
+int mbx_embedding_gradient(const void* grad, const void* ids, int itype, int64_t tokens, int dtype, int64_t words, int64_t hidden, int64_t padding, float scale,
+                           void* out, void* scratch, size_t scratch_bytes, mbx_stream_t stream);
+
+/* ---- the norm of many tensors together, and clipping by it ----
+ * No counterpart in the reference, whose trainer does it.  norm = (sum over all values of |x|^p)^(1/p) for p = 1 and 2, max |x| for p = inf (other p:
+ * MBX_EINVAL), in fp32; sums in 64 bits, in a fixed order; a NaN gives NaN, no value 0.  The arrays of `count` pointers, element counts and types are in host
+ * memory, read before the call returns.  Tensors may start at any address their type may.  scratch: mbx_global_norm_scratch_bytes(count) bytes, 8-byte aligned.
+ *
+ * mbx_clip_by_global_norm: out[i] = tensors[i] * min(1, most / (norm + 1e-6)), in fp32, rounded once to out_dtypes[i].  out[i] may be tensors[i] with the same
+ * type; where all are and the norm is short enough nothing is written.  MBX_EINVAL: outputs that overlap each other, or a tensor in another way. */
+size_t mbx_global_norm_scratch_bytes(int count);
+int mbx_global_norm(const void* const* tensors, const int64_t* numel, const int* dtypes, int count, float p, float* norm, void* scratch, size_t scratch_bytes,
+                    mbx_stream_t stream);
+int mbx_clip_by_global_norm(const void* const* tensors, void* const* out, const int64_t* numel, const int* dtypes, const int* out_dtypes, int count, float p,
+                            float most, float* norm, void* scratch, size_t scratch_bytes, mbx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,126 @@
+"""The norm of all gradients together, and clipping by it: what a training step does between its backward and its optimizer.  The reference leaves it to the
+trainer around it, whose expert weights it marks for that purpose (megablocks/layers/mpu.py)."""
+import ctypes
+import math
+
+import torch
+
+from megablocks_amd import _lib
+from megablocks_amd._lib import lib
+
+_is_contiguous, _get_device, _data_ptr, _numel = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
+
+
+def _check_norm(what, norm_type):
+    norm_type = float(norm_type)
+    if norm_type not in (1.0, 2.0, math.inf):
+        raise ValueError(f'{what}: norms are of type 1, 2 or inf, not {norm_type}')
+    return norm_type
+
+
+def _on_one_gpu(what, tensors):
+    """The tensors as a list, checked."""
+    tensors = list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+            raise RuntimeError(f'{what}: expected dense tensors')
+    devices = set(map(_get_device, tensors))
+    dtypes = {t.dtype for t in tensors}
+    if tensors and (len(devices) > 1 or min(devices) < 0 or not dtypes <= _lib.DTYPE.keys()):
+        raise RuntimeError(f'{what}: expected bfloat16, float16 or float32 tensors on one GPU but got {sorted({f"{t.dtype} on {t.device}" for t in tensors})}')
+    if getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0 or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
+        raise RuntimeError(f'{what}: norms and clipping have no gradient; call them under torch.no_grad(), on gradients')
+    return tensors
+
+
+def _operands(tensors):
+    """(addresses, element counts, types) as the library takes them."""
+    n = len(tensors)
+    return ((ctypes.c_void_p * n)(*map(_data_ptr, tensors)), (ctypes.c_int64 * n)(*map(_numel, tensors)),
+            (ctypes.c_int * n)(*[_lib.DTYPE[t.dtype] for t in tensors]))
+
+
+def _outputs(device, n):
+    scratch = torch.empty(lib.mbx_global_norm_scratch_bytes(n), dtype=torch.uint8, device=device)
+    return torch.empty((), dtype=torch.float32, device=device), scratch
+
+
+def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all values of the tensors together, as one number in fp32 on their device: (sum |x|^p)^(1/p) for p = 1 and 2, max |x| for inf.  tensors:
+    bf16, fp16 and fp32 ones, mixed as they come, of any shape.  Sums are held in 64 bits and come out the same from run to run; a NaN gives NaN.  No tensor:
+    0, on the CPU."""
+    norm_type = _check_norm('global_norm', norm_type)
+    tensors = _on_one_gpu('global_norm', tensors)
+    if not tensors:
+        return torch.zeros((), dtype=torch.float32)
+    plain = [t if c else t.contiguous() for t, c in zip(tensors, map(_is_contiguous, tensors))]      # kept until the launch is under way
+    norm, scratch = _outputs(plain[0].device, len(plain))
+    with _lib.device_of(norm):
+        _lib.check(lib.mbx_global_norm(*_operands(plain), len(plain), norm_type, norm.data_ptr(), scratch.data_ptr(), scratch.numel(), _lib.stream()), 'global_norm')
+    return norm
+
+
+def clip_by_global_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """Multiplies the tensors by min(1, max_norm / (norm + 1e-6)), norm = `global_norm` of them all, and returns the norm before that; a norm that is NaN makes all
+    values NaN, an infinite one zeros and NaN.  In place, where the launches that would write do nothing if the norm is short enough, or into `out`: as many tensors of
+    the same sizes, in bf16, fp16 or fp32 (the fp32 gradients an optimizer reads, for instance), rounded once.  No output may lie over another, or over a tensor
+    that is not its own."""
+    norm_type, max_norm = _check_norm('clip_by_global_norm_', norm_type), float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError('clip_by_global_norm_: the largest norm must be a number from 0 on')
+    tensors = _on_one_gpu('clip_by_global_norm_', tensors)
+    outputs = tensors if out is None else _on_one_gpu('clip_by_global_norm_', out)
+    if len(outputs) != len(tensors) or any(o.shape != t.shape for t, o in zip(tensors, outputs)):
+        raise ValueError('clip_by_global_norm_: an output of the same size for every tensor')
+    if not tensors:
+        return torch.zeros((), dtype=torch.float32)
+    if outputs[0].get_device() != tensors[0].get_device():
+        raise RuntimeError('clip_by_global_norm_: tensors and outputs must be on one GPU')
+    plain = [t if c else t.contiguous() for t, c in zip(tensors, map(_is_contiguous, tensors))]
+    if out is None:
+        to = plain
+    else:
+        to = [o if c else torch.empty_like(o, memory_format=torch.contiguous_format) for o, c in zip(outputs, map(_is_contiguous, outputs))]
+    strided = [(o, made) for o, made in zip(outputs, to) if made is not o]
+    if strided:
+        _refuse_overlaps(outputs, tensors)
+    norm, scratch = _outputs(plain[0].device, len(plain))
+    in_ptrs, numels, types = _operands(plain)
+    out_ptrs, _, out_types = (in_ptrs, numels, types) if to is plain else _operands(to)
+    with _lib.device_of(norm):
+        rc = lib.mbx_clip_by_global_norm(in_ptrs, out_ptrs, numels, types, out_types, len(plain), norm_type, max_norm, norm.data_ptr(), scratch.data_ptr(),
+                                         scratch.numel(), _lib.stream())
+    if rc == _lib.EINVAL:
+        raise ValueError('clip_by_global_norm_: an output lies over another one, or over a tensor that is not its own')
+    _lib.check(rc, 'clip_by_global_norm_')
+    for o, made in strided:
+        o.copy_(made)
+    torch.autograd.graph.increment_version([o for o in outputs if not o.is_inference()])
+    return norm
+
+
+def _refuse_overlaps(outputs, tensors):
+    """The library's check of its operands, on the tensors that some of these stand for: by the memory between their first and last values."""
+    def extent(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    ranges = sorted((*extent(o), i) for i, o in enumerate(outputs) if o.numel())
+    clash = any(a[1] > b[0] for a, b in zip(ranges, ranges[1:]))
+    for i, t in enumerate(tensors):
+        if t.numel() and t is not outputs[i]:
+            begin, end = extent(t)
+            clash = clash or any(a < end and begin < b for a, b, _ in ranges)
+    if clash or any(0 in o.stride() and o.numel() > 1 for o in outputs):
+        raise ValueError('clip_by_global_norm_: an output that is not contiguous lies over another one, over a tensor that is not its own, or over itself')
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clips the gradients of the parameters (or of one) in place by their global norm, as torch.nn.utils.clip_grad_norm_ does, and returns the norm.
+    error_if_nonfinite waits for the GPU: RuntimeError, and gradients as they were, where the norm is not finite."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad.detach() for p in parameters if p.grad is not None]
+    if error_if_nonfinite and grads:
+        norm = global_norm(grads, norm_type)
+        if not torch.isfinite(norm):
+            raise RuntimeError(f'clip_grad_norm_: the norm of order {float(norm_type)} of the gradients is not finite, so they cannot be clipped')
+    return clip_by_global_norm_(grads, max_norm, norm_type)
