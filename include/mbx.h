@@ -562,6 +562,19 @@ int mbx_choose_experts_backward(const void* grad_weights, const void* grad_score
 int mbx_balance_bias(const float* const* bias, const int32_t* const* counts, const int* rows, float* const* out, int layers, int num_experts, float rate,
                      mbx_stream_t stream);
 
+/* ---- a whole layer for a few tokens ----
+ * The forward without gradients of megablocks/layers/moe.py:457-475 with dropless experts, for decoding, by two products and the choice between them and the
+ * router: x [tokens, hidden], router [num_experts, hidden], the choice as mbx_choose_experts makes it of x router^T (exact products, sums in 64 bits, rounded
+ * nowhere), weights fp32 and indices int64 [tokens, top_k]; out[t] = sum over j of weights[t, j] (act(x[t] W1[e]^T) * (x[t] V1[e]^T)) W2[e] with e = indices[t, j], w1, v1
+ * (NULL: no gate) and w2 [num_experts, ffn, hidden], fp32 sums, the activation kept to 2^-17 (fp16: 2^-23), out rounded once.  Up to 64 tokens, 512 experts, 16 a
+ * token, 64 groups, bf16 or fp16, hidden and ffn multiples of 8, all matrices 16-byte aligned (else MBX_EUNSUPPORTED); matrices of an expert below 2 GiB (else
+ * MBX_ERANGE).  scratch: mbx_moe_layer_scratch_bytes bytes (gate: whether v1 is given; 0: such a call is refused, or has no tokens), 16-byte aligned.  workspace: 4096 bytes, zero before
+ * the call and zero again after it, of no other call that may run at the same time (the head of mbx_gmm_ws's is such memory). */
+size_t mbx_moe_layer_scratch_bytes(int64_t tokens, int64_t hidden, int64_t ffn, int num_experts, int top_k, int gate);
+int mbx_moe_layer(const void* x, int64_t tokens, int64_t hidden, int dtype, const void* router, int num_experts, int top_k, int score, const float* bias, int groups,
+                  int top_groups, int group_best, float norm_p, float scale, const void* w1, const void* v1, const void* w2, int64_t ffn, int act, void* out, float* weights,
+                  int64_t* indices, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, mbx_stream_t stream);
+
 /* ---- rows of a table by token ----
  * No counterpart in the reference.  out[i] = scale * table[ids[i]], in fp32, rounded once: table [words, hidden] of `dtype`, ids [tokens] (MBX_I32 or
  * MBX_I64), out [tokens, hidden]; an id outside [0, words) gives zeros.  All contiguous, at any address their types may have.

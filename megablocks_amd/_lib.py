@@ -89,6 +89,8 @@ _SIGNATURES = {
     'mbx_choose_experts': (_i, [_vp, _i, _i64, _i, _i, _i, _vp, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _vp, _vp, _vp]),
     'mbx_choose_experts_backward': (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp]),
     'mbx_balance_bias': (_i, [_vp, _vp, _vp, _vp, _i, _i, ctypes.c_float, _vp]),
+    'mbx_moe_layer_scratch_bytes': (_sz, [_i64, _i64, _i64, _i, _i, _i]),
+    'mbx_moe_layer': (_i, [_vp, _i64, _i64, _i, _vp, _i, _i, _i, _vp, _i, _i, _i, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _i64, _i, _vp, _vp, _vp, _vp, _sz, _vp, _sz, _vp]),
     'mbx_embedding': (_i, [_vp, _i, _i64, _vp, _i, _i64, _i64, ctypes.c_float, _vp, _vp]),
     'mbx_embedding_gradient_scratch_bytes': (_sz, [_i64, _i64, _i64]),
     'mbx_embedding_gradient': (_i, [_vp, _vp, _i, _i64, _i, _i64, _i64, _i64, ctypes.c_float, _vp, _vp, _sz, _vp]),

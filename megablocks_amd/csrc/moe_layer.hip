@@ -1,0 +1,685 @@
+// A whole mixture-of-experts layer for a few tokens (up to 64), without gradients: the router, the choice of experts, their products, the weighted sum.
+//
+//   l = x Wr^T;  s = softmax(l) or 1 / (1 + exp(-l));  the top_k experts by key (l, or s + bias; open groups only);  w = scale s / ||s||_p
+//   out[t] = sum_j w[t, j] (act(x[t] W1[e]^T) * (x[t] V1[e]^T)) W2[e],  e = the j-th expert of t
+//
+// What bounds it is reading the weights of the chosen experts, once, and, for a few small ones, the way between the launches.  Three of them:
+//
+//   choose   a wave per expert and token (or eight tokens): logits as exact products summed in 64 bits, so that no order of summation decides between
+//            neighbours; the workgroup that is last at a group of tokens chooses for them, and the last of all makes the table of which experts have which rows
+//   hidden   a workgroup per used expert and 16 to 64 rows of its first weights, a quarter of the reduction a wave; the activation is kept as the sum of two
+//            16-bit numbers, so that the second product sees it to 2^-17
+//   down     a workgroup per used expert, 128 columns and a part of the reduction; the parts meet in memory, and the workgroup that is last at its columns adds them up
+//            in a fixed order, weights them and writes the output
+//
+// "Last" is counted with device-wide atomics; nobody waits for anybody.  What goes from one workgroup to another inside a launch is stored and loaded past the
+// caches (the compute units are on eight L2s that do not see each other) and counted in when the stores have been acknowledged.  Sums are taken in an order that
+// does not depend on who came when.
+#include "gmm_common.h"
+
+#include <cmath>
+
+namespace mbx {
+namespace {
+
+constexpr int kLayerTokens = 64, kLayerTopK = 16, kLayerExperts = 512, kLayerGroups = 64;
+constexpr int kLayerSlots = kLayerTokens * kLayerTopK;
+constexpr int kLayerThreads = 256, kLayerWaves = kLayerThreads / kWave;
+constexpr int kLayerMaxParts = 16;                                     // of the second product's reduction
+constexpr int kDownColumns = 128;
+// counters: 0 .. 7 groups of tokens, 8 the groups that are done, from 16 on the second product's columns
+constexpr int kCounterAll = 8, kCounterColumns = 16;
+
+// which experts have which rows; a row is an assignment (token, j), sorted by expert
+struct LayerTable {
+  int4 used[kLayerExperts];         // expert, first row, rows, 0; rows 0 past the last used one
+  int32_t slot_of_row[kLayerSlots];
+  int32_t row_of_slot[kLayerSlots];
+  int32_t experts;                  // used ones
+};
+
+struct LayerChoice {
+  int tokens, hidden, experts, top_k, sigmoid, groups, top_groups, group_best, entries;
+  float norm_p, scale;
+};
+
+__device__ __forceinline__ void store_through(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t load_through(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void store_through(int32_t* p, int32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ int32_t load_through(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether this workgroup is the last of `all` to come here; what all of them have stored through the caches can then be loaded.  Leaves the counter zero.
+__device__ __forceinline__ bool last_to_come(int32_t* counter, int all, int* flag) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
+    if (last) *counter = 0;
+    *flag = last;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// larger keys first, NaN before all, -0 as 0; 0 is below every number's
+__device__ __forceinline__ uint64_t sortable(double key) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, key + 0.0);
+  return key != key ? ~0ull : (int64_t)u < 0 ? ~u : u | 1ull << 63;
+}
+
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+__device__ __forceinline__ double wave_max_f64(double v) {
+#pragma unroll
+  for (int off = 32; off; off >>= 1) {
+    const double o = __shfl_xor(v, off, kWave);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+  return wave_butterfly(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
+  return wave_butterfly(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
+// The choice for a token by one wave: expert 64 i + lane is in register i.  scratch: this wave's, a value for every expert (groups only).
+template <int R>
+__device__ __forceinline__ void choose_for(const LayerChoice& q, int token, const uint64_t* __restrict__ logits, const float* __restrict__ bias,
+                                           double* __restrict__ scratch, float* __restrict__ weights, int64_t* __restrict__ indices, int32_t* __restrict__ choice) {
+  const int lane = lane_id();
+  double score[R];
+  uint64_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int e = i * kWave + lane;
+    score[i] = e < q.experts ? __builtin_bit_cast(double, load_through(logits + (int64_t)token * q.experts + e)) : -INFINITY;
+    key[i] = e < q.experts ? sortable(score[i]) : 0;
+  }
+  if (q.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) score[i] = 1. / (1. + exp(-score[i]));
+  } else {
+    double most = -INFINITY, sum = 0.;
+#pragma unroll
+    for (int i = 0; i < R; ++i) most = score[i] > most ? score[i] : most;
+    most = wave_max_f64(most);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      score[i] = exp(score[i] - most);
+      sum += i * kWave + lane < q.experts ? score[i] : 0.;
+    }
+    sum = wave_sum_f64(sum);
+#pragma unroll
+    for (int i = 0; i < R; ++i) score[i] /= sum;
+  }
+  if (bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int e = i * kWave + lane;
+      if (e < q.experts) key[i] = sortable(score[i] + (double)bias[e]);
+    }
+  }
+  if (q.top_groups < q.groups) {
+    const int size = q.experts / q.groups;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int e = i * kWave + lane;
+      if (e < q.experts) scratch[e] = bias != nullptr ? score[i] + (double)bias[e] : score[i];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    double best = -INFINITY, second = -INFINITY;
+    if (lane < q.groups)
+      for (int i = 0; i < size; ++i) {
+        const double v = scratch[lane * size + i];
+        if (v > best || v != v) { second = best; best = v; }
+        else if (v > second) second = v;
+      }
+    const uint64_t mine = lane < q.groups ? sortable(q.group_best == 2 && size > 1 ? best + second : best) : 0;
+    int before = 0;
+    for (int g = 0; g < q.groups; ++g) {
+      const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), g) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, g);
+      before += other > mine || (other == mine && g < lane) ? 1 : 0;
+    }
+    const uint64_t open = __ballot(lane < q.groups && before < q.top_groups);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int e = i * kWave + lane;
+      if (e < q.experts && !(open >> (e / size) & 1)) key[i] = 0;
+    }
+  }
+  int my_expert = 0;          // lane j: the j-th of the choice
+  double my_score = 0.;
+  for (int j = 0; j < q.top_k; ++j) {
+    uint64_t best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < R; ++i)
+      if (key[i] > best) { best = key[i]; at = i; }
+    const uint32_t high = wave_max_u32((uint32_t)(best >> 32));
+    const bool high_is = (uint32_t)(best >> 32) == high;
+    const uint32_t low = wave_max_u32(high_is ? (uint32_t)best : 0u);
+    const int e = __builtin_amdgcn_readfirstlane((int)wave_min_u32(high_is && (uint32_t)best == low ? (uint32_t)(at * kWave + lane) : ~0u));
+    const int from = e % kWave, reg = e / kWave;
+    double s = 0.;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (i == reg) {
+        s = score[i];
+        if (lane == from) key[i] = 0;
+      }
+    const uint64_t bits = __builtin_bit_cast(uint64_t, s);
+    s = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(bits >> 32), from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)bits, from));
+    if (lane == j) {
+      my_expert = e;
+      my_score = s;
+    }
+  }
+  double norm = 1.;
+  if (q.norm_p > 0.f) {
+    const double p = q.norm_p, s = lane < q.top_k ? my_score : 0.;
+    norm = wave_sum_f64(p == 1. ? s : p == 2. ? s * s : lane < q.top_k ? pow(s, p) : 0.);
+    norm = p == 1. ? norm : p == 2. ? sqrt(norm) : pow(norm, 1. / p);
+  }
+  if (lane < q.top_k) {
+    const int64_t at = (int64_t)token * q.top_k + lane;
+    weights[at] = (float)(norm == 0. ? 0. : my_score / norm * (double)q.scale);
+    indices[at] = my_expert;
+    store_through(choice + at, my_expert);
+  }
+}
+
+// ---- choose ----
+// Workgroup (b, g): experts 4 b .. 4 b + 3, a wave each, tokens TB g .. ; TB 1 or 8.
+template <int DT, int TB, int R>
+__global__ void __launch_bounds__(kLayerThreads)
+layer_choose_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ router, LayerChoice q, const float* __restrict__ bias, uint64_t* __restrict__ logits,
+                    int32_t* __restrict__ choice, float* __restrict__ weights, int64_t* __restrict__ indices, LayerTable* __restrict__ table, int32_t* __restrict__ counters) {
+  __shared__ double scratch[kLayerWaves][R * kWave];
+  __shared__ int flag;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int e = (int)blockIdx.x * kLayerWaves + wave, t0 = (int)blockIdx.y * TB, tokens = q.tokens - t0 < TB ? q.tokens - t0 : TB;
+  typedef typename Elem<DT>::type E;
+  if (e < q.experts) {
+    constexpr int kAhead = TB == 1 ? 8 : 2, kStep = kWave * 8;
+    double acc[TB];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) acc[t] = 0.;
+    const uint16_t* const w_row = router + (int64_t)e * q.hidden;
+    for (int c0 = lane * 8; c0 < q.hidden; c0 += kAhead * kStep) {
+      u32x4 w[kAhead], v[kAhead][TB];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int c = c0 + u * kStep;
+        const bool here = c < q.hidden;
+        w[u] = here ? *(const u32x4*)(w_row + c) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int t = 0; t < TB; ++t) v[u][t] = here && t < tokens ? *(const u32x4*)(x + (int64_t)(t0 + t) * q.hidden + c) : u32x4{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const double wd = Elem<DT>::to_f32(__builtin_bit_cast(E, (uint16_t)(w[u][i >> 1] >> ((i & 1) * 16))));
+#pragma unroll
+          for (int t = 0; t < TB; ++t)
+            acc[t] = __builtin_fma(wd, (double)Elem<DT>::to_f32(__builtin_bit_cast(E, (uint16_t)(v[u][t][i >> 1] >> ((i & 1) * 16)))), acc[t]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const double l = wave_sum_f64(acc[t]);
+      if (lane == 0 && t < tokens) store_through(logits + (int64_t)(t0 + t) * q.experts + e, __builtin_bit_cast(uint64_t, l));
+    }
+  }
+  if (!last_to_come(counters + blockIdx.y, (int)gridDim.x, &flag)) return;
+  for (int t = t0 + wave; t < t0 + tokens; t += kLayerWaves) choose_for<R>(q, t, logits, bias, scratch[wave], weights, indices, choice);
+  if (!last_to_come(counters + kCounterAll, (int)gridDim.y, &flag)) return;
+  // the table: experts 2 i and 2 i + 1 are thread i's
+  __shared__ int32_t count[kLayerExperts], first[kLayerExperts], sums[kLayerWaves];
+  const int slots = q.tokens * q.top_k, i = threadIdx.x;
+  count[2 * i] = count[2 * i + 1] = 0;
+  __syncthreads();
+  int expert[kLayerSlots / kLayerThreads], rank[kLayerSlots / kLayerThreads];
+#pragma unroll
+  for (int n = 0; n < kLayerSlots / kLayerThreads; ++n) {
+    const int s = i + n * kLayerThreads;
+    expert[n] = s < slots ? load_through(choice + s) : 0;
+  }
+#pragma unroll
+  for (int n = 0; n < kLayerSlots / kLayerThreads; ++n)      // the order of an expert's rows is nobody's business: each is computed by itself
+    if (i + n * kLayerThreads < slots) rank[n] = atomicAdd(&count[expert[n]], 1);
+  __syncthreads();
+  const int c0 = count[2 * i], c1 = count[2 * i + 1];
+  const int mine = c0 + c1 | ((c0 > 0) + (c1 > 0)) << 16;    // rows, used experts
+  const int through = wave_inclusive_scan(mine);
+  if (lane == kWave - 1) sums[wave] = through;
+  __syncthreads();
+  int before = through - mine, all = 0;
+#pragma unroll
+  for (int w = 0; w < kLayerWaves; ++w) {
+    before += w < wave ? sums[w] : 0;
+    all += sums[w];
+  }
+  const int row = before & 0xffff, used = all >> 16;
+  int u = before >> 16;
+  first[2 * i] = row;
+  first[2 * i + 1] = row + c0;
+  if (c0 > 0) table->used[u++] = make_int4(2 * i, row, c0, 0);
+  if (c1 > 0) table->used[u] = make_int4(2 * i + 1, row + c0, c1, 0);
+  for (int n = used + i; n < q.entries; n += kLayerThreads) table->used[n] = make_int4(0, 0, 0, 0);
+  if (i == 0) table->experts = used;
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kLayerSlots / kLayerThreads; ++n) {
+    const int s = i + n * kLayerThreads;
+    if (s < slots) {
+      const int at = first[expert[n]] + rank[n];
+      table->slot_of_row[at] = s;
+      table->row_of_slot[s] = at;
+    }
+  }
+}
+
+// ---- products ----
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if (DT == MBX_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+constexpr uint32_t kNone = 0x80000000u;      // an offset past every buffer: the load brings zeros
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t at) { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0)); }
+
+__device__ __forceinline__ float activated(float x, int act) {
+  // silu: x / (1 + exp(-x));  gelu: x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+  const float z = act == MBX_ACT_SILU ? x * -1.44269504f : x * (-0.102943240f * (x * x) - 2.30220819f);
+  return x / (1.f + __builtin_amdgcn_exp2f(z));
+}
+
+// v as the sum of two 16-bit numbers
+template <int DT>
+__device__ __forceinline__ void in_two(float v, uint16_t& hi, uint16_t& lo) {
+  typedef typename Elem<DT>::type E;
+  const E h = Elem<DT>::from_f32(v);
+  const float rest = v - Elem<DT>::to_f32(h);
+  hi = __builtin_bit_cast(uint16_t, h);
+  lo = __builtin_bit_cast(uint16_t, Elem<DT>::from_f32(rest - rest == 0.f ? rest : 0.f));     // an infinity or NaN has no rest
+}
+
+// NF fragments of 16 weight rows (with the gate: half of them W1's, half V1's), up to R tiles of 16 token rows.  In a chunk of 64 columns lane (c = l % 16,
+// g = l / 16) has columns 16 g .. 16 g + 15 of weight row c and of token row c: 32 bytes each.
+template <int DT, bool GATE, int NF, int R>
+__global__ void __launch_bounds__(kLayerThreads)
+layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w1, const uint16_t* __restrict__ v1, const LayerTable* __restrict__ table, int tokens,
+                    int top_k, int hidden, int ffn, int tiles, int act, uint16_t* __restrict__ h_hi, uint16_t* __restrict__ h_lo) {
+  constexpr int kCols = GATE ? NF * 8 : NF * 16;          // output columns
+  constexpr int kPitch = NF * 16 + 4, kChunk = 64;
+  __shared__ __attribute__((aligned(16))) float sums[kLayerWaves][16][kPitch];
+  const int u = (int)blockIdx.x / tiles, f0 = ((int)blockIdx.x - u * tiles) * kCols;
+  const int4 it = table->used[u];
+  if (it.z == 0) return;
+  const int expert = it.x, first = it.y, rows = it.z, row_tiles = (rows + 15) / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const uint32_t pitch = (uint32_t)hidden * 2u;
+  const int64_t matrix = (int64_t)ffn * hidden;
+  const __amdgpu_buffer_rsrc_t rsrc_x = rsrc_of(x, (uint32_t)tokens * pitch), rsrc_w = rsrc_of(w1 + expert * matrix, (uint32_t)(matrix * 2));
+  const __amdgpu_buffer_rsrc_t rsrc_v = GATE ? rsrc_of(v1 + expert * matrix, (uint32_t)(matrix * 2)) : rsrc_w;
+  uint32_t x_off[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) {
+    const int r = t * 16 + c;
+    x_off[t] = r < rows ? (uint32_t)(table->slot_of_row[first + r] / top_k) * pitch + (uint32_t)g * 32u : kNone;
+  }
+  const uint32_t w_off = (uint32_t)(f0 + c) * pitch + (uint32_t)g * 32u;
+  struct Chunk { u32x4 a[R][2], b[NF][2]; };
+  const int chunks = (hidden + kChunk - 1) / kChunk;
+  auto fetch = [&](Chunk& q, int chunk) {
+    const uint32_t at = (uint32_t)chunk * (kChunk * 2);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t past = chunk * kChunk + 16 * g + 8 * s < hidden ? 0u : kNone;      // pieces past the row's end
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const int row = GATE ? f % (NF / 2 > 0 ? NF / 2 : 1) : f;
+        q.b[f][s] = load16(GATE && f >= NF / 2 ? rsrc_v : rsrc_w, (w_off + at + (uint32_t)(row * 16) * pitch + 16u * s) | past);
+      }
+#pragma unroll
+      for (int t = 0; t < R; ++t)
+        if (t == 0 || t < row_tiles) q.a[t][s] = load16(rsrc_x, (x_off[t] + at + 16u * s) | past | (x_off[t] & kNone));
+    }
+  };
+  f32x4 acc[R][NF];
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[t][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Chunk& q) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < R; ++t)
+        if (t == 0 || t < row_tiles)
+#pragma unroll
+          for (int f = 0; f < NF; ++f) acc[t][f] = mfma<DT>(q.b[f][s], q.a[t][s], acc[t][f]);
+  };
+  // the waves take the chunks in turn; past the last one nothing is fetched
+  Chunk q0, q1;
+  fetch(q0, wave);
+  for (int chunk = wave; chunk < chunks; chunk += 2 * kLayerWaves) {
+    fetch(q1, chunk + kLayerWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(q0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(q0, chunk + 2 * kLayerWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(q1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // accumulator t, f, register i of lane (c, g): token row 16 t + c, weight row 16 f + 4 g + i
+  constexpr int kEach = kCols / 16;
+  const int m = threadIdx.x / 16, col = threadIdx.x % 16 * kEach;
+  for (int t = 0; t < row_tiles; ++t) {
+    if (t > 0) __syncthreads();
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      f32x4 v = acc[0][f];
+#pragma unroll
+      for (int o = 1; o < R; ++o)
+        if (t == o) v = acc[o][f];
+      *(f32x4*)&sums[wave][c][f * 16 + 4 * g] = v;
+    }
+    __syncthreads();
+    const int r = t * 16 + m;
+    if (r < rows && f0 + col < ffn) {      // ffn is a multiple of 8, a thread's columns 1, 2 or 4
+      uint16_t hi[kEach], lo[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        float v = 0.f, gate = 0.f;
+#pragma unroll
+        for (int w = 0; w < kLayerWaves; ++w) {
+          v += sums[w][m][col + i];
+          if (GATE) gate += sums[w][m][kCols + col + i];
+        }
+        v = activated(v, act);
+        in_two<DT>(GATE ? v * gate : v, hi[i], lo[i]);
+      }
+      const int64_t at = (int64_t)(first + r) * ffn + f0 + col;
+      __builtin_memcpy(h_hi + at, hi, sizeof(hi));
+      __builtin_memcpy(h_lo + at, lo, sizeof(lo));
+    }
+  }
+}
+
+// Second product: 128 columns, in chunks of 32 rows of W2.  Lane (c, g) reads columns 8 c .. 8 c + 7 of rows 8 g .. 8 g + 7, 16 bytes each (256 contiguous bytes a
+// row), and turns the 8 x 8 values over with byte permutes: fragment j has column 8 c + j of those rows.
+template <int DT, int R>
+__global__ void __launch_bounds__(kLayerThreads)
+layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict__ h_lo, const uint16_t* __restrict__ w2, const LayerTable* __restrict__ table, int tokens,
+                  int top_k, int hidden, int ffn, int tiles, int parts, const float* __restrict__ weights, float* __restrict__ sums_of_parts, uint16_t* __restrict__ out,
+                  int32_t* __restrict__ counters) {
+  constexpr int kPitch = kDownColumns + 4, kChunk = 32, kThrough = 0x11;      // cache policy: past the caches
+  __shared__ __attribute__((aligned(16))) float sums[kLayerWaves][16][kPitch];
+  __shared__ int flag;
+  const int per_expert = tiles * parts, u = (int)blockIdx.x / per_expert, in = (int)blockIdx.x - u * per_expert;
+  const int part = in / tiles, tile = in - part * tiles, n0 = tile * kDownColumns;
+  const int4 it = table->used[u];
+  if (it.z == 0) return;
+  const int expert = it.x, first = it.y, rows = it.z, row_tiles = (rows + 15) / 16, slots = tokens * top_k;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), c = lane & 15, g = lane >> 4;
+  const uint32_t pitch = (uint32_t)hidden * 2u, h_pitch = (uint32_t)ffn * 2u;
+  const int64_t matrix = (int64_t)ffn * hidden;
+  const __amdgpu_buffer_rsrc_t rsrc_w = rsrc_of(w2 + expert * matrix, (uint32_t)(matrix * 2));
+  const __amdgpu_buffer_rsrc_t rsrc_hi = rsrc_of(h_hi, (uint32_t)slots * h_pitch), rsrc_lo = rsrc_of(h_lo, (uint32_t)slots * h_pitch);
+  const uint32_t w_off = n0 + 8 * c < hidden ? (uint32_t)(8 * g) * pitch + (uint32_t)(n0 + 8 * c) * 2u : kNone;
+  uint32_t h_off[R];
+#pragma unroll
+  for (int t = 0; t < R; ++t) h_off[t] = t * 16 + c < rows ? (uint32_t)(first + t * 16 + c) * h_pitch + (uint32_t)g * 16u : kNone;
+  const int chunks = (ffn + kChunk - 1) / kChunk, begin = (int)((int64_t)part * chunks / parts), end = (int)((int64_t)(part + 1) * chunks / parts);
+  struct Chunk { u32x4 hi[R], lo[R], b[8]; };
+  auto fetch = [&](Chunk& q, int chunk) {
+    const uint32_t none = chunk < end && w_off != kNone ? 0u : kNone;
+    const uint32_t at = w_off + (uint32_t)chunk * kChunk * pitch;      // rows past ffn are past the buffer
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q.b[i] = load16(rsrc_w, (at + (uint32_t)i * pitch) | none);
+    const uint32_t past = chunk < end && chunk * kChunk + 8 * g < ffn ? 0u : kNone;
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+      if (t == 0 || t < row_tiles) {
+        const uint32_t h_at = (h_off[t] + (uint32_t)chunk * (kChunk * 2)) | past | (h_off[t] & kNone);
+        q.hi[t] = load16(rsrc_hi, h_at);
+        q.lo[t] = load16(rsrc_lo, h_at);
+      }
+  };
+  f32x4 acc[R][8];
+#pragma unroll
+  for (int t = 0; t < R; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Chunk& q) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      u32x4 b;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) b[w] = __builtin_amdgcn_perm(q.b[2 * w + 1][j >> 1], q.b[2 * w][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < R; ++t)
+        if (t == 0 || t < row_tiles) {
+          acc[t][j] = mfma<DT>(b, q.hi[t], acc[t][j]);
+          acc[t][j] = mfma<DT>(b, q.lo[t], acc[t][j]);
+        }
+    }
+  };
+  Chunk q0, q1;
+  fetch(q0, begin + wave);
+  for (int chunk = begin + wave; chunk < end; chunk += 2 * kLayerWaves) {
+    fetch(q1, chunk + kLayerWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(q0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(q0, chunk + 2 * kLayerWaves);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(q1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // accumulator t, j, register i of lane (c, g): token row 16 t + c, column 8 (4 g + i) + j
+  const int m = threadIdx.x / 16, col = threadIdx.x % 16 * 8;
+  const bool mine = n0 + col < hidden;          // a multiple of 8
+  // a part's sums lie [part][row][column]
+  const __amdgpu_buffer_rsrc_t rsrc_parts = rsrc_of(sums_of_parts, (uint32_t)parts * (uint32_t)slots * (uint32_t)hidden * 4u);
+  for (int t = 0; t < row_tiles; ++t) {
+    if (t > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x4 lo, hi;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        lo[j] = acc[0][j][i];
+        hi[j] = acc[0][4 + j][i];
+#pragma unroll
+        for (int o = 1; o < R; ++o)
+          if (t == o) {
+            lo[j] = acc[o][j][i];
+            hi[j] = acc[o][4 + j][i];
+          }
+      }
+      *(f32x4*)&sums[wave][c][8 * (4 * g + i)] = lo;
+      *(f32x4*)&sums[wave][c][8 * (4 * g + i) + 4] = hi;
+    }
+    __syncthreads();
+    if (t * 16 + m < rows && mine) {
+      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+      for (int w = 0; w < kLayerWaves; ++w) {
+        lo += *(const f32x4*)&sums[w][m][col];
+        hi += *(const f32x4*)&sums[w][m][col + 4];
+      }
+      const uint32_t at = (((uint32_t)part * (uint32_t)slots + (uint32_t)(first + t * 16 + m)) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rsrc_parts, (int)at, 0, kThrough);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rsrc_parts, (int)at + 16, 0, kThrough);
+    }
+  }
+  if (!last_to_come(counters + kCounterColumns + tile, table->experts * parts, &flag)) return;
+  // all rows of these columns are there: a token's are weighted and added up, parts first, then experts as they were chosen
+  if (!mine) return;
+  for (int t = m; t < tokens; t += 16) {
+    constexpr int kAhead = 8;
+    const int pieces = top_k * parts;
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo, y_lo = lo, y_hi = lo;
+    for (int q = 0; q < pieces; q += kAhead) {
+      u32x4 a[kAhead], b[kAhead];
+      float w[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int now = q + i < pieces ? q + i : pieces - 1, j = now / parts, p = now - j * parts, s = t * top_k + j;
+        const uint32_t at = (((uint32_t)p * (uint32_t)slots + (uint32_t)table->row_of_slot[s]) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
+        a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc_parts, (int)at, 0, kThrough));
+        b[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc_parts, (int)at + 16, 0, kThrough));
+        w[i] = weights[s];
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (q + i >= pieces) break;
+        y_lo += __builtin_bit_cast(f32x4, a[i]);
+        y_hi += __builtin_bit_cast(f32x4, b[i]);
+        if ((q + i + 1) % parts == 0) {
+          lo += y_lo * w[i];
+          hi += y_hi * w[i];
+          y_lo = y_hi = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
+    }
+    const u32x4 v = {pack2<DT>(lo[0], lo[1]), pack2<DT>(lo[2], lo[3]), pack2<DT>(hi[0], hi[1]), pack2<DT>(hi[2], hi[3])};
+    *(u32x4*)(out + (int64_t)t * hidden + n0 + col) = v;
+  }
+}
+
+// ---- host ----
+struct LayerPlan {
+  int entries;              // experts that can have a row
+  int fragments, hidden_tiles;
+  int down_tiles, parts;
+  size_t table, choice, logits, h_hi, h_lo, sums, total = 0;
+
+  LayerPlan(int tokens, int hidden, int ffn, int experts, int top_k, bool gate) {
+    const int slots = tokens * top_k;
+    entries = slots < experts ? slots : experts;
+    // experts that get a row where tokens choose evenly
+    const double used = fmin(slots, experts * (1. - pow(1. - (double)top_k / experts, tokens)));
+    const int wide = gate ? 8 : 16;
+    fragments = 4;
+    while (fragments > (gate ? 2 : 1) && used * ceil_div(ffn, fragments * wide) < 512) fragments /= 2;
+    hidden_tiles = (int)ceil_div(ffn, fragments * wide);
+    down_tiles = (int)ceil_div(hidden, kDownColumns);
+    parts = 1;
+    while (parts < kLayerMaxParts && used * down_tiles * parts < 384 && ceil_div(ffn, 32) >= parts * 2 * kLayerWaves) parts *= 2;
+    auto take = [&](size_t bytes) {
+      const size_t at = total;
+      total += (bytes + 255) & ~(size_t)255;
+      return at;
+    };
+    table = take(sizeof(LayerTable));
+    choice = take((size_t)slots * 4);
+    logits = take((size_t)tokens * experts * 8);
+    h_hi = take((size_t)slots * ffn * 2);
+    h_lo = take((size_t)slots * ffn * 2);
+    sums = take((size_t)parts * slots * hidden * 4);
+  }
+};
+
+// 0, or why not
+int layer_sizes(int64_t tokens, int64_t hidden, int64_t ffn, int experts, int top_k) {
+  if (tokens < 0 || hidden < 0 || ffn < 0 || experts <= 0 || top_k <= 0 || top_k > experts) return MBX_EINVAL;
+  if (tokens > kLayerTokens || top_k > kLayerTopK || experts > kLayerExperts || hidden == 0 || ffn == 0 || hidden % 8 || ffn % 8) return MBX_EUNSUPPORTED;
+  // 32-bit offsets into an expert's matrix (and the rows past it that a tile's fragments ask for), into the hidden rows and the parts; a counter for every tile
+  if ((ffn + 64) * hidden * 2 >= (int64_t)1 << 31 || (hidden + 64) * ffn * 2 >= (int64_t)1 << 31 || hidden > (int64_t)(kWorkspaceCounters - kCounterColumns) * kDownColumns ||
+      tokens * top_k * ffn * 2 >= (int64_t)1 << 31 || tokens * top_k * hidden * 4 * kLayerMaxParts >= (int64_t)1 << 31 || experts * hidden * 2 >= (int64_t)1 << 31)
+    return MBX_ERANGE;
+  return 0;
+}
+
+template <int DT, int TB, int R>
+void launch_choose(const void* x, const void* router, const LayerChoice& q, const float* bias, char* base, const LayerPlan& plan, float* weights, int64_t* indices,
+                   int32_t* counters, hipStream_t s) {
+  layer_choose_kernel<DT, TB, R><<<dim3((unsigned)ceil_div(q.experts, kLayerWaves), (unsigned)ceil_div(q.tokens, TB)), kLayerThreads, 0, s>>>(
+      (const uint16_t*)x, (const uint16_t*)router, q, bias, (uint64_t*)(base + plan.logits), (int32_t*)(base + plan.choice), weights, indices, (LayerTable*)(base + plan.table), counters);
+}
+
+template <int DT, int R>
+void launch_products(const void* x, const void* w1, const void* v1, const void* w2, const LayerChoice& q, int ffn, int act, char* base, const LayerPlan& plan,
+                     const float* weights, void* out, int32_t* counters, hipStream_t s) {
+  const LayerTable* const table = (const LayerTable*)(base + plan.table);
+  uint16_t *const hi = (uint16_t*)(base + plan.h_hi), *const lo = (uint16_t*)(base + plan.h_lo);
+  const unsigned grid = (unsigned)(plan.entries * plan.hidden_tiles);
+#define MBX_LAYER_HIDDEN(GATE, NF) \
+  layer_hidden_kernel<DT, GATE, NF, R><<<grid, kLayerThreads, 0, s>>>((const uint16_t*)x, (const uint16_t*)w1, (const uint16_t*)v1, table, q.tokens, q.top_k, q.hidden, ffn, plan.hidden_tiles, act, hi, lo)
+  if (v1) {
+    if (plan.fragments == 4) MBX_LAYER_HIDDEN(true, 4); else MBX_LAYER_HIDDEN(true, 2);
+  } else {
+    if (plan.fragments == 4) MBX_LAYER_HIDDEN(false, 4); else if (plan.fragments == 2) MBX_LAYER_HIDDEN(false, 2); else MBX_LAYER_HIDDEN(false, 1);
+  }
+#undef MBX_LAYER_HIDDEN
+  layer_down_kernel<DT, R><<<(unsigned)(plan.entries * plan.down_tiles * plan.parts), kLayerThreads, 0, s>>>(
+      hi, lo, (const uint16_t*)w2, table, q.tokens, q.top_k, q.hidden, ffn, plan.down_tiles, plan.parts, weights, (float*)(base + plan.sums), (uint16_t*)out, counters);
+}
+
+template <int DT>
+int launch_layer(const void* x, const void* router, const void* w1, const void* v1, const void* w2, const LayerChoice& q, const float* bias, int ffn, int act, void* out,
+                 float* weights, int64_t* indices, char* base, const LayerPlan& plan, int32_t* counters, hipStream_t s) {
+#define MBX_LAYER_CHOOSE(TB) \
+  (q.experts <= 64 ? launch_choose<DT, TB, 1>(x, router, q, bias, base, plan, weights, indices, counters, s) \
+   : q.experts <= 256 ? launch_choose<DT, TB, 4>(x, router, q, bias, base, plan, weights, indices, counters, s) \
+                      : launch_choose<DT, TB, 8>(x, router, q, bias, base, plan, weights, indices, counters, s))
+  if (q.tokens <= 8) MBX_LAYER_CHOOSE(1); else MBX_LAYER_CHOOSE(8);
+#undef MBX_LAYER_CHOOSE
+  if (q.tokens <= 16) launch_products<DT, 1>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  else if (q.tokens <= 32) launch_products<DT, 2>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  else launch_products<DT, 4>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  return launch_status();
+}
+
+}  // namespace
+}  // namespace mbx
+
+using namespace mbx;
+
+extern "C" {
+
+size_t mbx_moe_layer_scratch_bytes(int64_t tokens, int64_t hidden, int64_t ffn, int num_experts, int top_k, int gate) {
+  if (layer_sizes(tokens, hidden, ffn, num_experts, top_k) || tokens == 0) return 0;
+  return LayerPlan((int)tokens, (int)hidden, (int)ffn, num_experts, top_k, gate != 0).total;
+}
+
+int mbx_moe_layer(const void* x, int64_t tokens, int64_t hidden, int dtype, const void* router, int num_experts, int top_k, int score, const float* bias, int groups,
+                  int top_groups, int group_best, float norm_p, float scale, const void* w1, const void* v1, const void* w2, int64_t ffn, int act, void* out, float* weights,
+                  int64_t* indices, void* scratch, size_t scratch_bytes, void* workspace, size_t workspace_bytes, mbx_stream_t stream) {
+  if (const int rc = layer_sizes(tokens, hidden, ffn, num_experts, top_k)) return rc;
+  if ((score != MBX_SCORE_SOFTMAX && score != MBX_SCORE_SIGMOID) || groups <= 0 || num_experts % groups || top_groups <= 0 || top_groups > groups ||
+      (group_best != 1 && group_best != 2) || top_k > top_groups * (num_experts / groups) || !(norm_p >= 0.f) || std::isinf(norm_p) || !std::isfinite(scale) ||
+      (act != MBX_ACT_SILU && act != MBX_ACT_GELU_TANH))
+    return MBX_EINVAL;
+  if ((dtype != MBX_BF16 && dtype != MBX_F16) || groups > kLayerGroups) return MBX_EUNSUPPORTED;
+  if (tokens == 0) return 0;
+  if (!x || !router || !w1 || !w2 || !out || !weights || !indices) return MBX_EINVAL;
+  if (((uintptr_t)x | (uintptr_t)router | (uintptr_t)w1 | (uintptr_t)v1 | (uintptr_t)w2 | (uintptr_t)out) & 15) return MBX_EUNSUPPORTED;
+  const LayerPlan plan((int)tokens, (int)hidden, (int)ffn, num_experts, top_k, v1 != nullptr);
+  if (!scratch || scratch_bytes < plan.total || ((uintptr_t)scratch & 15)) return MBX_ESCRATCH;
+  if (!workspace || workspace_bytes < kWorkspaceCounters * sizeof(int32_t) || ((uintptr_t)workspace & 3)) return MBX_ESCRATCH;
+  const LayerChoice q{(int)tokens, (int)hidden, num_experts, top_k, score == MBX_SCORE_SIGMOID, groups, top_groups, group_best, plan.entries, norm_p, scale};
+  hipStream_t s = as_stream(stream);
+  return dtype == MBX_BF16 ? launch_layer<MBX_BF16>(x, router, w1, v1, w2, q, bias, (int)ffn, act, out, weights, indices, (char*)scratch, plan, (int32_t*)workspace, s)
+                           : launch_layer<MBX_F16>(x, router, w1, v1, w2, q, bias, (int)ffn, act, out, weights, indices, (char*)scratch, plan, (int32_t*)workspace, s);
+}
+
+}  // extern "C"

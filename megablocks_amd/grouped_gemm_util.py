@@ -98,8 +98,11 @@ _captured_workspaces = {}   # (device, stream) -> (capture, buffer), of the last
 
 def _workspace(device):
     """(pointer, bytes) of the current stream's workspace on `device`; (None, 0) if switched off."""
-    if not GMM_WORKSPACE:
-        return None, 0
+    return _counters(device) if GMM_WORKSPACE else (None, 0)
+
+
+def _counters(device):
+    """The workspace whether or not the products may use it: its head is counters that are zero between launches (`mbx_moe_layer` needs them)."""
     stream = _lib.stream()
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream.value)
     if torch.cuda.is_current_stream_capturing():

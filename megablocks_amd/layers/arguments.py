@@ -79,11 +79,17 @@ class Arguments:
     moe_router_group_best: int = 2
     moe_router_scale: float = 1.0
 
+    # Decoding: a dropless layer in evaluation and without gradients runs up to this many tokens (64 at most; 0: none) as one operator (ops.moe_layer),
+    # whose results are rounded in fewer places than the separate ones'.
+    moe_fused_tokens: int = 0
+
     def __post_init__(self):
         if self.moe_expert_model_parallelism:
             raise NotImplementedError('expert model parallelism is not part of this single-GPU build')
         if self.shared_expert:
             raise NotImplementedError('the shared expert is not part of the dropless-MoE hot path')
+        if not 0 <= self.moe_fused_tokens <= 64:
+            raise ValueError(f'moe_fused_tokens must be from 0 to 64, not {self.moe_fused_tokens}')
         if self.shared_expert_hidden_size is None:
             self.shared_expert_hidden_size = self.ffn_hidden_size
 

@@ -8,6 +8,8 @@ import numpy as np
 import torch
 
 import megablocks_amd.ops as ops
+from megablocks_amd import _lib
+from megablocks_amd.ops import few_tokens
 from megablocks_amd.ops import routing as ops_routing
 from megablocks_amd import grouped_gemm_util as gg
 from megablocks_amd.layers import common, dmlp_registry, moe, mpu, router
@@ -266,6 +268,36 @@ class dMoE(moe.MoE):
 
     def _init_experts_mlp(self, args: Arguments):
         return ParallelDroplessMLP(args)
+
+    def _few_tokens(self, x: torch.Tensor):
+        """Up to args.moe_fused_tokens tokens by ops.moe_layer, in evaluation and without gradients, where the layer, its router and its experts are the built-in ones and
+        nobody looks at one of them by itself; else None."""
+        args, gate, experts = self.experts.args, self.router, self.experts
+        if args.moe_fused_tokens == 0 or torch.is_grad_enabled() or type(x) is not torch.Tensor or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or \
+                type(self) is not dMoE or type(gate) is not router.LearnedRouter or type(experts) is not ParallelDroplessMLP or \
+                self.training or gate.training or experts.training:
+            return None
+        hidden = x.shape[-1]
+        tokens = x.numel() // hidden if hidden else 0
+        if not 0 < tokens <= args.moe_fused_tokens or args.uniform_expert_assignment or args.moe_zloss_weight != 0 or args.mlp_impl != 'grouped' or not _only_computed() or \
+                any(router._has_hooks(m) for m in (gate, gate.layer, experts, experts.mlp)) or type(gate.layer) is not torch.nn.Linear or gate.layer.bias is not None or \
+                not gate.__dict__.keys().isdisjoint(('route', '_top_k', '_choose')) or experts.forward_fn != experts.forward_once or \
+                not experts.__dict__.keys().isdisjoint(('forward_once', 'grouped_forward_once')):
+            return None
+        known = experts._one_call_experts()
+        if known is None:
+            return None
+        act, w1, v1, w2 = known
+        weight, num_experts, top_k = gate.layer.weight, args.moe_num_experts, args.moe_top_k
+        ffn = w1.numel() // (num_experts * hidden)
+        if any(type(w) is not torch.nn.Parameter or w.dtype != x.dtype or w.device != x.device or not w.is_contiguous() or w.data_ptr() % 16
+               for w in (weight, w1, v1, w2) if w is not None) or weight.shape != (num_experts, hidden) or \
+                any(w.numel() != num_experts * ffn * hidden for w in (w1, v1, w2) if w is not None) or not few_tokens.takes(tokens, hidden, ffn, num_experts, top_k):
+            return None
+        out, _, _ = few_tokens.launch(x.reshape(-1, hidden), weight, w1, v1, w2, ffn, top_k, act, args.moe_router_score, getattr(gate, 'balance_bias', None),
+                                      args.moe_router_groups, args.moe_router_top_groups, args.moe_router_group_best, float(args.moe_normalize_expert_weights or 0),
+                                      float(args.moe_router_scale))
+        return out.view(x.shape)
 
     def quantize_experts_(self, group_size: int = 128, zero_points: bool = False):
         """The experts' weights in 4 bits, for serving (ParallelDroplessMLP.quantize_experts_).  Returns the layer."""

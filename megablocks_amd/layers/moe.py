@@ -171,7 +171,9 @@ class ParallelMLP(torch.nn.Module):
         self.tokens_per_expert = tokens_per_expert if self.args.moe_router_bias and self.training and torch.is_grad_enabled() else None
         if self.training and self.args.moe_loss_weight > 0:
             save_load_balancing_loss((tokens_per_expert, scores))
-        x = x.view(in_shape)
+        return self.with_bias(x.view(in_shape))
+
+    def with_bias(self, x):
         if self.bias is not None:
             if self.args.return_bias:
                 return x, self.bias
@@ -191,8 +193,15 @@ class MoE(torch.nn.Module):
     def _init_experts_mlp(self, args: Arguments):
         return ParallelMLP(args)
 
+    def _few_tokens(self, x: torch.Tensor):
+        """The layer's output, without its bias, where it is computed as one operator; None: as router and experts."""
+        return None
+
     def forward(self, x: torch.Tensor):
         x = common.cast_if_autocast_enabled(x)
+        out = self._few_tokens(x)
+        if out is not None:
+            return self.experts.with_bias(out)
         # Called as a module (moe.py:468), so that hooks on the router and routers that only define forward() work.
         # LearnedRouter hangs the int32 copy of its indices, which its kernel writes anyway, on the int64 tensor it
         # returns; the routing takes that copy (no cast, moe.py:160) unless something has replaced or rewritten the

@@ -1,0 +1,66 @@
+"""What the layer for a few tokens refuses, without a GPU."""
+import math
+
+import pytest
+import torch
+
+import megablocks_amd.ops as ops
+from megablocks_amd import _lib
+from megablocks_amd.layers.arguments import Arguments
+from megablocks_amd.ops import few_tokens
+
+W = torch.zeros(4, 16, 8, dtype=torch.bfloat16)
+CALL = dict(x=torch.zeros(2, 8, dtype=torch.bfloat16), router=torch.zeros(4, 8, dtype=torch.bfloat16), w1=W, v1=W, w2=W, top_k=2, act=0)
+
+
+@pytest.mark.parametrize('changed', [
+    dict(x=torch.zeros(2, 16)), dict(x=torch.zeros(8)), dict(x=torch.zeros(1, 2, 8)), dict(x=torch.zeros(65, 8)), dict(router=torch.zeros(5, 8)), dict(router=torch.zeros(4, 9)),
+    dict(w1=torch.zeros(64, 8)), dict(w1=torch.zeros(4, 24, 8)), dict(v1=torch.zeros(4, 24, 8)), dict(w2=torch.zeros(4, 8, 16)), dict(act=2), dict(act=-1), dict(top_k=0), dict(top_k=5),
+    dict(score='tanh'), dict(groups=3), dict(groups=4, top_groups=1), dict(group_best=3), dict(norm_p=-1), dict(norm_p=math.inf), dict(scale=math.nan), dict(bias=torch.zeros(5)),
+    dict(bias=torch.zeros(1, 4)), dict(x=torch.zeros(2, 12), router=torch.zeros(4, 12), w1=torch.zeros(4, 16, 12), v1=None, w2=torch.zeros(4, 16, 12)),
+    dict(w1=torch.zeros(4, 12, 8), v1=None, w2=torch.zeros(4, 12, 8)), dict(w1=torch.zeros(4, 0, 8), v1=None, w2=torch.zeros(4, 0, 8)),
+    dict(x=torch.zeros(2, 8), router=torch.zeros(32, 8), w1=torch.zeros(32, 8, 8), v1=None, w2=torch.zeros(32, 8, 8), top_k=17),
+    dict(router=torch.zeros(600, 8), w1=torch.zeros(600, 8, 8), v1=None, w2=torch.zeros(600, 8, 8))])
+def test_calls_that_are_none_are_refused(changed):
+    with pytest.raises(ValueError):
+        ops.moe_layer(**(CALL | changed))
+
+
+def test_tensors_off_the_gpu_are_refused():
+    with pytest.raises(RuntimeError):
+        ops.moe_layer(**CALL)
+
+
+@pytest.mark.parametrize('sizes,taken', [
+    ((1, 8, 8, 1, 1), True), ((64, 4096, 14336, 8, 2), True), ((65, 8, 8, 1, 1), False), ((1, 8, 8, 512, 16), True), ((1, 8, 8, 513, 1), False), ((1, 8, 8, 32, 17), False),
+    ((1, 8, 8, 4, 5), False), ((1, 12, 8, 4, 1), False), ((1, 8, 12, 4, 1), False), ((1, 0, 8, 4, 1), False), ((1, 32768, 32704, 4, 1), False), ((1, 32768, 32640, 4, 1), True),
+    ((1, 16, 1 << 26, 4, 1), False), ((1, 1008 * 128, 64, 4, 1), True), ((1, 1008 * 128 + 8, 64, 4, 1), False), ((64, 32768, 8, 16, 16), False), ((64, 8192, 8, 16, 16), True)])
+def test_sizes_that_are_taken(sizes, taken):
+    """Offsets that the kernels keep in 32 bits, and the counters of the workspace."""
+    assert few_tokens.takes(*sizes) == taken
+
+
+def test_entry_point_refuses_without_touching_the_gpu():
+    lib = _lib.lib
+
+    def call(tokens=2, hidden=8, dtype=0, experts=4, top_k=2, score=0, groups=1, top_groups=1, best=2, p=0., scale=1., ffn=16, act=0, x=16, w=16, out=16, scratch=None, nbytes=0,
+             workspace=None, workspace_bytes=0):
+        return lib.mbx_moe_layer(x, tokens, hidden, dtype, w, experts, top_k, score, None, groups, top_groups, best, p, scale, w, w, w, ffn, act, out, 16, 16, scratch, nbytes,
+                                 workspace, workspace_bytes, None)
+    for bad in (dict(tokens=-1), dict(hidden=-8), dict(ffn=-8), dict(experts=0), dict(top_k=0), dict(top_k=5), dict(score=2), dict(groups=3), dict(groups=4, top_groups=1),
+                dict(groups=2, top_groups=3), dict(best=0), dict(p=-1.), dict(p=math.inf), dict(p=math.nan), dict(scale=math.inf), dict(act=2), dict(x=None), dict(w=None), dict(out=None)):
+        assert call(**bad) == _lib.EINVAL
+    for bad in (dict(tokens=65), dict(hidden=12), dict(ffn=12), dict(hidden=0), dict(dtype=2), dict(experts=513), dict(experts=40, top_k=17), dict(x=8), dict(w=24), dict(out=18),
+                dict(experts=65, groups=65, top_groups=65)):
+        assert call(**bad) == _lib.EUNSUPPORTED
+    assert call(tokens=0) == 0
+    nbytes = lib.mbx_moe_layer_scratch_bytes(2, 8, 16, 4, 2, 1)
+    assert call() == _lib.ESCRATCH and call(scratch=16, nbytes=nbytes - 1, workspace=16, workspace_bytes=4096) == _lib.ESCRATCH
+    assert call(scratch=16, nbytes=nbytes) == _lib.ESCRATCH and call(scratch=16, nbytes=nbytes, workspace=16, workspace_bytes=4095) == _lib.ESCRATCH
+    assert call(scratch=8, nbytes=nbytes, workspace=16, workspace_bytes=4096) == _lib.ESCRATCH
+
+
+@pytest.mark.parametrize('tokens', [-1, 65])
+def test_arguments_refuse_other_numbers_of_tokens(tokens):
+    with pytest.raises(ValueError):
+        Arguments(device=torch.device('cpu'), moe_fused_tokens=tokens)
