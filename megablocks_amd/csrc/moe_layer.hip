@@ -27,13 +27,13 @@ constexpr int kLayerSlots = kLayerTokens * kLayerTopK;
 constexpr int kLayerThreads = 256, kLayerWaves = kLayerThreads / kWave;
 constexpr int kLayerMaxParts = 16;                                     // of the second product's reduction
 constexpr int kDownColumns = 128;
-// counters: 0 .. 7 groups of tokens, 8 the groups that are done, from 16 on the second product's columns
-constexpr int kCounterAll = 8, kCounterColumns = 16;
+// counters: from 0 on groups of tokens, then the groups that are done, then the second product's columns
+constexpr int kCounterAll = kLayerTokens, kCounterColumns = kLayerTokens + 1;
 
 // which experts have which rows; a row is an assignment (token, j), sorted by expert
 struct LayerTable {
   int4 used[kLayerExperts];         // expert, first row, rows, 0; rows 0 past the last used one
-  int32_t slot_of_row[kLayerSlots];
+  int32_t token_of_row[kLayerSlots];
   int32_t row_of_slot[kLayerSlots];
   int32_t experts;                  // used ones
 };
@@ -67,18 +67,30 @@ __device__ __forceinline__ uint64_t sortable(double key) {
   return key != key ? ~0ull : (int64_t)u < 0 ? ~u : u | 1ull << 63;
 }
 
+// v of all lanes combined, in all of them: wave_butterfly of two registers a value
+template <typename F>
+__device__ __forceinline__ double wave_butterfly_f64(double v, F&& op) {
+  const auto value = [](uint32_t lo, uint32_t hi) { return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
+  const auto low = [](double x) { return (uint32_t)__builtin_bit_cast(uint64_t, x); };
+  const auto high = [](double x) { return (uint32_t)(__builtin_bit_cast(uint64_t, x) >> 32); };
+  {
+    const auto lo = __builtin_amdgcn_permlane32_swap(low(v), low(v), false, false), hi = __builtin_amdgcn_permlane32_swap(high(v), high(v), false, false);
+    v = op(value(lo[0], hi[0]), value(lo[1], hi[1]));
+  }
+  {
+    const auto lo = __builtin_amdgcn_permlane16_swap(low(v), low(v), false, false), hi = __builtin_amdgcn_permlane16_swap(high(v), high(v), false, false);
+    v = op(value(lo[0], hi[0]), value(lo[1], hi[1]));
+  }
+  v = op(v, value(lane_xor_dpp<8>(low(v)), lane_xor_dpp<8>(high(v))));
+  v = op(v, value(lane_xor_dpp<4>(low(v)), lane_xor_dpp<4>(high(v))));
+  v = op(v, value(lane_xor_dpp<2>(low(v)), lane_xor_dpp<2>(high(v))));
+  return op(v, value(lane_xor_dpp<1>(low(v)), lane_xor_dpp<1>(high(v))));
+}
 __device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, kWave);
-  return v;
+  return wave_butterfly_f64(v, [](double a, double b) { return a + b; });
 }
 __device__ __forceinline__ double wave_max_f64(double v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) {
-    const double o = __shfl_xor(v, off, kWave);
-    v = o > v ? o : v;
-  }
-  return v;
+  return wave_butterfly_f64(v, [](double a, double b) { return a > b ? a : b; });
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
   return wave_butterfly(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
@@ -88,16 +100,17 @@ __device__ __forceinline__ uint32_t wave_min_u32(uint32_t v) {
 }
 
 // The choice for a token by one wave: expert 64 i + lane is in register i.  scratch: this wave's, a value for every expert (groups only).
-template <int R>
-__device__ __forceinline__ void choose_for(const LayerChoice& q, int token, const uint64_t* __restrict__ logits, const float* __restrict__ bias,
-                                           double* __restrict__ scratch, float* __restrict__ weights, int64_t* __restrict__ indices, int32_t* __restrict__ choice) {
+// logit(e): the token's; put(j, e): its j-th expert.
+template <int R, typename L, typename P>
+__device__ __forceinline__ void choose_for(const LayerChoice& q, int token, L&& logit, const float* __restrict__ bias, double* __restrict__ scratch,
+                                           float* __restrict__ weights, int64_t* __restrict__ indices, P&& put) {
   const int lane = lane_id();
   double score[R];
   uint64_t key[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int e = i * kWave + lane;
-    score[i] = e < q.experts ? __builtin_bit_cast(double, load_through(logits + (int64_t)token * q.experts + e)) : -INFINITY;
+    score[i] = e < q.experts ? logit(e) : -INFINITY;
     key[i] = e < q.experts ? sortable(score[i]) : 0;
   }
   if (q.sigmoid) {
@@ -162,8 +175,14 @@ __device__ __forceinline__ void choose_for(const LayerChoice& q, int token, cons
       if (key[i] > best) { best = key[i]; at = i; }
     const uint32_t high = wave_max_u32((uint32_t)(best >> 32));
     const bool high_is = (uint32_t)(best >> 32) == high;
-    const uint32_t low = wave_max_u32(high_is ? (uint32_t)best : 0u);
-    const int e = __builtin_amdgcn_readfirstlane((int)wave_min_u32(high_is && (uint32_t)best == low ? (uint32_t)(at * kWave + lane) : ~0u));
+    const uint64_t tied = __ballot(high_is);
+    int e;
+    if ((tied & (tied - 1)) == 0) {      // nearly always
+      e = __builtin_amdgcn_readlane(at * kWave + lane, __builtin_ctzll(tied));
+    } else {
+      const uint32_t low = wave_max_u32(high_is ? (uint32_t)best : 0u);
+      e = __builtin_amdgcn_readfirstlane((int)wave_min_u32(high_is && (uint32_t)best == low ? (uint32_t)(at * kWave + lane) : ~0u));
+    }
     const int from = e % kWave, reg = e / kWave;
     double s = 0.;
 #pragma unroll
@@ -189,11 +208,143 @@ __device__ __forceinline__ void choose_for(const LayerChoice& q, int token, cons
     const int64_t at = (int64_t)token * q.top_k + lane;
     weights[at] = (float)(norm == 0. ? 0. : my_score / norm * (double)q.scale);
     indices[at] = my_expert;
-    store_through(choice + at, my_expert);
+    put(lane, my_expert);
   }
 }
 
 // ---- choose ----
+// sums of exact products in 64 bits of EB rows of the router and TB tokens, in all lanes
+template <int DT, int EB, int TB>
+__device__ __forceinline__ void dot_f64(const uint16_t* __restrict__ router, int e0, int experts, const uint16_t* __restrict__ x, int t0, int tokens, int hidden,
+                                        double (&acc)[EB][TB]) {
+  typedef typename Elem<DT>::type E;
+  constexpr int kAhead = EB * TB == 1 ? 8 : 2, kStep = kWave * 8;
+#pragma unroll
+  for (int e = 0; e < EB; ++e)
+#pragma unroll
+    for (int t = 0; t < TB; ++t) acc[e][t] = 0.;
+  for (int c0 = lane_id() * 8; c0 < hidden; c0 += kAhead * kStep) {
+    u32x4 w[kAhead][EB], v[kAhead][TB];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int c = c0 + u * kStep;
+      const bool here = c < hidden;
+#pragma unroll
+      for (int e = 0; e < EB; ++e) w[u][e] = here && e0 + e < experts ? *(const u32x4*)(router + (int64_t)(e0 + e) * hidden + c) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int t = 0; t < TB; ++t) v[u][t] = here && t0 + t < tokens ? *(const u32x4*)(x + (int64_t)(t0 + t) * hidden + c) : u32x4{0u, 0u, 0u, 0u};
+    }
+    const auto value = [](const u32x4& p, int i) { return (double)Elem<DT>::to_f32(__builtin_bit_cast(E, (uint16_t)(p[i >> 1] >> ((i & 1) * 16)))); };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        double wd[EB];
+#pragma unroll
+        for (int e = 0; e < EB; ++e) wd[e] = value(w[u][e], i);
+#pragma unroll
+        for (int t = 0; t < TB; ++t) {
+          const double vd = value(v[u][t], i);
+#pragma unroll
+          for (int e = 0; e < EB; ++e) acc[e][t] = __builtin_fma(wd[e], vd, acc[e][t]);
+        }
+      }
+  }
+#pragma unroll
+  for (int e = 0; e < EB; ++e)
+#pragma unroll
+    for (int t = 0; t < TB; ++t) acc[e][t] = wave_sum_f64(acc[e][t]);
+}
+
+// The table, by one workgroup; expert_of(s): the s-th assignment's.
+template <int THREADS, typename X>
+__device__ __forceinline__ void make_table(const LayerChoice& q, X&& expert_of, LayerTable* __restrict__ table) {
+  static_assert(kLayerExperts <= 2 * THREADS && THREADS >= kWave, "two experts a thread");
+  constexpr int kEach = (kLayerSlots + THREADS - 1) / THREADS, kPair = kLayerExperts / 2;      // thread i: experts 2 i and 2 i + 1
+  __shared__ int32_t count[kLayerExperts], first[kLayerExperts], sums[kPair / kWave];
+  const int slots = q.tokens * q.top_k, i = threadIdx.x, wave = i / kWave;
+  if (i < kPair) count[2 * i] = count[2 * i + 1] = 0;
+  __syncthreads();
+  int expert[kEach], rank[kEach];
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) {
+    const int s = i + n * THREADS;
+    expert[n] = s < slots ? expert_of(s) : 0;
+  }
+#pragma unroll
+  for (int n = 0; n < kEach; ++n)      // the order of an expert's rows is nobody's business: each is computed by itself
+    if (i + n * THREADS < slots) rank[n] = atomicAdd(&count[expert[n]], 1);
+  __syncthreads();
+  int c0 = 0, c1 = 0, through = 0;
+  if (i < kPair) {
+    c0 = count[2 * i];
+    c1 = count[2 * i + 1];
+    through = wave_inclusive_scan(c0 + c1 | ((c0 > 0) + (c1 > 0)) << 16);    // rows, used experts
+    if (i % kWave == kWave - 1) sums[wave] = through;
+  }
+  __syncthreads();
+  if (i < kPair) {
+    int before = through - (c0 + c1 | ((c0 > 0) + (c1 > 0)) << 16), all = 0;
+#pragma unroll
+    for (int w = 0; w < kPair / kWave; ++w) {
+      before += w < wave ? sums[w] : 0;
+      all += sums[w];
+    }
+    const int row = before & 0xffff, used = all >> 16;
+    int u = before >> 16;
+    first[2 * i] = row;
+    first[2 * i + 1] = row + c0;
+    if (c0 > 0) table->used[u++] = make_int4(2 * i, row, c0, 0);
+    if (c1 > 0) table->used[u] = make_int4(2 * i + 1, row + c0, c1, 0);
+    for (int n = used + i; n < q.entries; n += kPair) table->used[n] = make_int4(0, 0, 0, 0);
+    if (i == 0) table->experts = used;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) {
+    const int s = i + n * THREADS;
+    if (s < slots) {
+      const int at = first[expert[n]] + rank[n];
+      table->token_of_row[at] = s / q.top_k;
+      table->row_of_slot[s] = at;
+    }
+  }
+}
+
+// The table of a lone token: its j-th expert has row j.
+__device__ __forceinline__ void row_of_lone_token(const LayerChoice& q, int j, int expert, LayerTable* __restrict__ table) {
+  table->used[j] = make_int4(expert, j, 1, 0);
+  table->token_of_row[j] = 0;
+  table->row_of_slot[j] = j;
+  if (j == 0) table->experts = q.top_k;
+}
+
+// A workgroup a token, of sixteen waves: for routers a compute unit reads in the time that the exchange between several takes.
+constexpr int kWholeThreads = 1024, kWholeWaves = kWholeThreads / kWave;
+template <int DT, int EB, int R>
+__global__ void __launch_bounds__(kWholeThreads)
+layer_choose_whole_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ router, LayerChoice q, const float* __restrict__ bias, int32_t* __restrict__ choice,
+                          float* __restrict__ weights, int64_t* __restrict__ indices, LayerTable* __restrict__ table, int32_t* __restrict__ counters) {
+  __shared__ double logits[R * kWave], scratch[R * kWave];
+  __shared__ int flag;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), token = blockIdx.x;
+  for (int e0 = wave * EB; e0 < q.experts; e0 += kWholeWaves * EB) {
+    double acc[EB][1];
+    dot_f64<DT, EB, 1>(router, e0, q.experts, x, token, q.tokens, q.hidden, acc);
+#pragma unroll
+    for (int e = 0; e < EB; ++e)
+      if (lane_id() == e && e0 + e < q.experts) logits[e0 + e] = acc[e][0];
+  }
+  __syncthreads();
+  if (wave == 0)
+    choose_for<R>(q, token, [&](int e) { return logits[e]; }, bias, scratch, weights, indices, [&](int j, int e) {
+      if (gridDim.x > 1) store_through(choice + (int64_t)token * q.top_k + j, e);
+      else row_of_lone_token(q, j, e, table);
+    });
+  if (gridDim.x > 1 && last_to_come(counters + kCounterAll, (int)gridDim.x, &flag))
+    make_table<kWholeThreads>(q, [&](int s) { return load_through(choice + s); }, table);
+}
+
 // Workgroup (b, g): experts 4 b .. 4 b + 3, a wave each, tokens TB g .. ; TB 1 or 8.
 template <int DT, int TB, int R>
 __global__ void __launch_bounds__(kLayerThreads)
@@ -201,88 +352,24 @@ layer_choose_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
                     int32_t* __restrict__ choice, float* __restrict__ weights, int64_t* __restrict__ indices, LayerTable* __restrict__ table, int32_t* __restrict__ counters) {
   __shared__ double scratch[kLayerWaves][R * kWave];
   __shared__ int flag;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int e = (int)blockIdx.x * kLayerWaves + wave, t0 = (int)blockIdx.y * TB, tokens = q.tokens - t0 < TB ? q.tokens - t0 : TB;
-  typedef typename Elem<DT>::type E;
   if (e < q.experts) {
-    constexpr int kAhead = TB == 1 ? 8 : 2, kStep = kWave * 8;
-    double acc[TB];
+    double acc[1][TB];
+    dot_f64<DT, 1, TB>(router, e, q.experts, x, t0, q.tokens, q.hidden, acc);
 #pragma unroll
-    for (int t = 0; t < TB; ++t) acc[t] = 0.;
-    const uint16_t* const w_row = router + (int64_t)e * q.hidden;
-    for (int c0 = lane * 8; c0 < q.hidden; c0 += kAhead * kStep) {
-      u32x4 w[kAhead], v[kAhead][TB];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int c = c0 + u * kStep;
-        const bool here = c < q.hidden;
-        w[u] = here ? *(const u32x4*)(w_row + c) : u32x4{0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int t = 0; t < TB; ++t) v[u][t] = here && t < tokens ? *(const u32x4*)(x + (int64_t)(t0 + t) * q.hidden + c) : u32x4{0u, 0u, 0u, 0u};
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const double wd = Elem<DT>::to_f32(__builtin_bit_cast(E, (uint16_t)(w[u][i >> 1] >> ((i & 1) * 16))));
-#pragma unroll
-          for (int t = 0; t < TB; ++t)
-            acc[t] = __builtin_fma(wd, (double)Elem<DT>::to_f32(__builtin_bit_cast(E, (uint16_t)(v[u][t][i >> 1] >> ((i & 1) * 16)))), acc[t]);
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const double l = wave_sum_f64(acc[t]);
-      if (lane == 0 && t < tokens) store_through(logits + (int64_t)(t0 + t) * q.experts + e, __builtin_bit_cast(uint64_t, l));
-    }
+    for (int t = 0; t < TB; ++t)
+      if (lane_id() == t && t < tokens) store_through(logits + (int64_t)(t0 + t) * q.experts + e, __builtin_bit_cast(uint64_t, acc[0][t]));
   }
   if (!last_to_come(counters + blockIdx.y, (int)gridDim.x, &flag)) return;
-  for (int t = t0 + wave; t < t0 + tokens; t += kLayerWaves) choose_for<R>(q, t, logits, bias, scratch[wave], weights, indices, choice);
-  if (!last_to_come(counters + kCounterAll, (int)gridDim.y, &flag)) return;
-  // the table: experts 2 i and 2 i + 1 are thread i's
-  __shared__ int32_t count[kLayerExperts], first[kLayerExperts], sums[kLayerWaves];
-  const int slots = q.tokens * q.top_k, i = threadIdx.x;
-  count[2 * i] = count[2 * i + 1] = 0;
-  __syncthreads();
-  int expert[kLayerSlots / kLayerThreads], rank[kLayerSlots / kLayerThreads];
-#pragma unroll
-  for (int n = 0; n < kLayerSlots / kLayerThreads; ++n) {
-    const int s = i + n * kLayerThreads;
-    expert[n] = s < slots ? load_through(choice + s) : 0;
-  }
-#pragma unroll
-  for (int n = 0; n < kLayerSlots / kLayerThreads; ++n)      // the order of an expert's rows is nobody's business: each is computed by itself
-    if (i + n * kLayerThreads < slots) rank[n] = atomicAdd(&count[expert[n]], 1);
-  __syncthreads();
-  const int c0 = count[2 * i], c1 = count[2 * i + 1];
-  const int mine = c0 + c1 | ((c0 > 0) + (c1 > 0)) << 16;    // rows, used experts
-  const int through = wave_inclusive_scan(mine);
-  if (lane == kWave - 1) sums[wave] = through;
-  __syncthreads();
-  int before = through - mine, all = 0;
-#pragma unroll
-  for (int w = 0; w < kLayerWaves; ++w) {
-    before += w < wave ? sums[w] : 0;
-    all += sums[w];
-  }
-  const int row = before & 0xffff, used = all >> 16;
-  int u = before >> 16;
-  first[2 * i] = row;
-  first[2 * i + 1] = row + c0;
-  if (c0 > 0) table->used[u++] = make_int4(2 * i, row, c0, 0);
-  if (c1 > 0) table->used[u] = make_int4(2 * i + 1, row + c0, c1, 0);
-  for (int n = used + i; n < q.entries; n += kLayerThreads) table->used[n] = make_int4(0, 0, 0, 0);
-  if (i == 0) table->experts = used;
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < kLayerSlots / kLayerThreads; ++n) {
-    const int s = i + n * kLayerThreads;
-    if (s < slots) {
-      const int at = first[expert[n]] + rank[n];
-      table->slot_of_row[at] = s;
-      table->row_of_slot[s] = at;
-    }
-  }
+  for (int t = t0 + wave; t < t0 + tokens; t += kLayerWaves)
+    choose_for<R>(q, t, [&](int e) { return __builtin_bit_cast(double, load_through(logits + (int64_t)t * q.experts + e)); }, bias, scratch[wave], weights, indices,
+                  [&](int j, int e) {
+                    if (q.tokens == 1) row_of_lone_token(q, j, e, table);
+                    else store_through(choice + (int64_t)t * q.top_k + j, e);
+                  });
+  if (q.tokens > 1 && last_to_come(counters + kCounterAll, (int)gridDim.y, &flag))
+    make_table<kLayerThreads>(q, [&](int s) { return load_through(choice + s); }, table);
 }
 
 // ---- products ----
@@ -318,8 +405,8 @@ __device__ __forceinline__ void in_two(float v, uint16_t& hi, uint16_t& lo) {
   lo = __builtin_bit_cast(uint16_t, Elem<DT>::from_f32(rest - rest == 0.f ? rest : 0.f));     // an infinity or NaN has no rest
 }
 
-// NF fragments of 16 weight rows (with the gate: half of them W1's, half V1's), up to R tiles of 16 token rows.  In a chunk of 64 columns lane (c = l % 16,
-// g = l / 16) has columns 16 g .. 16 g + 15 of weight row c and of token row c: 32 bytes each.
+// NF fragments of 16 weight rows (with the gate: half of them W1's, half V1's), up to R tiles of 16 token rows.  Of a chunk of 64 columns lane (c = l % 16,
+// g = l / 16) has columns 8 g .. 8 g + 7 and 32 + 8 g .. 32 + 8 g + 7 of weight row c and of token row c, 16 bytes each: whole 64-byte pieces a load.
 template <int DT, bool GATE, int NF, int R>
 __global__ void __launch_bounds__(kLayerThreads)
 layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w1, const uint16_t* __restrict__ v1, const LayerTable* __restrict__ table, int tokens,
@@ -330,35 +417,38 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
   const int u = (int)blockIdx.x / tiles, f0 = ((int)blockIdx.x - u * tiles) * kCols;
   const int4 it = table->used[u];
   if (it.z == 0) return;
-  const int expert = it.x, first = it.y, rows = it.z, row_tiles = (rows + 15) / 16;
+  const int expert = it.x, all_rows = it.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), c = lane & 15, g = lane >> 4;
   const uint32_t pitch = (uint32_t)hidden * 2u;
   const int64_t matrix = (int64_t)ffn * hidden;
   const __amdgpu_buffer_rsrc_t rsrc_x = rsrc_of(x, (uint32_t)tokens * pitch), rsrc_w = rsrc_of(w1 + expert * matrix, (uint32_t)(matrix * 2));
   const __amdgpu_buffer_rsrc_t rsrc_v = GATE ? rsrc_of(v1 + expert * matrix, (uint32_t)(matrix * 2)) : rsrc_w;
+  for (int done = 0; done < all_rows; done += 16 * R) {      // once, but for experts of many rows
+  const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
   uint32_t x_off[R];
 #pragma unroll
   for (int t = 0; t < R; ++t) {
     const int r = t * 16 + c;
-    x_off[t] = r < rows ? (uint32_t)(table->slot_of_row[first + r] / top_k) * pitch + (uint32_t)g * 32u : kNone;
+    x_off[t] = r < rows ? (uint32_t)table->token_of_row[first + r] * pitch + (uint32_t)g * 16u : kNone;
   }
-  const uint32_t w_off = (uint32_t)(f0 + c) * pitch + (uint32_t)g * 32u;
+  const uint32_t w_off = (uint32_t)(f0 + c) * pitch + (uint32_t)g * 16u;
   struct Chunk { u32x4 a[R][2], b[NF][2]; };
   const int chunks = (hidden + kChunk - 1) / kChunk;
   auto fetch = [&](Chunk& q, int chunk) {
     const uint32_t at = (uint32_t)chunk * (kChunk * 2);
+    const uint32_t past[2] = {chunk * kChunk + 8 * g < hidden ? 0u : kNone, chunk * kChunk + 8 * g + 32 < hidden ? 0u : kNone};      // pieces past the row's end
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint32_t past = chunk * kChunk + 16 * g + 8 * s < hidden ? 0u : kNone;      // pieces past the row's end
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         const int row = GATE ? f % (NF / 2 > 0 ? NF / 2 : 1) : f;
-        q.b[f][s] = load16(GATE && f >= NF / 2 ? rsrc_v : rsrc_w, (w_off + at + (uint32_t)(row * 16) * pitch + 16u * s) | past);
+        q.b[f][s] = load16(GATE && f >= NF / 2 ? rsrc_v : rsrc_w, (w_off + at + (uint32_t)(row * 16) * pitch + 64u * s) | past[s]);
       }
 #pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
       for (int t = 0; t < R; ++t)
-        if (t == 0 || t < row_tiles) q.a[t][s] = load16(rsrc_x, (x_off[t] + at + 16u * s) | past | (x_off[t] & kNone));
-    }
+        if (t == 0 || t < row_tiles) q.a[t][s] = load16(rsrc_x, (x_off[t] + at + 64u * s) | past[s] | (x_off[t] & kNone));
   };
   f32x4 acc[R][NF];
 #pragma unroll
@@ -374,15 +464,22 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
 #pragma unroll
           for (int f = 0; f < NF; ++f) acc[t][f] = mfma<DT>(q.b[f][s], q.a[t][s], acc[t][f]);
   };
-  // the waves take the chunks in turn; past the last one nothing is fetched
+  // The waves take the chunks in turn, every workgroup from another one on and round: started together at the rows' beginnings they would all ask for bytes that
+  // are a power of two apart, of a few memory channels (1 token, 2 of 8 experts of [14336, 4096]: the layer 164 us, now 148).
+  const int steps = chunks > wave ? (chunks - wave + kLayerWaves - 1) / kLayerWaves : 0;      // this wave's
+  const int turn = steps > 0 ? (int)(((uint32_t)(f0 / kCols) * 5u + (uint32_t)u * 3u) % (uint32_t)steps) : 0;
+  auto chunk_of = [&](int step) {
+    const int at = step + turn < steps ? step + turn : step + turn - steps;
+    return step < steps ? at * kLayerWaves + wave : chunks;      // past the last one nothing is fetched
+  };
   Chunk q0, q1;
-  fetch(q0, wave);
-  for (int chunk = wave; chunk < chunks; chunk += 2 * kLayerWaves) {
-    fetch(q1, chunk + kLayerWaves);
-    __builtin_amdgcn_sched_barrier(0);
+  fetch(q0, chunk_of(0));
+  for (int step = 0; step < steps; step += 2) {
+    fetch(q1, chunk_of(step + 1));
+    __builtin_amdgcn_sched_barrier(0);      // a chunk's loads are all issued before the products of the one before it
     multiply(q0);
     __builtin_amdgcn_sched_barrier(0);
-    fetch(q0, chunk + 2 * kLayerWaves);
+    fetch(q0, chunk_of(step + 2));
     __builtin_amdgcn_sched_barrier(0);
     multiply(q1);
     __builtin_amdgcn_sched_barrier(0);
@@ -391,7 +488,7 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
   constexpr int kEach = kCols / 16;
   const int m = threadIdx.x / 16, col = threadIdx.x % 16 * kEach;
   for (int t = 0; t < row_tiles; ++t) {
-    if (t > 0) __syncthreads();
+    if (t > 0 || done > 0) __syncthreads();
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
       f32x4 v = acc[0][f];
@@ -420,6 +517,7 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
       __builtin_memcpy(h_lo + at, lo, sizeof(lo));
     }
   }
+  }
 }
 
 // Second product: 128 columns, in chunks of 32 rows of W2.  Lane (c, g) reads columns 8 c .. 8 c + 7 of rows 8 g .. 8 g + 7, 16 bytes each (256 contiguous bytes a
@@ -436,13 +534,19 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
   const int part = in / tiles, tile = in - part * tiles, n0 = tile * kDownColumns;
   const int4 it = table->used[u];
   if (it.z == 0) return;
-  const int expert = it.x, first = it.y, rows = it.z, row_tiles = (rows + 15) / 16, slots = tokens * top_k;
+  const int expert = it.x, all_rows = it.z, slots = tokens * top_k;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), c = lane & 15, g = lane >> 4;
   const uint32_t pitch = (uint32_t)hidden * 2u, h_pitch = (uint32_t)ffn * 2u;
   const int64_t matrix = (int64_t)ffn * hidden;
   const __amdgpu_buffer_rsrc_t rsrc_w = rsrc_of(w2 + expert * matrix, (uint32_t)(matrix * 2));
   const __amdgpu_buffer_rsrc_t rsrc_hi = rsrc_of(h_hi, (uint32_t)slots * h_pitch), rsrc_lo = rsrc_of(h_lo, (uint32_t)slots * h_pitch);
   const uint32_t w_off = n0 + 8 * c < hidden ? (uint32_t)(8 * g) * pitch + (uint32_t)(n0 + 8 * c) * 2u : kNone;
+  const int m = threadIdx.x / 16, col = threadIdx.x % 16 * 8;
+  const bool mine = n0 + col < hidden;          // a multiple of 8
+  // a part's sums lie [part][row][column]
+  const __amdgpu_buffer_rsrc_t rsrc_parts = rsrc_of(sums_of_parts, (uint32_t)parts * (uint32_t)slots * (uint32_t)hidden * 4u);
+  for (int done = 0; done < all_rows; done += 16 * R) {      // once, but for experts of many rows
+  const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
   uint32_t h_off[R];
 #pragma unroll
   for (int t = 0; t < R; ++t) h_off[t] = t * 16 + c < rows ? (uint32_t)(first + t * 16 + c) * h_pitch + (uint32_t)g * 16u : kNone;
@@ -494,12 +598,8 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
     __builtin_amdgcn_sched_barrier(0);
   }
   // accumulator t, j, register i of lane (c, g): token row 16 t + c, column 8 (4 g + i) + j
-  const int m = threadIdx.x / 16, col = threadIdx.x % 16 * 8;
-  const bool mine = n0 + col < hidden;          // a multiple of 8
-  // a part's sums lie [part][row][column]
-  const __amdgpu_buffer_rsrc_t rsrc_parts = rsrc_of(sums_of_parts, (uint32_t)parts * (uint32_t)slots * (uint32_t)hidden * 4u);
   for (int t = 0; t < row_tiles; ++t) {
-    if (t > 0) __syncthreads();
+    if (t > 0 || done > 0) __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f32x4 lo, hi;
@@ -530,36 +630,55 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
       __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rsrc_parts, (int)at + 16, 0, kThrough);
     }
   }
+  }
+  // Then a token's rows are weighted and added up.  Sixteen threads have a column; with few tokens several of them share a token's parts, and add up in order
+  // what each has.
+  constexpr int kAhead = 8;
+  int share = 1;
+  while (tokens * share * 2 <= 16) share *= 2;
+  const int pieces = top_k * parts, each = (pieces + share - 1) / share, my_share = m % share, stop = (my_share + 1) * each < pieces ? (my_share + 1) * each : pieces;
+  uint32_t place[kAhead];
+  float w[kAhead];
+  auto look_up = [&](int t, int q) {      // where the pieces q .. of token t lie, and their weights
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const bool here = q + i < stop && t < tokens && mine;
+      const int now = here ? q + i : 0, j = now / parts, p = now - j * parts, s = here ? t * top_k + j : 0;
+      const uint32_t at = (((uint32_t)p * (uint32_t)slots + (uint32_t)table->row_of_slot[s]) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
+      place[i] = here ? at : kNone;
+      w[i] = weights[s];
+    }
+  };
+  look_up(m / share, my_share * each);
   if (!last_to_come(counters + kCounterColumns + tile, table->experts * parts, &flag)) return;
-  // all rows of these columns are there: a token's are weighted and added up, parts first, then experts as they were chosen
-  if (!mine) return;
-  for (int t = m; t < tokens; t += 16) {
-    constexpr int kAhead = 8;
-    const int pieces = top_k * parts;
-    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo, y_lo = lo, y_hi = lo;
-    for (int q = 0; q < pieces; q += kAhead) {
+  for (int t = m / share; t < tokens; t += 16 / share) {
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    for (int q = my_share * each; q < stop; q += kAhead) {
+      if (t != m / share || q != my_share * each) look_up(t, q);
       u32x4 a[kAhead], b[kAhead];
-      float w[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const int now = q + i < pieces ? q + i : pieces - 1, j = now / parts, p = now - j * parts, s = t * top_k + j;
-        const uint32_t at = (((uint32_t)p * (uint32_t)slots + (uint32_t)table->row_of_slot[s]) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
-        a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc_parts, (int)at, 0, kThrough));
-        b[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc_parts, (int)at + 16, 0, kThrough));
-        w[i] = weights[s];
+        a[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc_parts, (int)place[i], 0, kThrough));
+        b[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc_parts, (int)place[i] + 16, 0, kThrough));
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (q + i >= pieces) break;
-        y_lo += __builtin_bit_cast(f32x4, a[i]);
-        y_hi += __builtin_bit_cast(f32x4, b[i]);
-        if ((q + i + 1) % parts == 0) {
-          lo += y_lo * w[i];
-          hi += y_hi * w[i];
-          y_lo = y_hi = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < kAhead; ++i)
+        if (q + i < stop) {
+          lo += __builtin_bit_cast(f32x4, a[i]) * w[i];
+          hi += __builtin_bit_cast(f32x4, b[i]) * w[i];
         }
+    }
+    if (share > 1) {      // one round: every token has its threads
+      *(f32x4*)&sums[0][m][col] = lo;
+      *(f32x4*)&sums[0][m][col + 4] = hi;
+      __syncthreads();
+      if (my_share != 0) return;
+      for (int o = 1; o < share; ++o) {
+        lo += *(const f32x4*)&sums[0][m + o][col];
+        hi += *(const f32x4*)&sums[0][m + o][col + 4];
       }
     }
+    if (!mine) return;
     const u32x4 v = {pack2<DT>(lo[0], lo[1]), pack2<DT>(lo[2], lo[3]), pack2<DT>(hi[0], hi[1]), pack2<DT>(hi[2], hi[3])};
     *(u32x4*)(out + (int64_t)t * hidden + n0 + col) = v;
   }
@@ -568,6 +687,7 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
 // ---- host ----
 struct LayerPlan {
   int entries;              // experts that can have a row
+  double used, rows;        // that get one, and how many those get, where tokens choose evenly
   int fragments, hidden_tiles;
   int down_tiles, parts;
   size_t table, choice, logits, h_hi, h_lo, sums, total = 0;
@@ -575,15 +695,24 @@ struct LayerPlan {
   LayerPlan(int tokens, int hidden, int ffn, int experts, int top_k, bool gate) {
     const int slots = tokens * top_k;
     entries = slots < experts ? slots : experts;
-    // experts that get a row where tokens choose evenly
-    const double used = fmin(slots, experts * (1. - pow(1. - (double)top_k / experts, tokens)));
-    const int wide = gate ? 8 : 16;
-    fragments = 4;
-    while (fragments > (gate ? 2 : 1) && used * ceil_div(ffn, fragments * wide) < 512) fragments /= 2;
-    hidden_tiles = (int)ceil_div(ffn, fragments * wide);
+    used = fmin(slots, experts * (1. - pow(1. - (double)top_k / experts, tokens)));
+    // Fragments of 16 weight rows a workgroup (half of them W1's, half V1's with a gate; us a layer by 2 / 4 / 8 of them).  From 12 rows an expert on the rows
+    // are read again by so many workgroups that eight pay: 64 tokens, 2 of 8 experts of [14336, 4096] 608 / 565 / 544, of [8192, 5120] 462 / 458 / 436, but
+    // 4 experts of [1024, 1024], which leave most compute units without a workgroup, 28 / 30 / 34.  Below, two: 1 token, 6 of 64 of [1408, 2048] 41 / 47 / 46, 2 of 8
+    // of [12288, 5120] 164 / 183 / 198, 16 tokens, 6 of 64 of [1408, 2048] 179 / 186 / 192; but rows that are a multiple of 8 KiB apart come faster in
+    // fours: 1 token, 2 of 8 of [14336, 4096] 180 / 166 / 169, of [8192, 4096] 105 / 100 / 104, where there are workgroups enough: of [2048, 4096] 38 / 43 / 60.  One without a gate,
+    // for a few small experts: 1 token, top-1 of 4 of [2048, 512] 14.7 instead of 15.2.
+    const int columns = gate ? 8 : 16;
+    const auto workgroups = [&](int n) { return used * ceil_div(ffn, n * columns); };
+    rows = slots / used;
+    fragments = rows >= 12 && workgroups(8) >= 256 ? 8 : hidden % 4096 == 0 && workgroups(4) >= 512 ? 4 : gate || workgroups(2) >= 512 ? 2 : 1;
+    hidden_tiles = (int)ceil_div(ffn, fragments * columns);
     down_tiles = (int)ceil_div(hidden, kDownColumns);
+    // Parts of the second product's reduction, as many as make a workgroup for most compute units, of two chunks a wave and more (us a layer by 1 / 2 / 4 / 8 of them:
+    // 1 token, 2 of 8 experts of [14336, 4096], 64 workgroups a part, 209 / 177 / 162 / 164; 6 of 64 of [1408, 2048], 96, 43 / 39 / 41 / 45; 8 of 64 of [2048, 7168],
+    // 448, 151 / 152 / 156 / 160; 64 tokens, 6 of 64 of [1408, 2048], 1024, 242 / 254 / 274 / 324).
     parts = 1;
-    while (parts < kLayerMaxParts && used * down_tiles * parts < 384 && ceil_div(ffn, 32) >= parts * 2 * kLayerWaves) parts *= 2;
+    while (parts < kLayerMaxParts && used * down_tiles * parts < 192 && ceil_div(ffn, 32) >= parts * 4 * kLayerWaves) parts *= 2;
     auto take = [&](size_t bytes) {
       const size_t at = total;
       total += (bytes + 255) & ~(size_t)255;
@@ -609,11 +738,25 @@ int layer_sizes(int64_t tokens, int64_t hidden, int64_t ffn, int experts, int to
   return 0;
 }
 
-template <int DT, int TB, int R>
-void launch_choose(const void* x, const void* router, const LayerChoice& q, const float* bias, char* base, const LayerPlan& plan, float* weights, int64_t* indices,
+template <int DT, int R>
+void launch_choose(const void* x_, const void* router_, const LayerChoice& q, const float* bias, char* base, const LayerPlan& plan, float* weights, int64_t* indices,
                    int32_t* counters, hipStream_t s) {
-  layer_choose_kernel<DT, TB, R><<<dim3((unsigned)ceil_div(q.experts, kLayerWaves), (unsigned)ceil_div(q.tokens, TB)), kLayerThreads, 0, s>>>(
-      (const uint16_t*)x, (const uint16_t*)router, q, bias, (uint64_t*)(base + plan.logits), (int32_t*)(base + plan.choice), weights, indices, (LayerTable*)(base + plan.table), counters);
+  const uint16_t *const x = (const uint16_t*)x_, *const router = (const uint16_t*)router_;
+  int32_t* const choice = (int32_t*)(base + plan.choice);
+  LayerTable* const table = (LayerTable*)(base + plan.table);
+  // up to 128 KiB of router by one workgroup a token (us, that / four experts a workgroup: 1 token, 8 of 4096 5.2 / 7.4; 16, 64 of 1024 7.9 / 9.4; 1, 64 of 2048 10.5 / 6.4)
+  if ((int64_t)q.experts * ((q.hidden + 1023) & ~1023) <= 1 << 16) {
+    if (q.experts <= kWholeWaves) layer_choose_whole_kernel<DT, 1, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices, table, counters);
+    else layer_choose_whole_kernel<DT, 4, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices, table, counters);
+    return;
+  }
+  const unsigned workgroups = (unsigned)ceil_div(q.experts, kLayerWaves);
+  // tokens one by one while all their waves are resident; eight of them read the router once together
+  uint64_t* const logits = (uint64_t*)(base + plan.logits);
+  if (q.experts * q.tokens <= 4096)
+    layer_choose_kernel<DT, 1, R><<<dim3(workgroups, (unsigned)q.tokens), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
+  else
+    layer_choose_kernel<DT, 8, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 8)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
 }
 
 template <int DT, int R>
@@ -624,11 +767,11 @@ void launch_products(const void* x, const void* w1, const void* v1, const void* 
   const unsigned grid = (unsigned)(plan.entries * plan.hidden_tiles);
 #define MBX_LAYER_HIDDEN(GATE, NF) \
   layer_hidden_kernel<DT, GATE, NF, R><<<grid, kLayerThreads, 0, s>>>((const uint16_t*)x, (const uint16_t*)w1, (const uint16_t*)v1, table, q.tokens, q.top_k, q.hidden, ffn, plan.hidden_tiles, act, hi, lo)
-  if (v1) {
-    if (plan.fragments == 4) MBX_LAYER_HIDDEN(true, 4); else MBX_LAYER_HIDDEN(true, 2);
-  } else {
-    if (plan.fragments == 4) MBX_LAYER_HIDDEN(false, 4); else if (plan.fragments == 2) MBX_LAYER_HIDDEN(false, 2); else MBX_LAYER_HIDDEN(false, 1);
-  }
+  if constexpr (R > 1)      // for rows enough
+    if (plan.fragments == 8) { if (v1) MBX_LAYER_HIDDEN(true, 8); else MBX_LAYER_HIDDEN(false, 8); }
+  if (plan.fragments == 4) { if (v1) MBX_LAYER_HIDDEN(true, 4); else MBX_LAYER_HIDDEN(false, 4); }
+  else if (plan.fragments == 2) { if (v1) MBX_LAYER_HIDDEN(true, 2); else MBX_LAYER_HIDDEN(false, 2); }
+  else if (plan.fragments == 1) MBX_LAYER_HIDDEN(false, 1);
 #undef MBX_LAYER_HIDDEN
   layer_down_kernel<DT, R><<<(unsigned)(plan.entries * plan.down_tiles * plan.parts), kLayerThreads, 0, s>>>(
       hi, lo, (const uint16_t*)w2, table, q.tokens, q.top_k, q.hidden, ffn, plan.down_tiles, plan.parts, weights, (float*)(base + plan.sums), (uint16_t*)out, counters);
@@ -637,14 +780,11 @@ void launch_products(const void* x, const void* w1, const void* v1, const void* 
 template <int DT>
 int launch_layer(const void* x, const void* router, const void* w1, const void* v1, const void* w2, const LayerChoice& q, const float* bias, int ffn, int act, void* out,
                  float* weights, int64_t* indices, char* base, const LayerPlan& plan, int32_t* counters, hipStream_t s) {
-#define MBX_LAYER_CHOOSE(TB) \
-  (q.experts <= 64 ? launch_choose<DT, TB, 1>(x, router, q, bias, base, plan, weights, indices, counters, s) \
-   : q.experts <= 256 ? launch_choose<DT, TB, 4>(x, router, q, bias, base, plan, weights, indices, counters, s) \
-                      : launch_choose<DT, TB, 8>(x, router, q, bias, base, plan, weights, indices, counters, s))
-  if (q.tokens <= 8) MBX_LAYER_CHOOSE(1); else MBX_LAYER_CHOOSE(8);
-#undef MBX_LAYER_CHOOSE
-  if (q.tokens <= 16) launch_products<DT, 1>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
-  else if (q.tokens <= 32) launch_products<DT, 2>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  if (q.experts <= 64) launch_choose<DT, 1>(x, router, q, bias, base, plan, weights, indices, counters, s);
+  else if (q.experts <= 256) launch_choose<DT, 4>(x, router, q, bias, base, plan, weights, indices, counters, s);
+  else launch_choose<DT, 8>(x, router, q, bias, base, plan, weights, indices, counters, s);
+  if (plan.rows < 12 && (q.tokens <= 16 || plan.rows <= 8)) launch_products<DT, 1>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  else if (q.tokens <= 32 || plan.rows <= 20) launch_products<DT, 2>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
   else launch_products<DT, 4>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
   return launch_status();
 }
