@@ -3,12 +3,12 @@
 //   out[i] = scale table[ids[i]]           dtable[v] = scale sum over {i : ids[i] = v} of dout[i], i ascending
 //
 // Both are bound by memory: the rows read and written once, for the gradient the whole table written, most of it zeros.  The gradient's sums are fp32 in
-// a fixed order: rows are added along the tokens sorted by word (stably), kPiece of them by a wave, whose runs of one word that end inside go straight
-// to the table; what a run that crosses pieces leaves in each is kept in fp32 and added up, in order, by a launch of its own.  So a word that is half of the text
-// costs no more than any other, and results do not depend on timing: no atomics.
+// a fixed order: rows are added along the tokens sorted by word (stably), a piece of 32 of them by a wave, whose runs of one word go straight to the table;
+// what a longer run leaves in each of its pieces is kept in fp32 and added up, in order, by a launch of its own.  So a word that is half of the text costs no
+// more than any other, and sums do not depend on timing.
 //
-// Sorting: workgroup w owns a range of words and goes through all tokens twice, once to count its own and those of smaller words, once to place them: no
-// exchange between workgroups, one launch.
+// Sorting: workgroup w owns a range of words and goes through all tokens, counts those of smaller words and lists its own, in order, in LDS: no exchange between
+// workgroups, one launch.
 //
 // A token outside the table gives a row of zeros and no gradient.  Tensors may start anywhere and rows have any length: the memory unit takes 16-byte
 // accesses at any address.
@@ -25,19 +25,24 @@ constexpr int kEmbThreads = 256, kEmbWaves = kEmbThreads / kWave;
 constexpr int kPer = 8;                               // columns of a lane
 constexpr int kSlice = kPer * kWave;                  // columns of a wave
 
+// kPer values as they lie in memory
 template <int DT>
-__device__ __forceinline__ void load8(const void* at, float (&v)[kPer]) {
-  if constexpr (DT == MBX_F32) {
-    const u32x4e a = *(const u32x4_at4*)at, b = *(const u32x4_at4*)((const float*)at + 4);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) { v[t] = __uint_as_float(a[t]); v[4 + t] = __uint_as_float(b[t]); }
-  } else {
-    const u32x4e a = *(const u32x4_at2*)at;
-#pragma unroll
-    for (int t = 0; t < kPer; ++t)
-      v[t] = Elem<DT>::to_f32(__builtin_bit_cast(typename Elem<DT>::type, (uint16_t)(a[t >> 1] >> ((t & 1) * 16))));
+struct Piece {
+  u32x4e part[DT == MBX_F32 ? 2 : 1];
+
+  __device__ __forceinline__ void load(const void* at) {
+    if constexpr (DT == MBX_F32) {
+      part[0] = *(const u32x4_at4*)at;
+      part[1] = *(const u32x4_at4*)((const float*)at + 4);
+    } else {
+      part[0] = *(const u32x4_at2*)at;
+    }
   }
-}
+  __device__ __forceinline__ float value(int t) const {
+    if constexpr (DT == MBX_F32) return __uint_as_float(part[t >> 2][t & 3]);
+    else return Elem<DT>::to_f32(__builtin_bit_cast(typename Elem<DT>::type, (uint16_t)(part[0][t >> 1] >> ((t & 1) * 16))));
+  }
+};
 
 template <int DT>
 __device__ __forceinline__ void store8(void* at, const float (&v)[kPer]) {
@@ -60,7 +65,10 @@ __device__ __forceinline__ void store8(void* at, const float (&v)[kPer]) {
 template <int DT>
 __device__ __forceinline__ void load_columns(const void* at, int left, float (&v)[kPer]) {
   if (left >= kPer) {
-    load8<DT>(at, v);
+    Piece<DT> piece;
+    piece.load(at);
+#pragma unroll
+    for (int t = 0; t < kPer; ++t) v[t] = piece.value(t);
   } else {
 #pragma unroll
     for (int t = 0; t < kPer; ++t) v[t] = t < left ? Elem<DT>::to_f32(((const typename Elem<DT>::type*)at)[t]) : 0.f;
@@ -105,106 +113,177 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_kernel(const I* __restr
   store_columns<DT>((E*)out + i * hidden + column, left, v);
 }
 
-// ---- tokens in the order of their words ----
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kSortRange = 1024, kSortAhead = 8;
+// the runs that are cut, as they come: the piece that one begins in, its word, how many pieces it has a part in
+struct EmbeddingRuns {
+  int32_t count, none[3];
+  int4 runs[1];
+};
 
-// Workgroup w: words [first, first + range).  Wave v of it goes through the tokens [v S, (v + 1) S), S a multiple of 64.
-// order: the places of the tokens that count, stably by word; sorted: their words; starts[v]: how many are of smaller words than v, v = 0 .. words.
+// ---- tokens in the order of their words ----
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / kWave, kSortRange = 1024, kSortList = 1024;
+static_assert(kSortRange == 1 << 10 && kSortThreads == kSortRange, "a word of the range: ten bits, and a thread");
+constexpr int kSortEach = 4, kSortBlock = kSortEach * kWave, kSortAhead = 4;      // neighbouring tokens of a lane, tokens of a wave at a time, loads under way
+
+// the words of kSortEach tokens from i on, ~0 for those that do not count: outside the table, past the end, padding
 template <typename I>
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const I* __restrict__ ids, int64_t tokens, int words, int range, int padding,
-                                                                      int32_t* __restrict__ order, int32_t* __restrict__ sorted, int32_t* __restrict__ starts) {
+__device__ __forceinline__ void load_words(const I* __restrict__ ids, int64_t i, int64_t end, uint32_t words, uint32_t padding, uint32_t (&w)[kSortEach]) {
+  I id[kSortEach];
+  if (i + kSortEach <= end) {
+    typedef I vector __attribute__((ext_vector_type(kSortEach), aligned(sizeof(I))));
+    const vector v = *(const vector*)(ids + i);
+#pragma unroll
+    for (int t = 0; t < kSortEach; ++t) id[t] = v[t];
+  } else {
+#pragma unroll
+    for (int t = 0; t < kSortEach; ++t) id[t] = i + t < end ? ids[i + t] : (I)-1;
+  }
+#pragma unroll
+  for (int t = 0; t < kSortEach; ++t) w[t] = (uint64_t)(int64_t)id[t] < words && (uint32_t)id[t] != padding ? (uint32_t)id[t] : ~0u;
+}
+
+// Workgroup w: words [first, first + range).  Wave v of it goes through the tokens [v S, (v + 1) S), S a multiple of kSortBlock.
+// order: the places of the tokens that count, stably by word; sorted: their words; starts[v]: how many are of smaller words than v, v = 0 .. words.
+// crossing: emptied for the launch behind.
+template <typename I>
+__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const I* __restrict__ ids, int64_t tokens, int words, int range, uint32_t padding,
+                                                                      int32_t* __restrict__ order, int32_t* __restrict__ sorted, int32_t* __restrict__ starts,
+                                                                      EmbeddingRuns* __restrict__ crossing) {
   __shared__ int32_t count[kSortWaves][kSortRange];
+  __shared__ uint32_t list[kSortWaves][kSortList];      // a wave's tokens of this workgroup's words, in order: place in the wave's share, word in the range
   __shared__ int32_t sums[kSortWaves], below_of[kSortWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   const int first = (int)blockIdx.x * range, mine = words - first < range ? words - first : range;
+  if (blockIdx.x == 0 && threadIdx.x == 0) crossing->count = 0;
   for (int r = threadIdx.x; r < kSortWaves * kSortRange; r += kSortThreads) (&count[0][0])[r] = 0;
   __syncthreads();
-  const int64_t share = (tokens + kSortThreads - 1) / kSortThreads * kWave;
+  const int64_t share = (tokens + kSortWaves * kSortBlock - 1) / (kSortWaves * kSortBlock) * kSortBlock;
   const int64_t begin = wave * share, end = begin + share < tokens ? begin + share : tokens;
-  // calls take(place, word or -1) for 64 tokens at a time
+  const uint64_t lower = (1ull << lane) - 1;
+  // calls take(place of the lane's first token in the share, words) for kSortBlock tokens at a time, in order
   auto walk = [&](auto&& take) {
-    for (int64_t at = begin; at < end; at += kSortAhead * kWave) {
-      int word[kSortAhead];
+    for (int64_t at = begin; at < end; at += kSortAhead * kSortBlock) {
+      uint32_t w[kSortAhead][kSortEach];
 #pragma unroll
-      for (int u = 0; u < kSortAhead; ++u) {
-        const int64_t i = at + u * kWave + lane;
-        word[u] = i < end ? word_of(ids, i, words) : -1;
-        if (word[u] == padding) word[u] = -1;
-      }
+      for (int u = 0; u < kSortAhead; ++u) load_words(ids, at + u * kSortBlock + lane * kSortEach, end, (uint32_t)words, padding, w[u]);
 #pragma unroll
-      for (int u = 0; u < kSortAhead; ++u) take((int)(at + u * kWave) + lane, word[u]);
+      for (int u = 0; u < kSortAhead; ++u) take((int)(at - begin + u * kSortBlock) + lane * kSortEach, w[u]);
     }
   };
-  // for each word of this workgroup's among the wave's 64 tokens: each(its place in the range, the lanes that have it)
-  auto match = [&](int word, auto&& each) {
-    uint64_t todo = __ballot((unsigned)(word - first) < (unsigned)mine && word >= 0);
+  // for each word among up to a wave's tokens, of which those in `todo` count: each(word, the lanes that have it)
+  auto match = [&](uint32_t word, uint64_t todo, auto&& each) {
     while (todo) {
-      const int it = __builtin_amdgcn_readlane(word, __builtin_ctzll(todo));
-      const uint64_t same = __ballot(word == it);
-      each(it - first, same);
+      const uint32_t it = (uint32_t)__builtin_amdgcn_readlane((int)word, __builtin_ctzll(todo));
+      const uint64_t same = __ballot(word == it) & todo;
+      each((int)it, same);
       todo &= ~same;
     }
   };
-  int below = 0;
-  walk([&](int, int word) {
-    below += word >= 0 && word < first ? 1 : 0;
-    match(word, [&](int r, uint64_t same) {
-      if (lane == 0) count[wave][r] += __popcll(same);
-    });
-  });
+  // the next places of word r for `n` tokens of the wave
+  auto claim = [&](int r, int n) {
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&count[wave][r], n);
+    return __builtin_amdgcn_readfirstlane(at);
+  };
+  int below = 0, listed = 0;
+  walk([&](int place, const uint32_t (&w)[kSortEach]) {
+    uint64_t here[kSortEach];
+    int n = 0;
 #pragma unroll
-  for (int off = 32; off; off >>= 1) below += __shfl_xor(below, off, kWave);
+    for (int t = 0; t < kSortEach; ++t) {
+      below += __popcll(__ballot(w[t] < (uint32_t)first));
+      here[t] = __ballot(w[t] - (uint32_t)first < (uint32_t)mine);
+      n += __popcll(here[t]);
+    }
+    if (n == 0) return;
+    int to = listed;      // behind the tokens of the lanes below
+#pragma unroll
+    for (int t = 0; t < kSortEach; ++t) to += __popcll(here[t] & lower);
+#pragma unroll
+    for (int t = 0; t < kSortEach; ++t)
+      if (here[t] >> lane & 1) {
+        if (to < kSortList) list[wave][to] = (uint32_t)(place + t) << 10 | (w[t] - (uint32_t)first);
+        ++to;
+      }
+    listed += n;
+  });
+  // more tokens than the list holds, as of a word that is much of the text: the share is gone through again instead, 64 tokens at a time
+  const bool all_listed = listed <= kSortList && share <= 1 << 22;
+  auto walk_all = [&](auto&& take) {
+    for (int64_t at = begin; at < end; at += kWave) {
+      const int64_t i = at + lane;
+      const int64_t id = i < end ? (int64_t)ids[i] : -1;
+      const uint32_t word = (uint64_t)id < (uint32_t)words && (uint32_t)id != padding ? (uint32_t)id - (uint32_t)first : ~0u;
+      match(word, __ballot(word < (uint32_t)mine), [&](int r, uint64_t same) { take((int)i, r, same); });
+    }
+  };
+  if (all_listed) {
+    for (int i = lane; i < listed; i += kWave) atomicAdd(&count[wave][list[wave][i] & (kSortRange - 1)], 1);
+  } else {
+    walk_all([&](int, int r, uint64_t same) {
+      if (lane == 0) atomicAdd(&count[wave][r], __popcll(same));
+    });
+  }
   if (lane == 0) below_of[wave] = below;
   __syncthreads();
   // thread r: word first + r
   const int r = threadIdx.x;
   int total = 0;
+#pragma unroll
   for (int v = 0; v < kSortWaves; ++v) total += count[v][r];
   const int through = wave_inclusive_scan(total);
   if (lane == kWave - 1) sums[wave] = through;
   __syncthreads();
   int start = through - total;
+#pragma unroll
   for (int v = 0; v < kSortWaves; ++v) start += below_of[v] + (v < wave ? sums[v] : 0);
   if (r < mine) {
     starts[first + r] = start;
     if (first + r == words - 1) starts[words] = start + total;
   }
+#pragma unroll
   for (int v = 0; v < kSortWaves; ++v) {
     const int n = count[v][r];
     count[v][r] = start;
     start += n;
   }
   __syncthreads();
-  walk([&](int place, int word) {
-    match(word, [&](int r, uint64_t same) {
-      const int at = count[wave][r];
-      if (word == r + first) {
-        const int to = at + __popcll(same & ((1ull << lane) - 1));
-        order[to] = place;
-        sorted[to] = word;
-      }
-      if (lane == 0) count[wave][r] = at + __popcll(same);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");     // the other lanes read it for the next word
-    });
-  });
+  auto put = [&](int place, int r, uint64_t same) {
+    const int at = claim(r, __popcll(same));
+    if (same >> lane & 1) {
+      const int to = at + __popcll(same & lower);
+      order[to] = place;
+      sorted[to] = first + r;
+    }
+  };
+  if (all_listed) {
+    for (int i0 = 0; i0 < listed; i0 += kWave) {
+      const uint32_t it = i0 + lane < listed ? list[wave][i0 + lane] : 0u;
+      match(it & (kSortRange - 1), __ballot(i0 + lane < listed), [&](int r, uint64_t same) { put((int)begin + (int)(it >> 10), r, same); });
+    }
+  } else {
+    walk_all(put);
+  }
 }
 
 // ---- sums along the order ----
-// Workgroups [0, piece_blocks): a wave per piece of `piece` places of the order and slice of columns; the others: rows of words without a token, zeroed.
+// Workgroups [0, piece_blocks): a wave per piece of kPiece places of the order and slice of columns; the others: rows of words without a token, zeroed.
 // heads[p] / tails[p]: what the run that piece p begins inside of / ends inside of leaves there; a run that goes through the whole piece: heads[p].
-constexpr int kZeroRows = 64;    // words of a wave
+constexpr int kZeroRows = 16;    // words of a wave
+// A run of up to kWholeRun tokens is added up by the piece that it begins in, which has it in its lanes; longer ones are cut at the pieces' ends.
+constexpr int kPiece = 32, kWholeRun = kWave - kPiece;
 
 template <int DT>
 __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* __restrict__ grad, const int32_t* __restrict__ order, const int32_t* __restrict__ sorted,
-                                                                    const int32_t* __restrict__ starts, int words, int hidden, int slices, int piece, int64_t piece_blocks,
-                                                                    float scale, float* __restrict__ heads, float* __restrict__ tails, void* __restrict__ out) {
+                                                                    const int32_t* __restrict__ starts, int words, int hidden, int slices, int64_t piece_blocks,
+                                                                    float scale, float* __restrict__ heads, float* __restrict__ tails, EmbeddingRuns* __restrict__ crossing,
+                                                                    void* __restrict__ out) {
   typedef typename Elem<DT>::type E;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   if ((int64_t)blockIdx.x >= piece_blocks) {
     const int64_t first = (((int64_t)blockIdx.x - piece_blocks) * kEmbWaves + wave) * kZeroRows;
     if (first >= words) return;
     const int64_t v = first + lane;
-    uint64_t todo = __ballot(v < words && starts[v < words ? v : words] == starts[v < words ? v + 1 : words]);
+    uint64_t todo = __ballot(lane < kZeroRows && v < words && starts[v < words ? v : words] == starts[v < words ? v + 1 : words]);
     const float none[kPer] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     while (todo) {
       E* const row = (E*)out + (first + __builtin_ctzll(todo)) * hidden;
@@ -214,102 +293,133 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* 
     return;
   }
   const int64_t unit = (int64_t)blockIdx.x * kEmbWaves + wave;
-  const int64_t p = unit / slices, from = p * piece;
+  const int64_t p = unit / slices, from = p * kPiece;
   const int total = starts[words];
   if (from >= total) return;
   const int column = (int)(unit - p * slices) * kSlice + lane * kPer, left = hidden - column;
-  const int n = total - from < piece ? (int)(total - from) : piece;          // up to a wave's lanes
-  const int my_word = lane < n ? sorted[from + lane] : -1, my_place = lane < n ? order[from + lane] : 0;
+  const int there = total - from < kWave ? (int)(total - from) : kWave, inside = there < kPiece ? there : kPiece;
+  const int my_word = lane < there ? sorted[from + lane] : -1, my_place = lane < there ? order[from + lane] : 0;
   int word = __builtin_amdgcn_readlane(my_word, 0);
-  bool from_before = from > 0 && sorted[from - 1] == word;
-  float acc[kPer] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  auto keep = [&](float* parts) {
-    if (left > 0) store_columns<MBX_F32>(parts + p * hidden + column, left, acc);
-  };
-  auto finish = [&]() {     // the run of `word` ends here
-    if (from_before) {
-      keep(heads);
-    } else if (left > 0) {
-      float v[kPer];
+  const int last_word = __builtin_amdgcn_readlane(my_word, inside - 1);
+  const int begin = starts[word], stop = starts[word + 1], last_begin = starts[last_word], last_stop = starts[last_word + 1];
+  const bool from_others = begin < from && stop - begin <= kWholeRun;
+  const int i0 = from_others ? (int)(stop - from) : 0;
+  if (i0 >= inside) return;
+  const int n = last_stop > from + inside && last_stop - last_begin <= kWholeRun ? (int)(last_stop - from) : inside;      // last_begin >= from: else i0 is past it
+  const bool goes_on = last_stop > from + n;
+  bool from_before = begin < from && !from_others;
+  word = __builtin_amdgcn_readlane(my_word, i0);
+  if (unit == p * slices && lane == 0 && goes_on && last_begin >= from)
+    crossing->runs[atomicAdd(&crossing->count, 1)] = make_int4((int)p, last_word, (int)((last_stop - 1) / kPiece - p + 1), 0);
+  // whole: all kPer columns are the row's
+  auto add_up = [&](auto whole) {
+    float acc[kPer] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto keep = [&](float* parts) { store_columns<MBX_F32>(parts + p * hidden + column, left, acc); };
+    auto finish = [&]() {     // the run of `word` ends here
+      if (from_before) {
+        keep(heads);
+      } else {
+        float v[kPer];
 #pragma unroll
-      for (int t = 0; t < kPer; ++t) v[t] = acc[t] * scale;
-      store_columns<DT>((E*)out + (int64_t)word * hidden + column, left, v);
-    }
-  };
-  constexpr int kAhead = 8;
-  for (int i = 0; i < n; i += kAhead) {
-    float v[kAhead][kPer];
+        for (int t = 0; t < kPer; ++t) v[t] = acc[t] * scale;
+        store_columns<DT>((E*)out + (int64_t)word * hidden + column, left, v);
+      }
+    };
+    constexpr int kAhead = 8;
+    for (int i = i0; i < n; i += kAhead) {
+      Piece<DT> v[kAhead];      // all under way before the first is looked at
+      if constexpr (decltype(whole)::value) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (i + u < n && left > 0)
-        load_columns<DT>((const E*)grad + (int64_t)__builtin_amdgcn_readlane(my_place, i + u) * hidden + column, left, v[u]);
+        for (int u = 0; u < kAhead; ++u)
+          v[u].load((const E*)grad + (int64_t)__builtin_amdgcn_readlane(my_place, i + u < n ? i + u : n - 1) * hidden + column);
+      }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (i + u < n) {
-        const int here = __builtin_amdgcn_readlane(my_word, i + u);
-        if (here != word) {
-          finish();
-          word = here;
-          from_before = false;
+      for (int u = 0; u < kAhead; ++u) {
+        if (i + u < n) {
+          const int here = __builtin_amdgcn_readlane(my_word, i + u);
+          if (here != word) {
+            finish();
+            word = here;
+            from_before = false;
 #pragma unroll
-          for (int t = 0; t < kPer; ++t) acc[t] = 0.f;
+            for (int t = 0; t < kPer; ++t) acc[t] = 0.f;
+          }
+          if constexpr (decltype(whole)::value) {
+#pragma unroll
+            for (int t = 0; t < kPer; ++t) acc[t] += v[u].value(t);
+          } else {
+            float last[kPer];
+            load_columns<DT>((const E*)grad + (int64_t)__builtin_amdgcn_readlane(my_place, i + u) * hidden + column, left, last);
+#pragma unroll
+            for (int t = 0; t < kPer; ++t) acc[t] += last[t];
+          }
         }
-#pragma unroll
-        for (int t = 0; t < kPer; ++t) acc[t] += v[u][t];
       }
     }
-  }
-  const bool goes_on = from + n < total && sorted[from + n] == word;
-  if (goes_on) keep(from_before ? heads : tails);
-  else finish();
+    if (!goes_on) finish();
+    else keep(from_before ? heads : tails);
+  };
+  if (left >= kPer) add_up(std::true_type{});
+  else if (left > 0) add_up(std::false_type{});
 }
 
-// ---- runs that cross pieces: a workgroup per piece that such a run begins in and kJoinColumns columns ----
-constexpr int kJoinColumns = kWave * 4;
+// ---- runs that are cut: a workgroup per run and kJoinColumns columns ----
+constexpr int kJoinColumns = kWave * 4, kJoinThreads = 512, kJoinWaves = kJoinThreads / kWave, kJoinRuns = 128;
 
 template <int DT>
-__global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const int32_t* __restrict__ sorted, const int32_t* __restrict__ starts, int words, int hidden,
-                                                                     int piece, float scale, const float* __restrict__ heads, const float* __restrict__ tails,
-                                                                     void* __restrict__ out) {
+__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden, float scale, const float* __restrict__ heads, const float* __restrict__ tails,
+                                                                      const EmbeddingRuns* __restrict__ crossing, void* __restrict__ out) {
   typedef typename Elem<DT>::type E;
-  __shared__ float sums[kEmbWaves][kJoinColumns];
-  const int64_t p = blockIdx.x, from = p * piece;
-  const int total = starts[words];
-  if (from + piece >= total) return;                     // nothing behind this piece
-  const int word = sorted[from + piece - 1];
-  const int begin = starts[word], end = starts[word + 1];
-  if (begin < from || end <= from + piece) return;
-  const int64_t last = (end - 1) / piece;                // pieces p .. last
+  __shared__ float sums[kJoinWaves][kJoinColumns];
   const int wave = threadIdx.x / kWave, lane = lane_id(), column = (int)blockIdx.y * kJoinColumns + lane * 4;
+  int4 it = crossing->runs[blockIdx.x];      // under way with the count: it may be none
+  const int runs = crossing->count;
+  for (int run = blockIdx.x; run < runs; run += gridDim.x) {
+  if (run != (int)blockIdx.x) it = crossing->runs[run];
+  const int64_t p = it.x, parts = it.z;
+  const int word = it.y;
   // the waves take consecutive runs of the pieces' parts, and are added in order
-  const int64_t parts = last - p + 1, share = (parts + kEmbWaves - 1) / kEmbWaves;
+  const int64_t share = (parts + kJoinWaves - 1) / kJoinWaves;
   const int64_t a = wave * share, b = a + share < parts ? a + share : parts;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t i = a; i < b; ++i) {
-    const float* const row = (i == 0 ? tails + p * hidden : heads + (p + i) * hidden) + column;
+  auto row = [&](int64_t n) { return (n == 0 ? tails + p * hidden : heads + (p + n) * hidden) + column; };
+  if (column + 4 <= hidden) {
+    constexpr int kAhead = 8;
+    for (int64_t i = a; i < b; i += kAhead) {
+      u32x4e v[kAhead];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (column + t < hidden) acc[t] += row[t];
+      for (int u = 0; u < kAhead; ++u) v[u] = *(const u32x4_at4*)row(i + u < b ? i + u : b - 1);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (i + u < b)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[t] += __uint_as_float(v[u][t]);
+    }
+  } else {
+    for (int64_t i = a; i < b; ++i)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (column + t < hidden) acc[t] += row(i)[t];
   }
 #pragma unroll
   for (int t = 0; t < 4; ++t) sums[wave][lane * 4 + t] = acc[t];
   __syncthreads();
   const int c = (int)blockIdx.y * kJoinColumns + (int)threadIdx.x;
-  if (c >= hidden) return;
-  float v = 0.f;
+  if (threadIdx.x < kJoinColumns && c < hidden) {
+    float v = 0.f;
 #pragma unroll
-  for (int w = 0; w < kEmbWaves; ++w) v += sums[w][threadIdx.x];
-  ((E*)out)[(int64_t)word * hidden + c] = Elem<DT>::from_f32(v * scale);
+    for (int w = 0; w < kJoinWaves; ++w) v += sums[w][threadIdx.x];
+    ((E*)out)[(int64_t)word * hidden + c] = Elem<DT>::from_f32(v * scale);
+  }
+  __syncthreads();      // the next run's sums
+  }
 }
-static_assert(kJoinColumns == kEmbThreads, "a column a thread");
 
 struct EmbeddingParts {
-  size_t order, sorted, starts, heads, tails, total = 0;
-  int piece;
+  size_t order, sorted, starts, heads, tails, crossing, total = 0;
   int64_t pieces;
   EmbeddingParts(int64_t tokens, int words, int hidden) {
-    piece = tokens <= (1 << 17) ? 32 : 64;
-    pieces = ceil_div(tokens, piece);
+    pieces = ceil_div(tokens, kPiece);
     auto take = [&](size_t bytes) {
       const size_t at = total;
       total += (bytes + 255) & ~(size_t)255;
@@ -320,6 +430,7 @@ struct EmbeddingParts {
     starts = take((size_t)(words + 1) * 4);
     heads = take((size_t)pieces * hidden * 4);
     tails = take((size_t)pieces * hidden * 4);
+    crossing = take(sizeof(EmbeddingRuns) + sizeof(int4) * (size_t)(pieces > kJoinRuns ? pieces : kJoinRuns));
   }
 };
 
@@ -333,12 +444,12 @@ int launch_embedding(const void* ids, int64_t tokens, const void* table, int wor
 }
 
 template <typename I>
-int launch_sort(const void* ids, int64_t tokens, int words, int64_t padding, int32_t* order, int32_t* sorted, int32_t* starts, hipStream_t s) {
+int launch_sort(const void* ids, int64_t tokens, int words, int64_t padding, int32_t* order, int32_t* sorted, int32_t* starts, EmbeddingRuns* crossing, hipStream_t s) {
   // a workgroup on every compute unit where there are words for them, and no more words each than it counts
   int range = (int)ceil_div(words, 256);
   if (range > kSortRange) range = kSortRange;
-  embedding_sort_kernel<I><<<(unsigned)ceil_div(words, range), kSortThreads, 0, s>>>((const I*)ids, tokens, words, range, padding < 0 || padding >= words ? -2 : (int)padding,
-                                                                                     order, sorted, starts);
+  embedding_sort_kernel<I><<<(unsigned)ceil_div(words, range), kSortThreads, 0, s>>>((const I*)ids, tokens, words, range, padding < 0 || padding >= words ? ~0u : (uint32_t)padding,
+                                                                                     order, sorted, starts, crossing);
   return launch_status();
 }
 
@@ -347,15 +458,16 @@ int launch_sums(const void* grad, int words, int hidden, float scale, const Embe
   const int32_t *const order = (const int32_t*)(scratch + parts.order), *const sorted = (const int32_t*)(scratch + parts.sorted);
   const int32_t* const starts = (const int32_t*)(scratch + parts.starts);
   float *const heads = (float*)(scratch + parts.heads), *const tails = (float*)(scratch + parts.tails);
+  EmbeddingRuns* const crossing = (EmbeddingRuns*)(scratch + parts.crossing);
   const int slices = (int)ceil_div(hidden, kSlice);
   const int64_t piece_blocks = ceil_div(parts.pieces * slices, kEmbWaves), zero_blocks = ceil_div(words, kEmbWaves * kZeroRows);
   if (piece_blocks + zero_blocks > 0x7fffffff) return MBX_ERANGE;
-  embedding_sum_kernel<DT><<<(unsigned)(piece_blocks + zero_blocks), kEmbThreads, 0, s>>>(grad, order, sorted, starts, words, hidden, slices, parts.piece, piece_blocks,
-                                                                                          scale, heads, tails, out);
+  embedding_sum_kernel<DT><<<(unsigned)(piece_blocks + zero_blocks), kEmbThreads, 0, s>>>(grad, order, sorted, starts, words, hidden, slices, piece_blocks,
+                                                                                          scale, heads, tails, crossing, out);
   if (const int rc = launch_status()) return rc;
   if (parts.pieces > 1) {
-    embedding_join_kernel<DT><<<dim3((unsigned)(parts.pieces - 1), (unsigned)ceil_div(hidden, kJoinColumns)), kEmbThreads, 0, s>>>(sorted, starts, words, hidden, parts.piece,
-                                                                                                                              scale, heads, tails, out);
+    const unsigned runs = (unsigned)(parts.pieces - 1 < kJoinRuns ? parts.pieces - 1 : kJoinRuns);
+    embedding_join_kernel<DT><<<dim3(runs, (unsigned)ceil_div(hidden, kJoinColumns)), kJoinThreads, 0, s>>>(hidden, scale, heads, tails, crossing, out);
     return launch_status();
   }
   return 0;
@@ -402,8 +514,9 @@ int mbx_embedding_gradient(const void* grad, const void* ids, int itype, int64_t
   char* const base = (char*)scratch;
   hipStream_t s = as_stream(stream);
   int32_t *const order = (int32_t*)(base + parts.order), *const sorted = (int32_t*)(base + parts.sorted), *const starts = (int32_t*)(base + parts.starts);
-  const int rc = itype == MBX_I32 ? launch_sort<int32_t>(ids, tokens, (int)words, padding, order, sorted, starts, s)
-                                  : launch_sort<int64_t>(ids, tokens, (int)words, padding, order, sorted, starts, s);
+  EmbeddingRuns* const crossing = (EmbeddingRuns*)(base + parts.crossing);
+  const int rc = itype == MBX_I32 ? launch_sort<int32_t>(ids, tokens, (int)words, padding, order, sorted, starts, crossing, s)
+                                  : launch_sort<int64_t>(ids, tokens, (int)words, padding, order, sorted, starts, crossing, s);
   if (rc) return rc;
   if (dtype == MBX_BF16) return launch_sums<MBX_BF16>(grad, (int)words, (int)hidden, scale, parts, base, out, s);
   if (dtype == MBX_F16) return launch_sums<MBX_F16>(grad, (int)words, (int)hidden, scale, parts, base, out, s);

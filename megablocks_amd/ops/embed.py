@@ -39,7 +39,9 @@ class EmbeddingOp(torch.autograd.Function):
     @staticmethod
     def backward(ctx: Any, grad):
         ids, = ctx.saved_tensors
-        return None, EmbeddingGradientOp.apply(grad, ids, *ctx.sizes), None, None
+        # a node of its own only where the backward is differentiated itself
+        gradient = EmbeddingGradientOp.apply if torch.is_grad_enabled() else _table_gradient
+        return None, gradient(grad, ids, *ctx.sizes), None, None
 
 
 class EmbeddingGradientOp(torch.autograd.Function):

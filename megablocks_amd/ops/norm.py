@@ -1,14 +1,18 @@
 """The norm of all gradients together, and clipping by it: what a training step does between its backward and its optimizer.  The reference leaves it to the
 trainer around it, whose expert weights it marks for that purpose (megablocks/layers/mpu.py)."""
-import ctypes
+import array
 import math
+import operator
 
 import torch
 
 from megablocks_amd import _lib
 from megablocks_amd._lib import lib
 
+# a property of all tensors at a time, by calls that are C throughout: for hundreds of small tensors the host's time is what a pass takes (300 and as many outputs: 393 us of it
+# a tensor's properties one after the other, now 219)
 _is_contiguous, _get_device, _data_ptr, _numel = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.numel
+_dtype, _requires_grad = operator.attrgetter('dtype'), operator.attrgetter('requires_grad')
 
 
 def _check_norm(what, norm_type):
@@ -18,29 +22,35 @@ def _check_norm(what, norm_type):
     return norm_type
 
 
-def _on_one_gpu(what, tensors):
-    """The tensors as a list, checked."""
-    tensors = list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
-            raise RuntimeError(f'{what}: expected dense tensors')
-    devices = set(map(_get_device, tensors))
-    dtypes = {t.dtype for t in tensors}
-    if tensors and (len(devices) > 1 or min(devices) < 0 or not dtypes <= _lib.DTYPE.keys()):
-        raise RuntimeError(f'{what}: expected bfloat16, float16 or float32 tensors on one GPU but got {sorted({f"{t.dtype} on {t.device}" for t in tensors})}')
-    if getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0 or (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
-        raise RuntimeError(f'{what}: norms and clipping have no gradient; call them under torch.no_grad(), on gradients')
-    return tensors
+class _Operands:
+    """Tensors on one GPU as the library takes them: arrays of addresses, element counts and types in host memory."""
+
+    def __init__(self, what, tensors):
+        self.tensors = tensors
+        try:
+            dtypes, devices = list(map(_dtype, tensors)), set(map(_get_device, tensors))
+            self.numel = array.array('q', map(_numel, tensors))
+            if tensors and (len(devices) > 1 or min(devices) < 0 or not _lib.DTYPE.keys() >= set(dtypes)):
+                raise RuntimeError(f'{what}: expected bfloat16, float16 or float32 tensors on one GPU but got {sorted({f"{t.dtype} on {t.device}" for t in tensors})}')
+            self.plain = tensors if all(map(_is_contiguous, tensors)) else [t if t.is_contiguous() else None for t in tensors]
+        except (TypeError, AttributeError):
+            raise RuntimeError(f'{what}: expected dense tensors') from None
+        self.device, self.types = devices, array.array('i', map(_lib.DTYPE.__getitem__, dtypes))
+        if getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0 or (torch.is_grad_enabled() and any(map(_requires_grad, tensors))):
+            raise RuntimeError(f'{what}: norms and clipping have no gradient; call them under torch.no_grad(), on gradients')
+
+    def fill(self, make):
+        """A contiguous tensor, make(t), for each t that is not."""
+        if self.plain is not self.tensors:
+            self.plain = [make(t) if p is None else p for t, p in zip(self.tensors, self.plain)]
+        self.addresses = array.array('Q', map(_data_ptr, self.plain))
 
 
-def _operands(tensors):
-    """(addresses, element counts, types) as the library takes them."""
-    n = len(tensors)
-    return ((ctypes.c_void_p * n)(*map(_data_ptr, tensors)), (ctypes.c_int64 * n)(*map(_numel, tensors)),
-            (ctypes.c_int * n)(*[_lib.DTYPE[t.dtype] for t in tensors]))
+def _address(values):
+    return values.buffer_info()[0]
 
 
-def _outputs(device, n):
+def _results(device, n):
     scratch = torch.empty(lib.mbx_global_norm_scratch_bytes(n), dtype=torch.uint8, device=device)
     return torch.empty((), dtype=torch.float32, device=device), scratch
 
@@ -49,53 +59,58 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all values of the tensors together, as one number in fp32 on their device: (sum |x|^p)^(1/p) for p = 1 and 2, max |x| for inf.  tensors:
     bf16, fp16 and fp32 ones, mixed as they come, of any shape.  Sums are held in 64 bits and come out the same from run to run; a NaN gives NaN.  No tensor:
     0, on the CPU."""
-    norm_type = _check_norm('global_norm', norm_type)
-    tensors = _on_one_gpu('global_norm', tensors)
+    norm_type, tensors = _check_norm('global_norm', norm_type), list(tensors)
+    given = _Operands('global_norm', tensors)
     if not tensors:
         return torch.zeros((), dtype=torch.float32)
-    plain = [t if c else t.contiguous() for t, c in zip(tensors, map(_is_contiguous, tensors))]      # kept until the launch is under way
-    norm, scratch = _outputs(plain[0].device, len(plain))
+    given.fill(torch.Tensor.contiguous)
+    norm, scratch = _results(tensors[0].device, len(tensors))
     with _lib.device_of(norm):
-        _lib.check(lib.mbx_global_norm(*_operands(plain), len(plain), norm_type, norm.data_ptr(), scratch.data_ptr(), scratch.numel(), _lib.stream()), 'global_norm')
+        _lib.check(lib.mbx_global_norm(_address(given.addresses), _address(given.numel), _address(given.types), len(tensors), norm_type, norm.data_ptr(),
+                                       scratch.data_ptr(), scratch.numel(), _lib.stream()), 'global_norm')
     return norm
 
 
 def clip_by_global_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Multiplies the tensors by min(1, max_norm / (norm + 1e-6)), norm = `global_norm` of them all, and returns the norm before that; a norm that is NaN makes all
     values NaN, an infinite one zeros and NaN.  In place, where the launches that would write do nothing if the norm is short enough, or into `out`: as many tensors of
-    the same sizes, in bf16, fp16 or fp32 (the fp32 gradients an optimizer reads, for instance), rounded once.  No output may lie over another, or over a tensor
+    as many elements, in bf16, fp16 or fp32 (the fp32 gradients an optimizer reads, for instance), rounded once.  No output may lie over another, or over a tensor
     that is not its own."""
-    norm_type, max_norm = _check_norm('clip_by_global_norm_', norm_type), float(max_norm)
+    what = 'clip_by_global_norm_'
+    norm_type, max_norm, tensors = _check_norm(what, norm_type), float(max_norm), list(tensors)
     if not max_norm >= 0:
-        raise ValueError('clip_by_global_norm_: the largest norm must be a number from 0 on')
-    tensors = _on_one_gpu('clip_by_global_norm_', tensors)
-    outputs = tensors if out is None else _on_one_gpu('clip_by_global_norm_', out)
-    if len(outputs) != len(tensors) or any(o.shape != t.shape for t, o in zip(tensors, outputs)):
-        raise ValueError('clip_by_global_norm_: an output of the same size for every tensor')
+        raise ValueError(f'{what}: the largest norm must be a number from 0 on')
+    given = _Operands(what, tensors)
+    to = given
+    if out is not None:
+        to = _Operands(what, list(out))
+        if to.numel != given.numel:
+            raise ValueError(f'{what}: an output of as many elements for every tensor')
     if not tensors:
         return torch.zeros((), dtype=torch.float32)
-    if outputs[0].get_device() != tensors[0].get_device():
-        raise RuntimeError('clip_by_global_norm_: tensors and outputs must be on one GPU')
-    plain = [t if c else t.contiguous() for t, c in zip(tensors, map(_is_contiguous, tensors))]
-    if out is None:
-        to = plain
-    else:
-        to = [o if c else torch.empty_like(o, memory_format=torch.contiguous_format) for o, c in zip(outputs, map(_is_contiguous, outputs))]
-    strided = [(o, made) for o, made in zip(outputs, to) if made is not o]
-    if strided:
+    if to.device != given.device:
+        raise RuntimeError(f'{what}: tensors and outputs must be on one GPU')
+    outputs = to.tensors
+    if to.plain is not outputs:
         _refuse_overlaps(outputs, tensors)
-    norm, scratch = _outputs(plain[0].device, len(plain))
-    in_ptrs, numels, types = _operands(plain)
-    out_ptrs, _, out_types = (in_ptrs, numels, types) if to is plain else _operands(to)
+    given.fill(torch.Tensor.contiguous)
+    if to is not given:
+        to.fill(lambda t: torch.empty_like(t, memory_format=torch.contiguous_format))
+    norm, scratch = _results(tensors[0].device, len(tensors))
     with _lib.device_of(norm):
-        rc = lib.mbx_clip_by_global_norm(in_ptrs, out_ptrs, numels, types, out_types, len(plain), norm_type, max_norm, norm.data_ptr(), scratch.data_ptr(),
-                                         scratch.numel(), _lib.stream())
+        rc = lib.mbx_clip_by_global_norm(_address(given.addresses), _address(to.addresses), _address(given.numel), _address(given.types), _address(to.types), len(tensors),
+                                         norm_type, max_norm, norm.data_ptr(), scratch.data_ptr(), scratch.numel(), _lib.stream())
     if rc == _lib.EINVAL:
-        raise ValueError('clip_by_global_norm_: an output lies over another one, or over a tensor that is not its own')
-    _lib.check(rc, 'clip_by_global_norm_')
-    for o, made in strided:
-        o.copy_(made)
-    torch.autograd.graph.increment_version([o for o in outputs if not o.is_inference()])
+        raise ValueError(f'{what}: an output lies over another one, or over a tensor that is not its own')
+    _lib.check(rc, what)
+    if to.plain is not outputs:
+        for o, made in zip(outputs, to.plain):
+            if made is not o:
+                o.copy_(made)
+    try:
+        torch.autograd.graph.increment_version(outputs)
+    except RuntimeError:      # tensors made in inference mode have no version
+        torch.autograd.graph.increment_version([o for o in outputs if not o.is_inference()])
     return norm
 
 
