@@ -5,9 +5,9 @@
 //
 // What bounds it is reading the weights of the chosen experts, once, and, for a few small ones, the way between the launches.  Three of them:
 //
-//   choose   a wave per expert and token (or eight tokens): logits as exact products summed in 64 bits, so that no order of summation decides between
+//   choose   a wave per expert and token (or four tokens): logits as exact products summed in 64 bits, so that no order of summation decides between
 //            neighbours; the workgroup that is last at a group of tokens chooses for them, and the last of all makes the table of which experts have which rows
-//   hidden   a workgroup per used expert and 16 to 64 rows of its first weights, a quarter of the reduction a wave; the activation is kept as the sum of two
+//   hidden   a workgroup per used expert and 16 to 128 rows of its first weights, a quarter of the reduction a wave; the activation is kept as the sum of two
 //            16-bit numbers, so that the second product sees it to 2^-17
 //   down     a workgroup per used expert, 128 columns and a part of the reduction; the parts meet in memory, and the workgroup that is last at its columns adds them up
 //            in a fixed order, weights them and writes the output
@@ -345,7 +345,7 @@ layer_choose_whole_kernel(const uint16_t* __restrict__ x, const uint16_t* __rest
     make_table<kWholeThreads>(q, [&](int s) { return load_through(choice + s); }, table);
 }
 
-// Workgroup (b, g): experts 4 b .. 4 b + 3, a wave each, tokens TB g .. ; TB 1 or 8.
+// Workgroup (b, g): experts 4 b .. 4 b + 3, a wave each, tokens TB g .. ; TB 1 or 4.
 template <int DT, int TB, int R>
 __global__ void __launch_bounds__(kLayerThreads)
 layer_choose_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ router, LayerChoice q, const float* __restrict__ bias, uint64_t* __restrict__ logits,
@@ -751,12 +751,13 @@ void launch_choose(const void* x_, const void* router_, const LayerChoice& q, co
     return;
   }
   const unsigned workgroups = (unsigned)ceil_div(q.experts, kLayerWaves);
-  // tokens one by one while all their waves are resident; eight of them read the router once together
+  // tokens one by one while there are few waves in all (us, one / two / four / eight of them a wave: 19 tokens, 256 experts of 1104 22 / 17 / 14 / 17, 64 tokens, 128 of
+  // 4096 26 / 23 / 20 / 24)
   uint64_t* const logits = (uint64_t*)(base + plan.logits);
   if (q.experts * q.tokens <= 4096)
     layer_choose_kernel<DT, 1, R><<<dim3(workgroups, (unsigned)q.tokens), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
   else
-    layer_choose_kernel<DT, 8, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 8)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
+    layer_choose_kernel<DT, 4, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 4)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
 }
 
 template <int DT, int R>

@@ -51,16 +51,20 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, w1: torch.Tensor, v1: Optio
         raise ValueError('moe_layer: act must be ACT_SILU or ACT_GELU_TANH')
     check_choice(experts, top_k, score, groups, top_groups, group_best, norm_p, scale)
     check_sizes(tokens, hidden, ffn, experts, top_k)
-    given = (x, router, w1, w2) if v1 is None else (x, router, w1, v1, w2)
-    device, dtype = x.device, x.dtype
-    if not x.is_cuda or any(t.device != device for t in given) or dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != dtype for t in given):
-        raise RuntimeError(f'moe_layer: expected bfloat16 or float16 tensors of one type on one GPU but got {sorted({f"{t.dtype} on {t.device}" for t in given})}')
+    device, dtype, recorded = x.device, x.dtype, torch.is_grad_enabled()
+    if not x.is_cuda or dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f'moe_layer: expected bfloat16 or float16 tensors on a GPU but got {dtype} on {device}')
+    if getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0 or (recorded and x.requires_grad):
+        raise RuntimeError('moe_layer: the layer for a few tokens has no gradient; call it under torch.no_grad()')
+    for w in (router, w1, w2) if v1 is None else (router, w1, v1, w2):
+        if w.device != device or w.dtype != dtype:
+            raise RuntimeError(f'moe_layer: expected {dtype} weights on {device}, as the tokens, but got {w.dtype} on {w.device}')
+        if recorded and w.requires_grad:
+            raise RuntimeError('moe_layer: the layer for a few tokens has no gradient; call it under torch.no_grad()')
+        if not w.is_contiguous() or w.data_ptr() % 16:
+            raise RuntimeError('moe_layer: the router and the weights must be contiguous and start at multiples of 16 bytes')
     if bias is not None and (bias.dtype != torch.float32 or bias.device != device):
         raise RuntimeError(f'moe_layer: expected a float32 bias on {device} but got {bias.dtype} on {bias.device}')
-    if getattr(torch.autograd.forward_ad, '_current_level', 0) >= 0 or (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
-        raise RuntimeError('moe_layer: the layer for a few tokens has no gradient; call it under torch.no_grad()')
-    if any(not w.is_contiguous() or w.data_ptr() % 16 for w in given[1:]):
-        raise RuntimeError('moe_layer: the router and the weights must be contiguous and start at multiples of 16 bytes')
     return launch(x, router, w1, v1, w2, ffn, top_k, act, score, bias, groups, top_groups, group_best, norm_p, scale)
 
 
