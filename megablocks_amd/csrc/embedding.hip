@@ -375,43 +375,43 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden
   int4 it = crossing->runs[blockIdx.x];      // under way with the count: it may be none
   const int runs = crossing->count;
   for (int run = blockIdx.x; run < runs; run += gridDim.x) {
-  if (run != (int)blockIdx.x) it = crossing->runs[run];
-  const int64_t p = it.x, parts = it.z;
-  const int word = it.y;
-  // the waves take consecutive runs of the pieces' parts, and are added in order
-  const int64_t share = (parts + kJoinWaves - 1) / kJoinWaves;
-  const int64_t a = wave * share, b = a + share < parts ? a + share : parts;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  auto row = [&](int64_t n) { return (n == 0 ? tails + p * hidden : heads + (p + n) * hidden) + column; };
-  if (column + 4 <= hidden) {
-    constexpr int kAhead = 8;
-    for (int64_t i = a; i < b; i += kAhead) {
-      u32x4e v[kAhead];
+    if (run != (int)blockIdx.x) it = crossing->runs[run];
+    const int64_t p = it.x, parts = it.z;
+    const int word = it.y;
+    // the waves take consecutive runs of the pieces' parts, and are added in order
+    const int64_t share = (parts + kJoinWaves - 1) / kJoinWaves;
+    const int64_t a = wave * share, b = a + share < parts ? a + share : parts;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    auto row = [&](int64_t n) { return (n == 0 ? tails + p * hidden : heads + (p + n) * hidden) + column; };
+    if (column + 4 <= hidden) {
+      constexpr int kAhead = 8;
+      for (int64_t i = a; i < b; i += kAhead) {
+        u32x4e v[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) v[u] = *(const u32x4_at4*)row(i + u < b ? i + u : b - 1);
+        for (int u = 0; u < kAhead; ++u) v[u] = *(const u32x4_at4*)row(i + u < b ? i + u : b - 1);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (i + u < b)
+        for (int u = 0; u < kAhead; ++u)
+          if (i + u < b)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) acc[t] += __uint_as_float(v[u][t]);
+            for (int t = 0; t < 4; ++t) acc[t] += __uint_as_float(v[u][t]);
+      }
+    } else {
+      for (int64_t i = a; i < b; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (column + t < hidden) acc[t] += row(i)[t];
     }
-  } else {
-    for (int64_t i = a; i < b; ++i)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (column + t < hidden) acc[t] += row(i)[t];
-  }
+    for (int t = 0; t < 4; ++t) sums[wave][lane * 4 + t] = acc[t];
+    __syncthreads();
+    const int c = (int)blockIdx.y * kJoinColumns + (int)threadIdx.x;
+    if (threadIdx.x < kJoinColumns && c < hidden) {
+      float v = 0.f;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) sums[wave][lane * 4 + t] = acc[t];
-  __syncthreads();
-  const int c = (int)blockIdx.y * kJoinColumns + (int)threadIdx.x;
-  if (threadIdx.x < kJoinColumns && c < hidden) {
-    float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kJoinWaves; ++w) v += sums[w][threadIdx.x];
-    ((E*)out)[(int64_t)word * hidden + c] = Elem<DT>::from_f32(v * scale);
-  }
-  __syncthreads();      // the next run's sums
+      for (int w = 0; w < kJoinWaves; ++w) v += sums[w][threadIdx.x];
+      ((E*)out)[(int64_t)word * hidden + c] = Elem<DT>::from_f32(v * scale);
+    }
+    __syncthreads();      // the next run's sums
   }
 }
 

@@ -424,99 +424,99 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
   const __amdgpu_buffer_rsrc_t rsrc_x = rsrc_of(x, (uint32_t)tokens * pitch), rsrc_w = rsrc_of(w1 + expert * matrix, (uint32_t)(matrix * 2));
   const __amdgpu_buffer_rsrc_t rsrc_v = GATE ? rsrc_of(v1 + expert * matrix, (uint32_t)(matrix * 2)) : rsrc_w;
   for (int done = 0; done < all_rows; done += 16 * R) {      // once, but for experts of many rows
-  const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
-  uint32_t x_off[R];
+    const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
+    uint32_t x_off[R];
 #pragma unroll
-  for (int t = 0; t < R; ++t) {
-    const int r = t * 16 + c;
-    x_off[t] = r < rows ? (uint32_t)table->token_of_row[first + r] * pitch + (uint32_t)g * 16u : kNone;
-  }
-  const uint32_t w_off = (uint32_t)(f0 + c) * pitch + (uint32_t)g * 16u;
-  struct Chunk { u32x4 a[R][2], b[NF][2]; };
-  const int chunks = (hidden + kChunk - 1) / kChunk;
-  auto fetch = [&](Chunk& q, int chunk) {
-    const uint32_t at = (uint32_t)chunk * (kChunk * 2);
-    const uint32_t past[2] = {chunk * kChunk + 8 * g < hidden ? 0u : kNone, chunk * kChunk + 8 * g + 32 < hidden ? 0u : kNone};      // pieces past the row's end
+    for (int t = 0; t < R; ++t) {
+      const int r = t * 16 + c;
+      x_off[t] = r < rows ? (uint32_t)table->token_of_row[first + r] * pitch + (uint32_t)g * 16u : kNone;
+    }
+    const uint32_t w_off = (uint32_t)(f0 + c) * pitch + (uint32_t)g * 16u;
+    struct Chunk { u32x4 a[R][2], b[NF][2]; };
+    const int chunks = (hidden + kChunk - 1) / kChunk;
+    auto fetch = [&](Chunk& q, int chunk) {
+      const uint32_t at = (uint32_t)chunk * (kChunk * 2);
+      const uint32_t past[2] = {chunk * kChunk + 8 * g < hidden ? 0u : kNone, chunk * kChunk + 8 * g + 32 < hidden ? 0u : kNone};      // pieces past the row's end
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const int row = GATE ? f % (NF / 2 > 0 ? NF / 2 : 1) : f;
+          q.b[f][s] = load16(GATE && f >= NF / 2 ? rsrc_v : rsrc_w, (w_off + at + (uint32_t)(row * 16) * pitch + 64u * s) | past[s]);
+        }
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+          if (t == 0 || t < row_tiles) q.a[t][s] = load16(rsrc_x, (x_off[t] + at + 64u * s) | past[s] | (x_off[t] & kNone));
+    };
+    f32x4 acc[R][NF];
+#pragma unroll
+    for (int t = 0; t < R; ++t)
+#pragma unroll
+      for (int f = 0; f < NF; ++f) acc[t][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Chunk& q) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+          if (t == 0 || t < row_tiles)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) acc[t][f] = mfma<DT>(q.b[f][s], q.a[t][s], acc[t][f]);
+    };
+    // The waves take the chunks in turn, every workgroup from another one on and round: started together at the rows' beginnings they would all ask for bytes that
+    // are a power of two apart, of a few memory channels (1 token, 2 of 8 experts of [14336, 4096]: the layer 164 us, now 148).
+    const int steps = chunks > wave ? (chunks - wave + kLayerWaves - 1) / kLayerWaves : 0;      // this wave's
+    const int turn = steps > 0 ? (int)(((uint32_t)(f0 / kCols) * 5u + (uint32_t)u * 3u) % (uint32_t)steps) : 0;
+    auto chunk_of = [&](int step) {
+      const int at = step + turn < steps ? step + turn : step + turn - steps;
+      return step < steps ? at * kLayerWaves + wave : chunks;      // past the last one nothing is fetched
+    };
+    Chunk q0, q1;
+    fetch(q0, chunk_of(0));
+    for (int step = 0; step < steps; step += 2) {
+      fetch(q1, chunk_of(step + 1));
+      __builtin_amdgcn_sched_barrier(0);      // a chunk's loads are all issued before the products of the one before it
+      multiply(q0);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(q0, chunk_of(step + 2));
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // accumulator t, f, register i of lane (c, g): token row 16 t + c, weight row 16 f + 4 g + i
+    constexpr int kEach = kCols / 16;
+    const int m = threadIdx.x / 16, col = threadIdx.x % 16 * kEach;
+    for (int t = 0; t < row_tiles; ++t) {
+      if (t > 0 || done > 0) __syncthreads();
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const int row = GATE ? f % (NF / 2 > 0 ? NF / 2 : 1) : f;
-        q.b[f][s] = load16(GATE && f >= NF / 2 ? rsrc_v : rsrc_w, (w_off + at + (uint32_t)(row * 16) * pitch + 64u * s) | past[s]);
+        f32x4 v = acc[0][f];
+#pragma unroll
+        for (int o = 1; o < R; ++o)
+          if (t == o) v = acc[o][f];
+        *(f32x4*)&sums[wave][c][f * 16 + 4 * g] = v;
       }
+      __syncthreads();
+      const int r = t * 16 + m;
+      if (r < rows && f0 + col < ffn) {      // ffn is a multiple of 8, a thread's columns 1, 2 or 4
+        uint16_t hi[kEach], lo[kEach];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < kEach; ++i) {
+          float v = 0.f, gate = 0.f;
 #pragma unroll
-      for (int t = 0; t < R; ++t)
-        if (t == 0 || t < row_tiles) q.a[t][s] = load16(rsrc_x, (x_off[t] + at + 64u * s) | past[s] | (x_off[t] & kNone));
-  };
-  f32x4 acc[R][NF];
-#pragma unroll
-  for (int t = 0; t < R; ++t)
-#pragma unroll
-    for (int f = 0; f < NF; ++f) acc[t][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const Chunk& q) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int t = 0; t < R; ++t)
-        if (t == 0 || t < row_tiles)
-#pragma unroll
-          for (int f = 0; f < NF; ++f) acc[t][f] = mfma<DT>(q.b[f][s], q.a[t][s], acc[t][f]);
-  };
-  // The waves take the chunks in turn, every workgroup from another one on and round: started together at the rows' beginnings they would all ask for bytes that
-  // are a power of two apart, of a few memory channels (1 token, 2 of 8 experts of [14336, 4096]: the layer 164 us, now 148).
-  const int steps = chunks > wave ? (chunks - wave + kLayerWaves - 1) / kLayerWaves : 0;      // this wave's
-  const int turn = steps > 0 ? (int)(((uint32_t)(f0 / kCols) * 5u + (uint32_t)u * 3u) % (uint32_t)steps) : 0;
-  auto chunk_of = [&](int step) {
-    const int at = step + turn < steps ? step + turn : step + turn - steps;
-    return step < steps ? at * kLayerWaves + wave : chunks;      // past the last one nothing is fetched
-  };
-  Chunk q0, q1;
-  fetch(q0, chunk_of(0));
-  for (int step = 0; step < steps; step += 2) {
-    fetch(q1, chunk_of(step + 1));
-    __builtin_amdgcn_sched_barrier(0);      // a chunk's loads are all issued before the products of the one before it
-    multiply(q0);
-    __builtin_amdgcn_sched_barrier(0);
-    fetch(q0, chunk_of(step + 2));
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(q1);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  // accumulator t, f, register i of lane (c, g): token row 16 t + c, weight row 16 f + 4 g + i
-  constexpr int kEach = kCols / 16;
-  const int m = threadIdx.x / 16, col = threadIdx.x % 16 * kEach;
-  for (int t = 0; t < row_tiles; ++t) {
-    if (t > 0 || done > 0) __syncthreads();
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      f32x4 v = acc[0][f];
-#pragma unroll
-      for (int o = 1; o < R; ++o)
-        if (t == o) v = acc[o][f];
-      *(f32x4*)&sums[wave][c][f * 16 + 4 * g] = v;
-    }
-    __syncthreads();
-    const int r = t * 16 + m;
-    if (r < rows && f0 + col < ffn) {      // ffn is a multiple of 8, a thread's columns 1, 2 or 4
-      uint16_t hi[kEach], lo[kEach];
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        float v = 0.f, gate = 0.f;
-#pragma unroll
-        for (int w = 0; w < kLayerWaves; ++w) {
-          v += sums[w][m][col + i];
-          if (GATE) gate += sums[w][m][kCols + col + i];
+          for (int w = 0; w < kLayerWaves; ++w) {
+            v += sums[w][m][col + i];
+            if (GATE) gate += sums[w][m][kCols + col + i];
+          }
+          v = activated(v, act);
+          in_two<DT>(GATE ? v * gate : v, hi[i], lo[i]);
         }
-        v = activated(v, act);
-        in_two<DT>(GATE ? v * gate : v, hi[i], lo[i]);
+        const int64_t at = (int64_t)(first + r) * ffn + f0 + col;
+        __builtin_memcpy(h_hi + at, hi, sizeof(hi));
+        __builtin_memcpy(h_lo + at, lo, sizeof(lo));
       }
-      const int64_t at = (int64_t)(first + r) * ffn + f0 + col;
-      __builtin_memcpy(h_hi + at, hi, sizeof(hi));
-      __builtin_memcpy(h_lo + at, lo, sizeof(lo));
     }
-  }
   }
 }
 
@@ -526,12 +526,13 @@ template <int DT, int R>
 __global__ void __launch_bounds__(kLayerThreads)
 layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict__ h_lo, const uint16_t* __restrict__ w2, const LayerTable* __restrict__ table, int tokens,
                   int top_k, int hidden, int ffn, int tiles, int parts, const float* __restrict__ weights, float* __restrict__ sums_of_parts, uint16_t* __restrict__ out,
-                  int32_t* __restrict__ counters) {
+                  int32_t* __restrict__ counters, int entries, bool by_xcd) {
   constexpr int kPitch = kDownColumns + 4, kChunk = 32, kThrough = 0x11;      // cache policy: past the caches
   __shared__ __attribute__((aligned(16))) float sums[kLayerWaves][16][kPitch];
   __shared__ int flag;
-  const int per_expert = tiles * parts, u = (int)blockIdx.x / per_expert, in = (int)blockIdx.x - u * per_expert;
+  const int in_order = by_xcd ? xcd_tile_id((int)blockIdx.x, tiles) : (int)blockIdx.x, u = in_order / (tiles * parts), in = in_order - u * tiles * parts;
   const int part = in / tiles, tile = in - part * tiles, n0 = tile * kDownColumns;
+  if (u >= entries) return;
   const int4 it = table->used[u];
   if (it.z == 0) return;
   const int expert = it.x, all_rows = it.z, slots = tokens * top_k;
@@ -546,90 +547,90 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
   // a part's sums lie [part][row][column]
   const __amdgpu_buffer_rsrc_t rsrc_parts = rsrc_of(sums_of_parts, (uint32_t)parts * (uint32_t)slots * (uint32_t)hidden * 4u);
   for (int done = 0; done < all_rows; done += 16 * R) {      // once, but for experts of many rows
-  const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
-  uint32_t h_off[R];
+    const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
+    uint32_t h_off[R];
 #pragma unroll
-  for (int t = 0; t < R; ++t) h_off[t] = t * 16 + c < rows ? (uint32_t)(first + t * 16 + c) * h_pitch + (uint32_t)g * 16u : kNone;
-  const int chunks = (ffn + kChunk - 1) / kChunk, begin = (int)((int64_t)part * chunks / parts), end = (int)((int64_t)(part + 1) * chunks / parts);
-  struct Chunk { u32x4 hi[R], lo[R], b[8]; };
-  auto fetch = [&](Chunk& q, int chunk) {
-    const uint32_t none = chunk < end && w_off != kNone ? 0u : kNone;
-    const uint32_t at = w_off + (uint32_t)chunk * kChunk * pitch;      // rows past ffn are past the buffer
+    for (int t = 0; t < R; ++t) h_off[t] = t * 16 + c < rows ? (uint32_t)(first + t * 16 + c) * h_pitch + (uint32_t)g * 16u : kNone;
+    const int chunks = (ffn + kChunk - 1) / kChunk, begin = (int)((int64_t)part * chunks / parts), end = (int)((int64_t)(part + 1) * chunks / parts);
+    struct Chunk { u32x4 hi[R], lo[R], b[8]; };
+    auto fetch = [&](Chunk& q, int chunk) {
+      const uint32_t none = chunk < end && w_off != kNone ? 0u : kNone;
+      const uint32_t at = w_off + (uint32_t)chunk * kChunk * pitch;      // rows past ffn are past the buffer
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q.b[i] = load16(rsrc_w, (at + (uint32_t)i * pitch) | none);
-    const uint32_t past = chunk < end && chunk * kChunk + 8 * g < ffn ? 0u : kNone;
-#pragma unroll
-    for (int t = 0; t < R; ++t)
-      if (t == 0 || t < row_tiles) {
-        const uint32_t h_at = (h_off[t] + (uint32_t)chunk * (kChunk * 2)) | past | (h_off[t] & kNone);
-        q.hi[t] = load16(rsrc_hi, h_at);
-        q.lo[t] = load16(rsrc_lo, h_at);
-      }
-  };
-  f32x4 acc[R][8];
-#pragma unroll
-  for (int t = 0; t < R; ++t)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const Chunk& q) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      u32x4 b;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) b[w] = __builtin_amdgcn_perm(q.b[2 * w + 1][j >> 1], q.b[2 * w][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+      for (int i = 0; i < 8; ++i) q.b[i] = load16(rsrc_w, (at + (uint32_t)i * pitch) | none);
+      const uint32_t past = chunk < end && chunk * kChunk + 8 * g < ffn ? 0u : kNone;
 #pragma unroll
       for (int t = 0; t < R; ++t)
         if (t == 0 || t < row_tiles) {
-          acc[t][j] = mfma<DT>(b, q.hi[t], acc[t][j]);
-          acc[t][j] = mfma<DT>(b, q.lo[t], acc[t][j]);
+          const uint32_t h_at = (h_off[t] + (uint32_t)chunk * (kChunk * 2)) | past | (h_off[t] & kNone);
+          q.hi[t] = load16(rsrc_hi, h_at);
+          q.lo[t] = load16(rsrc_lo, h_at);
         }
-    }
-  };
-  Chunk q0, q1;
-  fetch(q0, begin + wave);
-  for (int chunk = begin + wave; chunk < end; chunk += 2 * kLayerWaves) {
-    fetch(q1, chunk + kLayerWaves);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(q0);
-    __builtin_amdgcn_sched_barrier(0);
-    fetch(q0, chunk + 2 * kLayerWaves);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(q1);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  // accumulator t, j, register i of lane (c, g): token row 16 t + c, column 8 (4 g + i) + j
-  for (int t = 0; t < row_tiles; ++t) {
-    if (t > 0 || done > 0) __syncthreads();
+    };
+    f32x4 acc[R][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f32x4 lo, hi;
+    for (int t = 0; t < R; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        lo[j] = acc[0][j][i];
-        hi[j] = acc[0][4 + j][i];
+      for (int j = 0; j < 8; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Chunk& q) {
 #pragma unroll
-        for (int o = 1; o < R; ++o)
-          if (t == o) {
-            lo[j] = acc[o][j][i];
-            hi[j] = acc[o][4 + j][i];
+      for (int j = 0; j < 8; ++j) {
+        u32x4 b;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) b[w] = __builtin_amdgcn_perm(q.b[2 * w + 1][j >> 1], q.b[2 * w][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int t = 0; t < R; ++t)
+          if (t == 0 || t < row_tiles) {
+            acc[t][j] = mfma<DT>(b, q.hi[t], acc[t][j]);
+            acc[t][j] = mfma<DT>(b, q.lo[t], acc[t][j]);
           }
       }
-      *(f32x4*)&sums[wave][c][8 * (4 * g + i)] = lo;
-      *(f32x4*)&sums[wave][c][8 * (4 * g + i) + 4] = hi;
+    };
+    Chunk q0, q1;
+    fetch(q0, begin + wave);
+    for (int chunk = begin + wave; chunk < end; chunk += 2 * kLayerWaves) {
+      fetch(q1, chunk + kLayerWaves);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q0);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(q0, chunk + 2 * kLayerWaves);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(q1);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __syncthreads();
-    if (t * 16 + m < rows && mine) {
-      f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+    // accumulator t, j, register i of lane (c, g): token row 16 t + c, column 8 (4 g + i) + j
+    for (int t = 0; t < row_tiles; ++t) {
+      if (t > 0 || done > 0) __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kLayerWaves; ++w) {
-        lo += *(const f32x4*)&sums[w][m][col];
-        hi += *(const f32x4*)&sums[w][m][col + 4];
+      for (int i = 0; i < 4; ++i) {
+        f32x4 lo, hi;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = acc[0][j][i];
+          hi[j] = acc[0][4 + j][i];
+#pragma unroll
+          for (int o = 1; o < R; ++o)
+            if (t == o) {
+              lo[j] = acc[o][j][i];
+              hi[j] = acc[o][4 + j][i];
+            }
+        }
+        *(f32x4*)&sums[wave][c][8 * (4 * g + i)] = lo;
+        *(f32x4*)&sums[wave][c][8 * (4 * g + i) + 4] = hi;
       }
-      const uint32_t at = (((uint32_t)part * (uint32_t)slots + (uint32_t)(first + t * 16 + m)) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rsrc_parts, (int)at, 0, kThrough);
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rsrc_parts, (int)at + 16, 0, kThrough);
+      __syncthreads();
+      if (t * 16 + m < rows && mine) {
+        f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+        for (int w = 0; w < kLayerWaves; ++w) {
+          lo += *(const f32x4*)&sums[w][m][col];
+          hi += *(const f32x4*)&sums[w][m][col + 4];
+        }
+        const uint32_t at = (((uint32_t)part * (uint32_t)slots + (uint32_t)(first + t * 16 + m)) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rsrc_parts, (int)at, 0, kThrough);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rsrc_parts, (int)at + 16, 0, kThrough);
+      }
     }
-  }
   }
   // Then a token's rows are weighted and added up.  Sixteen threads have a column; with few tokens several of them share a token's parts, and add up in order
   // what each has.
@@ -690,6 +691,7 @@ struct LayerPlan {
   double used, rows;        // that get one, and how many those get, where tokens choose evenly
   int fragments, hidden_tiles;
   int down_tiles, parts;
+  bool by_xcd;              // the second product's tiles of an expert's part on one XCD
   size_t table, choice, logits, h_hi, h_lo, sums, total = 0;
 
   LayerPlan(int tokens, int hidden, int ffn, int experts, int top_k, bool gate) {
@@ -713,6 +715,9 @@ struct LayerPlan {
     // 448, 151 / 152 / 156 / 160; 64 tokens, 6 of 64 of [1408, 2048], 1024, 242 / 254 / 274 / 324).
     parts = 1;
     while (parts < kLayerMaxParts && used * down_tiles * parts < 192 && ceil_div(ffn, 32) >= parts * 4 * kLayerWaves) parts *= 2;
+    // Where rows begin inside a cache line, neighbouring tiles share one, which XCDs of their own would each fetch (5 tokens, 4 of 60 of [2728, 1032]: 162 MB for
+    // 113): a part's tiles to one XCD, where that leaves none without (us the other way / so: this one 79.6 / 76.3; 33 tokens, 6 of 64 of [1416, 2056] 246 / 234).
+    by_xcd = hidden % 64 != 0 && used * parts >= 2 * kXcds;
     auto take = [&](size_t bytes) {
       const size_t at = total;
       total += (bytes + 255) & ~(size_t)255;
@@ -774,8 +779,10 @@ void launch_products(const void* x, const void* w1, const void* v1, const void* 
   else if (plan.fragments == 2) { if (v1) MBX_LAYER_HIDDEN(true, 2); else MBX_LAYER_HIDDEN(false, 2); }
   else if (plan.fragments == 1) MBX_LAYER_HIDDEN(false, 1);
 #undef MBX_LAYER_HIDDEN
-  layer_down_kernel<DT, R><<<(unsigned)(plan.entries * plan.down_tiles * plan.parts), kLayerThreads, 0, s>>>(
-      hi, lo, (const uint16_t*)w2, table, q.tokens, q.top_k, q.hidden, ffn, plan.down_tiles, plan.parts, weights, (float*)(base + plan.sums), (uint16_t*)out, counters);
+  const int64_t down = (int64_t)plan.entries * plan.down_tiles * plan.parts;
+  layer_down_kernel<DT, R><<<(unsigned)(plan.by_xcd ? xcd_grid(down, plan.down_tiles) : down), kLayerThreads, 0, s>>>(
+      hi, lo, (const uint16_t*)w2, table, q.tokens, q.top_k, q.hidden, ffn, plan.down_tiles, plan.parts, weights, (float*)(base + plan.sums), (uint16_t*)out, counters,
+      plan.entries, plan.by_xcd);
 }
 
 template <int DT>

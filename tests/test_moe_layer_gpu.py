@@ -88,7 +88,7 @@ def check(o, top_k, act=gg.ACT_SILU, got=None, **choice):
 @pytest.mark.parametrize('gate', [True, False], ids=['gated', 'plain'])
 @pytest.mark.parametrize('tokens,hidden,ffn,experts,top_k', [
     (1, 8, 8, 1, 1), (1, 64, 64, 2, 1), (1, 2048, 1408, 16, 6), (1, 512, 4096, 8, 2), (2, 72, 40, 3, 3), (3, 1032, 264, 60, 4), (5, 128, 136, 130, 8), (7, 520, 1000, 512, 16),
-    (8, 256, 24, 4, 1), (9, 264, 512, 8, 2), (16, 1024, 512, 64, 1), (17, 136, 200, 5, 2), (31, 512, 512, 300, 10), (33, 200, 328, 8, 2), (48, 256, 256, 2, 1),
+    (8, 256, 24, 4, 1), (9, 264, 512, 8, 2), (11, 1048, 72, 29, 4), (16, 1024, 512, 64, 1), (17, 136, 200, 5, 2), (31, 512, 512, 300, 10), (33, 200, 328, 8, 2), (48, 256, 256, 2, 1),
     (63, 128, 72, 40, 16), (64, 640, 1088, 8, 2), (64, 64, 64, 1, 1)])
 def test_layer(tokens, hidden, ffn, experts, top_k, gate, dtype):
     check(make(tokens, hidden, ffn, experts, gate, dtype), top_k, gg.ACT_SILU if gate else gg.ACT_GELU_TANH)
