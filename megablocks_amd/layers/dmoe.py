@@ -4,11 +4,12 @@
     sparse:   the same over 128-padded expert groups, with the block-diagonal topology
               metadata the reference builds for stk
 """
+import math
+
 import numpy as np
 import torch
 
 import megablocks_amd.ops as ops
-from megablocks_amd import _lib
 from megablocks_amd.ops import few_tokens
 from megablocks_amd.ops import routing as ops_routing
 from megablocks_amd import grouped_gemm_util as gg
@@ -294,9 +295,13 @@ class dMoE(moe.MoE):
                for w in (weight, w1, v1, w2) if w is not None) or weight.shape != (num_experts, hidden) or \
                 any(w.numel() != num_experts * ffn * hidden for w in (w1, v1, w2) if w is not None) or not few_tokens.takes(tokens, hidden, ffn, num_experts, top_k):
             return None
-        out, _, _ = few_tokens.launch(x.reshape(-1, hidden), weight, w1, v1, w2, ffn, top_k, act, args.moe_router_score, getattr(gate, 'balance_bias', None),
-                                      args.moe_router_groups, args.moe_router_top_groups, args.moe_router_group_best, float(args.moe_normalize_expert_weights or 0),
-                                      float(args.moe_router_scale))
+        # a router without options of its own (`_chooses`) goes by the softmax and the norm alone, whatever the others say; a norm that is no finite one is the separate operators'
+        norm_p, bias = float(gate.args.moe_normalize_expert_weights or 0), gate.balance_bias if gate._chooses else None
+        if not 0 <= norm_p < math.inf or (bias is not None and (bias.dtype != torch.float32 or bias.device != x.device)):
+            return None
+        choice = (gate.args.moe_router_score, bias, gate.args.moe_router_groups, gate.args.moe_router_top_groups, gate.args.moe_router_group_best, norm_p,
+                  float(gate.args.moe_router_scale)) if gate._chooses else ('softmax', None, 1, 1, 2, norm_p, 1.0)
+        out, _, _ = few_tokens.launch(x.reshape(-1, hidden), weight, w1, v1, w2, ffn, top_k, act, *choice)
         return out.view(x.shape)
 
     def quantize_experts_(self, group_size: int = 128, zero_points: bool = False):

@@ -17,6 +17,7 @@ import megablocks_amd.ops as ops
 from megablocks_amd import grouped_gemm_util as gg
 from megablocks_amd.layers.arguments import DEFAULT_ACTIVATION_FN, Arguments
 from megablocks_amd.layers.dmoe import dMoE
+from megablocks_amd.layers.moe import clear_load_balancing_loss
 
 pytestmark = pytest.mark.gpu
 
@@ -270,6 +271,11 @@ def chosen_alike(layer, x):
     return (layer.router(x)[2].sort(1).values == exact.sort(1).values).all(1)
 
 
+def chosen_alike_plainly(layer, x):
+    _, exact = exact_choice(dict(x=x.reshape(-1, x.shape[-1]), router=layer.router.layer.weight.detach()), layer.experts.args.moe_top_k)
+    return (layer.router(x)[2].sort(1).values == exact.sort(1).values).all(1)
+
+
 def calls(monkeypatch):
     from megablocks_amd.ops import few_tokens
     made, launch = [], few_tokens.launch
@@ -312,6 +318,7 @@ def test_calls_that_stay_with_the_separate_operators(monkeypatch):
     with torch.no_grad():
         layer.train(), separate.train()
         assert torch.equal(layer(x), separate(x))
+        clear_load_balancing_loss()
         layer.eval(), separate.eval()
         for module in (layer.router, layer.router.layer, layer.experts, layer.experts.mlp):
             seen = []
@@ -330,6 +337,20 @@ def test_calls_that_stay_with_the_separate_operators(monkeypatch):
     with torch.no_grad():
         layer(x)
     assert len(made) == 1
+
+
+@pytest.mark.parametrize('changed', [dict(moe_normalize_expert_weights=float('inf')), dict(moe_router_groups=3, moe_router_top_groups=3, moe_router_group_best=5)], ids=str)
+def test_routers_that_look_at_no_options(changed, monkeypatch):
+    """A router with softmax scores, no bias and all groups open takes any norm and does not look at the groups: with an infinite norm the separate operators run, as they did."""
+    layer, separate = make_layer(**changed)
+    made = calls(monkeypatch)
+    x = torch.randn(3, 1, 256, device='cuda').bfloat16()
+    with torch.no_grad():
+        got, want = layer(x), separate(x)
+        alike = chosen_alike_plainly(separate, x)
+    assert len(made) == (0 if 'moe_normalize_expert_weights' in changed else 1)
+    got, want = got.double().view(-1, 256)[alike], want.double().view(-1, 256)[alike]
+    assert alike.any() and (got - want).norm() <= 1e-2 * want.norm()
 
 
 def test_layer_captured(monkeypatch):
