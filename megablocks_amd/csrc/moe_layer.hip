@@ -652,10 +652,11 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
   };
   look_up(m / share, my_share * each);
   if (!last_to_come(counters + kCounterColumns + tile, table->experts * parts, &flag)) return;
-  for (int t = m / share; t < tokens; t += 16 / share) {
+  for (int t0 = 0; t0 < tokens; t0 += 16 / share) {
+    const int t = t0 + m / share;
     f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
     for (int q = my_share * each; q < stop; q += kAhead) {
-      if (t != m / share || q != my_share * each) look_up(t, q);
+      if (t0 > 0 || q != my_share * each) look_up(t, q);
       u32x4 a[kAhead], b[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -679,9 +680,10 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
         hi += *(const f32x4*)&sums[0][m + o][col + 4];
       }
     }
-    if (!mine) return;
-    const u32x4 v = {pack2<DT>(lo[0], lo[1]), pack2<DT>(lo[2], lo[3]), pack2<DT>(hi[0], hi[1]), pack2<DT>(hi[2], hi[3])};
-    *(u32x4*)(out + (int64_t)t * hidden + n0 + col) = v;
+    if (t < tokens && mine) {
+      const u32x4 v = {pack2<DT>(lo[0], lo[1]), pack2<DT>(lo[2], lo[3]), pack2<DT>(hi[0], hi[1]), pack2<DT>(hi[2], hi[3])};
+      *(u32x4*)(out + (int64_t)t * hidden + n0 + col) = v;
+    }
   }
 }
 
