@@ -2,13 +2,16 @@
 //
 //   out[i] = scale table[ids[i]]           dtable[v] = scale sum over {i : ids[i] = v} of dout[i], i ascending
 //
-// Both are bound by memory: the rows read and written once, for the gradient the whole table written, most of it zeros.  The gradient's sums are fp32 in
-// a fixed order: rows are added along the tokens sorted by word (stably), a piece of 32 of them by a wave, whose runs of one word go straight to the table;
-// what a longer run leaves in each of its pieces is kept in fp32 and added up, in order, by a launch of its own.  So a word that is half of the text costs no
-// more than any other, and sums do not depend on timing.
+// Both are bound by memory: the rows read and written once, for the gradient the whole table written, most of it zeros.  The gradient's sums are fp32 in a fixed
+// order: rows are added along the tokens sorted by word (stably), a piece of 32 of them by a wave, whose runs of one word go straight to the table; what a run of
+// more than 32 tokens leaves in each of its pieces is kept in fp32 and added up, in order, by a launch of its own.  So a word that is half of the text costs no more
+// than any other, and sums do not depend on timing.
+//
+// Measured (us): 32767 tokens, two fifths of them padding, 100000 words of 2040 in fp16: rows 52 (268 MB, 5.2 TB/s; a copy moves 4.8), gradient 12.8 sorting, 99 sums and
+// zeros (0.49 GB, 5.0 TB/s; a fill writes 6.7), 7 joining.  16384 tokens, 50000 words of 1024 in bf16: 13.1 (5.1 TB/s) and 10.8 + 25.9 (136 MB, 5.3 TB/s) + 4.1.  16 tokens: 2.5.
 //
 // Sorting: workgroup w owns a range of words and goes through all tokens, counts those of smaller words and lists its own, in order, in LDS: no exchange between
-// workgroups, one launch.
+// workgroups, one launch.  Its time is latencies: of the loads, four of which are under way in a wave, and of the claims of places.
 //
 // A token outside the table gives a row of zeros and no gradient.  Tensors may start anywhere and rows have any length: the memory unit takes 16-byte
 // accesses at any address.
@@ -268,7 +271,8 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const I* _
 // ---- sums along the order ----
 // Workgroups [0, piece_blocks): a wave per piece of kPiece places of the order and slice of columns; the others: rows of words without a token, zeroed.
 // heads[p] / tails[p]: what the run that piece p begins inside of / ends inside of leaves there; a run that goes through the whole piece: heads[p].
-constexpr int kZeroRows = 16;    // words of a wave
+// Words of a wave that zeroes (us a pass by 16 / 8 / 4 / 2 / 1: 32767 tokens, 100000 words of 2040 179 / 176 / 173 / 172 / 172; 2000 tokens, 128000 of 4096 225 / 222 / 219 / 218 / 220).
+constexpr int kZeroRows = 2;
 // A run of up to kWholeRun tokens is added up by the piece that it begins in, which has it in its lanes; longer ones are cut at the pieces' ends.
 constexpr int kPiece = 32, kWholeRun = kWave - kPiece;
 

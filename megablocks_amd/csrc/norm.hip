@@ -8,6 +8,10 @@
 //
 // What bounds both passes is memory: a conversion and a multiply-add in 64 bits an element are a tenth of what the compute units issue meanwhile.  The second
 // pass goes through the tensors from behind: what the first one read last is still in the 256 MiB cache.
+//
+// Measured: the norm of 554 M bf16 values, 1.1 GB, 187 us + 4.5 for the join (5.9 TB/s); clipped into 554 M fp32 ones 234 (what is left of the last pass's output in the
+// cache is written meanwhile) + 663 (3.3 GB, 5.0 TB/s, a copy's rate; with stores past the cache 820); 0.55 GB in place that is short enough 95 + 4.6; 300 tensors of
+// 2 M values in all 6.2 and 6.9 a launch, of which there are three each way.
 #include "common.h"
 
 #include <algorithm>
