@@ -127,6 +127,47 @@ def test_layouts():
     check(ids, torch.randn(50, 66, device='cuda')[:, ::2], torch.randn(33, device='cuda').expand(15, 40, 33))
 
 
+def test_a_table_of_more_than_2_to_the_31_values():
+    words, hidden = (1 << 20) + 7, 2056
+    table = torch.zeros(words, hidden, dtype=BF16, device='cuda')
+    ids = torch.tensor([words - 1, 0, words - 2, words - 1, 1 << 20, 77], device='cuda')
+    table[ids] = torch.randn(len(ids), hidden, device='cuda').bfloat16()
+    grad = torch.randn(len(ids), hidden, device='cuda').bfloat16()
+    table.requires_grad_()
+    out = ops.embedding(ids, table)
+    assert torch.equal(out, table.detach()[ids])
+    got, = torch.autograd.grad(out, table, grad)
+    named = ids.unique()
+    assert torch.equal(got.any(1).nonzero().flatten(), named)
+    want, off = exact((ids.unsqueeze(1) == named).int().argmax(1), grad, len(named), 1.0)
+    assert ((got[named].double() - want).abs() <= off).all()
+
+
+def test_rows_of_more_than_2_to_the_31_values():
+    """Counts are exact in fp32, up to 2^24, and so are their parts."""
+    tokens, hidden = (1 << 20) + 7, 2056
+    ids = torch.randint(0, 3, (tokens,), device='cuda')
+    table = torch.randn(3, hidden, device='cuda').bfloat16().requires_grad_()
+    out = ops.embedding(ids, table)
+    assert torch.equal(out, table.detach()[ids])
+    grad = torch.ones_like(out)
+    grad[-1, -1] = 0
+    got, = torch.autograd.grad(out, table, grad)
+    want = torch.bincount(ids, minlength=3).unsqueeze(1).repeat(1, hidden)
+    want[ids[-1], -1] -= 1
+    assert torch.equal(got, want.float().bfloat16())
+
+
+def test_more_tokens_than_a_list_counts():
+    """Sixteen shares of more than 2^22 tokens."""
+    tokens = (1 << 26) + 12345
+    ids = torch.randint(0, 13, (tokens,), device='cuda', dtype=torch.int32)
+    table = torch.zeros(13, 1, device='cuda', requires_grad=True)
+    grad = (torch.arange(tokens, device='cuda') % 5 == 0).float().unsqueeze(1)      # sums below 2^24
+    got, = torch.autograd.grad(ops.embedding(ids, table), table, grad)
+    assert torch.equal(got.flatten().long(), torch.bincount(ids[::5], minlength=13))
+
+
 def test_sums_are_not_in_16_bits():
     ids = torch.zeros(40000, dtype=torch.int64, device='cuda')
     table = torch.zeros(2, 8, device='cuda', dtype=BF16, requires_grad=True)

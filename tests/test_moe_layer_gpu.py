@@ -122,6 +122,13 @@ def test_all_tokens_on_the_same_experts(tokens):
     assert (indices == torch.tensor([2, 7], device='cuda')).all()
 
 
+def test_the_largest_matrices():
+    """Experts of nearly 2 GiB a matrix, one behind the other."""
+    o = make(2, 16384, 65200, 2, gate=False, std=0.01)
+    _, _, indices = check(o, 1, gg.ACT_GELU_TANH, bias=torch.tensor([0.0, 9.0], device='cuda'))
+    assert (indices == 1).all()
+
+
 def test_equal_experts_go_to_the_lower_index():
     o = make(12, 128, 64, 100)
     for e in (10, 37, 99):

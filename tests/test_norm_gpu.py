@@ -102,6 +102,17 @@ def test_many_small_values_next_to_a_large_one():
     check_norm(ops.global_norm([t]), math.sqrt(1 + ((1 << 24) - 1) * 2.0 ** -26))
 
 
+def test_a_tensor_of_more_than_2_to_the_31_values():
+    n = (1 << 31) + 12345
+    t = torch.ones(n, dtype=BF16, device='cuda')
+    t[-3:] = 1024.0
+    norm = math.sqrt(n - 3 + 3 * 2.0 ** 20)
+    check_norm(ops.global_norm([t]), norm)
+    check_norm(ops.clip_by_global_norm_([t], norm / 64), norm)
+    # a 64th of each value, by a factor that is off by some steps of fp32 and rounds to it in 8 bits
+    assert (t[-3:] == 16.0).all() and (t[:-3] == 2.0 ** -6).all()
+
+
 @pytest.mark.parametrize('p', [2.0, 1.0, math.inf])
 @pytest.mark.parametrize('where', [0, 16383, 99_999, -1])
 def test_values_that_are_not_finite(where, p):
