@@ -3,7 +3,8 @@
 Tolerances, from the roundings there are.  Weights are rounded to fp32 once (2^-24; the arithmetic before is in 64 bits).  An output is off by
   - the first products' sums: of n terms in fp32 at most n 2^-24 of the sum of magnitudes, through an activation of slope up to 1.13;
   - the activation: 2^-20 of itself and of its argument (an exponential and a quotient in fp32);
-  - keeping it as two 16-bit numbers: half a step of half a step, 2^-18 (bf16) or 2^-22 (fp16, and 2^-25 where the second number is that small);
+  - keeping it as two 16-bit numbers: the first is off by at most half its step, 2^-8 (bf16) or 2^-11 (fp16) of the value's power of two, so the second lies below that, where half a
+    step is 2^-17 or 2^-23 (fp16 has no step below 2^-24: 2^-25 where the second number is that small);
   - the second product's sums, of ffn terms and top_k weighted parts, as the first's;
   - its rounding, half a step of its type.
 Since roundings seldom all point one way, the norm of the error is held to a quarter more than half a step of the output's as well."""
@@ -53,7 +54,7 @@ def exact_out(o, weights, indices, act):
     x, dtype = o['x'].double(), o['x'].dtype
     hidden, ffn = x.shape[1], o['w1'].shape[1]
     out, off = torch.zeros_like(x), torch.zeros_like(x)
-    keep = 2.0 ** -18 if dtype == BF16 else 2.0 ** -22
+    keep = 2.0 ** -17 if dtype == BF16 else 2.0 ** -23
     for e in indices.unique().tolist():
         t, j = (indices == e).nonzero(as_tuple=True)
         w1, w2 = o['w1'][e].double(), o['w2'][e].double()
