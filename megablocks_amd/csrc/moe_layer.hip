@@ -6,18 +6,18 @@
 // What bounds it is reading the weights of the chosen experts, once, and, for a few small ones, the way between the launches.  Three of them:
 //
 //   choose   a wave per expert and token (or four tokens): logits as exact products summed in 64 bits, so that no order of summation decides between
-//            neighbours; the workgroup that is last at a group of tokens chooses for them, and the last of all makes the table of which experts have which rows
+//            neighbours; the workgroup that is last at a group of tokens chooses for them
 //   hidden   a workgroup per used expert and 16 to 128 rows of its first weights, a quarter of the reduction a wave; the activation is kept as the sum of two
 //            16-bit numbers, so that the second product sees it to 2^-17
 //   down     a workgroup per used expert, 128 columns and a part of the reduction; the parts meet in memory, and the workgroup that is last at its columns adds them up
 //            in a fixed order, weights them and writes the output
 //
 // Measured (us: choose + hidden + down; the weights' rate in the last two, of 5.9 TB/s that a large read reaches):
-//    1 token,  6 of 64 gated experts of [1408, 2048]    6.5 +  19 +  12     3.7 and 2.8 TB/s: 528 and 192 workgroups of 5 to 8 chunks a wave, half of it the way to the first
-//    1 token,  2 of 8 of [14336, 4096]                  5.3 +  92 +  44     5.1 and 5.3
-//    16 tokens, 1 of 64 of [4096, 1024], no gate        8.2 +  23 +  27     5.1 and 4.4
-//    5 tokens, 4 of 60 of [2728, 1032], fp16            9.8 +  38 +  27     5.0 and 3.5: rows that begin inside cache lines
-//    64 tokens, 2 of 8 of [14336, 4096]                 7.6 + 351 + 182     5.4 and 5.2
+//    1 token,  6 of 64 gated experts of [1408, 2048]    6.3 +  19 +  12     3.7 and 2.9 TB/s: 528 and 192 workgroups of 5 to 8 chunks a wave, half of it the way to the first
+//    1 token,  2 of 8 of [14336, 4096]                  5.1 +  93 +  44     5.1 and 5.3
+//    16 tokens, 1 of 64 of [4096, 1024], no gate        6.3 +  24 +  27     4.9 and 4.4
+//    5 tokens, 4 of 60 of [2728, 1032], fp16            7.8 +  39 +  27     4.9 and 3.5: rows that begin inside cache lines
+//    64 tokens, 2 of 8 of [14336, 4096]                 5.5 + 355 + 183     5.3 and 5.1
 //
 // "Last" is counted with device-wide atomics; nobody waits for anybody.  What goes from one workgroup to another inside a launch is stored and loaded past the
 // caches (the compute units are on eight L2s that do not see each other) and counted in when the stores have been acknowledged.  Sums are taken in an order that
@@ -34,26 +34,16 @@ constexpr int kLayerSlots = kLayerTokens * kLayerTopK;
 constexpr int kLayerThreads = 256, kLayerWaves = kLayerThreads / kWave;
 constexpr int kLayerMaxParts = 16;                                     // of the second product's reduction
 constexpr int kDownColumns = 128;
-// counters: from 0 on groups of tokens, then the groups that are done, then the second product's columns
-constexpr int kCounterAll = kLayerTokens, kCounterColumns = kLayerTokens + 1;
-
-// which experts have which rows; a row is an assignment (token, j), sorted by expert
-struct LayerTable {
-  int4 used[kLayerExperts];         // expert, first row, rows, 0; rows 0 past the last used one
-  int32_t token_of_row[kLayerSlots];
-  int32_t row_of_slot[kLayerSlots];
-  int32_t experts;                  // used ones
-};
+// counters: from 0 on groups of tokens, then the second product's columns
+constexpr int kCounterColumns = kLayerTokens;
 
 struct LayerChoice {
-  int tokens, hidden, experts, top_k, sigmoid, groups, top_groups, group_best, entries;
+  int tokens, hidden, experts, top_k, sigmoid, groups, top_groups, group_best;
   float norm_p, scale;
 };
 
 __device__ __forceinline__ void store_through(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ uint64_t load_through(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void store_through(int32_t* p, int32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ int32_t load_through(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // Whether this workgroup is the last of `all` to come here; what all of them have stored through the caches can then be loaded.  Leaves the counter zero.
 __device__ __forceinline__ bool last_to_come(int32_t* counter, int all, int* flag) {
@@ -263,77 +253,13 @@ __device__ __forceinline__ void dot_f64(const uint16_t* __restrict__ router, int
     for (int t = 0; t < TB; ++t) acc[e][t] = wave_sum_f64(acc[e][t]);
 }
 
-// The table, by one workgroup; expert_of(s): the s-th assignment's.
-template <int THREADS, typename X>
-__device__ __forceinline__ void make_table(const LayerChoice& q, X&& expert_of, LayerTable* __restrict__ table) {
-  static_assert(kLayerExperts <= 2 * THREADS && THREADS >= kWave, "two experts a thread");
-  constexpr int kEach = (kLayerSlots + THREADS - 1) / THREADS, kPair = kLayerExperts / 2;      // thread i: experts 2 i and 2 i + 1
-  __shared__ int32_t count[kLayerExperts], first[kLayerExperts], sums[kPair / kWave];
-  const int slots = q.tokens * q.top_k, i = threadIdx.x, wave = i / kWave;
-  if (i < kPair) count[2 * i] = count[2 * i + 1] = 0;
-  __syncthreads();
-  int expert[kEach], rank[kEach];
-#pragma unroll
-  for (int n = 0; n < kEach; ++n) {
-    const int s = i + n * THREADS;
-    expert[n] = s < slots ? expert_of(s) : 0;
-  }
-#pragma unroll
-  for (int n = 0; n < kEach; ++n)      // the order of an expert's rows is nobody's business: each is computed by itself
-    if (i + n * THREADS < slots) rank[n] = atomicAdd(&count[expert[n]], 1);
-  __syncthreads();
-  int c0 = 0, c1 = 0, through = 0;
-  if (i < kPair) {
-    c0 = count[2 * i];
-    c1 = count[2 * i + 1];
-    through = wave_inclusive_scan(c0 + c1 | ((c0 > 0) + (c1 > 0)) << 16);    // rows, used experts
-    if (i % kWave == kWave - 1) sums[wave] = through;
-  }
-  __syncthreads();
-  if (i < kPair) {
-    int before = through - (c0 + c1 | ((c0 > 0) + (c1 > 0)) << 16), all = 0;
-#pragma unroll
-    for (int w = 0; w < kPair / kWave; ++w) {
-      before += w < wave ? sums[w] : 0;
-      all += sums[w];
-    }
-    const int row = before & 0xffff, used = all >> 16;
-    int u = before >> 16;
-    first[2 * i] = row;
-    first[2 * i + 1] = row + c0;
-    if (c0 > 0) table->used[u++] = make_int4(2 * i, row, c0, 0);
-    if (c1 > 0) table->used[u] = make_int4(2 * i + 1, row + c0, c1, 0);
-    for (int n = used + i; n < q.entries; n += kPair) table->used[n] = make_int4(0, 0, 0, 0);
-    if (i == 0) table->experts = used;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int n = 0; n < kEach; ++n) {
-    const int s = i + n * THREADS;
-    if (s < slots) {
-      const int at = first[expert[n]] + rank[n];
-      table->token_of_row[at] = s / q.top_k;
-      table->row_of_slot[s] = at;
-    }
-  }
-}
-
-// The table of a lone token: its j-th expert has row j.
-__device__ __forceinline__ void row_of_lone_token(const LayerChoice& q, int j, int expert, LayerTable* __restrict__ table) {
-  table->used[j] = make_int4(expert, j, 1, 0);
-  table->token_of_row[j] = 0;
-  table->row_of_slot[j] = j;
-  if (j == 0) table->experts = q.top_k;
-}
-
 // A workgroup a token, of sixteen waves: for routers a compute unit reads in the time that the exchange between several takes.
 constexpr int kWholeThreads = 1024, kWholeWaves = kWholeThreads / kWave;
 template <int DT, int EB, int R>
 __global__ void __launch_bounds__(kWholeThreads)
 layer_choose_whole_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ router, LayerChoice q, const float* __restrict__ bias, int32_t* __restrict__ choice,
-                          float* __restrict__ weights, int64_t* __restrict__ indices, LayerTable* __restrict__ table, int32_t* __restrict__ counters) {
+                          float* __restrict__ weights, int64_t* __restrict__ indices) {
   __shared__ double logits[R * kWave], scratch[R * kWave];
-  __shared__ int flag;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), token = blockIdx.x;
   for (int e0 = wave * EB; e0 < q.experts; e0 += kWholeWaves * EB) {
     double acc[EB][1];
@@ -344,19 +270,14 @@ layer_choose_whole_kernel(const uint16_t* __restrict__ x, const uint16_t* __rest
   }
   __syncthreads();
   if (wave == 0)
-    choose_for<R>(q, token, [&](int e) { return logits[e]; }, bias, scratch, weights, indices, [&](int j, int e) {
-      if (gridDim.x > 1) store_through(choice + (int64_t)token * q.top_k + j, e);
-      else row_of_lone_token(q, j, e, table);
-    });
-  if (gridDim.x > 1 && last_to_come(counters + kCounterAll, (int)gridDim.x, &flag))
-    make_table<kWholeThreads>(q, [&](int s) { return load_through(choice + s); }, table);
+    choose_for<R>(q, token, [&](int e) { return logits[e]; }, bias, scratch, weights, indices, [&](int j, int e) { choice[(int64_t)token * q.top_k + j] = e; });
 }
 
 // Workgroup (b, g): experts 4 b .. 4 b + 3, a wave each, tokens TB g .. ; TB 1 or 4.
 template <int DT, int TB, int R>
 __global__ void __launch_bounds__(kLayerThreads)
 layer_choose_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ router, LayerChoice q, const float* __restrict__ bias, uint64_t* __restrict__ logits,
-                    int32_t* __restrict__ choice, float* __restrict__ weights, int64_t* __restrict__ indices, LayerTable* __restrict__ table, int32_t* __restrict__ counters) {
+                    int32_t* __restrict__ choice, float* __restrict__ weights, int64_t* __restrict__ indices, int32_t* __restrict__ counters) {
   __shared__ double scratch[kLayerWaves][R * kWave];
   __shared__ int flag;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -371,12 +292,7 @@ layer_choose_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
   if (!last_to_come(counters + blockIdx.y, (int)gridDim.x, &flag)) return;
   for (int t = t0 + wave; t < t0 + tokens; t += kLayerWaves)
     choose_for<R>(q, t, [&](int e) { return __builtin_bit_cast(double, load_through(logits + (int64_t)t * q.experts + e)); }, bias, scratch[wave], weights, indices,
-                  [&](int j, int e) {
-                    if (q.tokens == 1) row_of_lone_token(q, j, e, table);
-                    else store_through(choice + (int64_t)t * q.top_k + j, e);
-                  });
-  if (q.tokens > 1 && last_to_come(counters + kCounterAll, (int)gridDim.y, &flag))
-    make_table<kLayerThreads>(q, [&](int s) { return load_through(choice + s); }, table);
+                  [&](int j, int e) { choice[(int64_t)t * q.top_k + j] = e; });
 }
 
 // ---- products ----
@@ -412,31 +328,86 @@ __device__ __forceinline__ void in_two(float v, uint16_t& hi, uint16_t& lo) {
   lo = __builtin_bit_cast(uint16_t, Elem<DT>::from_f32(rest - rest == 0.f ? rest : 0.f));     // an infinity or NaN has no rest
 }
 
+// The assignments (token top_k + j, one a token at most) of the u-th of the experts that have any, experts and tokens ascending: every workgroup finds them for
+// itself out of the choice, 4 KiB at most.  A table of them, made by the workgroup that is the last of all to choose, takes an exchange between workgroups and a way
+// to memory more (us a layer with it / so: 16 tokens, 1 of 64 experts of [4096, 1024] 63.5 / 62.3; 64 tokens, 1 of 4 of [1024, 1024] 27.8 / 26.0; 5, 4 of 60 of [2728, 1032] 76.2 / 75.5; but
+// 64 tokens, 16 of 256 of [512, 512], 9000 workgroups with little to do, 126 / 134).  A lone token's u-th expert is the u-th of its choice.
+struct LayerRows {
+  uint64_t used[kLayerExperts / 8];                // a byte an expert
+  int16_t slot_of[kLayerTokens];                   // -1: none
+  uint16_t slots[kLayerWaves][kLayerTokens];       // every wave's own copy
+};
+// the u-th used expert; rows: how many it has, all: how many are used; rows 0 where u is past them
+__device__ __forceinline__ int find_rows(const int32_t* __restrict__ choice, int tokens, int top_k, int u, LayerRows& of, int& rows, int& all) {
+  static_assert(kLayerTokens == kWave && kLayerExperts == 8 * kWave, "a token a lane, eight experts a lane");
+  constexpr int kEach = kLayerSlots / kLayerThreads;
+  const int slots = tokens * top_k, i = threadIdx.x, lane = lane_id(), wave = i / kWave;
+  if (tokens == 1) {
+    all = top_k;
+    rows = u < top_k ? 1 : 0;
+    if (lane == 0) of.slots[wave][0] = (uint16_t)u;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    return choice[u < top_k ? u : 0];
+  }
+  int e[kEach];
+#pragma unroll
+  for (int n = 0; n < kEach; ++n) e[n] = i + n * kLayerThreads < slots ? choice[i + n * kLayerThreads] : -1;
+  if (i < kWave) {
+    of.used[i] = 0;
+    of.slot_of[i] = -1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < kEach; ++n)
+    if (n * kLayerThreads < slots && e[n] >= 0) ((uint8_t*)of.used)[e[n]] = 1;
+  __syncthreads();
+  const uint64_t mine = of.used[lane];
+  const int count = __popcll(mine), through = wave_inclusive_scan(count);
+  all = __builtin_amdgcn_readlane(through, kWave - 1);
+  rows = 0;
+  if (u >= all) return 0;
+  const int at = __builtin_ctzll(__ballot(through > u));
+  uint64_t left = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), at) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+  for (int before = u - (__builtin_amdgcn_readlane(through, at) - __builtin_amdgcn_readlane(count, at)); before > 0; --before) left &= left - 1;
+  const int expert = at * 8 + __builtin_ctzll(left) / 8;
+#pragma unroll
+  for (int n = 0; n < kEach; ++n)
+    if (n * kLayerThreads < slots && e[n] == expert) of.slot_of[(i + n * kLayerThreads) / top_k] = (int16_t)(i + n * kLayerThreads);
+  __syncthreads();
+  const int slot = of.slot_of[lane];
+  const uint64_t has = __ballot(slot >= 0);
+  if (slot >= 0) of.slots[wave][__popcll(has & ((1ull << lane) - 1))] = (uint16_t)slot;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  rows = __popcll(has);
+  return expert;
+}
+
 // NF fragments of 16 weight rows (with the gate: half of them W1's, half V1's), up to R tiles of 16 token rows.  Of a chunk of 64 columns lane (c = l % 16,
 // g = l / 16) has columns 8 g .. 8 g + 7 and 32 + 8 g .. 32 + 8 g + 7 of weight row c and of token row c, 16 bytes each: whole 64-byte pieces a load.
 template <int DT, bool GATE, int NF, int R>
 __global__ void __launch_bounds__(kLayerThreads)
-layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w1, const uint16_t* __restrict__ v1, const LayerTable* __restrict__ table, int tokens,
+layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ w1, const uint16_t* __restrict__ v1, const int32_t* __restrict__ choice, int tokens,
                     int top_k, int hidden, int ffn, int tiles, int act, uint16_t* __restrict__ h_hi, uint16_t* __restrict__ h_lo) {
   constexpr int kCols = GATE ? NF * 8 : NF * 16;          // output columns
   constexpr int kPitch = NF * 16 + 4, kChunk = 64;
   __shared__ __attribute__((aligned(16))) float sums[kLayerWaves][16][kPitch];
+  __shared__ LayerRows of;
   const int u = (int)blockIdx.x / tiles, f0 = ((int)blockIdx.x - u * tiles) * kCols;
-  const int4 it = table->used[u];
-  if (it.z == 0) return;
-  const int expert = it.x, all_rows = it.z;
+  int all_rows, used;
+  const int expert = find_rows(choice, tokens, top_k, u, of, all_rows, used);
+  if (all_rows == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), c = lane & 15, g = lane >> 4;
   const uint32_t pitch = (uint32_t)hidden * 2u;
   const int64_t matrix = (int64_t)ffn * hidden;
   const __amdgpu_buffer_rsrc_t rsrc_x = rsrc_of(x, (uint32_t)tokens * pitch), rsrc_w = rsrc_of(w1 + expert * matrix, (uint32_t)(matrix * 2));
   const __amdgpu_buffer_rsrc_t rsrc_v = GATE ? rsrc_of(v1 + expert * matrix, (uint32_t)(matrix * 2)) : rsrc_w;
   for (int done = 0; done < all_rows; done += 16 * R) {      // once, but for experts of many rows
-    const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
+    const int rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
     uint32_t x_off[R];
 #pragma unroll
     for (int t = 0; t < R; ++t) {
       const int r = t * 16 + c;
-      x_off[t] = r < rows ? (uint32_t)table->token_of_row[first + r] * pitch + (uint32_t)g * 16u : kNone;
+      x_off[t] = r < rows ? (uint32_t)of.slots[wave][done + r] / (uint32_t)top_k * pitch + (uint32_t)g * 16u : kNone;
     }
     const uint32_t w_off = (uint32_t)(f0 + c) * pitch + (uint32_t)g * 16u;
     struct Chunk { u32x4 a[R][2], b[NF][2]; };
@@ -519,7 +490,7 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
           v = activated(v, act);
           in_two<DT>(GATE ? v * gate : v, hi[i], lo[i]);
         }
-        const int64_t at = (int64_t)(first + r) * ffn + f0 + col;
+        const int64_t at = (int64_t)of.slots[wave][done + r] * ffn + f0 + col;
         __builtin_memcpy(h_hi + at, hi, sizeof(hi));
         __builtin_memcpy(h_lo + at, lo, sizeof(lo));
       }
@@ -531,18 +502,18 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
 // row), and turns the 8 x 8 values over with byte permutes: fragment j has column 8 c + j of those rows.
 template <int DT, int R>
 __global__ void __launch_bounds__(kLayerThreads)
-layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict__ h_lo, const uint16_t* __restrict__ w2, const LayerTable* __restrict__ table, int tokens,
+layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict__ h_lo, const uint16_t* __restrict__ w2, const int32_t* __restrict__ choice, int tokens,
                   int top_k, int hidden, int ffn, int tiles, int parts, const float* __restrict__ weights, float* __restrict__ sums_of_parts, uint16_t* __restrict__ out,
-                  int32_t* __restrict__ counters, int entries, bool by_xcd) {
+                  int32_t* __restrict__ counters, bool by_xcd) {
   constexpr int kPitch = kDownColumns + 4, kChunk = 32, kThrough = 0x11;      // cache policy: past the caches
   __shared__ __attribute__((aligned(16))) float sums[kLayerWaves][16][kPitch];
+  __shared__ LayerRows of;
   __shared__ int flag;
   const int in_order = by_xcd ? xcd_tile_id((int)blockIdx.x, tiles) : (int)blockIdx.x, u = in_order / (tiles * parts), in = in_order - u * tiles * parts;
   const int part = in / tiles, tile = in - part * tiles, n0 = tile * kDownColumns;
-  if (u >= entries) return;
-  const int4 it = table->used[u];
-  if (it.z == 0) return;
-  const int expert = it.x, all_rows = it.z, slots = tokens * top_k;
+  int all_rows, used;
+  const int expert = find_rows(choice, tokens, top_k, u, of, all_rows, used), slots = tokens * top_k;
+  if (all_rows == 0) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id(), c = lane & 15, g = lane >> 4;
   const uint32_t pitch = (uint32_t)hidden * 2u, h_pitch = (uint32_t)ffn * 2u;
   const int64_t matrix = (int64_t)ffn * hidden;
@@ -554,10 +525,10 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
   // a part's sums lie [part][row][column]
   const __amdgpu_buffer_rsrc_t rsrc_parts = rsrc_of(sums_of_parts, (uint32_t)parts * (uint32_t)slots * (uint32_t)hidden * 4u);
   for (int done = 0; done < all_rows; done += 16 * R) {      // once, but for experts of many rows
-    const int first = it.y + done, rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
+    const int rows = all_rows - done < 16 * R ? all_rows - done : 16 * R, row_tiles = (rows + 15) / 16;
     uint32_t h_off[R];
 #pragma unroll
-    for (int t = 0; t < R; ++t) h_off[t] = t * 16 + c < rows ? (uint32_t)(first + t * 16 + c) * h_pitch + (uint32_t)g * 16u : kNone;
+    for (int t = 0; t < R; ++t) h_off[t] = t * 16 + c < rows ? (uint32_t)of.slots[wave][done + t * 16 + c] * h_pitch + (uint32_t)g * 16u : kNone;
     const int chunks = (ffn + kChunk - 1) / kChunk, begin = (int)((int64_t)part * chunks / parts), end = (int)((int64_t)(part + 1) * chunks / parts);
     struct Chunk { u32x4 hi[R], lo[R], b[8]; };
     auto fetch = [&](Chunk& q, int chunk) {
@@ -633,7 +604,7 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
           lo += *(const f32x4*)&sums[w][m][col];
           hi += *(const f32x4*)&sums[w][m][col + 4];
         }
-        const uint32_t at = (((uint32_t)part * (uint32_t)slots + (uint32_t)(first + t * 16 + m)) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
+        const uint32_t at = (((uint32_t)part * (uint32_t)slots + (uint32_t)of.slots[wave][done + t * 16 + m]) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rsrc_parts, (int)at, 0, kThrough);
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rsrc_parts, (int)at + 16, 0, kThrough);
       }
@@ -652,13 +623,13 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
     for (int i = 0; i < kAhead; ++i) {
       const bool here = q + i < stop && t < tokens && mine;
       const int now = here ? q + i : 0, j = now / parts, p = now - j * parts, s = here ? t * top_k + j : 0;
-      const uint32_t at = (((uint32_t)p * (uint32_t)slots + (uint32_t)table->row_of_slot[s]) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
+      const uint32_t at = (((uint32_t)p * (uint32_t)slots + (uint32_t)s) * (uint32_t)hidden + (uint32_t)(n0 + col)) * 4u;
       place[i] = here ? at : kNone;
       w[i] = weights[s];
     }
   };
   look_up(m / share, my_share * each);
-  if (!last_to_come(counters + kCounterColumns + tile, table->experts * parts, &flag)) return;
+  if (!last_to_come(counters + kCounterColumns + tile, used * parts, &flag)) return;
   for (int t0 = 0; t0 < tokens; t0 += 16 / share) {
     const int t = t0 + m / share;
     f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
@@ -701,7 +672,7 @@ struct LayerPlan {
   int fragments, hidden_tiles;
   int down_tiles, parts;
   bool by_xcd;              // the second product's tiles of an expert's part on one XCD
-  size_t table, choice, logits, h_hi, h_lo, sums, total = 0;
+  size_t choice, logits, h_hi, h_lo, sums, total = 0;
 
   LayerPlan(int tokens, int hidden, int ffn, int experts, int top_k, bool gate) {
     const int slots = tokens * top_k;
@@ -732,7 +703,6 @@ struct LayerPlan {
       total += (bytes + 255) & ~(size_t)255;
       return at;
     };
-    table = take(sizeof(LayerTable));
     choice = take((size_t)slots * 4);
     logits = take((size_t)tokens * experts * 8);
     h_hi = take((size_t)slots * ffn * 2);
@@ -757,11 +727,10 @@ void launch_choose(const void* x_, const void* router_, const LayerChoice& q, co
                    int32_t* counters, hipStream_t s) {
   const uint16_t *const x = (const uint16_t*)x_, *const router = (const uint16_t*)router_;
   int32_t* const choice = (int32_t*)(base + plan.choice);
-  LayerTable* const table = (LayerTable*)(base + plan.table);
   // up to 128 KiB of router by one workgroup a token (us, that / four experts a workgroup: 1 token, 8 of 4096 5.2 / 7.4; 16, 64 of 1024 7.9 / 9.4; 1, 64 of 2048 10.5 / 6.4)
   if ((int64_t)q.experts * ((q.hidden + 1023) & ~1023) <= 1 << 16) {
-    if (q.experts <= kWholeWaves) layer_choose_whole_kernel<DT, 1, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices, table, counters);
-    else layer_choose_whole_kernel<DT, 4, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices, table, counters);
+    if (q.experts <= kWholeWaves) layer_choose_whole_kernel<DT, 1, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);
+    else layer_choose_whole_kernel<DT, 4, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);
     return;
   }
   const unsigned workgroups = (unsigned)ceil_div(q.experts, kLayerWaves);
@@ -769,19 +738,19 @@ void launch_choose(const void* x_, const void* router_, const LayerChoice& q, co
   // 4096 26 / 23 / 20 / 24)
   uint64_t* const logits = (uint64_t*)(base + plan.logits);
   if (q.experts * q.tokens <= 4096)
-    layer_choose_kernel<DT, 1, R><<<dim3(workgroups, (unsigned)q.tokens), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
+    layer_choose_kernel<DT, 1, R><<<dim3(workgroups, (unsigned)q.tokens), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, counters);
   else
-    layer_choose_kernel<DT, 4, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 4)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, table, counters);
+    layer_choose_kernel<DT, 4, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 4)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, counters);
 }
 
 template <int DT, int R>
 void launch_products(const void* x, const void* w1, const void* v1, const void* w2, const LayerChoice& q, int ffn, int act, char* base, const LayerPlan& plan,
                      const float* weights, void* out, int32_t* counters, hipStream_t s) {
-  const LayerTable* const table = (const LayerTable*)(base + plan.table);
+  const int32_t* const choice = (const int32_t*)(base + plan.choice);
   uint16_t *const hi = (uint16_t*)(base + plan.h_hi), *const lo = (uint16_t*)(base + plan.h_lo);
   const unsigned grid = (unsigned)(plan.entries * plan.hidden_tiles);
 #define MBX_LAYER_HIDDEN(GATE, NF) \
-  layer_hidden_kernel<DT, GATE, NF, R><<<grid, kLayerThreads, 0, s>>>((const uint16_t*)x, (const uint16_t*)w1, (const uint16_t*)v1, table, q.tokens, q.top_k, q.hidden, ffn, plan.hidden_tiles, act, hi, lo)
+  layer_hidden_kernel<DT, GATE, NF, R><<<grid, kLayerThreads, 0, s>>>((const uint16_t*)x, (const uint16_t*)w1, (const uint16_t*)v1, choice, q.tokens, q.top_k, q.hidden, ffn, plan.hidden_tiles, act, hi, lo)
   if constexpr (R > 1)      // for rows enough
     if (plan.fragments == 8) { if (v1) MBX_LAYER_HIDDEN(true, 8); else MBX_LAYER_HIDDEN(false, 8); }
   if (plan.fragments == 4) { if (v1) MBX_LAYER_HIDDEN(true, 4); else MBX_LAYER_HIDDEN(false, 4); }
@@ -790,8 +759,8 @@ void launch_products(const void* x, const void* w1, const void* v1, const void* 
 #undef MBX_LAYER_HIDDEN
   const int64_t down = (int64_t)plan.entries * plan.down_tiles * plan.parts;
   layer_down_kernel<DT, R><<<(unsigned)(plan.by_xcd ? xcd_grid(down, plan.down_tiles) : down), kLayerThreads, 0, s>>>(
-      hi, lo, (const uint16_t*)w2, table, q.tokens, q.top_k, q.hidden, ffn, plan.down_tiles, plan.parts, weights, (float*)(base + plan.sums), (uint16_t*)out, counters,
-      plan.entries, plan.by_xcd);
+      hi, lo, (const uint16_t*)w2, choice, q.tokens, q.top_k, q.hidden, ffn, plan.down_tiles, plan.parts, weights, (float*)(base + plan.sums), (uint16_t*)out, counters,
+      plan.by_xcd);
 }
 
 template <int DT>
@@ -833,7 +802,7 @@ int mbx_moe_layer(const void* x, int64_t tokens, int64_t hidden, int dtype, cons
   const LayerPlan plan((int)tokens, (int)hidden, (int)ffn, num_experts, top_k, v1 != nullptr);
   if (!scratch || scratch_bytes < plan.total || ((uintptr_t)scratch & 15)) return MBX_ESCRATCH;
   if (!workspace || workspace_bytes < kWorkspaceCounters * sizeof(int32_t) || ((uintptr_t)workspace & 3)) return MBX_ESCRATCH;
-  const LayerChoice q{(int)tokens, (int)hidden, num_experts, top_k, score == MBX_SCORE_SIGMOID, groups, top_groups, group_best, plan.entries, norm_p, scale};
+  const LayerChoice q{(int)tokens, (int)hidden, num_experts, top_k, score == MBX_SCORE_SIGMOID, groups, top_groups, group_best, norm_p, scale};
   hipStream_t s = as_stream(stream);
   return dtype == MBX_BF16 ? launch_layer<MBX_BF16>(x, router, w1, v1, w2, q, bias, (int)ffn, act, out, weights, indices, (char*)scratch, plan, (int32_t*)workspace, s)
                            : launch_layer<MBX_F16>(x, router, w1, v1, w2, q, bias, (int)ffn, act, out, weights, indices, (char*)scratch, plan, (int32_t*)workspace, s);

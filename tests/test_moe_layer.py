@@ -34,7 +34,7 @@ def test_tensors_off_the_gpu_are_refused():
 @pytest.mark.parametrize('sizes,taken', [
     ((1, 8, 8, 1, 1), True), ((64, 4096, 14336, 8, 2), True), ((65, 8, 8, 1, 1), False), ((1, 8, 8, 512, 16), True), ((1, 8, 8, 513, 1), False), ((1, 8, 8, 32, 17), False),
     ((1, 8, 8, 4, 5), False), ((1, 12, 8, 4, 1), False), ((1, 8, 12, 4, 1), False), ((1, 0, 8, 4, 1), False), ((1, 32768, 32704, 4, 1), False), ((1, 32768, 32640, 4, 1), True),
-    ((1, 16, 1 << 26, 4, 1), False), ((1, 959 * 128, 64, 4, 1), True), ((1, 959 * 128 + 8, 64, 4, 1), False), ((64, 32768, 8, 16, 16), False), ((64, 8192, 8, 16, 16), True)])
+    ((1, 16, 1 << 26, 4, 1), False), ((1, 960 * 128, 64, 4, 1), True), ((1, 960 * 128 + 8, 64, 4, 1), False), ((64, 32768, 8, 16, 16), False), ((64, 8192, 8, 16, 16), True)])
 def test_sizes_that_are_taken(sizes, taken):
     """Offsets that the kernels keep in 32 bits, and the counters of the workspace."""
     assert few_tokens.takes(*sizes) == taken
