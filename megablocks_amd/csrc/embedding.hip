@@ -419,11 +419,92 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden
   }
 }
 
+// ---- up to kFewTokens tokens: the gradient by one launch ----
+// A workgroup has up to kFewWords words and kFewSlices slices of the columns: it lists the tokens of those words, in order, and a wave adds up those of a word for a slice.
+// Bound by the launch, or by the zeros of a large table.  Tokens of one word are added up one after the other, so it is for few of them (us of three launches / of this, forward
+// included: 64 tokens, 1000 words of 64 19.2 / 7.8; 256 tokens, 128000 words of 2040 121 / 111; 128 tokens of one word of 4096 17.2 / 18.2, 256 of them 18.2 / 33).
+constexpr int kFewTokens = kEmbThreads, kFewWords = 16, kFewSlices = kEmbWaves;
+
+template <int DT, typename I>
+__global__ void __launch_bounds__(kEmbThreads) embedding_few_kernel(const void* __restrict__ grad, const I* __restrict__ ids, int tokens, int words, int each, int hidden,
+                                                                    int slices, int padding, float scale, void* __restrict__ out) {
+  typedef typename Elem<DT>::type E;
+  __shared__ int32_t token_of[kFewTokens], place_of[kFewTokens], counts[kEmbWaves];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int64_t first = (int64_t)blockIdx.x * each;
+  int place = -1;
+  if ((int)threadIdx.x < tokens) {
+    const int word = word_of(ids, threadIdx.x, words);
+    if (word >= first && word < first + each && word != padding) place = word - (int)first;
+  }
+  const uint64_t here = __ballot(place >= 0);
+  if (lane == 0) counts[wave] = __popcll(here);
+  __syncthreads();
+  int to = __popcll(here & ((1ull << lane) - 1)), n = 0;
+#pragma unroll
+  for (int w = 0; w < kEmbWaves; ++w) {
+    to += w < wave ? counts[w] : 0;
+    n += counts[w];
+  }
+  if (place >= 0) {
+    token_of[to] = threadIdx.x;
+    place_of[to] = place;
+  }
+  __syncthreads();
+  const int first_slice = (int)blockIdx.y * kFewSlices, my_slices = slices - first_slice < kFewSlices ? slices - first_slice : kFewSlices;
+  const int units = (int)(words - first < each ? words - first : each) * my_slices;
+  for (int unit = wave; unit < units; unit += kEmbWaves) {
+    const int word = unit / my_slices, slice = first_slice + unit - word * my_slices, column = slice * kSlice + lane * kPer, left = hidden - column;
+    const bool whole = hidden % kPer == 0 || (slice + 1) * kSlice <= hidden;      // every lane has eight columns or none
+    float acc[kPer] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    bool any = false;
+    for (int c = 0; c < n; c += kWave) {
+      const int token = c + lane < n ? token_of[c + lane] : 0;
+      uint64_t todo = __ballot(c + lane < n && place_of[c + lane] == word);
+      any = any || todo != 0;
+      constexpr int kAhead = DT == MBX_F32 ? 8 : 16;
+      while (todo) {
+        const uint64_t now = todo;
+        const int count = __popcll(now) < kAhead ? __popcll(now) : kAhead;
+        int row[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          row[u] = __builtin_amdgcn_readlane(token, __builtin_ctzll(todo ? todo : now));
+          todo &= todo - 1;      // 0 stays 0
+        }
+        if (whole) {
+          Piece<DT> v[kAhead];      // all under way before the first is looked at
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) v[u].load((const E*)grad + (int64_t)row[u] * hidden + (left > 0 ? column : 0));
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (u < count)
+#pragma unroll
+              for (int t = 0; t < kPer; ++t) acc[t] += v[u].value(t);
+        } else if (left > 0) {
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u)
+            if (u < count) {
+              float v[kPer];
+              load_columns<DT>((const E*)grad + (int64_t)row[u] * hidden + column, left, v);
+#pragma unroll
+              for (int t = 0; t < kPer; ++t) acc[t] += v[t];
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kPer; ++t) acc[t] = any ? acc[t] * scale : 0.f;
+    if (left > 0) store_columns<DT>((E*)out + (first + word) * hidden + column, left, acc);
+  }
+}
+
 struct EmbeddingParts {
-  size_t order, sorted, starts, heads, tails, crossing, total = 0;
+  size_t order = 0, sorted = 0, starts = 0, heads = 0, tails = 0, crossing = 0, total = 0;
   int64_t pieces;
   EmbeddingParts(int64_t tokens, int words, int hidden) {
     pieces = ceil_div(tokens, kPiece);
+    if (tokens <= kFewTokens) return;      // none
     auto take = [&](size_t bytes) {
       const size_t at = total;
       total += (bytes + 255) & ~(size_t)255;
@@ -477,6 +558,14 @@ int launch_sums(const void* grad, int words, int hidden, float scale, const Embe
   return 0;
 }
 
+template <int DT, typename I>
+int launch_few(const void* grad, const void* ids, int tokens, int words, int hidden, int64_t padding, float scale, void* out, hipStream_t s) {
+  const int slices = (int)ceil_div(hidden, kSlice), each = words <= 256 ? 1 : words >= 256 * kFewWords ? kFewWords : (int)ceil_div(words, 256);
+  embedding_few_kernel<DT, I><<<dim3((unsigned)ceil_div(words, each), (unsigned)ceil_div(slices, kFewSlices)), kEmbThreads, 0, s>>>(
+      grad, (const I*)ids, tokens, words, each, hidden, slices, padding < 0 || padding >= words ? -1 : (int)padding, scale, out);
+  return launch_status();
+}
+
 bool embedding_sizes_ok(int64_t tokens, int64_t words, int64_t hidden) { return tokens >= 0 && words >= 0 && hidden >= 0; }
 // 32-bit places of tokens; the join's grid counts columns in 16 bits
 bool embedding_in_range(int64_t tokens, int64_t words, int64_t hidden) {
@@ -513,6 +602,12 @@ int mbx_embedding_gradient(const void* grad, const void* ids, int itype, int64_t
   if (!embedding_in_range(tokens, words, hidden)) return MBX_ERANGE;
   if (words == 0 || hidden == 0) return 0;
   if (!out || (tokens > 0 && (!ids || !grad))) return MBX_EINVAL;
+  if (tokens <= kFewTokens) {
+#define MBX_FEW(DT) (itype == MBX_I32 ? launch_few<DT, int32_t>(grad, ids, (int)tokens, (int)words, (int)hidden, padding, scale, out, as_stream(stream)) \
+                                      : launch_few<DT, int64_t>(grad, ids, (int)tokens, (int)words, (int)hidden, padding, scale, out, as_stream(stream)))
+    return dtype == MBX_BF16 ? MBX_FEW(MBX_BF16) : dtype == MBX_F16 ? MBX_FEW(MBX_F16) : MBX_FEW(MBX_F32);
+#undef MBX_FEW
+  }
   const EmbeddingParts parts(tokens, (int)words, (int)hidden);
   if (!scratch || scratch_bytes < parts.total || ((uintptr_t)scratch & 15)) return MBX_ESCRATCH;
   char* const base = (char*)scratch;

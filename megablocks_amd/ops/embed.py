@@ -19,12 +19,12 @@ def _rows(ids, table, scale):
 def _table_gradient(grad, ids, words, scale, padding):
     hidden = grad.shape[-1]
     grad = grad.contiguous()
-    out = torch.empty((words, hidden), dtype=grad.dtype, device=grad.device)
+    out = grad.new_empty((words, hidden))
     with _lib.device_of(grad):
         nbytes = lib.mbx_embedding_gradient_scratch_bytes(ids.numel(), words, hidden)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=grad.device) if nbytes else None      # none for a few tokens
         _lib.check(lib.mbx_embedding_gradient(grad.data_ptr(), ids.data_ptr(), _lib.ITYPE[ids.dtype], ids.numel(), _lib.DTYPE[grad.dtype], words, hidden, padding, scale,
-                                              out.data_ptr(), scratch.data_ptr(), nbytes, _lib.stream()), 'embedding_gradient')
+                                              out.data_ptr(), _lib.ptr(scratch), nbytes, _lib.stream()), 'embedding_gradient')
     return out
 
 

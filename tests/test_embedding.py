@@ -37,6 +37,6 @@ def test_entry_points_refuse_without_touching_the_gpu():
             assert call(**bad) == _lib.ERANGE
         assert call(hidden=0) == 0
     assert rows(table=None) == _lib.EINVAL and gradient(grad=None) == _lib.EINVAL and rows(tokens=0) == 0 and gradient(words=0) == 0
-    nbytes = lib.mbx_embedding_gradient_scratch_bytes(3, 5, 8)
-    assert gradient() == _lib.ESCRATCH and gradient(scratch=16, nbytes=nbytes - 1) == _lib.ESCRATCH and gradient(scratch=8, nbytes=nbytes) == _lib.ESCRATCH
-    assert lib.mbx_embedding_gradient_scratch_bytes(-1, 5, 8) == 0 and nbytes > 0
+    many, nbytes = dict(tokens=257), lib.mbx_embedding_gradient_scratch_bytes(257, 5, 8)      # fewer tokens need none
+    assert gradient(**many) == _lib.ESCRATCH and gradient(**many, scratch=16, nbytes=nbytes - 1) == _lib.ESCRATCH and gradient(**many, scratch=8, nbytes=nbytes) == _lib.ESCRATCH
+    assert lib.mbx_embedding_gradient_scratch_bytes(-1, 5, 8) == 0 and lib.mbx_embedding_gradient_scratch_bytes(256, 5, 8) == 0 and nbytes > 0

@@ -56,21 +56,23 @@ def check(ids, table, grad, scale=1.0, padding=None):
 
 @pytest.mark.parametrize('dtype', [BF16, FP16, FP32], ids=str)
 @pytest.mark.parametrize('tokens,words,hidden', [(1, 1, 8), (1, 50000, 1024), (2, 3, 1), (63, 1000, 64), (64, 70, 7), (65, 257, 513), (300, 255, 2040), (1000, 5, 1032),
-                                                 (4097, 30011, 100), (3, 100000, 512), (33, 4, 4100), (20000, 1025, 72)])
+                                                 (4097, 30011, 100), (3, 100000, 512), (33, 4, 4100), (20000, 1025, 72),
+                                                 (256, 300, 520), (255, 5000, 2056), (257, 300, 520), (258, 70, 7), (300, 3, 1), (321, 257, 513)])
 def test_rows_and_gradient(tokens, words, hidden, dtype):
     check(*make(tokens, words, hidden, dtype, wide=tokens % 2 == 0), scale=1.0)
 
 
 @pytest.mark.parametrize('kind', ['one', 'half', 'few', 'ascending', 'even'])
-@pytest.mark.parametrize('tokens,words,hidden', [(31, 9, 40), (32, 9, 40), (33, 9, 40), (64, 9, 40), (4096, 2000, 264), (9999, 300, 1030), (140000, 5000, 16)])
+@pytest.mark.parametrize('tokens,words,hidden', [(31, 9, 40), (32, 9, 40), (33, 9, 40), (64, 9, 40), (200, 30, 1028), (256, 700, 264), (257, 9, 40), (288, 9, 40), (289, 9, 40), (4096, 2000, 264), (9999, 300, 1030), (140000, 5000, 16)])
 def test_words_that_come_often(tokens, words, hidden, kind):
     check(*make(tokens, words, hidden, BF16, kind), scale=0.5)
 
 
 @pytest.mark.parametrize('padding', [0, 17, -1, 99])
 @pytest.mark.parametrize('kind', ['half', 'few', 'one'])
-def test_padding_learns_nothing(kind, padding):
-    ids, table, grad = make(3000, 100, 96, FP16, kind)
+@pytest.mark.parametrize('tokens', [3000, 150])
+def test_padding_learns_nothing(tokens, kind, padding):
+    ids, table, grad = make(tokens, 100, 96, FP16, kind)
     ids[::3] = padding % 100
     check(ids, table, grad, scale=32.0, padding=padding % 100)
     table.requires_grad_()
