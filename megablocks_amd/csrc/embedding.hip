@@ -27,6 +27,7 @@ typedef u32x4e __attribute__((aligned(4))) u32x4_at4;
 constexpr int kEmbThreads = 256, kEmbWaves = kEmbThreads / kWave;
 constexpr int kPer = 8;                               // columns of a lane
 constexpr int kSlice = kPer * kWave;                  // columns of a wave
+constexpr int64_t kEmbMaxBlocks = 1 << 23;            // of a launch, whose threads have to be fewer than 2^32
 
 // kPer values as they lie in memory
 template <int DT>
@@ -99,9 +100,9 @@ __device__ __forceinline__ int word_of(const I* __restrict__ ids, int64_t i, int
 // ---- out[i] = scale table[ids[i]]: a wave per row and slice of kSlice columns ----
 template <int DT, typename I>
 __global__ void __launch_bounds__(kEmbThreads) embedding_kernel(const I* __restrict__ ids, int64_t tokens, const void* __restrict__ table, int words, int hidden,
-                                                                int slices, float scale, void* __restrict__ out) {
+                                                                int slices, float scale, void* __restrict__ out, int64_t first_block) {
   typedef typename Elem<DT>::type E;
-  const int64_t unit = (int64_t)blockIdx.x * kEmbWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t unit = (first_block + blockIdx.x) * kEmbWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int64_t i = unit / slices;
   if (i >= tokens) return;
   const int column = (int)(unit - i * slices) * kSlice + lane_id() * kPer, left = hidden - column;
@@ -280,11 +281,12 @@ template <int DT>
 __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* __restrict__ grad, const int32_t* __restrict__ order, const int32_t* __restrict__ sorted,
                                                                     const int32_t* __restrict__ starts, int words, int hidden, int slices, int64_t piece_blocks,
                                                                     float scale, float* __restrict__ heads, float* __restrict__ tails, EmbeddingRuns* __restrict__ crossing,
-                                                                    void* __restrict__ out) {
+                                                                    void* __restrict__ out, int64_t first_block) {
   typedef typename Elem<DT>::type E;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
-  if ((int64_t)blockIdx.x >= piece_blocks) {
-    const int64_t first = (((int64_t)blockIdx.x - piece_blocks) * kEmbWaves + wave) * kZeroRows;
+  const int64_t block = first_block + blockIdx.x;
+  if (block >= piece_blocks) {
+    const int64_t first = ((block - piece_blocks) * kEmbWaves + wave) * kZeroRows;
     if (first >= words) return;
     const int64_t v = first + lane;
     uint64_t todo = __ballot(lane < kZeroRows && v < words && starts[v < words ? v : words] == starts[v < words ? v + 1 : words]);
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* 
     }
     return;
   }
-  const int64_t unit = (int64_t)blockIdx.x * kEmbWaves + wave;
+  const int64_t unit = block * kEmbWaves + wave;
   const int64_t p = unit / slices, from = p * kPiece;
   const int total = starts[words];
   if (from >= total) return;
@@ -427,11 +429,11 @@ constexpr int kFewTokens = kEmbThreads, kFewWords = 16, kFewSlices = kEmbWaves;
 
 template <int DT, typename I>
 __global__ void __launch_bounds__(kEmbThreads) embedding_few_kernel(const void* __restrict__ grad, const I* __restrict__ ids, int tokens, int words, int each, int hidden,
-                                                                    int slices, int padding, float scale, void* __restrict__ out) {
+                                                                    int slices, int padding, float scale, void* __restrict__ out, int64_t first_block) {
   typedef typename Elem<DT>::type E;
   __shared__ int32_t token_of[kFewTokens], place_of[kFewTokens], counts[kEmbWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
-  const int64_t first = (int64_t)blockIdx.x * each;
+  const int64_t first = (first_block + blockIdx.x) * each;
   int place = -1;
   if ((int)threadIdx.x < tokens) {
     const int word = word_of(ids, threadIdx.x, words);
@@ -519,12 +521,18 @@ struct EmbeddingParts {
   }
 };
 
+// launch(workgroups, the first of them) for all of them, in as many launches as that takes
+template <typename F>
+void in_launches(int64_t blocks, F&& launch) {
+  for (int64_t first = 0; first < blocks; first += kEmbMaxBlocks) launch((unsigned)(blocks - first < kEmbMaxBlocks ? blocks - first : kEmbMaxBlocks), first);
+}
+
 template <int DT, typename I>
 int launch_embedding(const void* ids, int64_t tokens, const void* table, int words, int hidden, float scale, void* out, hipStream_t s) {
   const int slices = (int)ceil_div(hidden, kSlice);
-  const int64_t blocks = ceil_div(tokens * slices, kEmbWaves);
-  if (blocks > 0x7fffffff) return MBX_ERANGE;
-  embedding_kernel<DT, I><<<(unsigned)blocks, kEmbThreads, 0, s>>>((const I*)ids, tokens, table, words, hidden, slices, scale, out);
+  in_launches(ceil_div(tokens * slices, kEmbWaves), [&](unsigned blocks, int64_t first) {
+    embedding_kernel<DT, I><<<blocks, kEmbThreads, 0, s>>>((const I*)ids, tokens, table, words, hidden, slices, scale, out, first);
+  });
   return launch_status();
 }
 
@@ -546,9 +554,9 @@ int launch_sums(const void* grad, int words, int hidden, float scale, const Embe
   EmbeddingRuns* const crossing = (EmbeddingRuns*)(scratch + parts.crossing);
   const int slices = (int)ceil_div(hidden, kSlice);
   const int64_t piece_blocks = ceil_div(parts.pieces * slices, kEmbWaves), zero_blocks = ceil_div(words, kEmbWaves * kZeroRows);
-  if (piece_blocks + zero_blocks > 0x7fffffff) return MBX_ERANGE;
-  embedding_sum_kernel<DT><<<(unsigned)(piece_blocks + zero_blocks), kEmbThreads, 0, s>>>(grad, order, sorted, starts, words, hidden, slices, piece_blocks,
-                                                                                          scale, heads, tails, crossing, out);
+  in_launches(piece_blocks + zero_blocks, [&](unsigned blocks, int64_t first) {
+    embedding_sum_kernel<DT><<<blocks, kEmbThreads, 0, s>>>(grad, order, sorted, starts, words, hidden, slices, piece_blocks, scale, heads, tails, crossing, out, first);
+  });
   if (const int rc = launch_status()) return rc;
   if (parts.pieces > 1) {
     const unsigned runs = (unsigned)(parts.pieces - 1 < kJoinRuns ? parts.pieces - 1 : kJoinRuns);
@@ -561,8 +569,10 @@ int launch_sums(const void* grad, int words, int hidden, float scale, const Embe
 template <int DT, typename I>
 int launch_few(const void* grad, const void* ids, int tokens, int words, int hidden, int64_t padding, float scale, void* out, hipStream_t s) {
   const int slices = (int)ceil_div(hidden, kSlice), each = words <= 256 ? 1 : words >= 256 * kFewWords ? kFewWords : (int)ceil_div(words, 256);
-  embedding_few_kernel<DT, I><<<dim3((unsigned)ceil_div(words, each), (unsigned)ceil_div(slices, kFewSlices)), kEmbThreads, 0, s>>>(
-      grad, (const I*)ids, tokens, words, each, hidden, slices, padding < 0 || padding >= words ? -1 : (int)padding, scale, out);
+  in_launches(ceil_div(words, each), [&](unsigned blocks, int64_t first) {
+    embedding_few_kernel<DT, I><<<dim3(blocks, (unsigned)ceil_div(slices, kFewSlices)), kEmbThreads, 0, s>>>(
+        grad, (const I*)ids, tokens, words, each, hidden, slices, padding < 0 || padding >= words ? -1 : (int)padding, scale, out, first);
+  });
   return launch_status();
 }
 

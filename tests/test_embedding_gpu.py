@@ -246,3 +246,33 @@ def test_inference_mode():
     with torch.inference_mode():
         ids, table = torch.arange(4, device='cuda'), torch.randn(5, 8, device='cuda')
         assert torch.equal(ops.embedding(ids, table), table[:4])
+
+
+def used_memory(*shape, **kw):
+    """What a tensor of this shape is likely to be made of next: no zeros."""
+    torch.full(shape, 9.0, device='cuda', **kw)
+
+
+def test_rows_of_more_workgroups_than_a_launch_has_threads_for():
+    """A launch has fewer than 2^32 threads, of which a token takes 64 at least."""
+    tokens = (1 << 26) + 12345
+    ids = torch.randint(0, 13, (tokens,), device='cuda', dtype=torch.int32)
+    table = torch.arange(1.0, 14.0, device='cuda').unsqueeze(1)
+    used_memory(tokens, 1)
+    assert torch.equal(ops.embedding(ids, table).flatten(), ids.float() + 1)
+
+
+@pytest.mark.parametrize('tokens,words', [(300, (1 << 27) + 77), (5, (1 << 28) + 77), (0, (1 << 28) + 77)])
+def test_gradients_of_more_workgroups_than_a_launch_has_threads_for(tokens, words):
+    """Rows of zeros too: eight words a workgroup next to the sums, sixteen where there are few tokens."""
+    ids = torch.randint(words - 1000, words, (tokens,), device='cuda')
+    ids[:tokens // 2] %= 1000
+    table = torch.zeros(words, 1, device='cuda', dtype=BF16, requires_grad=True)
+    out = ops.embedding(ids, table)
+    grad = torch.randint(1, 4, out.shape, device='cuda').to(BF16)
+    used_memory(words, 1, dtype=BF16)
+    got, = torch.autograd.grad(out, table, grad)
+    assert torch.equal(got.flatten().nonzero().flatten(), ids.unique())
+    named = ids.unique()
+    want, off = exact((ids.unsqueeze(1) == named).int().argmax(1) if tokens else ids, grad, len(named), 1.0)
+    assert ((got[named].double() - want).abs() <= off).all()
