@@ -719,6 +719,8 @@ int layer_sizes(int64_t tokens, int64_t hidden, int64_t ffn, int experts, int to
   if ((ffn + 64) * hidden * 2 >= (int64_t)1 << 31 || (hidden + 64) * ffn * 2 >= (int64_t)1 << 31 || hidden > (int64_t)(kWorkspaceCounters - kCounterColumns) * kDownColumns ||
       tokens * top_k * ffn * 2 >= (int64_t)1 << 31 || tokens * top_k * hidden * 4 * kLayerMaxParts >= (int64_t)1 << 31 || experts * hidden * 2 >= (int64_t)1 << 31)
     return MBX_ERANGE;
+  // a launch's threads have to be fewer than 2^32: a workgroup of the first product has 16 rows of an expert's weights or more
+  if ((tokens * top_k < experts ? tokens * top_k : experts) * ceil_div(ffn, 16) * kLayerThreads >= (int64_t)1 << 32) return MBX_ERANGE;
   return 0;
 }
 

@@ -64,3 +64,9 @@ def test_entry_point_refuses_without_touching_the_gpu():
 def test_arguments_refuse_other_numbers_of_tokens(tokens):
     with pytest.raises(ValueError):
         Arguments(device=torch.device('cpu'), moe_fused_tokens=tokens)
+
+
+@pytest.mark.parametrize('sizes,taken', [((64, 8, 1 << 22, 64, 1), False), ((63, 8, 1 << 22, 64, 1), True), ((64, 8, 1 << 22, 63, 1), True), ((32, 16, 1 << 22, 128, 2), False)])
+def test_a_launch_has_fewer_than_2_to_the_32_threads(sizes, taken):
+    """256 of them for 16 rows of the weights of an expert that a token may choose."""
+    assert few_tokens.takes(*sizes) == taken
