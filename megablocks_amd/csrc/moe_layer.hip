@@ -195,15 +195,16 @@ __device__ __forceinline__ void choose_for(const LayerChoice& q, int token, L&& 
       my_score = s;
     }
   }
-  double norm = 1.;
+  double weight = my_score;
   if (q.norm_p > 0.f) {
-    const double p = q.norm_p, s = lane < q.top_k ? my_score : 0.;
-    norm = wave_sum_f64(p == 1. ? s : p == 2. ? s * s : lane < q.top_k ? pow(s, p) : 0.);
-    norm = p == 1. ? norm : p == 2. ? sqrt(norm) : pow(norm, 1. / p);
+    // the norm as the largest times the norm of the scores over that: scores of 1e-20, or large p, have powers below the smallest number
+    const double p = q.norm_p, s = lane < q.top_k ? my_score : 0., most = wave_max_f64(s), part = p != 1. && most > 0. ? s / most : s;
+    const double sum = wave_sum_f64(p == 1. ? part : p == 2. ? part * part : pow(part, p));
+    weight = sum == 0. ? 0. : part / (p == 1. ? sum : p == 2. ? sqrt(sum) : pow(sum, 1. / p));      // scores that are all zero: weights of zero
   }
   if (lane < q.top_k) {
     const int64_t at = (int64_t)token * q.top_k + lane;
-    weights[at] = (float)(norm == 0. ? 0. : my_score / norm * (double)q.scale);
+    weights[at] = (float)(weight * (double)q.scale);
     indices[at] = my_expert;
     put(lane, my_expert);
   }

@@ -413,3 +413,58 @@ def test_a_model_trains_and_decodes():
         alike = chosen_alike(layer, x)
     whole, alone = whole.double().view(-1, hidden)[alike], alone.double().view(-1, hidden)[alike]
     assert alike.sum() >= tokens * 0.8 and (whole - alone).norm() <= 1e-2 * whole.norm()
+
+
+# ---- norms of scores whose powers leave every number's range ----
+
+def exact_weights_by_logarithms(logits, indices, score, norm_p, scale=1.0):
+    """scale s / ||s||_p in 64 bits, from log s: nothing is raised to a power."""
+    logs = (logits.log_softmax(1) if score == 'softmax' else F.logsigmoid(logits)).gather(1, indices)
+    return scale * (logs - (norm_p * logs).logsumexp(1, keepdim=True) / norm_p).exp()
+
+
+@pytest.mark.parametrize('norm_p', [0.5, 2, 16, 64, 119, 120, 130, 1000, 3e38])
+@pytest.mark.parametrize('score,experts,logit', [('softmax', 512, 0.0), ('softmax', 64, 3.0), ('sigmoid', 64, -50.0), ('sigmoid', 16, -600.0), ('sigmoid', 300, 5.0)])
+def test_norms_of_large_order_and_small_scores(score, experts, logit, norm_p):
+    """Logits around one number (softmax: flat but for a little), some of one number exactly."""
+    hidden, top_k = 64, 6
+    o = make(5, hidden, 72, experts, std=0.001)
+    o['x'][:, 0] = 1.0
+    o['router'][:, 0] = logit
+    o['router'][experts // 2:, 1:] = 0
+    out, weights, indices = ops.moe_layer(**o, top_k=top_k, act=gg.ACT_SILU, score=score, norm_p=norm_p, scale=1.5)
+    _, want_indices = exact_choice(o, top_k, score)
+    assert torch.equal(indices, want_indices)
+    logits = o['x'].double() @ o['router'].double().t()
+    want = exact_weights_by_logarithms(logits, indices, score, norm_p, 1.5)
+    # arithmetic in 64 bits, the logarithms' too: of numbers up to 601 times p, which is 2^-43 of an exponent there, divided by p again
+    assert ((weights.double() - want).abs() <= want * 1.01 * STEP + 2.0 ** -149).all()
+    want_out, off = exact_out(o, want, indices, gg.ACT_SILU)
+    assert ((out.double() - want_out).abs() <= off).all()
+
+
+def test_norms_of_scores_that_are_zero_or_no_numbers():
+    o = make(4, 64, 72, 16)
+    o['x'][:, 0], o['router'][:, 0] = 1.0, 0.0
+    o['x'][1, 0], o['x'][2, 3] = -30000.0, float('nan')
+    o['router'][:, 0] = 1.0
+    for norm_p in (1, 2, 64, 0.5):
+        out, weights, _ = ops.moe_layer(**o, top_k=3, act=0, score='sigmoid', norm_p=norm_p)
+        assert (weights[1] == 0).all() and (out[1] == 0).all() and weights[2].isnan().all() and out[2].isnan().all()
+        rest = torch.tensor([0, 3], device='cuda')
+        assert ((weights[rest].double().pow(norm_p).sum(1) - 1).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize('norm_p', [2, 130, 1000])
+def test_layers_with_norms_of_large_order(norm_p, monkeypatch):
+    """A dMoE's weights by either way: scores of about 1 / 512, of logits below 1, whose rounding to bf16 moves a score by 2^-9."""
+    layer, separate = make_layer(moe_num_experts=512, moe_top_k=4, ffn_hidden_size=128, moe_normalize_expert_weights=norm_p, moe_router_scale=2.0)
+    made = calls(monkeypatch)
+    with torch.no_grad():
+        for both in (layer, separate):
+            both.router.layer.weight *= 0.125
+        x = torch.randn(6, 1, 256, device='cuda').bfloat16()
+        got, want, alike = layer(x), separate(x), chosen_alike(separate, x)
+    assert len(made) == 1 and alike.any()
+    got, want = got.double().view(-1, 256)[alike], want.double().view(-1, 256)[alike]
+    assert want.norm() > 0 and (got - want).norm() <= 1e-2 * want.norm()
