@@ -273,9 +273,11 @@ class dMoE(moe.MoE):
     def _few_tokens(self, x: torch.Tensor):
         """Up to args.moe_fused_tokens tokens by ops.moe_layer, in evaluation and without gradients, where the layer, its router and its experts are the built-in ones and
         nobody looks at one of them by itself; else None."""
-        args, gate, experts = self.experts.args, self.router, self.experts
-        if args.moe_fused_tokens == 0 or torch.is_grad_enabled() or type(x) is not torch.Tensor or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or \
-                type(self) is not dMoE or type(gate) is not router.LearnedRouter or type(experts) is not ParallelDroplessMLP or \
+        gate, experts = self.router, self.experts
+        if torch.is_grad_enabled() or type(self) is not dMoE or type(gate) is not router.LearnedRouter or type(experts) is not ParallelDroplessMLP:      # others may have no arguments
+            return None
+        args = experts.args
+        if getattr(args, 'moe_fused_tokens', 0) == 0 or type(x) is not torch.Tensor or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or \
                 self.training or gate.training or experts.training:
             return None
         hidden = x.shape[-1]

@@ -7,6 +7,7 @@ import torch
 import megablocks_amd.ops as ops
 from megablocks_amd import _lib
 from megablocks_amd.layers.arguments import Arguments
+from megablocks_amd.layers.dmoe import dMoE
 from megablocks_amd.ops import few_tokens
 
 W = torch.zeros(4, 16, 8, dtype=torch.bfloat16)
@@ -70,3 +71,36 @@ def test_arguments_refuse_other_numbers_of_tokens(tokens):
 def test_a_launch_has_fewer_than_2_to_the_32_threads(sizes, taken):
     """256 of them for 16 rows of the weights of an expert that a token may choose."""
     assert few_tokens.takes(*sizes) == taken
+
+
+class Known(torch.nn.Module):
+    """A router's or experts' stand-in: no arguments, a result that tells it."""
+
+    def __init__(self, result):
+        super().__init__()
+        self.result = result
+
+    def forward(self, *given):
+        return self.result
+
+
+@pytest.mark.parametrize('recorded', [True, False])
+@pytest.mark.parametrize('tokens', [0, 16])
+def test_layers_whose_experts_have_no_arguments(tokens, recorded):
+    layer = dMoE(Arguments(device=torch.device('cpu'), hidden_size=16, ffn_hidden_size=32, moe_num_experts=4, moe_fused_tokens=tokens, mlp_impl='grouped', bf16=False, fp16=False))
+    layer.router, layer.experts = Known((None, None, torch.zeros(2, 1, dtype=torch.int64))), Known('experts')
+    with torch.set_grad_enabled(recorded):
+        for training in (True, False):
+            layer.train(training)
+            assert layer(torch.randn(2, 1, 16)) == 'experts'
+
+
+def test_arguments_without_a_number_of_fused_tokens():
+    class Few:
+        """Some other object that holds the layer's arguments."""
+    args = Arguments(device=torch.device('cpu'), hidden_size=16, ffn_hidden_size=32, moe_num_experts=4, mlp_impl='grouped', bf16=False, fp16=False)
+    layer = dMoE(args).eval()
+    layer.experts.args = Few()
+    layer.experts.args.__dict__.update({name: value for name, value in vars(args).items() if name != 'moe_fused_tokens'})
+    with torch.no_grad():
+        assert layer._few_tokens(torch.randn(2, 1, 16)) is None
