@@ -566,7 +566,8 @@ int mbx_balance_bias(const float* const* bias, const int32_t* const* counts, con
  * The forward without gradients of megablocks/layers/moe.py:457-475 with dropless experts, for decoding, by two products and the choice between them and the
  * router: x [tokens, hidden], router [num_experts, hidden], the choice as mbx_choose_experts makes it of x router^T (exact products, sums in 64 bits, rounded
  * nowhere), weights fp32 and indices int64 [tokens, top_k]; out[t] = sum over j of weights[t, j] (act(x[t] W1[e]^T) * (x[t] V1[e]^T)) W2[e] with e = indices[t, j], w1, v1
- * (NULL: no gate) and w2 [num_experts, ffn, hidden], fp32 sums, the activation kept to 2^-17 (fp16: 2^-23), out rounded once.  Up to 64 tokens, 512 experts, 16 a
+ * (NULL: no gate) and w2 [num_experts, ffn, hidden], fp32 sums, the activation kept to 2^-17 of it in bf16, in
+ * fp16 to 2^-23 of it or 2^-32 and up to 2^20 (infinite past that), out rounded once.  Up to 64 tokens, 512 experts, 16 a
  * token, 64 groups, bf16 or fp16, hidden and ffn multiples of 8, all matrices 16-byte aligned (else MBX_EUNSUPPORTED); matrices of an expert below 2 GiB, and fewer
  * than 2^24 pieces of 16 features of as many experts as there are choices (else MBX_ERANGE).  scratch: mbx_moe_layer_scratch_bytes bytes (gate: whether v1 is given; 0: such a call is refused, or has no tokens), 16-byte aligned.  workspace: 4096 bytes, zero before
  * the call and zero again after it, of no other call that may run at the same time (the head of mbx_gmm_ws's is such memory). */

@@ -7,8 +7,8 @@
 //
 //   choose   a wave per expert and token (or four tokens): logits as exact products summed in 64 bits, so that no order of summation decides between
 //            neighbours; the workgroup that is last at a group of tokens chooses for them
-//   hidden   a workgroup per used expert and 16 to 128 rows of its first weights, a quarter of the reduction a wave; the activation is kept as the sum of two
-//            16-bit numbers, so that the second product sees it to 2^-17
+//   hidden   a workgroup per used expert and 16 to 128 rows of its first weights, a quarter of the reduction a wave; the activation is kept as two 16-bit
+//            numbers, so that the second product sees it to 2^-17 (bf16) or 2^-23 (fp16, or to 2^-32, up to 2^20)
 //   down     a workgroup per used expert, 128 columns and a part of the reduction; the parts meet in memory, and the workgroup that is last at its columns adds them up
 //            in a fixed order, weights them and writes the output
 //
@@ -319,12 +319,15 @@ __device__ __forceinline__ float activated(float x, int act) {
   return x / (1.f + __builtin_amdgcn_exp2f(z));
 }
 
-// v as the sum of two 16-bit numbers
+// v as unit (hi + rest lo), two 16-bit numbers.  fp16 has no step below 2^-24 and nothing past 65504: what the first number leaves is kept times 2^11, which fits where
+// the first does, and both are sixteenths.  So v is kept to 2^-23 of it or 2^-32, up to 2^20.
+template <int DT> struct InTwo { static constexpr float unit = DT == MBX_F16 ? 16.f : 1.f, rest = DT == MBX_F16 ? 0x1p-11f : 1.f; };
 template <int DT>
 __device__ __forceinline__ void in_two(float v, uint16_t& hi, uint16_t& lo) {
   typedef typename Elem<DT>::type E;
+  v *= 1.f / InTwo<DT>::unit;
   const E h = Elem<DT>::from_f32(v);
-  const float rest = v - Elem<DT>::to_f32(h);
+  const float rest = (v - Elem<DT>::to_f32(h)) * (1.f / InTwo<DT>::rest);
   hi = __builtin_bit_cast(uint16_t, h);
   lo = __builtin_bit_cast(uint16_t, Elem<DT>::from_f32(rest - rest == 0.f ? rest : 0.f));     // an infinity or NaN has no rest
 }
@@ -502,7 +505,7 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
 // Second product: 128 columns, in chunks of 32 rows of W2.  Lane (c, g) reads columns 8 c .. 8 c + 7 of rows 8 g .. 8 g + 7, 16 bytes each (256 contiguous bytes a
 // row), and turns the 8 x 8 values over with byte permutes: fragment j has column 8 c + j of those rows.
 template <int DT, int R>
-__global__ void __launch_bounds__(kLayerThreads)
+__global__ void __launch_bounds__(kLayerThreads, R == 4 ? 1 : 2)
 layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict__ h_lo, const uint16_t* __restrict__ w2, const int32_t* __restrict__ choice, int tokens,
                   int top_k, int hidden, int ffn, int tiles, int parts, const float* __restrict__ weights, float* __restrict__ sums_of_parts, uint16_t* __restrict__ out,
                   int32_t* __restrict__ counters, bool by_xcd) {
@@ -561,7 +564,13 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
         for (int t = 0; t < R; ++t)
           if (t == 0 || t < row_tiles) {
             acc[t][j] = mfma<DT>(b, q.hi[t], acc[t][j]);
-            acc[t][j] = mfma<DT>(b, q.lo[t], acc[t][j]);
+            if constexpr (InTwo<DT>::rest == 1.f) {
+              acc[t][j] = mfma<DT>(b, q.lo[t], acc[t][j]);
+            } else {
+              const f32x4 rest = mfma<DT>(b, q.lo[t], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[t][j][i] = fmaf(rest[i], InTwo<DT>::rest, acc[t][j][i]);
+            }
           }
       }
     };
@@ -660,6 +669,8 @@ layer_down_kernel(const uint16_t* __restrict__ h_hi, const uint16_t* __restrict_
       }
     }
     if (t < tokens && mine) {
+      lo *= InTwo<DT>::unit;
+      hi *= InTwo<DT>::unit;
       const u32x4 v = {pack2<DT>(lo[0], lo[1]), pack2<DT>(lo[2], lo[3]), pack2<DT>(hi[0], hi[1]), pack2<DT>(hi[2], hi[3])};
       *(u32x4*)(out + (int64_t)t * hidden + n0 + col) = v;
     }

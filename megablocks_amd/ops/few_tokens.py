@@ -35,8 +35,9 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, w1: torch.Tensor, v1: Optio
         out[t]  = sum_j weights[t, j] (activation(x[t] @ w1[e]^T) * (x[t] @ v1[e]^T)) @ w2[e], e = indices[t, j]
 
     w1, v1 (None: no gate) and w2: [experts, ffn, hidden], contiguous, all of x's type, bf16 or fp16; hidden and ffn multiples of 8; up to 16 experts a token.  act: ACT_SILU or
-    ACT_GELU_TANH of `grouped_gemm_util`.  Logits are sums of exact products in 64 bits and are rounded nowhere, nor are weights and products on the way: out is
-    rounded once.  (A layer called as a module rounds each of them to its type, so the two agree to a few steps of that.)"""
+    ACT_GELU_TANH of `grouped_gemm_util`.  Logits are sums of exact products in 64 bits and are rounded nowhere, weights to fp32, products are fp32 sums,
+    and out is rounded once.  On the way the activation is kept to 2^-17 of it in bf16; in fp16 to 2^-23 of it or 2^-32, whichever is more, and it is infinite from
+    about 2^20 on, where the separate operators' is from 65520 on.  (A layer called as a module rounds each of them to its type, so the two agree to a few steps of that.)"""
     from megablocks_amd import grouped_gemm_util as gg
     norm_p, scale = float(norm_p or 0), float(scale)
     if x.ndim != 2 or router.ndim != 2 or w1.ndim != 3:

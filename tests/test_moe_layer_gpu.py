@@ -468,3 +468,63 @@ def test_layers_with_norms_of_large_order(norm_p, monkeypatch):
     assert len(made) == 1 and alike.any()
     got, want = got.double().view(-1, 256)[alike], want.double().view(-1, 256)[alike]
     assert want.norm() > 0 and (got - want).norm() <= 1e-2 * want.norm()
+
+
+# ---- fp16: the activation in two numbers that keep their bits whatever its size ----
+
+def exact_out_of_fp16(o, weights, indices):
+    """exact_out for fp16: the activation (silu) is kept to 2^-23 of it or 2^-32."""
+    x = o['x'].double()
+    hidden, ffn = x.shape[1], o['w1'].shape[1]
+    out, off = torch.zeros_like(x), torch.zeros_like(x)
+    largest = smallest = None
+    for e in indices.unique().tolist():
+        t, j = (indices == e).nonzero(as_tuple=True)
+        w1, w2 = o['w1'][e].double(), o['w2'][e].double()
+        p, dp = x[t] @ w1.t(), hidden * STEP * (x[t].abs() @ w1.abs().t())
+        a, da = F.silu(p), 1.13 * dp + 2.0 ** -20 * (F.silu(p).abs() + p.abs())
+        if o['v1'] is not None:
+            v1 = o['v1'][e].double()
+            q, dq = x[t] @ v1.t(), hidden * STEP * (x[t].abs() @ v1.abs().t())
+            a, da = a * q, da * (q.abs() + dq) + a.abs() * dq + a.abs() * q.abs() * STEP
+        da = da + 2.0 ** -23 * a.abs() + 2.0 ** -32
+        w = weights[t, j].unsqueeze(1)
+        out[t] += w * (a @ w2)
+        off[t] += w.abs() * (da @ w2.abs() + (ffn + indices.shape[1] + 20) * STEP * (a.abs() @ w2.abs()))
+        largest = max(largest or 0, a.abs().max().item())
+    return out, off, largest
+
+
+@pytest.mark.parametrize('gate', [True, False], ids=['gated', 'plain'])
+@pytest.mark.parametrize('tokens,experts', [(1, 4), (9, 4), (40, 3), (64, 2)])
+@pytest.mark.parametrize('size', [2.0 ** -18, 1e-5, 1e-4, 2.0 ** -12, 1e-2, 1.0, 1e3, 3e4], ids=lambda s: f'{s:.0e}')
+def test_fp16_activations_of_every_size(size, tokens, experts, gate):
+    """Activations of about `size`, past 65504 too, and second weights that bring the output to about 1: its own rounding is all there is."""
+    o = make(tokens, 128, 264, experts, gate, FP16, std=0.1)
+    # first weights that make the gate's product (or, plain, the activation) that small or large; silu(p) is p / 2 near 0 and p far from it
+    if gate:
+        o['v1'] = (o['v1'].float() * min(size * 2, 1e3)).half()
+        o['w1'] = (o['w1'].float() * max(1.0, size / 1e3)).half()
+    else:
+        o['w1'] = (o['w1'].float() * (size if size > 1 else 2 * size)).half()
+    o['w2'] = (o['w2'].float() / min(max(size, 2.0 ** -9), 1e3)).half()
+    if size > 1e3:
+        o['w2'] = (o['w2'].float() / (size / 1e3)).half()
+    out, weights, indices = ops.moe_layer(**o, top_k=2, act=gg.ACT_SILU, norm_p=1)
+    want_weights, _ = exact_choice(o, 2, norm_p=1)
+    want, off, largest = exact_out_of_fp16(o, want_weights, indices)
+    assert largest < 2.0 ** 20 and (size < 1e4 or largest > 65504)
+    error = (out.double() - want).abs()
+    half = want.abs().clamp(min=2.0 ** -14) * 2.0 ** -11      # half a step, also of the numbers below the normal ones
+    assert (error <= off + half).all()
+    assert error.norm() <= 1.01 * half.norm()
+
+
+def test_fp16_activations_past_what_two_numbers_hold_are_infinite():
+    o = make(1, 64, 8, 1, gate=False, dtype=FP16)
+    o['x'].fill_(0)
+    o['x'][0, 0], o['w1'][0], o['w2'][0] = 32768.0, 0.0, 0.0
+    o['w1'][0, 2, 0], o['w2'][0, 2, 5] = 31.0, 2.0 ** -8
+    assert ops.moe_layer(**o, top_k=1, act=gg.ACT_SILU)[0][0, 5].item() == 31.0 * 2 ** 15 / 2 ** 8       # 1015808, below 2^20
+    o['w1'][0, 2, 0] = 32.0
+    assert ops.moe_layer(**o, top_k=1, act=gg.ACT_SILU)[0][0, 5].item() == float('inf')
