@@ -682,6 +682,7 @@ struct LayerPlan {
   int entries;              // experts that can have a row
   double used, rows;        // that get one, and how many those get, where tokens choose evenly
   int fragments, hidden_tiles;
+  int row_tiles;            // of 16 rows of an expert that a workgroup has at a time: 1, 2, 4
   int down_tiles, parts;
   bool by_xcd;              // the second product's tiles of an expert's part on one XCD
   size_t choice, logits, h_hi, h_lo, sums, total = 0;
@@ -701,6 +702,7 @@ struct LayerPlan {
     rows = slots / used;
     fragments = rows >= 12 && workgroups(8) >= 256 ? 8 : hidden % 4096 == 0 && workgroups(4) >= 512 ? 4 : gate || workgroups(2) >= 512 ? 2 : 1;
     hidden_tiles = (int)ceil_div(ffn, fragments * columns);
+    row_tiles = rows < 12 && (tokens <= 16 || rows <= 8) ? 1 : tokens <= 32 || rows <= 20 ? 2 : 4;
     down_tiles = (int)ceil_div(hidden, kDownColumns);
     // Parts of the second product's reduction, as many as make a workgroup for most compute units, of two chunks a wave and more (us a layer by 1 / 2 / 4 / 8 of them:
     // 1 token, 2 of 8 experts of [14336, 4096], 64 workgroups a part, 209 / 177 / 162 / 164; 6 of 64 of [1408, 2048], 96, 43 / 39 / 41 / 45; 8 of 64 of [2048, 7168],
@@ -783,8 +785,8 @@ int launch_layer(const void* x, const void* router, const void* w1, const void* 
   if (q.experts <= 64) launch_choose<DT, 1>(x, router, q, bias, base, plan, weights, indices, counters, s);
   else if (q.experts <= 256) launch_choose<DT, 4>(x, router, q, bias, base, plan, weights, indices, counters, s);
   else launch_choose<DT, 8>(x, router, q, bias, base, plan, weights, indices, counters, s);
-  if (plan.rows < 12 && (q.tokens <= 16 || plan.rows <= 8)) launch_products<DT, 1>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
-  else if (q.tokens <= 32 || plan.rows <= 20) launch_products<DT, 2>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  if (plan.row_tiles == 1) launch_products<DT, 1>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
+  else if (plan.row_tiles == 2) launch_products<DT, 2>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
   else launch_products<DT, 4>(x, w1, v1, w2, q, ffn, act, base, plan, weights, out, counters, s);
   return launch_status();
 }
@@ -795,6 +797,17 @@ int launch_layer(const void* x, const void* router, const void* w1, const void* 
 using namespace mbx;
 
 extern "C" {
+
+// For tests: how such a layer is computed -- {fragments, row tiles, parts, by_xcd} of LayerPlan, or why it is not.
+int mbx_debug_moe_layer_plan(int64_t tokens, int64_t hidden, int64_t ffn, int num_experts, int top_k, int gate, int* of) {
+  if (const int rc = layer_sizes(tokens, hidden, ffn, num_experts, top_k)) return rc;
+  const LayerPlan plan((int)tokens, (int)hidden, (int)ffn, num_experts, top_k, gate != 0);
+  of[0] = plan.fragments;
+  of[1] = plan.row_tiles;
+  of[2] = plan.parts;
+  of[3] = plan.by_xcd;
+  return 0;
+}
 
 size_t mbx_moe_layer_scratch_bytes(int64_t tokens, int64_t hidden, int64_t ffn, int num_experts, int top_k, int gate) {
   if (layer_sizes(tokens, hidden, ffn, num_experts, top_k) || tokens == 0) return 0;

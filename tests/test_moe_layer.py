@@ -1,4 +1,5 @@
 """What the layer for a few tokens refuses, without a GPU."""
+import ctypes
 import math
 
 import pytest
@@ -104,3 +105,29 @@ def test_arguments_without_a_number_of_fused_tokens():
     layer.experts.args.__dict__.update({name: value for name, value in vars(args).items() if name != 'moe_fused_tokens'})
     with torch.no_grad():
         assert layer._few_tokens(torch.randn(2, 1, 16)) is None
+
+
+# Layers that are computed in every way there is, and end inside of tiles: (tokens, hidden, ffn, experts, top_k), gate -> weight fragments of a workgroup of the first product, row
+# tiles, parts of the second product's reduction, whether its tiles are neighbours on an XCD
+PLANS = [
+    ((64, 136, 2056, 8, 2), True, (8, 2, 8, 1)), ((64, 136, 4104, 8, 2), False, (8, 2, 16, 1)), ((48, 72, 8200, 2, 1), True, (8, 4, 16, 1)), ((48, 72, 16392, 2, 1), False, (8, 4, 16, 1)),
+    ((1, 4096, 8200, 3, 2), True, (4, 1, 4, 0)), ((1, 4096, 16392, 3, 2), False, (4, 1, 4, 0)), ((20, 4096, 4104, 4, 2), True, (4, 2, 2, 0)), ((20, 4096, 8200, 4, 2), False, (4, 2, 2, 0)),
+    ((1, 72, 4104, 8, 4), False, (2, 1, 16, 1)), ((64, 136, 2056, 8, 2), False, (2, 2, 8, 1)), ((48, 72, 8200, 2, 1), False, (2, 4, 16, 1)),
+    ((5, 1032, 1064, 60, 4), True, (2, 1, 2, 1)), ((17, 200, 520, 4, 2), True, (2, 2, 2, 0)), ((40, 200, 200, 2, 1), True, (2, 4, 1, 0)), ((33, 2056, 264, 64, 6), True, (2, 1, 1, 1)),
+    ((30, 1160, 40, 64, 16), True, (2, 1, 1, 1)), ((60, 1160, 40, 64, 16), True, (2, 2, 1, 1)), ((50, 1032, 40, 32, 16), True, (2, 4, 1, 1)),
+    ((2, 264, 200, 5, 2), False, (1, 1, 1, 0)), ((16, 264, 200, 5, 2), False, (1, 1, 1, 0)), ((30, 264, 200, 4, 2), False, (1, 2, 1, 0)), ((60, 264, 200, 3, 2), False, (1, 4, 1, 0))]
+
+
+def plan_of(sizes, gate):
+    plan = (ctypes.c_int * 4)()
+    assert _lib.lib.mbx_debug_moe_layer_plan(*map(ctypes.c_int64, sizes[:3]), *sizes[3:], gate, plan) == 0
+    return tuple(plan)
+
+
+def test_layers_are_computed_in_every_way_there_is():
+    for sizes, gate, plan in PLANS:
+        assert plan_of(sizes, gate) == plan, sizes
+    products = {(gate, *plan[:2]) for _, gate, plan in PLANS}
+    # eight fragments are for 12 rows an expert and more, four for fewer, one for layers without a gate
+    assert products == {(gate, n, r) for gate in (True, False) for n, r in ((8, 2), (8, 4), (4, 1), (4, 2), (2, 1), (2, 2), (2, 4))} | {(False, 1, r) for r in (1, 2, 4)}
+    assert {plan[1:] for _, _, plan in PLANS} >= {(r, 1, x) for r in (1, 2, 4) for x in (0, 1)} | {(1, 2, 1), (2, 8, 1), (4, 16, 1), (1, 4, 0), (2, 2, 0)}

@@ -19,6 +19,7 @@ from megablocks_amd import grouped_gemm_util as gg
 from megablocks_amd.layers.arguments import DEFAULT_ACTIVATION_FN, Arguments
 from megablocks_amd.layers.dmoe import dMoE
 from megablocks_amd.layers.moe import clear_load_balancing_loss
+from test_moe_layer import PLANS, plan_of
 
 pytestmark = pytest.mark.gpu
 
@@ -528,3 +529,18 @@ def test_fp16_activations_past_what_two_numbers_hold_are_infinite():
     assert ops.moe_layer(**o, top_k=1, act=gg.ACT_SILU)[0][0, 5].item() == 31.0 * 2 ** 15 / 2 ** 8       # 1015808, below 2^20
     o['w1'][0, 2, 0] = 32.0
     assert ops.moe_layer(**o, top_k=1, act=gg.ACT_SILU)[0][0, 5].item() == float('inf')
+
+
+# ---- every way in which the products are computed ----
+
+@pytest.mark.parametrize('dtype', [BF16, FP16], ids=str)
+@pytest.mark.parametrize('sizes,gate,plan', PLANS, ids=lambda v: '-'.join(map(str, v)) if isinstance(v, tuple) else 'gated' if v else 'plain')
+def test_every_way_of_the_products(sizes, gate, plan, dtype):
+    assert plan_of(sizes, gate) == plan
+    tokens, hidden, ffn, experts, top_k = sizes
+    o = make(tokens, hidden, ffn, experts, gate, dtype, std=min(0.1, 1.5 / hidden ** 0.5))
+    check(o, top_k, gg.ACT_SILU if gate else gg.ACT_GELU_TANH)
+    # all rows on the same experts: one or more rounds of row tiles, the last of which is not full
+    bias = torch.zeros(experts, device='cuda')
+    bias[-top_k:] = 9.0
+    check(o, top_k, gg.ACT_GELU_TANH if gate else gg.ACT_SILU, score='sigmoid', bias=bias, norm_p=1)
