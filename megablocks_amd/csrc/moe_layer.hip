@@ -481,7 +481,7 @@ layer_hidden_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__
       }
       __syncthreads();
       const int r = t * 16 + m;
-      if (r < rows && f0 + col < ffn) {      // ffn is a multiple of 8, a thread's columns 1, 2 or 4
+      if (r < rows && f0 + col < ffn) {      // ffn is a multiple of 8, a thread's columns 1, 2, 4 or 8
         uint16_t hi[kEach], lo[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -744,19 +744,22 @@ void launch_choose(const void* x_, const void* router_, const LayerChoice& q, co
   const uint16_t *const x = (const uint16_t*)x_, *const router = (const uint16_t*)router_;
   int32_t* const choice = (int32_t*)(base + plan.choice);
   // up to 128 KiB of router by one workgroup a token (us, that / four experts a workgroup: 1 token, 8 of 4096 5.2 / 7.4; 16, 64 of 1024 7.9 / 9.4; 1, 64 of 2048 10.5 / 6.4)
-  if ((int64_t)q.experts * ((q.hidden + 1023) & ~1023) <= 1 << 16) {
-    if (q.experts <= kWholeWaves) layer_choose_whole_kernel<DT, 1, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);
-    else layer_choose_whole_kernel<DT, 4, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);
-    return;
-  }
+  if constexpr (R == 1)      // up to 64 experts, as such a router has
+    if ((int64_t)q.experts * ((q.hidden + 1023) & ~1023) <= 1 << 16) {
+      if (q.experts <= kWholeWaves) layer_choose_whole_kernel<DT, 1, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);
+      else layer_choose_whole_kernel<DT, 4, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);
+      return;
+    }
   const unsigned workgroups = (unsigned)ceil_div(q.experts, kLayerWaves);
   // tokens one by one while there are few waves in all (us, one / two / four / eight of them a wave: 19 tokens, 256 experts of 1104 22 / 17 / 14 / 17, 64 tokens, 128 of
   // 4096 26 / 23 / 20 / 24)
   uint64_t* const logits = (uint64_t*)(base + plan.logits);
-  if (q.experts * q.tokens <= 4096)
-    layer_choose_kernel<DT, 1, R><<<dim3(workgroups, (unsigned)q.tokens), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, counters);
-  else
-    layer_choose_kernel<DT, 4, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 4)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, counters);
+  if constexpr (R > 1)      // 64 experts of 64 tokens are no more
+    if (q.experts * q.tokens > 4096) {
+      layer_choose_kernel<DT, 4, R><<<dim3(workgroups, (unsigned)ceil_div(q.tokens, 4)), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, counters);
+      return;
+    }
+  layer_choose_kernel<DT, 1, R><<<dim3(workgroups, (unsigned)q.tokens), kLayerThreads, 0, s>>>(x, router, q, bias, logits, choice, weights, indices, counters);
 }
 
 template <int DT, int R>
@@ -767,10 +770,11 @@ void launch_products(const void* x, const void* w1, const void* v1, const void* 
   const unsigned grid = (unsigned)(plan.entries * plan.hidden_tiles);
 #define MBX_LAYER_HIDDEN(GATE, NF) \
   layer_hidden_kernel<DT, GATE, NF, R><<<grid, kLayerThreads, 0, s>>>((const uint16_t*)x, (const uint16_t*)w1, (const uint16_t*)v1, choice, q.tokens, q.top_k, q.hidden, ffn, plan.hidden_tiles, act, hi, lo)
-  if constexpr (R > 1)      // for rows enough
+  if constexpr (R > 1)      // from 12 rows an expert on
     if (plan.fragments == 8) { if (v1) MBX_LAYER_HIDDEN(true, 8); else MBX_LAYER_HIDDEN(false, 8); }
-  if (plan.fragments == 4) { if (v1) MBX_LAYER_HIDDEN(true, 4); else MBX_LAYER_HIDDEN(false, 4); }
-  else if (plan.fragments == 2) { if (v1) MBX_LAYER_HIDDEN(true, 2); else MBX_LAYER_HIDDEN(false, 2); }
+  if constexpr (R < 4)      // below: where eight are too few workgroups, so are four
+    if (plan.fragments == 4) { if (v1) MBX_LAYER_HIDDEN(true, 4); else MBX_LAYER_HIDDEN(false, 4); }
+  if (plan.fragments == 2) { if (v1) MBX_LAYER_HIDDEN(true, 2); else MBX_LAYER_HIDDEN(false, 2); }
   else if (plan.fragments == 1) MBX_LAYER_HIDDEN(false, 1);
 #undef MBX_LAYER_HIDDEN
   const int64_t down = (int64_t)plan.entries * plan.down_tiles * plan.parts;
