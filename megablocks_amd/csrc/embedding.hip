@@ -2,9 +2,9 @@
 //
 //   out[i] = scale table[ids[i]]           dtable[v] = scale sum over {i : ids[i] = v} of dout[i], i ascending
 //
-// Both are bound by memory: the rows read and written once, for the gradient the whole table written, most of it zeros.  The gradient's sums are fp32 in a fixed
-// order: rows are added along the tokens sorted by word (stably), a piece of 32 of them by a wave, whose runs of one word go straight to the table; what a run of
-// more than 32 tokens leaves in each of its pieces is kept in fp32 and added up, in order, by a launch of its own.  So a word that is half of the text costs no more
+// Both are bound by memory: the rows read and written once, for the gradient the whole table written, most of it zeros.  The gradient's sums are fp32 (64 bits for
+// an fp32 table) in a fixed order: rows are added along the tokens sorted by word (stably), a piece of 32 of them by a wave, whose runs of one word go straight to the table; what a run of
+// more than 32 tokens leaves in each of its pieces is kept as it is and added up, in order, by a launch of its own.  So a word that is half of the text costs no more
 // than any other, and sums do not depend on timing.
 //
 // Measured (us): 32767 tokens, two fifths of them padding, 100000 words of 2040 in fp16: rows 52 (268 MB, 5.2 TB/s; a copy moves 4.8), gradient 12.8 sorting, 99 sums and
@@ -16,6 +16,8 @@
 // A token outside the table gives a row of zeros and no gradient.  Tensors may start anywhere and rows have any length: the memory unit takes 16-byte
 // accesses at any address.
 #include "common.h"
+
+#include <type_traits>
 
 namespace mbx {
 namespace {
@@ -64,6 +66,28 @@ __device__ __forceinline__ void store8(void* at, const float (&v)[kPer]) {
     *(u32x4_at2*)at = a;
   }
 }
+
+// What gradients are added up in: where the result has 24 bits, thousands of sums in 24 would be off by several of its last.  It is bound by memory either way (us a pass,
+// fp32 / 64 bits: 16384 tokens, 50000 words of 1024 101 / 101; 32767, two fifths of them padding, 49999 of 2040 231 / 240, of which 17 MB are the wider sums of cut runs).
+template <int DT> using Sum = std::conditional_t<DT == MBX_F32, double, float>;
+
+// N sums as they lie in memory
+template <int N, typename S>
+struct Sums {
+  typedef S vector __attribute__((ext_vector_type(16 / sizeof(S)), aligned(sizeof(S))));
+  static constexpr int kEach = 16 / sizeof(S);
+  vector part[N / kEach];
+
+  __device__ __forceinline__ void load(const S* at) {
+#pragma unroll
+    for (int i = 0; i < N / kEach; ++i) part[i] = *(const vector*)(at + i * kEach);
+  }
+  __device__ __forceinline__ void store(S* at) const {
+#pragma unroll
+    for (int i = 0; i < N / kEach; ++i) *(vector*)(at + i * kEach) = part[i];
+  }
+  __device__ __forceinline__ S value(int t) const { return part[t / kEach][t % kEach]; }
+};
 
 // up to kPer columns from `at`, of which `left` are the row's
 template <int DT>
@@ -280,7 +304,7 @@ constexpr int kPiece = 32, kWholeRun = kWave - kPiece;
 template <int DT>
 __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* __restrict__ grad, const int32_t* __restrict__ order, const int32_t* __restrict__ sorted,
                                                                     const int32_t* __restrict__ starts, int words, int hidden, int slices, int64_t piece_blocks,
-                                                                    float scale, float* __restrict__ heads, float* __restrict__ tails, EmbeddingRuns* __restrict__ crossing,
+                                                                    float scale, Sum<DT>* __restrict__ heads, Sum<DT>* __restrict__ tails, EmbeddingRuns* __restrict__ crossing,
                                                                     void* __restrict__ out, int64_t first_block) {
   typedef typename Elem<DT>::type E;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
@@ -319,15 +343,27 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* 
     crossing->runs[atomicAdd(&crossing->count, 1)] = make_int4((int)p, last_word, (int)((last_stop - 1) / kPiece - p + 1), 0);
   // whole: all kPer columns are the row's
   auto add_up = [&](auto whole) {
-    float acc[kPer] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    auto keep = [&](float* parts) { store_columns<MBX_F32>(parts + p * hidden + column, left, acc); };
+    Sum<DT> acc[kPer] = {};
+    auto keep = [&](Sum<DT>* parts) {
+      Sum<DT>* const at = parts + p * hidden + column;
+      if constexpr (decltype(whole)::value) {
+        Sums<kPer, Sum<DT>> v;
+#pragma unroll
+        for (int t = 0; t < kPer; ++t) v.part[t / v.kEach][t % v.kEach] = acc[t];
+        v.store(at);
+      } else {
+#pragma unroll
+        for (int t = 0; t < kPer; ++t)
+          if (t < left) at[t] = acc[t];
+      }
+    };
     auto finish = [&]() {     // the run of `word` ends here
       if (from_before) {
         keep(heads);
       } else {
         float v[kPer];
 #pragma unroll
-        for (int t = 0; t < kPer; ++t) v[t] = acc[t] * scale;
+        for (int t = 0; t < kPer; ++t) v[t] = (float)(acc[t] * scale);
         store_columns<DT>((E*)out + (int64_t)word * hidden + column, left, v);
       }
     };
@@ -348,7 +384,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* 
             word = here;
             from_before = false;
 #pragma unroll
-            for (int t = 0; t < kPer; ++t) acc[t] = 0.f;
+            for (int t = 0; t < kPer; ++t) acc[t] = 0;
           }
           if constexpr (decltype(whole)::value) {
 #pragma unroll
@@ -373,10 +409,10 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_sum_kernel(const void* 
 constexpr int kJoinColumns = kWave * 4, kJoinThreads = 512, kJoinWaves = kJoinThreads / kWave, kJoinRuns = 128;
 
 template <int DT>
-__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden, float scale, const float* __restrict__ heads, const float* __restrict__ tails,
+__global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden, float scale, const Sum<DT>* __restrict__ heads, const Sum<DT>* __restrict__ tails,
                                                                       const EmbeddingRuns* __restrict__ crossing, void* __restrict__ out) {
   typedef typename Elem<DT>::type E;
-  __shared__ float sums[kJoinWaves][kJoinColumns];
+  __shared__ Sum<DT> sums[kJoinWaves][kJoinColumns];
   const int wave = threadIdx.x / kWave, lane = lane_id(), column = (int)blockIdx.y * kJoinColumns + lane * 4;
   int4 it = crossing->runs[blockIdx.x];      // under way with the count: it may be none
   const int runs = crossing->count;
@@ -387,19 +423,19 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden
     // the waves take consecutive runs of the pieces' parts, and are added in order
     const int64_t share = (parts + kJoinWaves - 1) / kJoinWaves;
     const int64_t a = wave * share, b = a + share < parts ? a + share : parts;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    Sum<DT> acc[4] = {};
     auto row = [&](int64_t n) { return (n == 0 ? tails + p * hidden : heads + (p + n) * hidden) + column; };
     if (column + 4 <= hidden) {
       constexpr int kAhead = 8;
       for (int64_t i = a; i < b; i += kAhead) {
-        u32x4e v[kAhead];
+        Sums<4, Sum<DT>> v[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) v[u] = *(const u32x4_at4*)row(i + u < b ? i + u : b - 1);
+        for (int u = 0; u < kAhead; ++u) v[u].load(row(i + u < b ? i + u : b - 1));
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
           if (i + u < b)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[t] += __uint_as_float(v[u][t]);
+            for (int t = 0; t < 4; ++t) acc[t] += v[u].value(t);
       }
     } else {
       for (int64_t i = a; i < b; ++i)
@@ -412,10 +448,10 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden
     __syncthreads();
     const int c = (int)blockIdx.y * kJoinColumns + (int)threadIdx.x;
     if (threadIdx.x < kJoinColumns && c < hidden) {
-      float v = 0.f;
+      Sum<DT> v = 0;
 #pragma unroll
       for (int w = 0; w < kJoinWaves; ++w) v += sums[w][threadIdx.x];
-      ((E*)out)[(int64_t)word * hidden + c] = Elem<DT>::from_f32(v * scale);
+      ((E*)out)[(int64_t)word * hidden + c] = Elem<DT>::from_f32((float)(v * scale));
     }
     __syncthreads();      // the next run's sums
   }
@@ -458,7 +494,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_few_kernel(const void* 
   for (int unit = wave; unit < units; unit += kEmbWaves) {
     const int word = unit / my_slices, slice = first_slice + unit - word * my_slices, column = slice * kSlice + lane * kPer, left = hidden - column;
     const bool whole = hidden % kPer == 0 || (slice + 1) * kSlice <= hidden;      // every lane has eight columns or none
-    float acc[kPer] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    Sum<DT> acc[kPer] = {};
     bool any = false;
     for (int c = 0; c < n; c += kWave) {
       const int token = c + lane < n ? token_of[c + lane] : 0;
@@ -495,9 +531,10 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_few_kernel(const void* 
         }
       }
     }
+    float sums[kPer];
 #pragma unroll
-    for (int t = 0; t < kPer; ++t) acc[t] = any ? acc[t] * scale : 0.f;
-    if (left > 0) store_columns<DT>((E*)out + (first + word) * hidden + column, left, acc);
+    for (int t = 0; t < kPer; ++t) sums[t] = any ? (float)(acc[t] * scale) : 0.f;
+    if (left > 0) store_columns<DT>((E*)out + (first + word) * hidden + column, left, sums);
   }
 }
 
@@ -515,8 +552,8 @@ struct EmbeddingParts {
     order = take((size_t)tokens * 4);
     sorted = take((size_t)tokens * 4);
     starts = take((size_t)(words + 1) * 4);
-    heads = take((size_t)pieces * hidden * 4);
-    tails = take((size_t)pieces * hidden * 4);
+    heads = take((size_t)pieces * hidden * sizeof(Sum<MBX_F32>));      // enough for all types
+    tails = take((size_t)pieces * hidden * sizeof(Sum<MBX_F32>));
     crossing = take(sizeof(EmbeddingRuns) + sizeof(int4) * (size_t)(pieces > kJoinRuns ? pieces : kJoinRuns));
   }
 };
@@ -550,7 +587,7 @@ template <int DT>
 int launch_sums(const void* grad, int words, int hidden, float scale, const EmbeddingParts& parts, char* scratch, void* out, hipStream_t s) {
   const int32_t *const order = (const int32_t*)(scratch + parts.order), *const sorted = (const int32_t*)(scratch + parts.sorted);
   const int32_t* const starts = (const int32_t*)(scratch + parts.starts);
-  float *const heads = (float*)(scratch + parts.heads), *const tails = (float*)(scratch + parts.tails);
+  Sum<DT> *const heads = (Sum<DT>*)(scratch + parts.heads), *const tails = (Sum<DT>*)(scratch + parts.tails);
   EmbeddingRuns* const crossing = (EmbeddingRuns*)(scratch + parts.crossing);
   const int slices = (int)ceil_div(hidden, kSlice);
   const int64_t piece_blocks = ceil_div(parts.pieces * slices, kEmbWaves), zero_blocks = ceil_div(words, kEmbWaves * kZeroRows);

@@ -66,7 +66,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     """scale * table[ids], [*ids.shape, hidden], for int32 or int64 ids of any shape and a table [words, hidden] in bf16, fp16 or fp32, rounded once.  An id outside
     [0, words) gives a row of zeros.
 
-    The table's gradient is dense, its sums in fp32 in the order of the tokens, rounded once, the same from run to run; a row that no id names gets zeros, and so does
+    The table's gradient is dense, its sums in fp32 (of an fp32 table in 64 bits) in the order of the tokens, rounded once, the same from run to run; a row that no id names gets zeros, and so does
     that of padding_idx (from the end if negative), whose values are given out like any other's.  It is differentiable itself.  Forward and backward can be captured into a
     graph; as with all of torch's operations no eager graph of the same table may be alive then."""
     scale = float(scale)

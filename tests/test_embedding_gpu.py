@@ -276,3 +276,18 @@ def test_gradients_of_more_workgroups_than_a_launch_has_threads_for(tokens, word
     named = ids.unique()
     want, off = exact((ids.unsqueeze(1) == named).int().argmax(1) if tokens else ids, grad, len(named), 1.0)
     assert ((got[named].double() - want).abs() <= off).all()
+
+
+@pytest.mark.parametrize('kind', ['one', 'half', 'few', 'even', 'text'])
+@pytest.mark.parametrize('tokens,words,hidden', [(2, 3, 9), (100, 30, 1028), (256, 700, 264), (257, 9, 40), (9999, 300, 1030), (16384, 50000, 256), (40000, 5000, 16)])
+def test_fp32_gradients_are_rounded_once(tokens, words, hidden, kind):
+    """Sums in 64 bits, 2^-53 of the magnitudes a term, rounded to fp32 at the end: half a step of 2^-24, and what the 64 bits are off by."""
+    ids, table, grad = make(tokens, words, hidden, FP32, 'even' if kind == 'text' else kind)
+    if kind == 'text':       # the p-th most frequent word with a probability of about 1 / p
+        ids = (torch.rand(tokens, device='cuda', dtype=torch.float64) * math.log(words + 1)).exp().long().clamp(1, words) - 1
+    table.requires_grad_()
+    got, = torch.autograd.grad(ops.embedding(ids, table, 3.0), table, grad)
+    zeros = lambda: torch.zeros(words, hidden, dtype=torch.float64, device='cuda')
+    want, size = zeros().index_add_(0, ids, grad.double()) * 3.0, zeros().index_add_(0, ids, grad.double().abs()) * 3.0
+    terms = torch.bincount(ids, minlength=words).double().unsqueeze(1)
+    assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -24 + 2 * (terms + 2) * 2.0 ** -53 * size).all()
