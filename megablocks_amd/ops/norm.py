@@ -91,7 +91,7 @@ def clip_by_global_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=N
     if to.device != given.device:
         raise RuntimeError(f'{what}: tensors and outputs must be on one GPU')
     outputs = to.tensors
-    if to.plain is not outputs:
+    if to.plain is not outputs or given.plain is not tensors:      # of which the library sees others
         _refuse_overlaps(outputs, tensors)
     given.fill(torch.Tensor.contiguous)
     if to is not given:
@@ -114,19 +114,52 @@ def clip_by_global_norm_(tensors, max_norm: float, norm_type: float = 2.0, out=N
     return norm
 
 
+class _Place:
+    """Where a tensor's values lie: the bytes from begin to end, and (stride in bytes, size) of the dimensions that have more than one, by stride."""
+
+    def __init__(self, t):
+        self.item, self.begin = t.element_size(), t.data_ptr()
+        self.dims = sorted((stride * self.item, size) for stride, size in zip(t.stride(), t.shape) if size > 1)
+        self.end = self.begin + self.item + sum(stride * (size - 1) for stride, size in self.dims)
+        self.same = self.begin, self.dims, t.dtype
+
+    def over_itself(self):
+        """Whether two values may lie over each other: one step of a dimension is within what the narrower ones reach."""
+        reach = self.item
+        for stride, size in self.dims:
+            if stride < reach:
+                return True
+            reach += stride * (size - 1)
+        return False
+
+    def apart_from(self, other):
+        """Whether no value lies over one of the other's: the ranges of bytes do not meet, or all values of either are in a range of their own of every period."""
+        if self.end <= other.begin or other.end <= self.begin:
+            return True
+        for period in {stride for stride, _ in self.dims + other.dims if stride}:
+            mine, its = (p.item + sum(stride * (size - 1) for stride, size in p.dims if stride % period) for p in (self, other))
+            if (other.begin - self.begin) % period >= mine and (self.begin - other.begin) % period >= its:
+                return True
+        return False
+
+
 def _refuse_overlaps(outputs, tensors):
-    """The library's check of its operands, on the tensors that some of these stand for: by the memory between their first and last values."""
-    def extent(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    ranges = sorted((*extent(o), i) for i, o in enumerate(outputs) if o.numel())
-    clash = any(a[1] > b[0] for a, b in zip(ranges, ranges[1:]))
+    """The library's check of its operands, on tensors of any strides.  Layouts that no program makes of slices, steps and transposes of a tensor may be refused too."""
+    outs = [_Place(o) if o.numel() else None for o in outputs]
+    places = [(p.begin, p, i, True) for i, p in enumerate(outs) if p is not None]
     for i, t in enumerate(tensors):
-        if t.numel() and t is not outputs[i]:
-            begin, end = extent(t)
-            clash = clash or any(a < end and begin < b for a, b, _ in ranges)
-    if clash or any(0 in o.stride() and o.numel() > 1 for o in outputs):
-        raise ValueError('clip_by_global_norm_: an output that is not contiguous lies over another one, over a tensor that is not its own, or over itself')
+        if t is not outputs[i] and t.numel():
+            p = _Place(t)
+            if p.same != outs[i].same:
+                places.append((p.begin, p, i, False))
+    clash = any(p.over_itself() for p in outs if p is not None)
+    near = []      # those that reach past where the next one begins
+    for begin, p, _, writes in sorted(places, key=operator.itemgetter(0)):
+        near = [n for n in near if n[0].end > begin]
+        clash = clash or any((writes or n_writes) and not p.apart_from(n) for n, n_writes in near)
+        near.append((p, writes))
+    if clash:
+        raise ValueError('clip_by_global_norm_: an output lies over another one, over a tensor that is not its own, or over itself')
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:

@@ -73,3 +73,65 @@ def test_entry_points_refuse_without_touching_the_gpu():
     assert lib.mbx_global_norm_scratch_bytes(0) == 0
     sizes = [lib.mbx_global_norm_scratch_bytes(n) for n in (1, 128, 129, 1000)]
     assert sizes == sorted(sizes) and sizes[0] >= 2048 * 8
+
+
+def _views():
+    g = torch.zeros(64, 96)
+    cube = torch.zeros(4, 6, 10)
+    line = torch.zeros(100)
+    return [
+        # apart
+        ([g[:, :48], g[:, 48:]], None, True),                                  # column halves
+        ([g[:, ::2], g[:, 1::2]], None, True),                                 # every other column
+        ([g.t()[:, ::2], g.t()[:, 1::2]], None, True),                         # every other row, transposed
+        ([g[::2, ::2], g[1::2], g[::2, 1::2]], None, True),
+        ([cube[:, :3], cube[:, 3:, :5], cube[:, 3:, 5:]], None, True),
+        ([cube[..., i] for i in range(10)], None, True),
+        ([line[::3], line[1::3], line[2::3]], None, True),
+        ([line.as_strided((1, 5), (0, 2))], None, True),                       # one row: its step does not count
+        ([line[:0], line[::2]], None, True),
+        ([g[:, :48], g[:, 48:]], [line[:50].expand(64, 50)[:, :48].contiguous(), torch.zeros(64, 48)], True),
+        ([line[::2]], [line[1::2]], True),                                     # between the values of its tensor
+        ([line[::2]], [line[::2]], True),                                      # another view of the same values
+        ([line[:50].expand(2, 50)], [torch.zeros(50, 2).t()], True),           # a tensor that repeats itself is only read
+        # over each other, or itself
+        ([g[:, :49], g[:, 48:]], None, False),
+        ([g[:, ::2], g[:, ::3]], None, False),
+        ([g[:, ::2], g[5]], None, False),
+        ([line.as_strided((4, 3), (2, 1))], None, False),
+        ([line[:50:2].expand(2, 25)], None, False),
+        ([g[:, :48], g[:, 48:]], [g[:, 48:], g[:, :48]], False),               # over each other's
+        ([line[::2]], [line[:50]], False),                                     # a contiguous output over its strided tensor
+        ([torch.zeros(50), line[::2]], [line[20:70], torch.zeros(50)], False),   # over another's
+        ([torch.zeros(25, 2).t()], [line.as_strided((2, 25), (1, 1))], False),
+        ([g[:, :48].bfloat16()[:, ::2], g[:, :24]], [g.view(torch.bfloat16)[:, 48:96:2], torch.zeros(64, 24)], True),
+        ([g[:, :48].bfloat16()[:, ::2], g[:, :24]], [g.view(torch.bfloat16)[:, 46:94:2], torch.zeros(64, 24)], False)]
+
+
+@pytest.mark.parametrize('case', range(len(_views())))
+def test_which_views_lie_over_each_other(case):
+    from megablocks_amd.ops import norm
+    tensors, out, apart = _views()[case]
+    tensors = [t for t in tensors]
+    if apart:
+        norm._refuse_overlaps(tensors if out is None else out, tensors)
+    else:
+        with pytest.raises(ValueError):
+            norm._refuse_overlaps(tensors if out is None else out, tensors)
+
+
+def test_views_of_a_buffer_that_are_apart_are_shown_to_be():
+    """Every pair of slices with steps of a small matrix: what is said to be apart has no value in common, and little that has none is refused."""
+    from megablocks_amd.ops import norm
+    m = torch.arange(6 * 8, dtype=torch.float32).view(6, 8)
+    views = [m[a:b:s, c:d:u] for a, b, s in ((0, 6, 1), (0, 3, 1), (3, 6, 1), (0, 6, 2), (1, 6, 2), (2, 3, 1)) for c, d, u in ((0, 8, 1), (0, 4, 1), (4, 8, 1), (3, 6, 1), (0, 8, 2), (1, 8, 2), (5, 6, 1))]
+    views += [v.t() for v in views]
+    refused = 0
+    for x in views:
+        for y in views:
+            apart = not set(x.flatten().tolist()) & set(y.flatten().tolist())
+            said = norm._Place(x).apart_from(norm._Place(y))
+            assert apart or not said
+            refused += apart and not said
+        assert not norm._Place(x).over_itself()
+    assert refused == 0

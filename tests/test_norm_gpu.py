@@ -217,3 +217,31 @@ def test_captured_and_replayed():
         check_norm(norm, exact_norm(tensors, 2.0))
         check_clipped(outs, tensors, 1.0, exact_norm(tensors, 2.0))
         assert ops.global_norm(tensors).item() == norm.item()
+
+
+def test_gradients_that_are_slices_of_one_buffer():
+    """As torch clips them: parts of a matrix's columns, every other row, and one that is contiguous."""
+    params = [torch.nn.Parameter(torch.zeros(64, 48, device='cuda')) for _ in range(2)] + [torch.nn.Parameter(torch.zeros(8, 30, device='cuda')) for _ in range(2)]
+    params.append(torch.nn.Parameter(torch.zeros(1000, device='cuda')))
+    columns, rows = torch.randn(64, 97, device='cuda'), torch.randn(16, 30, device='cuda')
+    grads = [columns[:, :48], columns[:, 49:], rows[::2], rows[1::2], torch.randn(1000, device='cuda')]
+    before, between = [g.clone() for g in grads], columns[:, 48].clone()
+    for p, g in zip(params, grads):
+        p.grad = g
+    norm = exact_norm(grads, 2.0)
+    check_norm(ops.clip_grad_norm_(params, 2.0), norm)
+    check_clipped(grads, before, 2.0, norm)
+    assert torch.equal(columns[:, 48], between) and all(p.grad is g for p, g in zip(params, grads))
+    for p, b in zip(params, before):
+        p.grad = b.clone()
+    torch.nn.utils.clip_grad_norm_(params, 2.0)
+    for p, g in zip(params, grads):
+        torch.testing.assert_close(g, p.grad, rtol=2e-6, atol=0)
+
+
+def test_outputs_over_strided_tensors_are_refused_before_anything_is_written():
+    line = torch.ones(100, device='cuda')
+    for tensors, out in (([line[::2]], [line[:50]]), ([torch.ones(50, device='cuda'), line[::2]], [line[20:70], torch.ones(50, device='cuda')]), ([line.as_strided((4, 3), (2, 1))], None)):
+        with pytest.raises(ValueError):
+            ops.clip_by_global_norm_(tensors, 0.1, out=out)
+    assert (line == 1).all()
