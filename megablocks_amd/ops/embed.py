@@ -6,6 +6,7 @@ import torch
 
 from megablocks_amd import _lib
 from megablocks_amd._lib import lib
+from megablocks_amd.ops.choose import _has_memory
 
 
 def _rows(ids, table, scale):
@@ -28,6 +29,25 @@ def _table_gradient(grad, ids, words, scale, padding):
     return out
 
 
+def _plain_rows(ids, table, scale):
+    """_rows in torch's operations, of a batch of tables (is_grads_batched), which has no memory of its own."""
+    words = table.shape[0]
+    if words == 0:
+        return table.new_zeros((*ids.shape, table.shape[1]))
+    inside = (ids >= 0) & (ids < words)
+    rows = table.index_select(0, torch.where(inside, ids, 0).long().flatten()).double() * scale
+    return rows.masked_fill(~inside.flatten().unsqueeze(1), 0.).to(table.dtype).reshape(*ids.shape, table.shape[1])
+
+
+def _plain_table_gradient(grad, ids, words, scale, padding):
+    """_table_gradient in torch's operations, of a batch of gradients: sums in 64 bits, the same from run to run."""
+    ids, hidden = ids.flatten().long(), grad.shape[-1]
+    counts = (ids >= 0) & (ids < words) & (ids != padding)
+    zeros = torch.zeros((words + 1, hidden), dtype=torch.float64, device=ids.device)       # the last row: tokens that do not count
+    sums = zeros.index_put((torch.where(counts, ids, words),), grad.reshape(len(ids), hidden).double(), accumulate=True)
+    return (sums.narrow(0, 0, words) * scale).to(grad.dtype)
+
+
 class EmbeddingOp(torch.autograd.Function):
 
     @staticmethod
@@ -39,8 +59,8 @@ class EmbeddingOp(torch.autograd.Function):
     @staticmethod
     def backward(ctx: Any, grad):
         ids, = ctx.saved_tensors
-        # a node of its own only where the backward is differentiated itself
-        gradient = EmbeddingGradientOp.apply if torch.is_grad_enabled() else _table_gradient
+        # a node of its own only where the backward is differentiated itself; a batch of gradients at once (is_grads_batched) by torch
+        gradient = _plain_table_gradient if not _has_memory(grad) else EmbeddingGradientOp.apply if torch.is_grad_enabled() else _table_gradient
         return None, gradient(grad, ids, *ctx.sizes), None, None
 
 
@@ -59,7 +79,8 @@ class EmbeddingGradientOp(torch.autograd.Function):
         scale, padding = ctx.choice
         if padding >= 0:
             ids = ids.masked_fill(ids == padding, -1)      # rows of zeros
-        return EmbeddingOp.apply(ids, grad.contiguous(), scale, -1), None, None, None, None
+        rows = EmbeddingOp.apply(ids, grad.contiguous(), scale, -1) if _has_memory(grad) else _plain_rows(ids, grad, scale)
+        return rows, None, None, None, None
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
@@ -67,7 +88,8 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     [0, words) gives a row of zeros.
 
     The table's gradient is dense, its sums in fp32 (of an fp32 table in 64 bits) in the order of the tokens, rounded once, the same from run to run; a row that no id names gets zeros, and so does
-    that of padding_idx (from the end if negative), whose values are given out like any other's.  It is differentiable itself.  Forward and backward can be captured into a
+    that of padding_idx (from the end if negative), whose values are given out like any other's.  It is differentiable itself;
+    several gradients at once (is_grads_batched) are computed by torch's operations.  Forward and backward can be captured into a
     graph; as with all of torch's operations no eager graph of the same table may be alive then."""
     scale = float(scale)
     if table.ndim != 2:

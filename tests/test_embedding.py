@@ -40,3 +40,25 @@ def test_entry_points_refuse_without_touching_the_gpu():
     many, nbytes = dict(tokens=257), lib.mbx_embedding_gradient_scratch_bytes(257, 5, 8)      # fewer tokens need none
     assert gradient(**many) == _lib.ESCRATCH and gradient(**many, scratch=16, nbytes=nbytes - 1) == _lib.ESCRATCH and gradient(**many, scratch=8, nbytes=nbytes) == _lib.ESCRATCH
     assert lib.mbx_embedding_gradient_scratch_bytes(-1, 5, 8) == 0 and lib.mbx_embedding_gradient_scratch_bytes(256, 5, 8) == 0 and nbytes > 0
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize('padding', [-1, 2])
+def test_batches_of_gradients_in_plain_operations(padding, dtype):
+    """What a backward of several gradients at once computes, one gradient after the other: whole numbers, of which sums are exact."""
+    from torch._vmap_internals import _vmap
+
+    from megablocks_amd.ops import embed
+    ids = torch.tensor([[1, 3, 3], [0, 2, -1], [5, 1, 2 ** 31 - 1]], dtype=torch.int32)
+    grads, tables = torch.randint(-9, 10, (4, 3, 3, 8)).to(dtype), torch.randint(-9, 10, (4, 5, 8)).to(dtype)
+    want = torch.zeros(4, 5, 8)
+    for b in range(4):
+        for i, word in enumerate(ids.flatten().tolist()):
+            if 0 <= word < 5 and word != padding:
+                want[b, word] += 2 * grads[b].view(9, 8)[i].float()
+    got = _vmap(lambda g: embed._plain_table_gradient(g, ids, 5, 2.0, padding))(grads)
+    assert got.dtype == dtype and torch.equal(got.float(), want)
+    rows = _vmap(lambda t: embed._plain_rows(ids, t, 2.0))(tables)
+    inside = (ids >= 0) & (ids < 5)
+    assert rows.dtype == dtype and torch.equal(rows[:, inside], 2 * tables[:, ids[inside].long()]) and (rows[:, ~inside] == 0).all()
+    assert embed._plain_rows(ids, tables[0, :0], 2.0).shape == (3, 3, 8) and embed._plain_table_gradient(grads[0], ids, 0, 2.0, -1).shape == (0, 8)

@@ -291,3 +291,27 @@ def test_fp32_gradients_are_rounded_once(tokens, words, hidden, kind):
     want, size = zeros().index_add_(0, ids, grad.double()) * 3.0, zeros().index_add_(0, ids, grad.double().abs()) * 3.0
     terms = torch.bincount(ids, minlength=words).double().unsqueeze(1)
     assert ((got.double() - want).abs() <= want.abs() * 2.0 ** -24 + 2 * (terms + 2) * 2.0 ** -53 * size).all()
+
+
+@pytest.mark.parametrize('tokens', [40, 3000])
+def test_several_gradients_at_once(tokens):
+    ids, table, _ = make(tokens, 50, 24, FP32, 'half')
+    ids[5] = -1
+    table.requires_grad_()
+    out = ops.embedding(ids, table, 1.5, padding_idx=3)
+    grads = torch.randn(3, tokens, 24, device='cuda')
+    got, = torch.autograd.grad(out, table, grads, is_grads_batched=True, retain_graph=True)
+    want = torch.stack([torch.autograd.grad(out, table, g, retain_graph=True)[0] for g in grads])
+    torch.testing.assert_close(got, want, rtol=2.0 ** -23, atol=1e-12)        # either is the sum in 64 bits, rounded once
+    # a gradient's gradient, of several vectors at once: rows of the vectors by token, added up by word again
+    first, = torch.autograd.grad((ops.embedding(ids, table, 1.5, padding_idx=3) ** 2).sum(), table, create_graph=True)
+    vectors = torch.randn(2, 50, 24, device='cuda')
+    got, = torch.autograd.grad(first, table, vectors, is_grads_batched=True, retain_graph=True)
+    want = torch.stack([torch.autograd.grad(first, table, v, retain_graph=True)[0] for v in vectors])
+    torch.testing.assert_close(got, want, rtol=2.0 ** -21, atol=1e-12)
+    # and the gradients of several gradients themselves
+    weights = torch.randn(tokens, 24, device='cuda', requires_grad=True)
+    both, = torch.autograd.grad(ops.embedding(ids, table, 1.5, padding_idx=3), table, torch.stack([weights, 2 * weights]), is_grads_batched=True, create_graph=True)
+    got, = torch.autograd.grad(both.sum(), weights)
+    counts = (ids >= 0) & (ids != 3)
+    torch.testing.assert_close(got, 4.5 * counts.unsqueeze(1).float().expand(tokens, 24), rtol=0, atol=0)
