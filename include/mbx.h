@@ -578,7 +578,7 @@ int mbx_moe_layer(const void* x, int64_t tokens, int64_t hidden, int dtype, cons
 
 /* ---- rows of a table by token ----
  * No counterpart in the reference.  out[i] = scale * table[ids[i]], in fp32, rounded once: table [words, hidden] of `dtype`, ids [tokens] (MBX_I32 or
- * MBX_I64), out [tokens, hidden]; an id outside [0, words) gives zeros.  All contiguous, at any address their types may have.
+ * MBX_I64), out [tokens, hidden]; an id outside [0, words) gives zeros.  All contiguous, at any address their types may have; scale finite.
  * mbx_embedding_gradient: out[v] = scale * (the sum of grad[i] over ids[i] = v, i ascending, in fp32, for MBX_F32 in 64 bits), rounded once, for all words; zeros for the word `padding`
  * (negative: none) and those no id names.  The order of a sum depends on the ids alone.  scratch: mbx_embedding_gradient_scratch_bytes bytes (none, and NULL, for up to 256 tokens),
  * 16-byte aligned.  MBX_ERANGE: 2^31 - 256 tokens, 2^31 - 1 words or 2^24 columns and more. */

@@ -17,6 +17,7 @@
 // accesses at any address.
 #include "common.h"
 
+#include <cmath>
 #include <type_traits>
 
 namespace mbx {
@@ -627,7 +628,7 @@ using namespace mbx;
 extern "C" {
 
 int mbx_embedding(const void* ids, int itype, int64_t tokens, const void* table, int dtype, int64_t words, int64_t hidden, float scale, void* out, mbx_stream_t stream) {
-  if (!embedding_sizes_ok(tokens, words, hidden) || (itype != MBX_I32 && itype != MBX_I64) || dtype < MBX_BF16 || dtype > MBX_F32) return MBX_EINVAL;
+  if (!embedding_sizes_ok(tokens, words, hidden) || (itype != MBX_I32 && itype != MBX_I64) || dtype < MBX_BF16 || dtype > MBX_F32 || !std::isfinite(scale)) return MBX_EINVAL;
   if (!embedding_in_range(tokens, words, hidden)) return MBX_ERANGE;
   if (tokens == 0 || hidden == 0) return 0;
   if (!ids || !out || (words > 0 && !table)) return MBX_EINVAL;
@@ -645,7 +646,7 @@ size_t mbx_embedding_gradient_scratch_bytes(int64_t tokens, int64_t words, int64
 
 int mbx_embedding_gradient(const void* grad, const void* ids, int itype, int64_t tokens, int dtype, int64_t words, int64_t hidden, int64_t padding, float scale,
                            void* out, void* scratch, size_t scratch_bytes, mbx_stream_t stream) {
-  if (!embedding_sizes_ok(tokens, words, hidden) || (itype != MBX_I32 && itype != MBX_I64) || dtype < MBX_BF16 || dtype > MBX_F32) return MBX_EINVAL;
+  if (!embedding_sizes_ok(tokens, words, hidden) || (itype != MBX_I32 && itype != MBX_I64) || dtype < MBX_BF16 || dtype > MBX_F32 || !std::isfinite(scale)) return MBX_EINVAL;
   if (!embedding_in_range(tokens, words, hidden)) return MBX_ERANGE;
   if (words == 0 || hidden == 0) return 0;
   if (!out || (tokens > 0 && (!ids || !grad))) return MBX_EINVAL;

@@ -1,5 +1,4 @@
 """Rows of a table by token, and the table's gradient by sorted tokens.  The reference has neither: its models' embedding is the trainer's."""
-import math
 from typing import Any, Optional
 
 import torch
@@ -94,8 +93,8 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0, paddin
     scale = float(scale)
     if table.ndim != 2:
         raise ValueError('embedding: the table must be [words, hidden]')
-    if not math.isfinite(scale):
-        raise ValueError('embedding: the scale must be finite')
+    if not abs(scale) <= torch.finfo(torch.float32).max:
+        raise ValueError('embedding: the scale must be finite, in fp32')
     words = table.shape[0]
     padding = -1
     if padding_idx is not None:

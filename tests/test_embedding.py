@@ -62,3 +62,12 @@ def test_batches_of_gradients_in_plain_operations(padding, dtype):
     inside = (ids >= 0) & (ids < 5)
     assert rows.dtype == dtype and torch.equal(rows[:, inside], 2 * tables[:, ids[inside].long()]) and (rows[:, ~inside] == 0).all()
     assert embed._plain_rows(ids, tables[0, :0], 2.0).shape == (3, 3, 8) and embed._plain_table_gradient(grads[0], ids, 0, 2.0, -1).shape == (0, 8)
+
+
+@pytest.mark.parametrize('scale', [1e39, -1e300, math.inf, -math.inf, math.nan])
+def test_scales_that_are_not_finite_in_fp32(scale):
+    """1e39 is a number as Python has it, and infinite as the library gets it: 0 times it would be none."""
+    with pytest.raises(ValueError):
+        ops.embedding(IDS, TABLE, scale)
+    assert _lib.lib.mbx_embedding(16, 2, 3, 16, 0, 5, 8, scale, 16, None) == _lib.EINVAL
+    assert _lib.lib.mbx_embedding_gradient(16, 16, 2, 3, 0, 5, 8, -1, scale, 16, None, 0, None) == _lib.EINVAL
