@@ -4,8 +4,6 @@
     sparse:   the same over 128-padded expert groups, with the block-diagonal topology
               metadata the reference builds for stk
 """
-import math
-
 import numpy as np
 import torch
 
@@ -297,9 +295,9 @@ class dMoE(moe.MoE):
                for w in (weight, w1, v1, w2) if w is not None) or weight.shape != (num_experts, hidden) or \
                 any(w.numel() != num_experts * ffn * hidden for w in (w1, v1, w2) if w is not None) or not few_tokens.takes(tokens, hidden, ffn, num_experts, top_k):
             return None
-        # a router without options of its own (`_chooses`) goes by the softmax and the norm alone, whatever the others say; a norm that is no finite one is the separate operators'
+        # a router without options of its own (`_chooses`) goes by the softmax and the norm alone, whatever the others say; a norm that is not finite in fp32 is the separate operators'
         norm_p, bias = float(gate.args.moe_normalize_expert_weights or 0), gate.balance_bias if gate._chooses else None
-        if not 0 <= norm_p < math.inf or (bias is not None and (bias.dtype != torch.float32 or bias.device != x.device)):
+        if not 0 <= norm_p <= torch.finfo(torch.float32).max or (bias is not None and (bias.dtype != torch.float32 or bias.device != x.device)):
             return None
         choice = (gate.args.moe_router_score, bias, gate.args.moe_router_groups, gate.args.moe_router_top_groups, gate.args.moe_router_group_best, norm_p,
                   float(gate.args.moe_router_scale)) if gate._chooses else ('softmax', None, 1, 1, 2, norm_p, 1.0)

@@ -544,3 +544,13 @@ def test_every_way_of_the_products(sizes, gate, plan, dtype):
     bias = torch.zeros(experts, device='cuda')
     bias[-top_k:] = 9.0
     check(o, top_k, gg.ACT_GELU_TANH if gate else gg.ACT_SILU, score='sigmoid', bias=bias, norm_p=1)
+
+
+def test_layers_with_norms_that_are_infinite_in_fp32(monkeypatch):
+    """An order of 1e39 is a number to the separate operators, and none to the one for a few tokens."""
+    layer, separate = make_layer(moe_normalize_expert_weights=1e39)
+    made = calls(monkeypatch)
+    x = torch.randn(3, 1, 256, device='cuda').bfloat16()
+    with torch.no_grad():
+        got, want = layer(x), separate(x)
+    assert not made and torch.equal(got, want)
