@@ -694,13 +694,17 @@ struct LayerPlan {
     // Fragments of 16 weight rows a workgroup (half of them W1's, half V1's with a gate; us a layer by 2 / 4 / 8 of them).  From 12 rows an expert on the rows
     // are read again by so many workgroups that eight pay: 64 tokens, 2 of 8 experts of [14336, 4096] 608 / 565 / 544, of [8192, 5120] 462 / 458 / 436, but
     // 4 experts of [1024, 1024], which leave most compute units without a workgroup, 28 / 30 / 34.  Below, two: 1 token, 6 of 64 of [1408, 2048] 41 / 47 / 46, 2 of 8
-    // of [12288, 5120] 164 / 183 / 198, 16 tokens, 6 of 64 of [1408, 2048] 179 / 186 / 192; but rows that are a multiple of 8 KiB apart come faster in
-    // fours: 1 token, 2 of 8 of [14336, 4096] 180 / 166 / 169, of [8192, 4096] 105 / 100 / 104, where there are workgroups enough: of [2048, 4096] 38 / 43 / 60.  One without a gate,
+    // of [12288, 5120] 164 / 183 / 198, 16 tokens, 6 of 64 of [1408, 2048] 179 / 186 / 192.  But rows that are 8 KiB apart come faster in
+    // fours: 1 token, 2 of 8 of [14336, 4096] 180 / 166 / 169, of [8192, 4096] 92 / 85, 8 tokens, 4 of 32 of [2048, 4096] 217 / 204, where there are workgroups enough: 1 token, 2 of 8 of
+    // [2048, 4096] 38 / 43 / 60.  With a gate no others do (those two with rows of 4160 92 / 98 and 203 / 226, of 8192 153 / 167 and 401 / 397 (8 tokens, 2 of 16 of [4096, 8192] 363 / 413), of 12288 225 / 234 and 577 / 633, of 16384
+    // 288 / 284 and 781 / 786); without one the larger powers of two do somewhat (1 token, 2 of 4 of [16384, h], 8 tokens, 4 of 32 of [4096, h]: 4096 105 / 103 and 257 / 261, 8192
+    // 206 / 201 and 535 / 503, 12288 296 / 295 and 769 / 800, 16384 374 / 364 and 1012 / 1032).  One without a gate,
     // for a few small experts: 1 token, top-1 of 4 of [2048, 512] 14.7 instead of 15.2.
     const int columns = gate ? 8 : 16;
     const auto workgroups = [&](int n) { return used * ceil_div(ffn, n * columns); };
     rows = slots / used;
-    fragments = rows >= 12 && workgroups(8) >= 256 ? 8 : hidden % 4096 == 0 && workgroups(4) >= 512 ? 4 : gate || workgroups(2) >= 512 ? 2 : 1;
+    const bool in_fours = gate ? hidden == 4096 : hidden >= 4096 && (hidden & (hidden - 1)) == 0;
+    fragments = rows >= 12 && workgroups(8) >= 256 ? 8 : in_fours && workgroups(4) >= 512 ? 4 : gate || workgroups(2) >= 512 ? 2 : 1;
     hidden_tiles = (int)ceil_div(ffn, fragments * columns);
     row_tiles = rows < 12 && (tokens <= 16 || rows <= 8) ? 1 : tokens <= 32 || rows <= 20 ? 2 : 4;
     down_tiles = (int)ceil_div(hidden, kDownColumns);
@@ -743,7 +747,9 @@ void launch_choose(const void* x_, const void* router_, const LayerChoice& q, co
                    int32_t* counters, hipStream_t s) {
   const uint16_t *const x = (const uint16_t*)x_, *const router = (const uint16_t*)router_;
   int32_t* const choice = (int32_t*)(base + plan.choice);
-  // up to 128 KiB of router by one workgroup a token (us, that / four experts a workgroup: 1 token, 8 of 4096 5.2 / 7.4; 16, 64 of 1024 7.9 / 9.4; 1, 64 of 2048 10.5 / 6.4)
+  // up to 128 KiB of router by one workgroup a token (us, that / four experts a workgroup: 1 token, 8 of 4096 5.2 / 7.4; 16, 64 of 1024 7.9 / 9.4; 1, 64 of 2048 10.5 / 6.4; small
+  // layers of 1, 16 and 64 tokens at that border, 64 of 1024 16.8 / 16.4, 21.4 / 22.9, 29.6 / 33.9; 32 of 2048 18.7 / 18.3, 24.6 / 25.2, 32 / 34; 16 of 4096 23.5 / 22.2, 29.0 / 28.0,
+  // 36 / 36; 8 of 8192 31 / 31, 38 / 38, 50 / 50; and behind it, 64 of 2048 20.8 / 18.4, 27.4 / 27.4, 40 / 43; 32 of 4096 25 / 22, 31 / 30, 42 / 42)
   if constexpr (R == 1)      // up to 64 experts, as such a router has
     if ((int64_t)q.experts * ((q.hidden + 1023) & ~1023) <= 1 << 16) {
       if (q.experts <= kWholeWaves) layer_choose_whole_kernel<DT, 1, R><<<q.tokens, kWholeThreads, 0, s>>>(x, router, q, bias, choice, weights, indices);

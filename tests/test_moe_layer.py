@@ -131,3 +131,10 @@ def test_layers_are_computed_in_every_way_there_is():
     # eight fragments are for 12 rows an expert and more, four for fewer, one for layers without a gate
     assert products == {(gate, n, r) for gate in (True, False) for n, r in ((8, 2), (8, 4), (4, 1), (4, 2), (2, 1), (2, 2), (2, 4))} | {(False, 1, r) for r in (1, 2, 4)}
     assert {plan[1:] for _, _, plan in PLANS} >= {(r, 1, x) for r in (1, 2, 4) for x in (0, 1)} | {(1, 2, 1), (2, 8, 1), (4, 16, 1), (1, 4, 0), (2, 2, 0)}
+
+
+@pytest.mark.parametrize('tokens,ffn,experts,top_k,gate,fours', [(1, 8192, 4, 2, True, [4096]), (8, 2048, 32, 4, True, [4096]), (1, 16384, 4, 2, False, [4096, 8192, 16384])])
+def test_rows_that_come_faster_in_fours(tokens, ffn, experts, top_k, gate, fours):
+    """Measured up to 10 % shorter with two weight fragments of a workgroup for all other rows."""
+    for hidden in (1024, 2048, 3584, 4032, 4096, 4160, 4608, 5120, 6144, 8192, 8256, 10240, 12288, 16384):
+        assert plan_of((tokens, hidden, ffn, experts, top_k), gate)[0] == (4 if hidden in fours else 2), hidden
