@@ -139,7 +139,8 @@ __device__ __forceinline__ void choose_for(const LayerChoice& q, int token, L&& 
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int e = i * kWave + lane;
-      if (e < q.experts) scratch[e] = bias != nullptr ? score[i] + (double)bias[e] : score[i];
+      // without a bias a group that goes by its best expert goes by that one's logit, as the choice does: scores of 1 - 1e-17 are all 1
+      if (e < q.experts) scratch[e] = bias != nullptr ? score[i] + (double)bias[e] : q.group_best == 1 ? logit(e) : score[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     double best = -INFINITY, second = -INFINITY;

@@ -554,3 +554,22 @@ def test_layers_with_norms_that_are_infinite_in_fp32(monkeypatch):
     with torch.no_grad():
         got, want = layer(x), separate(x)
     assert not made and torch.equal(got, want)
+
+
+@pytest.mark.parametrize('score,logit', [('sigmoid', 48.0), ('sigmoid', -800.0), ('softmax', 48.0)])
+@pytest.mark.parametrize('tokens,experts,groups', [(1, 32, 8), (6, 64, 4), (20, 256, 8)])
+def test_groups_by_their_best_expert_where_scores_are_all_alike(tokens, experts, groups, score, logit):
+    """Logits of 40 to 56, whose sigmoid scores are 1 in 64 bits, or of -800, whose are 0; groups go by the largest logit, as in choose_experts."""
+    o = make(tokens, 128, 72, experts, std=0.02)
+    o['x'] = (o['x'].float() * 4).bfloat16()
+    o['x'][:, 0], o['router'][:, 0] = 1.0, logit
+    if score == 'softmax':
+        o['router'][0, 0] = 1000.0         # next to which all others have a score of 0
+    logits = o['x'].double() @ o['router'].double().t()
+    of = logits.view(tokens, groups, -1)
+    ranks = of.amax(2).sort(dim=1, descending=True, stable=True).indices.argsort(1)
+    keys = of.masked_fill((ranks >= 2).unsqueeze(2), -float('inf')).flatten(1)
+    want = keys.sort(dim=1, descending=True, stable=True).indices[:, :3]
+    _, _, indices = ops.moe_layer(**o, top_k=3, act=0, score=score, groups=groups, top_groups=2, group_best=1)
+    assert torch.equal(indices, want)
+    assert torch.equal(ops.choose_experts(logits.float(), 3, score, groups=groups, top_groups=2, group_best=1)[2], want)
