@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kJoinThreads) embedding_join_kernel(int hidden
 // ---- up to kFewTokens tokens: the gradient by one launch ----
 // A workgroup has up to kFewWords words and kFewSlices slices of the columns: it lists the tokens of those words, in order, and a wave adds up those of a word for a slice.
 // Bound by the launch, or by the zeros of a large table.  Tokens of one word are added up one after the other, so it is for few of them (us of three launches / of this, forward
-// included: 64 tokens, 1000 words of 64 19.2 / 7.8; 256 tokens, 128000 words of 2040 121 / 111; 128 tokens of one word of 4096 17.2 / 18.2, 256 of them 18.2 / 33).
+// included: 64 tokens, 1000 words of 64 19.2 / 5.9; 256 tokens, 128000 words of 2040 121 / 110; but 128 tokens of one word of 4096 17.2 / 19.0, 256 of them 18.2 / 35.5).
 constexpr int kFewTokens = kEmbThreads, kFewWords = 16, kFewSlices = kEmbWaves;
 
 template <int DT, typename I>

@@ -31,7 +31,7 @@ def moe_layer(x: torch.Tensor, router: torch.Tensor, w1: torch.Tensor, v1: Optio
     """(out, weights, indices) of a mixture-of-experts layer for up to 64 tokens x [tokens, hidden], without gradients:
 
         logits  = x @ router^T, router [experts, hidden]
-        weights, indices = the choice of `choose_experts` with the options of that name, [tokens, top_k], fp32 and int64
+        weights, indices = the choice of `choose_experts` with the options of that name, [tokens, top_k], fp32 and int64; scores in 64 bits
         out[t]  = sum_j weights[t, j] (activation(x[t] @ w1[e]^T) * (x[t] @ v1[e]^T)) @ w2[e], e = indices[t, j]
 
     w1, v1 (None: no gate) and w2: [experts, ffn, hidden], contiguous, all of x's type, bf16 or fp16; hidden and ffn multiples of 8; up to 16 experts a token.  act: ACT_SILU or
