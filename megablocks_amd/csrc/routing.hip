@@ -742,11 +742,15 @@ int mbx_cumsum(const void* x, int itype, int64_t rows, int64_t n, int exclusive,
   if (!x || !out) return MBX_EINVAL;
   if (rows > 0x7fffffff) return MBX_ERANGE;
   hipStream_t s = as_stream(stream);
-  switch (itype) {
-    case MBX_I16: cumsum_kernel<int16_t><<<(unsigned)rows, 256, 0, s>>>((const int16_t*)x, n, exclusive, (int16_t*)out); break;
-    case MBX_I32: cumsum_kernel<int32_t><<<(unsigned)rows, 256, 0, s>>>((const int32_t*)x, n, exclusive, (int32_t*)out); break;
-    case MBX_I64: cumsum_kernel<int64_t><<<(unsigned)rows, 256, 0, s>>>((const int64_t*)x, n, exclusive, (int64_t*)out); break;
-    default: return MBX_EINVAL;
+  constexpr int64_t kMaxRows = 1 << 23;      // of a launch, whose threads have to be fewer than 2^32
+  for (int64_t first = 0; first < rows; first += kMaxRows) {
+    const unsigned grid = (unsigned)(rows - first < kMaxRows ? rows - first : kMaxRows);
+    switch (itype) {
+      case MBX_I16: cumsum_kernel<int16_t><<<grid, 256, 0, s>>>((const int16_t*)x + first * n, n, exclusive, (int16_t*)out + first * n); break;
+      case MBX_I32: cumsum_kernel<int32_t><<<grid, 256, 0, s>>>((const int32_t*)x + first * n, n, exclusive, (int32_t*)out + first * n); break;
+      case MBX_I64: cumsum_kernel<int64_t><<<grid, 256, 0, s>>>((const int64_t*)x + first * n, n, exclusive, (int64_t*)out + first * n); break;
+      default: return MBX_EINVAL;
+    }
   }
   return launch_status();
 }

@@ -795,3 +795,12 @@ def test_round_up_in_one_launch(ops):
         assert torch.equal(ops.round_up(x.cuda(), value).cpu(), want)
         assert torch.equal(ops.round_up(x.cuda()[::3], value).cpu(), want[::3])
     assert ops.round_up(x[:0].cuda(), 128).shape == (0,) and ops.round_up(x.cuda().view(10, 100), 128).shape == (10, 100)
+
+
+@pytest.mark.parametrize('rows', [2 ** 23 + 3, 2 ** 24 + 5])
+def test_cumsum_of_more_rows_than_a_launch_has_threads_for(ops, rows):
+    """A workgroup of 256 threads has a row; a launch has fewer than 2^32 threads."""
+    x = torch.randint(0, 100, (rows, 2), device='cuda', dtype=torch.int16)
+    torch.full_like(x, 9)
+    assert torch.equal(ops.inclusive_cumsum(x, 1), torch.stack([x[:, 0], x[:, 0] + x[:, 1]], 1))
+    assert torch.equal(ops.exclusive_cumsum(x, 1), torch.stack([torch.zeros_like(x[:, 0]), x[:, 0]], 1))
