@@ -452,7 +452,7 @@ int mbx_router_forward(const void* logits, int dtype, int64_t tokens, int num_ex
 /* The linear layer in front of it as well, megablocks/layers/router.py:96-106, for 16-bit types in one launch:
  * logits = round(x @ weight^T) with x [tokens, hidden], weight [num_experts, hidden], then the above (the logits are not
  * written).  Meant for a few tokens.  MBX_EUNSUPPORTED: fp32, hidden not a multiple of 8, x or weight not 16-byte
- * aligned, more than 128 experts, top_k above 64. */
+ * aligned, more than 128 experts, top_k above 64, 2^22 tokens and more. */
 int mbx_router_linear_forward(const void* x, const void* weight, int dtype, int64_t tokens, int hidden, int num_experts, int top_k,
                               float norm_p, void* scores, void* weights, int64_t* indices, int32_t* indices32, mbx_stream_t stream);
 

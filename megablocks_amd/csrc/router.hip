@@ -585,7 +585,7 @@ int mbx_router_linear_forward(const void* x, const void* weight, int dtype, int6
   if (tokens < 0 || hidden <= 0 || num_experts <= 0 || top_k <= 0 || top_k > num_experts || !(norm_p >= 0.f)) return MBX_EINVAL;
   if (dtype != MBX_BF16 && dtype != MBX_F16 && dtype != MBX_F32) return MBX_EINVAL;
   if (dtype == MBX_F32 || hidden % 8 || num_experts > kLinearMaxExperts || top_k > kWave || (int64_t)num_experts * hidden * 2 >= ((int64_t)1 << 30) ||
-      tokens > 0x7fffffff || (((uintptr_t)x | (uintptr_t)weight) & 15u)) return MBX_EUNSUPPORTED;
+      tokens * (kLinearWaves * kWave) >= (int64_t)1 << 32 || (((uintptr_t)x | (uintptr_t)weight) & 15u)) return MBX_EUNSUPPORTED;     // a launch's threads are fewer
   if (tokens == 0) return 0;
   if (!x || !weight || !scores || !weights || !indices) return MBX_EINVAL;
   hipStream_t s = as_stream(stream);

@@ -155,3 +155,10 @@ def test_bench_refuses_more_than_one_gpu():
                          timeout=120)
     assert run.returncode != 0
     assert 'one GPU' in run.stderr and run.stdout.strip() == ''
+
+
+def test_the_fused_router_refuses_tokens_past_what_a_launch_has_threads_for():
+    """A token is a workgroup of 1024 threads, and a launch has fewer than 2^32."""
+    from megablocks_amd._lib import lib, EUNSUPPORTED, EINVAL
+    for tokens, code in (((1 << 22) - 1, EINVAL), (1 << 22, EUNSUPPORTED), ((1 << 22) + 5, EUNSUPPORTED)):      # sizes that are taken: refused for a missing operand only
+        assert lib.mbx_router_linear_forward(None, None, 0, tokens, 64, 8, 2, 0.0, None, None, None, None, None) == code
