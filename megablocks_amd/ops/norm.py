@@ -119,9 +119,10 @@ class _Place:
 
     def __init__(self, t):
         self.item, self.begin = t.element_size(), t.data_ptr()
-        self.dims = sorted((stride * self.item, size) for stride, size in zip(t.stride(), t.shape) if size > 1)
+        dims = [(stride * self.item, size) for stride, size in zip(t.stride(), t.shape) if size > 1]
+        self.dims = sorted(dims)
         self.end = self.begin + self.item + sum(stride * (size - 1) for stride, size in self.dims)
-        self.same = self.begin, self.dims, t.dtype
+        self.same = self.begin, dims, t.dtype      # value by value
 
     def over_itself(self):
         """Whether two values may lie over each other: one step of a dimension is within what the narrower ones reach."""

@@ -120,6 +120,15 @@ def test_which_views_lie_over_each_other(case):
             norm._refuse_overlaps(tensors if out is None else out, tensors)
 
 
+def test_an_output_in_the_place_of_its_tensor_in_another_order_is_refused():
+    from megablocks_amd.ops import norm
+    square, line = torch.zeros(8, 8), torch.zeros(100)
+    for t, o in ((square, square.t()), (square[:, ::2], square[::2].t()), (line.as_strided((3, 5), (20, 2)), line.as_strided((5, 3), (2, 20)))):
+        with pytest.raises(ValueError):
+            norm._refuse_overlaps([o], [t])
+    norm._refuse_overlaps([square[:, ::2]], [square[:, ::2]])
+
+
 def test_views_of_a_buffer_that_are_apart_are_shown_to_be():
     """Every pair of slices with steps of a small matrix: what is said to be apart has no value in common, and little that has none is refused."""
     from megablocks_amd.ops import norm
